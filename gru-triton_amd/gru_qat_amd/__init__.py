@@ -31,6 +31,7 @@ from .struct_proj import structured_input_projection
 from .quantizers import FakeQuantizePerTensor, QuantizerConfig
 from .observe import gru_scan_observe, hidden_map_dense
 from .calibration import calibrate, freeze_all
+from .gated_linear import gated_linear_scan, gated_linear_step
 from .export import dequantize_int_weights, export_int_weights, quantize_rows
 
 __all__ = [
@@ -48,6 +49,8 @@ __all__ = [
     "fast_dispatch_eligible",
     "freeze_all",
     "forward_fast_dispatch",
+    "gated_linear_scan",
+    "gated_linear_step",
     "gru_scan",
     "gru_scan_butterfly_forward",
     "gru_scan_butterfly_persistent",

@@ -64,6 +64,11 @@ EXPORTS = (
     "gs_observe_tensor_scratch_bytes",
     "gs_observe_scan",
     "gs_observe_scan_scratch_bytes",
+    "gs_glr_scratch_bytes",
+    "gs_glr_fwd",
+    "gs_glr_bwd_scratch_bytes",
+    "gs_glr_bwd",
+    "gs_glr_step",
     "gs_workspace_bytes",
     "gs_bwd_workspace_bytes",
     "gs_bwd_scratch_bytes",
@@ -72,7 +77,7 @@ EXPORTS = (
     "gs_abi_version",
 )
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 QuantTuple = Optional[Tuple[float, int, int]]
 
@@ -349,6 +354,38 @@ class GsObserveArgs(ctypes.Structure):
     ]
 
 
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+ACT_NONE = 0
+ACT_TANH = 1
+
+
+class GsGlrArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("gi", "h0", "reset", "out", "h_last", "scratch")]
+        + [(k, ctypes.c_int64) for k in ("scratch_bytes", "T", "B", "H", "sg_t", "sg_b", "sh0_b", "sr_t", "sr_b",
+                                         "so_t", "so_b")]
+        + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
+    )
+
+
+class GsGlrBwdArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("gi", "h0", "reset", "out", "dout", "dh_last", "dgi", "dh0", "scratch")]
+        + [(k, ctypes.c_int64) for k in ("scratch_bytes", "T", "B", "H", "sg_t", "sg_b", "sh0_b", "sr_t", "sr_b",
+                                         "so_t", "so_b", "sd_t", "sd_b", "sdg_t", "sdg_b")]
+        + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
+    )
+
+
+class GsGlrStepArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("gi", "state", "slots", "out")]
+        + [(k, ctypes.c_int64) for k in ("B", "H", "S", "sg_b", "ss", "so_b")]
+        + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
+    )
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -397,6 +434,15 @@ def load() -> ctypes.CDLL:
             size = getattr(lib, name + "_scratch_bytes")
             size.argtypes = [ctypes.POINTER(argt)]
             size.restype = ctypes.c_int64
+        for name, argt in (("gs_glr", GsGlrArgs), ("gs_glr_bwd", GsGlrBwdArgs)):
+            run = getattr(lib, name if name != "gs_glr" else "gs_glr_fwd")
+            run.argtypes = [ctypes.POINTER(argt), ctypes.c_void_p]
+            run.restype = ctypes.c_int
+            size = getattr(lib, name + "_scratch_bytes")
+            size.argtypes = [ctypes.POINTER(argt)]
+            size.restype = ctypes.c_int64
+        lib.gs_glr_step.argtypes = [ctypes.POINTER(GsGlrStepArgs), ctypes.c_void_p]
+        lib.gs_glr_step.restype = ctypes.c_int
         lib.gs_hidden_map_grad.argtypes = [ctypes.POINTER(GsMapArgs), ctypes.c_void_p, ctypes.c_void_p,
                                            ctypes.c_void_p]
         lib.gs_hidden_map_grad.restype = ctypes.c_int
@@ -641,6 +687,11 @@ PROJ_ARGS = struct.Struct("<7Q5q" "ifii" "ifii" "2Q")
 PROJ_BWD_ARGS = struct.Struct("<8Q7q" "ifii" "2Q" "ifii")
 SPROJ_ARGS = struct.Struct("<i4x8Q9q" "ifii" "ifii" "ifii" "ifii")
 SPROJ_BWD_ARGS = struct.Struct("<i4x10Q10q" "ifii" "ifii" "ifii" "ifii")
+
+# Those of the gated linear recurrence (GsGlrArgs, GsGlrBwdArgs, GsGlrStepArgs).
+GLR_ARGS = struct.Struct("<6Q11q2i")
+GLR_BWD_ARGS = struct.Struct("<9Q15q2i")
+GLR_STEP_ARGS = struct.Struct("<4Q6q2i")
 
 
 def raw_size(lib: ctypes.CDLL, fn_name: str, packed: bytes) -> int:

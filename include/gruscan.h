@@ -62,7 +62,7 @@
 extern "C" {
 #endif
 
-#define GS_ABI_VERSION 5
+#define GS_ABI_VERSION 6
 
 #define GS_OK 0
 #define GS_ERR_INVALID (-1)  /* bad pointer, shape, stride or quant parameter (Python: ValueError) */
@@ -589,6 +589,73 @@ typedef struct gs_observe_args {
 
 int64_t gs_observe_scan_scratch_bytes(const gs_observe_args* args);
 int gs_observe_scan(const gs_observe_args* args, hipStream_t stream);
+
+/* ---- gated linear recurrence (ABI version 6) -------------------------------------
+ * The GRU update without a hidden map, over rows of gi = [gi_z, gi_n]:
+ *   z = sigmoid(gi_z), n = tanh(gi_n) (GS_ACT_TANH) or gi_n (GS_ACT_NONE),
+ *   h_t = z h_{t-1} + (1 - z) n,  out[t] = h_t rounded to the tensors' type
+ * so the sequence is a scan of B H independent channels. reset[t][b] != 0 takes
+ * h_{t-1} as 0 at step t (a new sequence starts in the row), whatever it held.
+ * gi, out, dout and dgi are of one type; states, their gradients and every sum
+ * are fp32. No counterpart in the reference. */
+#define GS_DTYPE_F32 0
+#define GS_DTYPE_BF16 1
+#define GS_ACT_NONE 0
+#define GS_ACT_TANH 1
+
+typedef struct gs_glr_args {
+  const void* gi;        /* [T, B, 2H], strides sg_t, sg_b, 1 (either of T, B outermost)  */
+  const float* h0;       /* [B, H], strides sh0_b, 1, or NULL for zeros                   */
+  const uint8_t* reset;  /* [T, B], strides sr_t, sr_b (bytes), or NULL                   */
+  void* out;             /* [T, B, H], strides so_t, so_b, 1; rows must not overlap       */
+  float* h_last;         /* [B, H] contiguous: h_{T-1} in fp32, or NULL                   */
+  void* scratch;         /* gs_glr_scratch_bytes() bytes, 256-byte aligned                */
+  int64_t scratch_bytes;
+  int64_t T, B, H;
+  int64_t sg_t, sg_b, sh0_b, sr_t, sr_b, so_t, so_b;
+  int32_t dtype, activation;
+} gs_glr_args;
+
+int64_t gs_glr_scratch_bytes(const gs_glr_args* args);
+int gs_glr_fwd(const gs_glr_args* args, hipStream_t stream);
+
+/* Gradients of gs_glr_fwd: dgi, and dh0 (zero where step 0 is a reset). The
+ * gates are recomputed from gi; h_{t-1} is the stored out[t-1] (in the tensors' type). */
+typedef struct gs_glr_bwd_args {
+  const void* gi;
+  const float* h0;
+  const uint8_t* reset;
+  const void* out;       /* the forward's output                                          */
+  const void* dout;      /* [T, B, H], strides sd_t, sd_b, 1                              */
+  const float* dh_last;  /* [B, H] contiguous: gradient of h_last, or NULL                */
+  void* dgi;             /* [T, B, 2H], strides sdg_t, sdg_b, 1; rows must not overlap    */
+  float* dh0;            /* [B, H] contiguous, or NULL                                    */
+  void* scratch;         /* gs_glr_bwd_scratch_bytes() bytes, 256-byte aligned            */
+  int64_t scratch_bytes;
+  int64_t T, B, H;
+  int64_t sg_t, sg_b, sh0_b, sr_t, sr_b, so_t, so_b, sd_t, sd_b, sdg_t, sdg_b;
+  int32_t dtype, activation;
+} gs_glr_bwd_args;
+
+int64_t gs_glr_bwd_scratch_bytes(const gs_glr_bwd_args* args);
+int gs_glr_bwd(const gs_glr_bwd_args* args, hipStream_t stream);
+
+/* One step for serving: row b of gi [B, 2H] advances state slots[b] of a cache
+ * [S, H] in place and writes out [B, H]. slots NULL: row b uses state b. A
+ * negative slot marks an empty row (out 0, no state touched); a slot of S or more
+ * touches no state either and gives NaN. Slots that are in the cache must be
+ * distinct. */
+typedef struct gs_glr_step_args {
+  const void* gi;        /* [B, 2H], strides sg_b, 1                                      */
+  float* state;          /* [S, H], strides ss, 1                                         */
+  const int32_t* slots;  /* [B] or NULL                                                   */
+  void* out;             /* [B, H], strides so_b, 1                                       */
+  int64_t B, H, S;
+  int64_t sg_b, ss, so_b;
+  int32_t dtype, activation;
+} gs_glr_step_args;
+
+int gs_glr_step(const gs_glr_step_args* args, hipStream_t stream);
 
 /* Message for the last failing call on this thread ("" if none). */
 const char* gs_last_error(void);
