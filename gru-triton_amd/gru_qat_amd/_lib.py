@@ -69,6 +69,8 @@ EXPORTS = (
     "gs_glr_bwd_scratch_bytes",
     "gs_glr_bwd",
     "gs_glr_step",
+    "gs_adamw_step",
+    "gs_adamw_dequantize",
     "gs_workspace_bytes",
     "gs_bwd_workspace_bytes",
     "gs_bwd_scratch_bytes",
@@ -386,6 +388,23 @@ class GsGlrStepArgs(ctypes.Structure):
     )
 
 
+class GsAdamwTensor(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale",
+                                        "master")]
+        + [("n", ctypes.c_int64)]
+    )
+
+
+class GsAdamwArgs(ctypes.Structure):
+    _fields_ = (
+        [("tensors", ctypes.POINTER(GsAdamwTensor)), ("count", ctypes.c_int64)]
+        + [(k, ctypes.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+        + [("step", ctypes.c_int64), ("grad_scale", ctypes.c_void_p)]
+        + [(k, ctypes.c_int32) for k in ("param_dtype", "grad_dtype", "state_bits", "has_master")]
+    )
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -441,6 +460,11 @@ def load() -> ctypes.CDLL:
             size = getattr(lib, name + "_scratch_bytes")
             size.argtypes = [ctypes.POINTER(argt)]
             size.restype = ctypes.c_int64
+        lib.gs_adamw_step.argtypes = [ctypes.POINTER(GsAdamwArgs), ctypes.c_void_p]
+        lib.gs_adamw_step.restype = ctypes.c_int
+        lib.gs_adamw_dequantize.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                            ctypes.c_int32, ctypes.c_void_p]
+        lib.gs_adamw_dequantize.restype = ctypes.c_int
         lib.gs_glr_step.argtypes = [ctypes.POINTER(GsGlrStepArgs), ctypes.c_void_p]
         lib.gs_glr_step.restype = ctypes.c_int
         lib.gs_hidden_map_grad.argtypes = [ctypes.POINTER(GsMapArgs), ctypes.c_void_p, ctypes.c_void_p,
@@ -692,6 +716,8 @@ SPROJ_BWD_ARGS = struct.Struct("<i4x10Q10q" "ifii" "ifii" "ifii" "ifii")
 GLR_ARGS = struct.Struct("<6Q11q2i")
 GLR_BWD_ARGS = struct.Struct("<9Q15q2i")
 GLR_STEP_ARGS = struct.Struct("<4Q6q2i")
+# gs_adamw_args; its tensor array (GsAdamwTensor) is packed as 8 words a tensor.
+ADAMW_ARGS = struct.Struct("<Qq5dqQ4i")
 
 
 def raw_size(lib: ctypes.CDLL, fn_name: str, packed: bytes) -> int:

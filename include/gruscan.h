@@ -657,6 +657,45 @@ typedef struct gs_glr_step_args {
 
 int gs_glr_step(const gs_glr_step_args* args, hipStream_t stream);
 
+/* ---- AdamW (ABI version 6) ---------------------------------------------------------
+ * One step over many tensors:
+ *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ *   p = (1 - lr weight_decay) p - (lr / c1) m / (sqrt(v) / sqrt(c2) + eps), ck = 1 - bk^step.
+ * Tensors are contiguous; the array of them is read on the host during the call.
+ * Parameters are fp32, or bf16 with or without an fp32 master (the parameter is then
+ * its rounding; without one, updates under half a unit of bf16 are lost). Moments are
+ * fp32 (state_bits 32), or codes of 8 bits with one fp32 scale A per 256 elements:
+ * int8 c for A sign(c) (c / 127)^2, and uint8 c for A (c / 255)^4. A block with a NaN
+ * or an infinity becomes NaN as a whole. grad_scale (device, optional) multiplies the
+ * gradients; where it is not finite the whole step is skipped. No counterpart in the
+ * reference. */
+typedef struct gs_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;            /* float, or int8_t codes                             */
+  void* exp_avg_sq;         /* float, or uint8_t codes                            */
+  float* exp_avg_scale;     /* [ceil(n / 256)] (state_bits 8), else NULL          */
+  float* exp_avg_sq_scale;
+  float* master;            /* [n] (has_master), else NULL                        */
+  int64_t n;
+} gs_adamw_tensor;
+
+typedef struct gs_adamw_args {
+  const gs_adamw_tensor* tensors; /* host array                                   */
+  int64_t count;
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;             /* 1 at the first step                                */
+  const float* grad_scale;  /* device scalar or NULL                              */
+  int32_t param_dtype, grad_dtype, state_bits, has_master;
+} gs_adamw_args;
+
+int gs_adamw_step(const gs_adamw_args* args, hipStream_t stream);
+
+/* out[i] = the value of code i of n codes with one scale per 256; second != 0: the
+ * uint8 codes of exp_avg_sq, otherwise the int8 ones of exp_avg. */
+int gs_adamw_dequantize(const void* codes, const float* scale, float* out, int64_t n, int32_t second,
+                        hipStream_t stream);
+
 /* Message for the last failing call on this thread ("" if none). */
 const char* gs_last_error(void);
 
