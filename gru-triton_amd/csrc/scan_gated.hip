@@ -123,18 +123,6 @@ struct Pack {
   }
 };
 
-// tanh within a few units in the last place also near 0, where h is small beside
-// tanh_fast's absolute error of 3e-7: x + x^3 p(x^2) below 0.55, with p the polynomial
-// of least largest relative error there (1.7 units with fp32's rounding).
-__device__ __forceinline__ float tanh_near(float x) {
-  const float t = x * x;
-  float p = __builtin_fmaf(0.016437569f, t, -0.052671809f);
-  p = __builtin_fmaf(p, t, 0.13320725f);
-  p = __builtin_fmaf(p, t, -0.33332947f);
-  const float small = __builtin_fmaf(x * t, p, x);
-  return __builtin_fabsf(x) < 0.55f ? small : tanh_fast(x);
-}
-
 template <bool TANH>
 __device__ __forceinline__ void gates(float gz, float gn, float& z, float& n) {
   z = sigmoid(gz);

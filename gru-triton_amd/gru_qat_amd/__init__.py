@@ -32,6 +32,7 @@ from .quantizers import FakeQuantizePerTensor, QuantizerConfig
 from .observe import gru_scan_observe, hidden_map_dense
 from .calibration import calibrate, freeze_all
 from .gated_linear import gated_linear_scan, gated_linear_step
+from .linear import linear_act
 from .optim import AdamW, adamw_dequantize_state, adamw_step
 from .export import dequantize_int_weights, export_int_weights, quantize_rows
 
@@ -70,6 +71,7 @@ __all__ = [
     "hidden_map_dense",
     "input_projection",
     "layer_forward",
+    "linear_act",
     "load_library",
     "quantize_input_weights",
     "quantize_rows",

@@ -69,6 +69,10 @@ EXPORTS = (
     "gs_glr_bwd_scratch_bytes",
     "gs_glr_bwd",
     "gs_glr_step",
+    "gs_linear_scratch_bytes",
+    "gs_linear_fwd",
+    "gs_linear_bwd_scratch_bytes",
+    "gs_linear_bwd",
     "gs_adamw_step",
     "gs_adamw_dequantize",
     "gs_workspace_bytes",
@@ -360,6 +364,10 @@ DTYPE_F32 = 0
 DTYPE_BF16 = 1
 ACT_NONE = 0
 ACT_TANH = 1
+ACT_RELU = 2
+ACT_GELU = 3
+ACT_SILU = 4
+ACT_SIGMOID = 5
 
 
 class GsGlrArgs(ctypes.Structure):
@@ -384,6 +392,22 @@ class GsGlrStepArgs(ctypes.Structure):
     _fields_ = (
         [(k, ctypes.c_void_p) for k in ("gi", "state", "slots", "out")]
         + [(k, ctypes.c_int64) for k in ("B", "H", "S", "sg_b", "ss", "so_b")]
+        + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
+    )
+
+
+class GsLinearArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("x", "w", "bias", "residual", "y", "pre", "scratch")]
+        + [(k, ctypes.c_int64) for k in ("scratch_bytes", "M", "N", "K", "sx", "sr", "sy")]
+        + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
+    )
+
+
+class GsLinearBwdArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("x", "w", "pre", "dy", "dx", "dw", "dbias", "scratch")]
+        + [(k, ctypes.c_int64) for k in ("scratch_bytes", "M", "N", "K", "sx", "sdy")]
         + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
     )
 
@@ -453,8 +477,9 @@ def load() -> ctypes.CDLL:
             size = getattr(lib, name + "_scratch_bytes")
             size.argtypes = [ctypes.POINTER(argt)]
             size.restype = ctypes.c_int64
-        for name, argt in (("gs_glr", GsGlrArgs), ("gs_glr_bwd", GsGlrBwdArgs)):
-            run = getattr(lib, name if name != "gs_glr" else "gs_glr_fwd")
+        for name, argt in (("gs_glr", GsGlrArgs), ("gs_glr_bwd", GsGlrBwdArgs), ("gs_linear", GsLinearArgs),
+                           ("gs_linear_bwd", GsLinearBwdArgs)):
+            run = getattr(lib, name if name.endswith("_bwd") else name + "_fwd")
             run.argtypes = [ctypes.POINTER(argt), ctypes.c_void_p]
             run.restype = ctypes.c_int
             size = getattr(lib, name + "_scratch_bytes")
@@ -712,10 +737,12 @@ PROJ_BWD_ARGS = struct.Struct("<8Q7q" "ifii" "2Q" "ifii")
 SPROJ_ARGS = struct.Struct("<i4x8Q9q" "ifii" "ifii" "ifii" "ifii")
 SPROJ_BWD_ARGS = struct.Struct("<i4x10Q10q" "ifii" "ifii" "ifii" "ifii")
 
-# Those of the gated linear recurrence (GsGlrArgs, GsGlrBwdArgs, GsGlrStepArgs).
+# Those of the gated linear recurrence (GsGlrArgs, GsGlrBwdArgs, GsGlrStepArgs) and of the linear operator.
 GLR_ARGS = struct.Struct("<6Q11q2i")
 GLR_BWD_ARGS = struct.Struct("<9Q15q2i")
 GLR_STEP_ARGS = struct.Struct("<4Q6q2i")
+LINEAR_ARGS = struct.Struct("<7Q7q2i")
+LINEAR_BWD_ARGS = struct.Struct("<8Q6q2i")
 # gs_adamw_args; its tensor array (GsAdamwTensor) is packed as 8 words a tensor.
 ADAMW_ARGS = struct.Struct("<Qq5dqQ4i")
 

@@ -602,6 +602,10 @@ int gs_observe_scan(const gs_observe_args* args, hipStream_t stream);
 #define GS_DTYPE_BF16 1
 #define GS_ACT_NONE 0
 #define GS_ACT_TANH 1
+#define GS_ACT_RELU 2    /* gs_linear_* only from here */
+#define GS_ACT_GELU 3    /* x (1 + erf(x / sqrt 2)) / 2 */
+#define GS_ACT_SILU 4    /* x sigmoid(x) */
+#define GS_ACT_SIGMOID 5
 
 typedef struct gs_glr_args {
   const void* gi;        /* [T, B, 2H], strides sg_t, sg_b, 1 (either of T, B outermost)  */
@@ -656,6 +660,50 @@ typedef struct gs_glr_step_args {
 } gs_glr_step_args;
 
 int gs_glr_step(const gs_glr_step_args* args, hipStream_t stream);
+
+/* ---- linear with activation and residual (ABI version 6) ----------------------------
+ *   pre = x w^T + bias,  y = act(pre) + residual
+ * x [M, K], w [N, K], all tensors of one type (GS_DTYPE_*), every sum in fp32 (bf16
+ * operands on the bf16 MFMA, fp32 ones on the fp32 MFMA). A training forward with an
+ * activation also stores pre, rounded to the type, for the backward. No counterpart in
+ * the reference (its projections are gs_input_proj's). */
+typedef struct gs_linear_args {
+  const void* x;         /* [M, K], row stride sx                                         */
+  const void* w;         /* [N, K] contiguous                                             */
+  const void* bias;      /* [N] or NULL                                                   */
+  const void* residual;  /* [M, N], row stride sr, or NULL                                */
+  void* y;               /* [M, N], row stride sy                                         */
+  void* pre;             /* [M, N] contiguous, or NULL                                    */
+  void* scratch;         /* gs_linear_scratch_bytes() bytes, 256-byte aligned             */
+  int64_t scratch_bytes;
+  int64_t M, N, K;
+  int64_t sx, sr, sy;
+  int32_t dtype, activation;
+} gs_linear_args;
+
+int64_t gs_linear_scratch_bytes(const gs_linear_args* args);
+int gs_linear_fwd(const gs_linear_args* args, hipStream_t stream);
+
+/* With dpre = dy act'(pre) (in bf16 rounded to bf16, as an operand of the products):
+ * dx = dpre w, dw = dpre^T x, dbias = column sums of dy act'(pre). Each of dx, dw, dbias
+ * may be NULL. The residual's gradient is dy itself. */
+typedef struct gs_linear_bwd_args {
+  const void* x;         /* [M, K], row stride sx (dw)                                    */
+  const void* w;         /* [N, K] contiguous (dx)                                        */
+  const void* pre;       /* the forward's, contiguous (activation other than none)        */
+  const void* dy;        /* [M, N], row stride sdy                                        */
+  void* dx;              /* [M, K] contiguous, or NULL                                    */
+  void* dw;              /* [N, K] contiguous, or NULL                                    */
+  void* dbias;           /* [N], or NULL                                                  */
+  void* scratch;         /* gs_linear_bwd_scratch_bytes() bytes, 256-byte aligned         */
+  int64_t scratch_bytes;
+  int64_t M, N, K;
+  int64_t sx, sdy;
+  int32_t dtype, activation;
+} gs_linear_bwd_args;
+
+int64_t gs_linear_bwd_scratch_bytes(const gs_linear_bwd_args* args);
+int gs_linear_bwd(const gs_linear_bwd_args* args, hipStream_t stream);
 
 /* ---- AdamW (ABI version 6) ---------------------------------------------------------
  * One step over many tensors:
