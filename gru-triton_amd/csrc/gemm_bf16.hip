@@ -2,16 +2,17 @@
 // (NT), dpre w (NN) and dpre^T x (TN), with the bias, activation and residual of the
 // forward in the epilogue.
 //
-// A workgroup computes a BM x BN tile of C, K in slices of 64, double-buffered in LDS.
-// The MFMA takes B's tile as its first operand, so that a lane holds four consecutive
-// columns of one row of C (D VGPR v of lane l: C[l % 16][4 (l / 16) + v]) and stores
-// them at once.
+// A workgroup computes a T x T tile of C, T = 256 with 8 waves (each 128 x 64 of it) or
+// 128 or 64 with 4 (each a quarter), K in slices of 32. The MFMA takes B's tile as its first operand, so that
+// a lane holds four consecutive columns of one row of C (D VGPR v of lane l:
+// C[l % 16][4 (l / 16) + v]) and stores them at once. While a slice's products run, the
+// next slice's operands are read from LDS into a second set of registers, so that after
+// the barrier that ends a slice the matrix pipe goes on at once.
 //
 // LDS layouts (16-byte granules, no padding):
-//   operand contiguous along k: row r is 8 granules of 8 k; granule c sits in slot
-//     c ^ (r % 8). A lane reads k = 8 (l / 16) + 32 kk of row l % 16 in 16 bytes; the
-//     16 lanes of a pass (rows r < 8 of one k-group and r >= 8 of another) then cover
-//     all 64 banks.
+//   operand contiguous along k: row r is 4 granules of 8 k; granule c sits in slot
+//     c ^ swz(r). A lane reads k = 8 (l / 16) of row l % 16 in 16 bytes; the 16 lanes of
+//     a pass (rows r < 8 of one k-group and r >= 8 of another) then cover all 64 banks.
 //   operand contiguous along its rows: k-row k is R / 8 granules of 8 rows; granule g
 //     sits in slot g ^ swz(k). ds_read_b64_tr_b16 gives lane l of each 16 four
 //     consecutive k of row l % 16 (lane l supplies the address of k = l / 4, rows
@@ -19,9 +20,9 @@
 //     of k) sit in different 32-byte bank groups.
 // Operands whose rows are 16-byte aligned come straight from memory to LDS
 // (buffer_load ... lds, 16 bytes a lane; the swizzle is in the address each lane asks
-// for, a lane past an edge asks for an offset out of range and gets zeros). Others go
-// through registers, in 16-byte loads at any address, element by element where a
-// granule crosses the end of a row.
+// for, a lane past an edge asks for an offset out of range and gets zeros), four slices
+// deep. Others go through registers, in 16-byte loads at any address, element by element
+// where a granule crosses the end of a row.
 #include "gs_gemm_bf16.h"
 
 namespace gs {
@@ -38,51 +39,50 @@ typedef unsigned int u4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef __attribute__((address_space(3))) void LdsVoid;
 typedef __attribute__((address_space(3))) s4v LdsS4;
 
-constexpr int BK = 64;
+constexpr int BK = 32;
 
-// One operand's tile of a slice: R rows x 64 k in LDS.
+// One operand's tile of a slice: R rows x BK k in LDS.
 template <int R, bool KC, int THREADS>
 struct Tile {
-  static constexpr int kBytes = R * BK * 2, kWaves = THREADS / 64;
+  static constexpr int kBytes = R * BK * 2;
   static constexpr int kLoads = kBytes / 16 / THREADS;  // granules of a thread
+  static constexpr int kReads = KC ? 1 : 2;              // LDS reads of a fragment
   static_assert(kLoads >= 1, "a granule for every thread");
 
-  static __device__ __forceinline__ int swz(int k) {
-    return R >= 128 ? 2 * ((k & 3) | ((k >> 1) & 4)) : 2 * (((k >> 1) & 1) | ((k >> 2) & 2));
+  static __device__ __forceinline__ int swz(int x) {  // of a row (KC) or a k
+    if constexpr (KC) return ((x >> 2) & 3) ^ ((x >> 3) & 1);
+    return R >= 128 ? 2 * ((x & 3) | ((x >> 1) & 4)) : 2 * (((x >> 1) & 1) | ((x >> 2) & 2));
   }
   // row (the first of 8, if not KC) and k (the first of 8, if KC) of the granule at byte `at` of the tile
   static __device__ __forceinline__ void granule(int at, int* row, int* k) {
     if constexpr (KC) {
-      *row = at >> 7;
-      *k = (((at >> 4) & 7) ^ (*row & 7)) * 8;
+      *row = at >> 6;
+      *k = (((at >> 4) & 3) ^ swz(*row)) * 8;
     } else {
       *k = at / (2 * R);
       *row = (((at % (2 * R)) >> 4) ^ swz(*k)) * 8;
     }
   }
-
-  // 16-byte fragment of MFMA step kk, rows row0 .. row0 + 15 (row0 a multiple of 16)
-  static __device__ __forceinline__ bf8 fragment(const char* lds, int row0, int kk, int lane) {
+  // rows row0 .. row0 + 15 (row0 a multiple of 16) of the slice, as an MFMA takes them
+  static __device__ __forceinline__ bf8 fragment(const char* lds, int row0, int lane) {
     const int r = lane & 15, g = lane >> 4;
     if constexpr (KC) {
-      const int at = (row0 + r) * 128 + (((4 * kk + g) ^ (r & 7)) << 4);
-      return *reinterpret_cast<const bf8*>(lds + at);
+      return *reinterpret_cast<const bf8*>(lds + (row0 + r) * 64 + ((g ^ swz(r)) << 4));
     } else {
-      const int k = 8 * g + (r >> 2);  // + 32 kk + 4 h: neither changes swz
-      const int at = k * 2 * R + ((((row0 >> 3) + ((r & 3) >> 1)) ^ swz(k)) << 4) + ((r & 1) << 3) + kk * 64 * R;
+      const int k = 8 * g + (r >> 2);  // and k + 4: the same swz
+      const int at = k * 2 * R + ((((row0 >> 3) + ((r & 3) >> 1)) ^ swz(k)) << 4) + ((r & 1) << 3);
       union {
         s4v h[2];
         bf8 v;
       } u;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4*)(lds + at + h * 8 * R));
+      for (int h = 0; h < 2; ++h) u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4*)(lds + at + h * 8 * R));
       return u.v;
     }
   }
 };
 
-// Rows and k that exist: a load past them gives zeros.
+// Straight to LDS. Rows and k that do not exist, and slices from n on, load zeros.
 template <int R, bool KC, int THREADS>
 struct Direct : Tile<R, KC, THREADS> {
   typedef Tile<R, KC, THREADS> T;
@@ -102,16 +102,17 @@ struct Direct : Tile<R, KC, THREADS> {
     }
   }
   __device__ __forceinline__ void load(int s, int n, char* lds) const {
-    const uint32_t last = s == n - 1 ? ~0u : 0u;
+    const uint32_t last = s == n - 1 ? ~0u : 0u, past = s >= n ? kOffNone : 0u;
     const auto r = bounded_rsrc(base + s * step, 0x7fffffffu);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int e = 0; e < T::kLoads; ++e)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsVoid*)(lds + (wave * T::kLoads + e) * 1024), 16,
-                                               (int)(off[e] | (tail[e] & last)), 0, 0, 0);
+                                               (int)(off[e] | (tail[e] & last) | past), 0, 0, 0);
   }
 };
 
+// Through registers.
 template <int R, bool KC, int THREADS>
 struct Staged : Tile<R, KC, THREADS> {
   typedef Tile<R, KC, THREADS> T;
@@ -127,16 +128,17 @@ struct Staged : Tile<R, KC, THREADS> {
     kend = kend_;
   }
   __device__ __forceinline__ void load(int s, u4v (&x)[T::kLoads]) const {
+    const int k0 = kbeg + s * BK;
+    const __bf16* base = KC ? p + (int64_t)row0 * ld + k0 : p + (int64_t)k0 * ld + row0;
+    const bool inside = row0 + R <= lim && k0 + BK <= kend;  // uniform
 #pragma unroll
     for (int e = 0; e < T::kLoads; ++e) {
       int row, k;
       T::granule((threadIdx.x + e * THREADS) * 16, &row, &k);
-      row += row0;
-      k += kbeg + s * BK;
+      const __bf16* q = base + (KC ? row * ld + k : k * ld + row);
       // elements along the contiguous side that exist
-      const int have = KC ? (row < lim ? kend - k : 0) : (k < kend ? lim - row : 0);
-      const __bf16* q = p + (KC ? row * ld + k : k * ld + row);
-      if (have >= 8) {
+      const int have = KC ? (row0 + row < lim ? kend - k0 - k : 0) : (k0 + k < kend ? lim - row0 - row : 0);
+      if (inside || have >= 8) {
         x[e] = *reinterpret_cast<const u4u*>(q);
       } else {
         unsigned int w[4] = {0u, 0u, 0u, 0u};
@@ -155,76 +157,93 @@ struct Staged : Tile<R, KC, THREADS> {
   }
 };
 
-typedef unsigned int u2u __attribute__((ext_vector_type(2), aligned(2)));
-
-// Four elements of a row from column j on, as far as they exist.
-__device__ __forceinline__ void load_row4(const __bf16* p, int j, int N, float (&x)[4]) {
-  if (j + 4 <= N) {
-    const u2u w = *reinterpret_cast<const u2u*>(p + j);
+// Eight elements of a row from column j on, as far as they exist, at any alignment.
+__device__ __forceinline__ void load_row8(const void* row, int j, int N, float (&x)[8]) {
+  const __bf16* p = static_cast<const __bf16*>(row) + j;
+  if (j + 8 <= N) {
+    const u4u w = *reinterpret_cast<const u4u*>(p);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       x[2 * i] = __uint_as_float(w[i] << 16);
       x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = j + i < N ? (float)p[j + i] : 0.0f;
+    for (int i = 0; i < 8; ++i) x[i] = j + i < N ? (float)p[i] : 0.0f;
   }
 }
-__device__ __forceinline__ void store_row4(__bf16* p, int j, int N, const float (&x)[4]) {
-  if (j + 4 <= N) {
-    u2u w;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      w[i] = __builtin_bit_cast(unsigned int, __builtin_convertvector((f2v{x[2 * i], x[2 * i + 1]}), bf2v));
-    *reinterpret_cast<u2u*>(p + j) = w;
-  } else {
+__device__ __forceinline__ void store_row8(void* row, int j, int N, const float (&x)[8]) {
+  __bf16* p = static_cast<__bf16*>(row) + j;
+  if (j + 8 <= N) {
+    u4u w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (j + i < N) p[j + i] = (__bf16)x[i];
+      w[i] = __builtin_bit_cast(unsigned int, __builtin_convertvector((f2v{x[2 * i], x[2 * i + 1]}), bf2v));
+    *reinterpret_cast<u4u*>(p) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (j + i < N) p[i] = (__bf16)x[i];
   }
 }
 
-// What follows the sums of columns j .. j + 3 of row i (< M; columns from N on do not exist).
-__device__ __forceinline__ void finish4(const LinearEpilogue& e, __bf16* y, int64_t ldy, int i, int j, int N,
-                                        const float (&bias)[4], float (&x)[4]) {
+// What follows the sums of columns j .. j + 7 of row i (< M; columns from N on do not exist).
+__device__ __forceinline__ void finish8(const LinearEpilogue& e, __bf16* y, int64_t ldy, int i, int j, int N,
+                                        const float (&bias)[8], float (&x)[8]) {
 #pragma unroll
-  for (int v = 0; v < 4; ++v) x[v] += bias[v];
-  if (e.pre != nullptr) store_row4(static_cast<__bf16*>(e.pre) + (int64_t)i * N, j, N, x);
-  if (e.act != GS_ACT_NONE) {
-#pragma unroll
-    for (int v = 0; v < 4; ++v) x[v] = act_value(x[v], e.act);
-  }
+  for (int v = 0; v < 8; ++v) x[v] += bias[v];
+  if (e.pre != nullptr) store_row8(static_cast<__bf16*>(e.pre) + (int64_t)i * N, j, N, x);
+  if (e.act != GS_ACT_NONE) act_values(x, e.act);
   if (e.residual != nullptr) {
-    float r[4];
-    load_row4(static_cast<const __bf16*>(e.residual) + i * e.ldr, j, N, r);
+    float r[8];
+    load_row8(static_cast<const __bf16*>(e.residual) + i * e.ldr, j, N, r);
 #pragma unroll
-    for (int v = 0; v < 4; ++v) x[v] += r[v];
+    for (int v = 0; v < 8; ++v) x[v] += r[v];
   }
-  store_row4(y + i * ldy, j, N, x);
+  store_row8(y + i * ldy, j, N, x);
 }
 
-template <int BM, int BN, int WM, int WN, int LAYOUT, bool DIRECT, bool PART>
-__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_bf16_kernel(GemmBf16Args g) {
-  constexpr int THREADS = 64 * WM * WN, TI = BM / WM / 16, TJ = BN / WN / 16;
+// The order of a slice's NM MFMAs and, between them, NR LDS reads, NW LDS writes and NV
+// loads: the reads first, one per MFMA or two, then the others.
+template <int NM, int NR, int NW, int NV>
+__device__ __forceinline__ void interleave() {
+  constexpr int kPer = NR * 2 <= NM ? 1 : 2, kFirst = (NR + kPer - 1) / kPer;
+  constexpr int kRest = NM - kFirst > 0 ? NM - kFirst : 1, kPut = (NW + NV + kRest - 1) / kRest;
+  static_for<0, NM>([&](auto I) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+    if constexpr (I < kFirst) {
+      __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);  // LDS read
+    } else {
+      constexpr int at = (I - kFirst) * kPut;
+      if constexpr (at < NW) __builtin_amdgcn_sched_group_barrier(0x200, kPut, 0);
+      if constexpr (at >= NW && at < NW + NV) __builtin_amdgcn_sched_group_barrier(0x020, kPut, 0);
+    }
+  });
+}
+
+// A workgroup's waves are 2 along the rows by WJ along the columns.
+template <int BT, int WJ, int LAYOUT, bool DIRECT, bool PART>
+__global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) {
+  constexpr int THREADS = 128 * WJ, TI = BT / 32, TJ = BT / WJ / 16;  // a wave's fragments
   constexpr bool A_KC = LAYOUT != kGemmTN, B_KC = LAYOUT == kGemmNT;
-  typedef typename std::conditional<DIRECT, Direct<BM, A_KC, THREADS>, Staged<BM, A_KC, THREADS>>::type LA;
-  typedef typename std::conditional<DIRECT, Direct<BN, B_KC, THREADS>, Staged<BN, B_KC, THREADS>>::type LB;
+  typedef typename std::conditional<DIRECT, Direct<BT, A_KC, THREADS>, Staged<BT, A_KC, THREADS>>::type LA;
+  typedef typename std::conditional<DIRECT, Direct<BT, B_KC, THREADS>, Staged<BT, B_KC, THREADS>>::type LB;
+  constexpr int kLoads = LA::kLoads + LB::kLoads;
   __shared__ __attribute__((aligned(1024))) char A0[LA::kBytes];
   __shared__ __attribute__((aligned(1024))) char A1[LA::kBytes];
   __shared__ __attribute__((aligned(1024))) char B0[LB::kBytes];
   __shared__ __attribute__((aligned(1024))) char B1[LB::kBytes];
   // Each XCD (workgroup mod 8) takes a run of tiles, in patches of 1024 rows.
-  const int mt = (g.M + BM - 1) / BM, nt = (g.N + BN - 1) / BN, total = mt * nt, per = (total + 7) / 8;
+  const int mt = (g.M + BT - 1) / BT, nt = (g.N + BT - 1) / BT, total = mt * nt, per = (total + 7) / 8;
   const int tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per || tile >= total) return;  // uniform
-  constexpr int kPatch = 1024 / BM;
+  constexpr int kPatch = 1024 / BT;
   const int patch = tile / (kPatch * nt), in_patch = tile - patch * kPatch * nt;
   const int pm = min(kPatch, mt - patch * kPatch);
-  const int i0 = (patch * kPatch + in_patch % pm) * BM, j0 = in_patch / pm * BN;
+  const int i0 = (patch * kPatch + in_patch % pm) * BT, j0 = in_patch / pm * BT;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wi = (wave / WN) * TI * 16, wj = (wave % WN) * TJ * 16;
+  const int wi = wave / WJ * (BT / 2), wj = wave % WJ * (BT / WJ);
   const int kper = ((g.K + g.ksplit - 1) / g.ksplit + BK - 1) / BK * BK;
   const int kbeg = blockIdx.z * kper, kend = min(g.K, kbeg + kper);
   const int n = kend > kbeg ? (kend - kbeg + BK - 1) / BK : 0;
@@ -239,124 +258,169 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_bf16_kernel(GemmBf16Args
   for (int a = 0; a < TI; ++a)
 #pragma unroll
     for (int b = 0; b < TJ; ++b) acc[a][b] = f4v{0.f, 0.f, 0.f, 0.f};
-
-  auto products = [&](const char* A, const char* B) __attribute__((always_inline)) {
-#pragma unroll
-    for (int kk = 0; kk < BK / 32; ++kk) {
-      bf8 fa[TI], fb[TJ];
-#pragma unroll
-      for (int a = 0; a < TI; ++a) fa[a] = LA::fragment(A, wi + 16 * a, kk, lane);
-#pragma unroll
-      for (int b = 0; b < TJ; ++b) fb[b] = LB::fragment(B, wj + 16 * b, kk, lane);
-#pragma unroll
-      for (int a = 0; a < TI; ++a)
-#pragma unroll
-        for (int b = 0; b < TJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[b], fa[a], acc[a][b], 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+  struct Operands {
+    bf8 a[TI], b[TJ];
   };
-  // A slice is read after the barrier that follows its arrival; the buffer it leaves is
-  // filled again after the next one.
+  Operands f0, f1;
+  auto read = [&](const char* A, const char* B, Operands& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < TJ; ++b) f.b[b] = LB::fragment(B, wj + 16 * b, lane);
+#pragma unroll
+    for (int a = 0; a < TI; ++a) f.a[a] = LA::fragment(A, wi + 16 * a, lane);
+  };
+  auto products = [&](const Operands& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < TI; ++a)
+#pragma unroll
+      for (int b = 0; b < TJ; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.b[b], f.a[a], acc[a][b], 0, 0, 0);
+  };
+  constexpr int kReads = TI * LA::kReads + TJ * LB::kReads;
   if constexpr (DIRECT) {
-    auto arrive = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    if (n > 0) {
-      la.load(0, n, A0);
-      lb.load(0, n, B0);
+    __shared__ __attribute__((aligned(1024))) char A2[LA::kBytes];
+    __shared__ __attribute__((aligned(1024))) char A3[LA::kBytes];
+    __shared__ __attribute__((aligned(1024))) char B2[LB::kBytes];
+    __shared__ __attribute__((aligned(1024))) char B3[LB::kBytes];
+    auto load = [&](int s, char* A, char* B) __attribute__((always_inline)) {
+      la.load(s, n, A);
+      lb.load(s, n, B);
+    };
+    // All but the last `kYoung` slices loaded have arrived for every wave, and this wave's
+    // LDS reads are done: two slices stay in flight across a barrier.
+    auto arrive = [&](auto young) __attribute__((always_inline)) {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(young)::value * kLoads) : "memory");
+    };
+    constexpr std::integral_constant<int, 2> I2{};
+    constexpr std::integral_constant<int, 3> I3{};
+    load(0, A0, B0);
+    load(1, A1, B1);
+    load(2, A2, B2);
+    load(3, A3, B3);
+    arrive(I3);
+    read(A0, B0, f0);
+    arrive(I2);
+    // Slice s: its operands are in registers; slice s + 1 has arrived and is read; slice
+    // s + 4 goes where s was, which every wave read before the last barrier.
+    auto slice = [&](int s, const Operands& f, Operands& next, const char* A, const char* B, char* Af,
+                     char* Bf) __attribute__((always_inline)) {
+      read(A, B, next);
+      load(s + 4, Af, Bf);
+      products(f);
+      interleave<TI * TJ, kReads, 0, kLoads>();
+      arrive(I2);
+    };
+    for (int s = 0; s < n; s += 4) {  // slices from n on are zeros
+      slice(s, f0, f1, A1, B1, A0, B0);
+      slice(s + 1, f1, f0, A2, B2, A1, B1);
+      slice(s + 2, f0, f1, A3, B3, A2, B2);
+      slice(s + 3, f1, f0, A0, B0, A3, B3);
     }
-    int s = 0;
-    for (; s + 1 < n; s += 2) {  // in pairs, so that the loop has one exit
-      arrive();
-      la.load(s + 1, n, A1);
-      lb.load(s + 1, n, B1);
-      products(A0, B0);
-      arrive();
-      if (s + 2 < n) {
-        la.load(s + 2, n, A0);
-        lb.load(s + 2, n, B0);
-      }
-      products(A1, B1);
-    }
-    if (s < n) {
-      arrive();
-      products(A0, B0);
-    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
   } else {
-    u4v xa[LA::kLoads], xb[LB::kLoads];
-    auto load = [&](int s) __attribute__((always_inline)) {
-      la.load(s, xa);
-      lb.load(s, xb);
+    u4v xa[2][LA::kLoads], xb[2][LB::kLoads];
+    auto load = [&](int s, auto I) __attribute__((always_inline)) {
+      la.load(s, xa[I]);
+      lb.load(s, xb[I]);
     };
-    auto stage = [&](char* A, char* B) __attribute__((always_inline)) {
-      la.stage(A, xa);
-      lb.stage(B, xb);
+    auto put = [&](int s, auto I, char* A, char* B) __attribute__((always_inline)) {  // slice s to LDS, its registers take s + 2
+      la.stage(A, xa[I]);
+      lb.stage(B, xb[I]);
+      load(s + 2, I);
     };
-    if (n > 0) {
-      load(0);
-      stage(A0, B0);
-    }
-    int s = 0;
-    for (; s + 1 < n; s += 2) {
+    constexpr std::integral_constant<int, 0> I0{};
+    constexpr std::integral_constant<int, 1> I1{};
+    load(0, I0);
+    load(1, I1);
+    put(0, I0, A0, B0);
+    put(1, I1, A1, B1);
+    lds_barrier();
+    read(A0, B0, f0);
+    lds_barrier();
+    auto slice = [&](int s, auto I, const Operands& f, Operands& next, const char* A, const char* B, char* Af,
+                     char* Bf) __attribute__((always_inline)) {
+      read(A, B, next);
+      put(s + 2, I, Af, Bf);
+      products(f);
+      interleave<TI * TJ, kReads, kLoads, kLoads>();
       lds_barrier();
-      load(s + 1);
-      products(A0, B0);
-      stage(A1, B1);
-      lds_barrier();
-      if (s + 2 < n) load(s + 2);
-      products(A1, B1);
-      if (s + 2 < n) stage(A0, B0);
-    }
-    if (s < n) {
-      lds_barrier();
-      products(A0, B0);
+    };
+    for (int s = 0; s < n; s += 2) {
+      slice(s, I0, f0, f1, A1, B1, A0, B0);
+      slice(s + 1, I1, f1, f0, A0, B0, A1, B1);
     }
   }
 
+  // Each wave passes its part of C through LDS, 16 rows at a time, so that a lane gets
+  // eight consecutive columns of a row and a row's bytes are stored together: stored as
+  // the MFMA leaves them (8 bytes a lane, 32 of a row at once), the epilogue of M = 32768,
+  // N = 2048 took 93 us.
+  constexpr int kCols = 16 * TJ, kStride = kCols + 4, kLanes = kCols / 8;  // kLanes lanes hold a row
+  static_assert(16 * kStride * 4 <= LA::kBytes / (THREADS / 256), "a wave's share of a buffer");
+  lds_barrier();  // every wave has read its last operands
+  char* room;
+  if constexpr (DIRECT)
+    room = (wave & 3) == 0 ? A0 : (wave & 3) == 1 ? A1 : (wave & 3) == 2 ? B0 : B1;
+  else
+    room = wave == 0 ? A0 : wave == 1 ? A1 : wave == 2 ? B0 : B1;
+  float* mine = reinterpret_cast<float*>(room + (wave >> 2) * (LA::kBytes / (THREADS / 256)));
   const int r16 = lane & 15, q4 = (lane >> 4) * 4;
+  const int j = j0 + wj + 8 * (lane % kLanes);
+  float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (!PART && g.epi.bias != nullptr && j < g.N) load_row8(g.epi.bias, j, g.N, bias);
 #pragma unroll
-  for (int b = 0; b < TJ; ++b) {
-    const int j = j0 + wj + 16 * b + q4;
-    if (j >= g.N) continue;
-    float bias[4] = {0.f, 0.f, 0.f, 0.f};
-    if (!PART && g.epi.bias != nullptr) load_row4(static_cast<const __bf16*>(g.epi.bias), j, g.N, bias);
+  for (int a = 0; a < TI; ++a) {
 #pragma unroll
-    for (int a = 0; a < TI; ++a) {
-      const int i = i0 + wi + 16 * a + r16;
-      if (i >= g.M) continue;
-      float x[4];
+    for (int b = 0; b < TJ; ++b) *reinterpret_cast<f4v*>(mine + r16 * kStride + 16 * b + q4) = acc[a][b];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int v = 0; v < 4; ++v) x[v] = acc[a][b][v];
+    for (int rr = 0; rr < 16; rr += 64 / kLanes) {
+      const int row = rr + lane / kLanes, i = i0 + wi + 16 * a + row;
+      float x[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f4v w = *reinterpret_cast<const f4v*>(mine + row * kStride + 8 * (lane % kLanes) + 4 * h);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) x[4 * h + v] = w[v];
+      }
+      if (i >= g.M || j >= g.N) continue;
       if constexpr (PART) {
         float* c = g.part + ((int64_t)blockIdx.z * g.M + i) * g.N + j;
         typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
-        if (j + 4 <= g.N) {
-          *reinterpret_cast<f4u*>(c) = f4u{x[0], x[1], x[2], x[3]};
+        if (j + 8 <= g.N) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<f4u*>(c + 4 * h) = f4u{x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]};
         } else {
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
+          for (int v = 0; v < 8; ++v)
             if (j + v < g.N) c[v] = x[v];
         }
       } else {
-        finish4(g.epi, g.y, g.ldy, i, j, g.N, bias, x);
+        finish8(g.epi, g.y, g.ldy, i, j, g.N, bias, x);
       }
     }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
-// y from the splits' sums, added in order: four columns a thread.
+// y from the splits' sums, added in order: eight columns a thread.
 __global__ __launch_bounds__(256) void gemm_bf16_finish_kernel(GemmBf16Args g) {
-  const int quads = (g.N + 3) / 4;
-  const int64_t all = (int64_t)g.M * quads;
+  const int octets = (g.N + 7) / 8;
+  const int64_t all = (int64_t)g.M * octets, stride = (int64_t)g.M * g.N;
   for (int64_t q = blockIdx.x * (int64_t)256 + threadIdx.x; q < all; q += (int64_t)gridDim.x * 256) {
-    const int i = (int)(q / quads), j = (int)(q - (int64_t)i * quads) * 4;
-    float x[4] = {0.f, 0.f, 0.f, 0.f}, bias[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < g.ksplit; ++s) {
-      const float* c = g.part + ((int64_t)s * g.M + i) * g.N + j;
+    const int i = (int)(q / octets), j = (int)(q - (int64_t)i * octets) * 8;
+    float x[8], bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const float* c = g.part + (int64_t)i * g.N + j;
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
+    for (int v = 0; v < 8; ++v) x[v] = j + v < g.N ? c[v] : 0.0f;
+    for (int s = 1; s < g.ksplit; ++s) {
+      c += stride;
+#pragma unroll
+      for (int v = 0; v < 8; ++v)
         if (j + v < g.N) x[v] += c[v];
     }
-    if (g.epi.bias != nullptr) load_row4(static_cast<const __bf16*>(g.epi.bias), j, g.N, bias);
-    finish4(g.epi, g.y, g.ldy, i, j, g.N, bias, x);
+    if (g.epi.bias != nullptr) load_row8(g.epi.bias, j, g.N, bias);
+    finish8(g.epi, g.y, g.ldy, i, j, g.N, bias, x);
   }
 }
 
@@ -377,16 +441,16 @@ bool direct_ok(const void* p, int64_t ld, int64_t extent, bool kc) {
 
 typedef void (*GemmBf16Fn)(GemmBf16Args);
 
-template <int LAYOUT, int BT, int WM, int WN, bool DIRECT>
+template <int LAYOUT, int BT, int WJ, bool DIRECT>
 GemmBf16Fn pick(bool part) {
-  return part ? gemm_bf16_kernel<BT, BT, WM, WN, LAYOUT, DIRECT, true> : gemm_bf16_kernel<BT, BT, WM, WN, LAYOUT, DIRECT, false>;
+  return part ? gemm_bf16_kernel<BT, WJ, LAYOUT, DIRECT, true> : gemm_bf16_kernel<BT, WJ, LAYOUT, DIRECT, false>;
 }
 
 template <int LAYOUT>
 GemmBf16Fn kernel_of(int T, bool direct, bool part) {
-  if (T == 256) return pick<LAYOUT, 256, 2, 4, true>(part);
-  if (T == 128) return direct ? pick<LAYOUT, 128, 2, 2, true>(part) : pick<LAYOUT, 128, 2, 2, false>(part);
-  return direct ? pick<LAYOUT, 64, 2, 2, true>(part) : pick<LAYOUT, 64, 2, 2, false>(part);
+  if (T == 256) return pick<LAYOUT, 256, 4, true>(part);
+  if (T == 128) return direct ? pick<LAYOUT, 128, 2, true>(part) : pick<LAYOUT, 128, 2, false>(part);
+  return direct ? pick<LAYOUT, 64, 2, true>(part) : pick<LAYOUT, 64, 2, false>(part);
 }
 
 }  // namespace
@@ -414,8 +478,8 @@ int gemm_bf16(const GemmBf16Args& g, hipStream_t stream, const char* who) {
   hipLaunchKernelGGL(fn, dim3((unsigned)tiles, 1, (unsigned)g.ksplit), dim3(T == 256 ? 512 : 256), 0, stream, g);
   GS_CHECK_HIP(hipGetLastError());
   if (part) {
-    const int64_t quads = (int64_t)g.M * ((g.N + 3) / 4);
-    hipLaunchKernelGGL(gemm_bf16_finish_kernel, dim3((unsigned)std::min<int64_t>((quads + 255) / 256, 4096)), dim3(256),
+    const int64_t octets = (int64_t)g.M * ((g.N + 7) / 8);
+    hipLaunchKernelGGL(gemm_bf16_finish_kernel, dim3((unsigned)std::min<int64_t>((octets + 255) / 256, 8192)), dim3(256),
                        0, stream, g);
     GS_CHECK_HIP(hipGetLastError());
   }

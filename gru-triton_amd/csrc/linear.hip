@@ -12,12 +12,69 @@ namespace gs {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 64;  // rows of one workgroup of the dpre pass
+constexpr int kRows = 128;  // rows of one workgroup of the dpre pass
 
+typedef unsigned int u4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f2v __attribute__((ext_vector_type(2)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
+
+// V consecutive elements (16 bytes) at any alignment; those from `have` on are zeros.
 template <typename T>
-__device__ __forceinline__ float get(const void* p, int64_t e) {
-  return (float)static_cast<const T*>(p)[e];
-}
+struct Wide;
+template <>
+struct Wide<float> {
+  static constexpr int V = 4;
+  static __device__ __forceinline__ void load(const float* p, int have, float (&x)[4]) {
+    if (have >= 4) {
+      const f4u w = *reinterpret_cast<const f4u*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = i < have ? p[i] : 0.0f;
+    }
+  }
+  static __device__ __forceinline__ void store(float* p, int have, const float (&x)[4]) {
+    if (have >= 4) {
+      *reinterpret_cast<f4u*>(p) = f4u{x[0], x[1], x[2], x[3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < have) p[i] = x[i];
+    }
+  }
+};
+template <>
+struct Wide<__bf16> {
+  static constexpr int V = 8;
+  static __device__ __forceinline__ void load(const __bf16* p, int have, float (&x)[8]) {
+    if (have >= 8) {
+      const u4u w = *reinterpret_cast<const u4u*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = i < have ? (float)p[i] : 0.0f;
+    }
+  }
+  static __device__ __forceinline__ void store(__bf16* p, int have, const float (&x)[8]) {
+    if (have >= 8) {
+      u4u w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = __builtin_bit_cast(unsigned int, __builtin_convertvector((f2v{x[2 * i], x[2 * i + 1]}), bf2v));
+      *reinterpret_cast<u4u*>(p) = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < have) p[i] = (__bf16)x[i];
+    }
+  }
+};
 
 struct DpreArgs {
   const void* pre;  // NULL: no activation, only the column sums
@@ -28,35 +85,72 @@ struct DpreArgs {
   int M, N, act;
 };
 
-// A workgroup takes 64 columns by kRows rows; its 4 waves take every fourth row.
+// A workgroup takes 16 lanes of columns (16 bytes each) by kRows rows; its 16 row lanes
+// take every 16th row, four at a time, and their sums are joined through LDS in order.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void dpre_kernel(DpreArgs p) {
-  __shared__ float red[4][64];
-  const int jl = threadIdx.x & 63, w = threadIdx.x >> 6, j = blockIdx.x * 64 + jl;
-  const int r0 = blockIdx.y * kRows, r1 = min(p.M, r0 + kRows);
-  float sum = 0.0f;
-  if (j < p.N) {
-    for (int r = r0 + w; r < r1; r += 4) {
-      float d = get<T>(p.dy, r * p.sdy + j);
-      if (p.pre != nullptr) d *= act_slope(get<T>(p.pre, (int64_t)r * p.N + j), p.act);
-      sum += d;
-      if (p.dpre != nullptr) static_cast<T*>(p.dpre)[(int64_t)r * p.N + j] = (T)d;
+  constexpr int V = Wide<T>::V, kAhead = 4;
+  __shared__ float red[16][16 * V + 1];
+  const int jl = threadIdx.x & 15, rl = threadIdx.x >> 4, j = (blockIdx.x * 16 + jl) * V;
+  const int r0 = blockIdx.y * kRows, r1 = min(p.M, r0 + kRows), have = p.N - j;
+  float sum[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum[v] = 0.0f;
+  if (have > 0) {
+    const T* dy = static_cast<const T*>(p.dy) + j;
+    const T* pre = static_cast<const T*>(p.pre) + j;
+    T* dpre = static_cast<T*>(p.dpre) + j;
+    for (int r = r0 + rl; r < r1; r += 16 * kAhead) {
+      float d[kAhead][V], x[kAhead][V];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int q = r + 16 * u;
+        Wide<T>::load(dy + q * p.sdy, q < r1 ? have : 0, d[u]);
+        if (p.pre != nullptr) Wide<T>::load(pre + (int64_t)q * p.N, q < r1 ? have : 0, x[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int q = r + 16 * u;
+        if (p.pre != nullptr) {
+          act_slopes(x[u], p.act);
+#pragma unroll
+          for (int v = 0; v < V; ++v) d[u][v] *= x[u][v];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] += d[u][v];
+        if (p.dpre != nullptr && q < r1) Wide<T>::store(dpre + (int64_t)q * p.N, have, d[u]);
+      }
     }
   }
   if (p.part == nullptr) return;
-  red[w][jl] = sum;
+#pragma unroll
+  for (int v = 0; v < V; ++v) red[rl][jl * V + v] = sum[v];
   __syncthreads();
-  if (w == 0 && j < p.N) p.part[(int64_t)blockIdx.y * p.N + j] = ((red[0][jl] + red[1][jl]) + red[2][jl]) + red[3][jl];
+  const int c = threadIdx.x, col = blockIdx.x * 16 * V + c;
+  if (c < 16 * V && col < p.N) {
+    float s = red[0][c];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += red[k][c];
+    p.part[(int64_t)blockIdx.y * p.N + col] = s;
+  }
 }
 
-// dst[e] = sum over parts of src[part * n + e], rounded to the tensor's type.
+// dst[e] = sum over parts of src[part * n + e], rounded to the tensor's type: a workgroup
+// takes 16 columns, its 16 part lanes every 16th part, joined through LDS in order.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sum_parts_kernel(T* dst, const float* src, int64_t n, int parts) {
-  const int64_t e = blockIdx.x * (int64_t)kThreads + threadIdx.x;
-  if (e >= n) return;
-  float s = src[e];
-  for (int k = 1; k < parts; ++k) s += src[k * n + e];
-  dst[e] = (T)s;
+__global__ __launch_bounds__(kThreads) void sum_columns_kernel(T* dst, const float* src, int n, int parts) {
+  __shared__ float red[16][17];
+  const int c = threadIdx.x & 15, l = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
+  float s = 0.0f;
+  if (e < n)
+    for (int k = l; k < parts; k += 16) s += src[(int64_t)k * n + e];
+  red[l][c] = s;
+  __syncthreads();
+  if (l == 0 && e < n) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += red[k][c];
+    dst[e] = (T)s;
+  }
 }
 
 // fp32: what follows the product's sums (with the bias already added), in place in y.
@@ -73,7 +167,9 @@ __global__ __launch_bounds__(kThreads) void post_kernel(PostArgs p) {
     const int j = (int)(e - i * p.N);
     float x = p.y[i * p.ldy + j];
     if (p.e.pre != nullptr) static_cast<float*>(p.e.pre)[e] = x;
-    x = act_value(x, p.e.act);
+    float v[1] = {x};
+    act_values(v, p.e.act);
+    x = v[0];
     if (p.e.residual != nullptr) x += static_cast<const float*>(p.e.residual)[i * p.e.ldr + j];
     p.y[i * p.ldy + j] = x;
   }
@@ -153,14 +249,6 @@ BwdPlan bwd_plan(const gs_linear_bwd_args* a) {
   p.dw = take(a->dw != nullptr && p.split_w > 1, p.split_w * a->N * a->K * 4);
   p.total = at;
   return p;
-}
-
-template <typename T>
-int sum_parts(void* dst, const float* src, int64_t n, int parts, hipStream_t stream) {
-  hipLaunchKernelGGL(sum_parts_kernel<T>, dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream,
-                     static_cast<T*>(dst), src, n, parts);
-  GS_CHECK_HIP(hipGetLastError());
-  return GS_OK;
 }
 
 }  // namespace
@@ -257,7 +345,8 @@ extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {
       if (q.dpre) q.dpre = static_cast<char*>(q.dpre) + r * a->N * size;
       if (q.part) q.part += (int64_t)first * a->N;
       auto fn = bf16 ? dpre_kernel<__bf16> : dpre_kernel<float>;
-      hipLaunchKernelGGL(fn, dim3((unsigned)((a->N + 63) / 64), (unsigned)((q.M + kRows - 1) / kRows)), dim3(kThreads),
+      const int cols = bf16 ? 128 : 64;
+      hipLaunchKernelGGL(fn, dim3((unsigned)((a->N + cols - 1) / cols), (unsigned)((q.M + kRows - 1) / kRows)), dim3(kThreads),
                          0, stream, q);
       GS_CHECK_HIP(hipGetLastError());
     }
@@ -327,13 +416,21 @@ extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {
       g.ksplit = plan.split_w;
       g.layout = kGemmTN;
       rc = gemm_f32(g, stream, who);
-      if (!rc && plan.dw >= 0) rc = sum_parts<float>(a->dw, g.c, a->N * a->K, plan.split_w, stream);
+      if (!rc && plan.dw >= 0)
+        rc = sum_partials(static_cast<float*>(a->dw), g.c, a->N * a->K, plan.split_w, a->N * a->K, stream, who);
     }
     if (rc) return rc;
   }
   if (a->dbias != nullptr) {
     const float* part = static_cast<const float*>(at(plan.cols));
-    rc = bf16 ? sum_parts<__bf16>(a->dbias, part, a->N, chunks, stream) : sum_parts<float>(a->dbias, part, a->N, chunks, stream);
+    const dim3 grid((unsigned)((a->N + 15) / 16));
+    if (bf16)
+      hipLaunchKernelGGL(sum_columns_kernel<__bf16>, grid, dim3(kThreads), 0, stream, static_cast<__bf16*>(a->dbias),
+                         part, (int)a->N, chunks);
+    else
+      hipLaunchKernelGGL(sum_columns_kernel<float>, grid, dim3(kThreads), 0, stream, static_cast<float*>(a->dbias),
+                         part, (int)a->N, chunks);
+    GS_CHECK_HIP(hipGetLastError());
   }
   return rc;
 }
