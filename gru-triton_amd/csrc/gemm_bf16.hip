@@ -33,9 +33,6 @@ typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
 typedef float f4v __attribute__((ext_vector_type(4)));
 typedef float f2v __attribute__((ext_vector_type(2)));
 typedef short s4v __attribute__((ext_vector_type(4)));
-typedef unsigned int u2v __attribute__((ext_vector_type(2)));
-typedef unsigned int u4v __attribute__((ext_vector_type(4)));
-typedef unsigned int u4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef __attribute__((address_space(3))) void LdsVoid;
 typedef __attribute__((address_space(3))) s4v LdsS4;
 
@@ -127,59 +124,53 @@ struct Staged : Tile<R, KC, THREADS> {
     kbeg = kbeg_;
     kend = kend_;
   }
-  __device__ __forceinline__ void load(int s, u4v (&x)[T::kLoads]) const {
+  __device__ __forceinline__ bool inside(int s) const {  // uniform
+    return row0 + R <= lim && kbeg + s * BK + BK <= kend;
+  }
+  // elements of granule e of slice s that exist, along the contiguous side
+  __device__ __forceinline__ int have(int s, int e, int* row, int* k) const {
+    T::granule((threadIdx.x + e * THREADS) * 16, row, k);
+    const int r = row0 + *row, kk = kbeg + s * BK + *k;
+    return KC ? (r < lim ? kend - kk : 0) : (kk < kend ? lim - r : 0);
+  }
+  __device__ __forceinline__ void load(int s, Granule (&x)[T::kLoads]) const {
     const int k0 = kbeg + s * BK;
     const __bf16* base = KC ? p + (int64_t)row0 * ld + k0 : p + (int64_t)k0 * ld + row0;
-    const bool inside = row0 + R <= lim && k0 + BK <= kend;  // uniform
+    const bool in = inside(s);
 #pragma unroll
     for (int e = 0; e < T::kLoads; ++e) {
       int row, k;
-      T::granule((threadIdx.x + e * THREADS) * 16, &row, &k);
+      const int h = have(s, e, &row, &k);
       const __bf16* q = base + (KC ? row * ld + k : k * ld + row);
-      // elements along the contiguous side that exist
-      const int have = KC ? (row0 + row < lim ? kend - k0 - k : 0) : (k0 + k < kend ? lim - row0 - row : 0);
-      if (inside || have >= 8) {
-        x[e] = *reinterpret_cast<const u4u*>(q);
-      } else {
-        unsigned int w[4] = {0u, 0u, 0u, 0u};
-        const unsigned short* h = reinterpret_cast<const unsigned short*>(q);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < have) w[i >> 1] |= (unsigned int)h[i] << (16 * (i & 1));
-        x[e] = u4v{w[0], w[1], w[2], w[3]};
-      }
+      if (in)
+        x[e] = *reinterpret_cast<const GranuleAt*>(q);
+      else
+        x[e] = granule_load(q, h, KC ? k0 + k : row0 + row);
     }
   }
-  __device__ __forceinline__ void stage(char* lds, const u4v (&x)[T::kLoads]) const {
+  __device__ __forceinline__ void stage(int s, char* lds, Granule (&x)[T::kLoads]) const {
+    const bool in = inside(s);
 #pragma unroll
-    for (int e = 0; e < T::kLoads; ++e)
-      *reinterpret_cast<u4v*>(lds + (threadIdx.x + e * THREADS) * 16) = x[e];
+    for (int e = 0; e < T::kLoads; ++e) {
+      int row, k;
+      if (!in) x[e] = granule_settle(x[e], have(s, e, &row, &k));
+      *reinterpret_cast<Granule*>(lds + (threadIdx.x + e * THREADS) * 16) = x[e];
+    }
   }
 };
 
 // Eight elements of a row from column j on, as far as they exist, at any alignment.
 __device__ __forceinline__ void load_row8(const void* row, int j, int N, float (&x)[8]) {
-  const __bf16* p = static_cast<const __bf16*>(row) + j;
-  if (j + 8 <= N) {
-    const u4u w = *reinterpret_cast<const u4u*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = j + i < N ? (float)p[i] : 0.0f;
-  }
+  granule_floats(granule_settle(granule_load(static_cast<const __bf16*>(row) + j, N - j, j), N - j), x);
 }
 __device__ __forceinline__ void store_row8(void* row, int j, int N, const float (&x)[8]) {
   __bf16* p = static_cast<__bf16*>(row) + j;
   if (j + 8 <= N) {
-    u4u w;
+    GranuleAt w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       w[i] = __builtin_bit_cast(unsigned int, __builtin_convertvector((f2v{x[2 * i], x[2 * i + 1]}), bf2v));
-    *reinterpret_cast<u4u*>(p) = w;
+    *reinterpret_cast<GranuleAt*>(p) = w;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -233,10 +224,16 @@ __global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) 
   __shared__ __attribute__((aligned(1024))) char A1[LA::kBytes];
   __shared__ __attribute__((aligned(1024))) char B0[LB::kBytes];
   __shared__ __attribute__((aligned(1024))) char B1[LB::kBytes];
-  // Each XCD (workgroup mod 8) takes a run of tiles, in patches of 1024 rows.
-  const int mt = (g.M + BT - 1) / BT, nt = (g.N + BT - 1) / BT, total = mt * nt, per = (total + 7) / 8;
-  const int tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || tile >= total) return;  // uniform
+  // Each XCD (workgroup mod 8) takes one split, or as few as there are, and of its tiles a
+  // run, in patches of 1024 rows: its L2 then holds what its workgroups share. (With the
+  // tiles of every split spread over all XCDs, dw of M = 32768, N = 2048, K = 1024 read
+  // 670 MB instead of 200.)
+  const int mt = (g.M + BT - 1) / BT, nt = (g.N + BT - 1) / BT, total = mt * nt;
+  const int xcd = blockIdx.x & 7, spread = g.ksplit < 8 ? 8 / g.ksplit : 1;  // XCDs of a split
+  const int per = (total + spread - 1) / spread, slot = blockIdx.x >> 3;
+  const int split = g.ksplit < 8 ? xcd % g.ksplit : xcd + 8 * (slot / per);
+  const int tile = g.ksplit < 8 ? xcd / g.ksplit * per + slot : slot % per;
+  if ((g.ksplit < 8 && slot >= per) || split >= g.ksplit || tile >= total) return;  // uniform
   constexpr int kPatch = 1024 / BT;
   const int patch = tile / (kPatch * nt), in_patch = tile - patch * kPatch * nt;
   const int pm = min(kPatch, mt - patch * kPatch);
@@ -245,7 +242,7 @@ __global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ * (BT / 2), wj = wave % WJ * (BT / WJ);
   const int kper = ((g.K + g.ksplit - 1) / g.ksplit + BK - 1) / BK * BK;
-  const int kbeg = blockIdx.z * kper, kend = min(g.K, kbeg + kper);
+  const int kbeg = split * kper, kend = min(g.K, kbeg + kper);
   const int n = kend > kbeg ? (kend - kbeg + BK - 1) / BK : 0;
 
   LA la;
@@ -316,14 +313,14 @@ __global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) 
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
   } else {
-    u4v xa[2][LA::kLoads], xb[2][LB::kLoads];
+    Granule xa[2][LA::kLoads], xb[2][LB::kLoads];
     auto load = [&](int s, auto I) __attribute__((always_inline)) {
       la.load(s, xa[I]);
       lb.load(s, xb[I]);
     };
     auto put = [&](int s, auto I, char* A, char* B) __attribute__((always_inline)) {  // slice s to LDS, its registers take s + 2
-      la.stage(A, xa[I]);
-      lb.stage(B, xb[I]);
+      la.stage(s, A, xa[I]);
+      lb.stage(s, B, xb[I]);
       load(s + 2, I);
     };
     constexpr std::integral_constant<int, 0> I0{};
@@ -384,7 +381,7 @@ __global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) 
       }
       if (i >= g.M || j >= g.N) continue;
       if constexpr (PART) {
-        float* c = g.part + ((int64_t)blockIdx.z * g.M + i) * g.N + j;
+        float* c = g.part + ((int64_t)split * g.M + i) * g.N + j;
         typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
         if (j + 8 <= g.N) {
 #pragma unroll
@@ -403,21 +400,38 @@ __global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) 
   }
 }
 
-// y from the splits' sums, added in order: eight columns a thread.
+// y from the splits' sums, added in order: eight columns a thread, the loads of up to
+// eight splits in flight.
 __global__ __launch_bounds__(256) void gemm_bf16_finish_kernel(GemmBf16Args g) {
+  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
   const int octets = (g.N + 7) / 8;
   const int64_t all = (int64_t)g.M * octets, stride = (int64_t)g.M * g.N;
   for (int64_t q = blockIdx.x * (int64_t)256 + threadIdx.x; q < all; q += (int64_t)gridDim.x * 256) {
     const int i = (int)(q / octets), j = (int)(q - (int64_t)i * octets) * 8;
     float x[8], bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < 8; ++v) x[v] = 0.0f;
     const float* c = g.part + (int64_t)i * g.N + j;
+    for (int s = 0; s < g.ksplit; s += 8) {
+      f4u w[8][2];
 #pragma unroll
-    for (int v = 0; v < 8; ++v) x[v] = j + v < g.N ? c[v] : 0.0f;
-    for (int s = 1; s < g.ksplit; ++s) {
-      c += stride;
+      for (int u = 0; u < 8; ++u) {
+        const float* d = c + (s + u) * stride;
+        w[u][0] = w[u][1] = f4u{0.f, 0.f, 0.f, 0.f};
+        if (s + u >= g.ksplit) continue;
+        if (j + 8 <= g.N) {
+          w[u][0] = *reinterpret_cast<const f4u*>(d);
+          w[u][1] = *reinterpret_cast<const f4u*>(d + 4);
+        } else {
 #pragma unroll
-      for (int v = 0; v < 8; ++v)
-        if (j + v < g.N) x[v] += c[v];
+          for (int v = 0; v < 8; ++v)
+            if (j + v < g.N) w[u][v >> 2][v & 3] = d[v];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int v = 0; v < 8; ++v) x[v] += w[u][v >> 2][v & 3];
     }
     if (g.epi.bias != nullptr) load_row8(g.epi.bias, j, g.N, bias);
     finish8(g.epi, g.y, g.ldy, i, j, g.N, bias, x);
@@ -428,14 +442,30 @@ __global__ __launch_bounds__(256) void gemm_bf16_finish_kernel(GemmBf16Args g) {
 
 int64_t tiles_of(int M, int N, int T) { return (int64_t)((M + T - 1) / T) * ((N + T - 1) / T); }
 
-int pick_tile(int M, int N, int ksplit) {
-  if (tiles_of(M, N, 256) * ksplit >= 200) return 256;
-  if (tiles_of(M, N, 128) * ksplit >= 200) return 128;
-  return 64;
+constexpr int kTileSizes[3] = {256, 128, 64};
+
+// Microseconds of a product with tile T and `split` splits of K, from runs on the chip:
+// a launch takes 3; a CU does a tile's slice in `slice` and its first loads and last
+// stores in `ends`, tile after tile; splits write their sums and a second launch reads
+// them. (M, N, K, layout; predicted and measured: 32768 x 2048 x 1024 NT T 256 138, 139;
+// 4096 x 1024 x 1024 NT T 128 13, 13; 2048 x 1024 x 512 NT T 64 7.3, 6.8, T 128 9.5, 8.8.)
+double tile_us(int M, int N, int K, int T, int split) {
+  const double slice = T == 256 ? 0.84 : T == 128 ? 0.235 : 0.1, ends = T == 256 ? 7.0 : T == 128 ? 2.7 : 0.55;
+  const int64_t slices = ((K + split - 1) / split + BK - 1) / BK, per_cu = (tiles_of(M, N, T) * split + 255) / 256;
+  return 3.0 + per_cu * (slices * slice + ends) + (split > 1 ? 5.0 + 8e-6 * split * M * N / 4.5 : 0.0);
 }
 
-bool direct_ok(const void* p, int64_t ld, int64_t extent, bool kc) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0 && extent % 8 == 0 &&
+int pick_tile(int M, int N, int K, int split, bool direct) {
+  int best = 64;
+  for (int T : kTileSizes)
+    if ((T < 256 || direct) && tile_us(M, N, K, T, split) < tile_us(M, N, K, best, split)) best = T;
+  return best;
+}
+
+// Whether an operand's rows are whole 16-byte granules (pads: because zeros follow them
+// up to one): its tile can go straight to LDS.
+bool direct_ok(const void* p, int64_t ld, int64_t extent, bool kc, bool pads) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0 && (extent % 8 == 0 || pads) &&
          (kc ? 256 * ld + 64 : 64 * ld + 256) < (int64_t(1) << 29);
 }
 
@@ -456,26 +486,35 @@ GemmBf16Fn kernel_of(int T, bool direct, bool part) {
 }  // namespace
 
 int gemm_bf16_pick_split(int M, int N, int K) {
-  const int64_t tiles = tiles_of(M, N, 128);
-  int s = 1;
-  while (s < 32 && tiles * s < 256 && K / (s * 2) >= 256) s *= 2;
-  return s;
+  int best = 1;
+  double least = 1e30;
+  for (int split = 1; split <= 32 && (split == 1 || K / split >= 4 * BK); split *= 2)
+    for (int T : kTileSizes) {
+      const double us = tile_us(M, N, K, T, split);
+      if (us < least) {
+        least = us;
+        best = split;
+      }
+    }
+  return best;
 }
 
 int gemm_bf16(const GemmBf16Args& g, hipStream_t stream, const char* who) {
-  if (g.M < 1 || g.N < 1 || g.K < 1 || g.ksplit < 1 || g.ksplit > 65535)
+  if (g.M < 1 || g.N < 1 || g.K < 1 || g.ksplit < 1 || g.ksplit > 32)
     return set_error(GS_ERR_INVALID, "%s: GEMM dims must be positive (M=%d, N=%d, K=%d, ksplit=%d)", who, g.M, g.N,
                      g.K, g.ksplit);
+  if ((g.ksplit & (g.ksplit - 1)) != 0) return set_error(GS_ERR_INVALID, "%s: ksplit must be a power of 2", who);
   const bool a_kc = g.layout != kGemmTN, b_kc = g.layout == kGemmNT;
-  const bool direct = direct_ok(g.a, g.lda, a_kc ? g.K : g.M, a_kc) && direct_ok(g.b, g.ldb, b_kc ? g.K : g.N, b_kc);
-  const int T = std::min(pick_tile(g.M, g.N, g.ksplit), direct ? 256 : 128);
+  const bool direct = direct_ok(g.a, g.lda, a_kc ? g.K : g.M, a_kc, g.a_pads) && direct_ok(g.b, g.ldb, b_kc ? g.K : g.N, b_kc, g.b_pads);
+  const int T = pick_tile(g.M, g.N, g.K, g.ksplit, direct);
   const bool part = g.ksplit > 1;
   GemmBf16Fn fn = g.layout == kGemmNT   ? kernel_of<kGemmNT>(T, direct, part)
                   : g.layout == kGemmNN ? kernel_of<kGemmNN>(T, direct, part)
                                         : kernel_of<kGemmTN>(T, direct, part);
-  const int64_t tiles = 8 * ((tiles_of(g.M, g.N, T) + 7) / 8);
-  if (tiles > (1 << 22)) return set_error(GS_ERR_INVALID, "%s: GEMM of too many tiles (M=%d, N=%d)", who, g.M, g.N);
-  hipLaunchKernelGGL(fn, dim3((unsigned)tiles, 1, (unsigned)g.ksplit), dim3(T == 256 ? 512 : 256), 0, stream, g);
+  const int64_t tiles = tiles_of(g.M, g.N, T), spread = g.ksplit < 8 ? 8 / g.ksplit : 1;
+  const int64_t groups = 8 * ((tiles + spread - 1) / spread) * (g.ksplit < 8 ? 1 : (g.ksplit + 7) / 8);
+  if (groups > (1 << 22)) return set_error(GS_ERR_INVALID, "%s: GEMM of too many tiles (M=%d, N=%d)", who, g.M, g.N);
+  hipLaunchKernelGGL(fn, dim3((unsigned)groups), dim3(T == 256 ? 512 : 256), 0, stream, g);
   GS_CHECK_HIP(hipGetLastError());
   if (part) {
     const int64_t octets = (int64_t)g.M * ((g.N + 7) / 8);

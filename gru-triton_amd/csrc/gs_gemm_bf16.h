@@ -25,12 +25,56 @@ struct GemmBf16Args {
   int64_t ldy = 0;
   float* part = nullptr;  // ksplit > 1: split s writes its sums to part + s M N ([M, N] contiguous)
   LinearEpilogue epi;
+  bool a_pads = false, b_pads = false;  // zeros follow the operand's rows up to a multiple of 8 elements
   int M = 0, N = 0, K = 0, ksplit = 1, layout = kGemmNT;
 };
 
 // Splits of K with which a product fills the device (1: none).
 int gemm_bf16_pick_split(int M, int N, int K);
 int gemm_bf16(const GemmBf16Args& g, hipStream_t stream, const char* who);
+
+// Granules: eight consecutive bf16 of a row, at any alignment. Where a row ends inside
+// one, the row's last eight elements are loaded instead and moved down, zeros behind
+// them: one load like any other (element by element, a tile at the edge of an operand
+// took eight dependent loads a slice).
+typedef unsigned int Granule __attribute__((ext_vector_type(4)));
+typedef unsigned int GranuleAt __attribute__((ext_vector_type(4), aligned(2)));
+
+// The load of the granule at p, `have` elements of which are in the row (any number; none:
+// zeros) and `before` elements of the row in front of it; settle() with the same `have`
+// then gives the granule.
+__device__ __forceinline__ Granule granule_load(const __bf16* p, int have, int before) {
+  Granule w = {0u, 0u, 0u, 0u};
+  if (have >= 8) {
+    w = *reinterpret_cast<const GranuleAt*>(p);
+  } else if (have > 0) {
+    if (before >= 8 - have) {
+      w = *reinterpret_cast<const GranuleAt*>(p + have - 8);
+    } else {  // a row of fewer than eight: its elements where settle() looks for them
+      const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = i - (8 - have);
+        if (at >= 0) w[i >> 1] |= (unsigned int)h[at] << (16 * (i & 1));
+      }
+    }
+  }
+  return w;
+}
+__device__ __forceinline__ Granule granule_settle(Granule w, int have) {
+  const int down = have > 0 && have < 8 ? 8 - have : 0;
+  if (down & 4) w = Granule{w[2], w[3], 0u, 0u};
+  if (down & 2) w = Granule{w[1], w[2], w[3], 0u};
+  if (down & 1) w = Granule{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16};
+  return w;
+}
+__device__ __forceinline__ void granule_floats(const Granule& w, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
 
 // The normal distribution's Phi(x) and phi(x) = Phi'(x), Phi within 8e-8: the rational
 // approximation of erf in Abramowitz and Stegun, Handbook of Mathematical Functions,

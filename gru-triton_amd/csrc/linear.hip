@@ -14,33 +14,36 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRows = 128;  // rows of one workgroup of the dpre pass
 
-typedef unsigned int u4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f2v __attribute__((ext_vector_type(2)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
 
-// V consecutive elements (16 bytes) at any alignment; those from `have` on are zeros.
+// 16 bytes of a row at any alignment: `have` elements exist from p on (the rest reads as
+// zeros, and is not written) and `before` elements of the row in front of it.
 template <typename T>
 struct Wide;
 template <>
 struct Wide<float> {
   static constexpr int V = 4;
-  static __device__ __forceinline__ void load(const float* p, int have, float (&x)[4]) {
-    if (have >= 4) {
-      const f4u w = *reinterpret_cast<const f4u*>(p);
+  typedef f4u Raw;
+  static __device__ __forceinline__ Raw load(const float* p, int have, int) {
+    if (have >= 4) return *reinterpret_cast<const f4u*>(p);
+    f4u w = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = w[i];
-    } else {
+    for (int i = 0; i < 3; ++i)
+      if (i < have) w[i] = p[i];
+    return w;
+  }
+  static __device__ __forceinline__ void values(const Raw& w, int, float (&x)[4]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = i < have ? p[i] : 0.0f;
-    }
+    for (int i = 0; i < 4; ++i) x[i] = w[i];
   }
   static __device__ __forceinline__ void store(float* p, int have, const float (&x)[4]) {
     if (have >= 4) {
       *reinterpret_cast<f4u*>(p) = f4u{x[0], x[1], x[2], x[3]};
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 3; ++i)
         if (i < have) p[i] = x[i];
     }
   }
@@ -48,29 +51,23 @@ struct Wide<float> {
 template <>
 struct Wide<__bf16> {
   static constexpr int V = 8;
-  static __device__ __forceinline__ void load(const __bf16* p, int have, float (&x)[8]) {
-    if (have >= 8) {
-      const u4u w = *reinterpret_cast<const u4u*>(p);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = i < have ? (float)p[i] : 0.0f;
-    }
+  typedef Granule Raw;
+  static __device__ __forceinline__ Raw load(const __bf16* p, int have, int before) {
+    return granule_load(p, have, before);
+  }
+  static __device__ __forceinline__ void values(const Raw& w, int have, float (&x)[8]) {
+    granule_floats(granule_settle(w, have), x);
   }
   static __device__ __forceinline__ void store(__bf16* p, int have, const float (&x)[8]) {
     if (have >= 8) {
-      u4u w;
+      GranuleAt w;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         w[i] = __builtin_bit_cast(unsigned int, __builtin_convertvector((f2v{x[2 * i], x[2 * i + 1]}), bf2v));
-      *reinterpret_cast<u4u*>(p) = w;
+      *reinterpret_cast<GranuleAt*>(p) = w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 7; ++i)
         if (i < have) p[i] = (__bf16)x[i];
     }
   }
@@ -79,9 +76,9 @@ struct Wide<__bf16> {
 struct DpreArgs {
   const void* pre;  // NULL: no activation, only the column sums
   const void* dy;
-  void* dpre;       // contiguous, or NULL (column sums only)
+  void* dpre;       // row stride ldp >= N, zeros from column N on; or NULL (column sums only)
   float* part;      // [ceil(M / kRows)][N], or NULL
-  int64_t sdy;
+  int64_t sdy, ldp;
   int M, N, act;
 };
 
@@ -101,24 +98,27 @@ __global__ __launch_bounds__(kThreads) void dpre_kernel(DpreArgs p) {
     const T* pre = static_cast<const T*>(p.pre) + j;
     T* dpre = static_cast<T*>(p.dpre) + j;
     for (int r = r0 + rl; r < r1; r += 16 * kAhead) {
-      float d[kAhead][V], x[kAhead][V];
+      typename Wide<T>::Raw rd[kAhead], rx[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int q = r + 16 * u;
-        Wide<T>::load(dy + q * p.sdy, q < r1 ? have : 0, d[u]);
-        if (p.pre != nullptr) Wide<T>::load(pre + (int64_t)q * p.N, q < r1 ? have : 0, x[u]);
+        rd[u] = Wide<T>::load(dy + q * p.sdy, q < r1 ? have : 0, j);
+        if (p.pre != nullptr) rx[u] = Wide<T>::load(pre + (int64_t)q * p.N, q < r1 ? have : 0, j);
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int q = r + 16 * u;
+        float d[V], x[V];
+        Wide<T>::values(rd[u], q < r1 ? have : 0, d);
         if (p.pre != nullptr) {
-          act_slopes(x[u], p.act);
+          Wide<T>::values(rx[u], q < r1 ? have : 0, x);
+          act_slopes(x, p.act);
 #pragma unroll
-          for (int v = 0; v < V; ++v) d[u][v] *= x[u][v];
+          for (int v = 0; v < V; ++v) d[v] *= x[v];
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] += d[u][v];
-        if (p.dpre != nullptr && q < r1) Wide<T>::store(dpre + (int64_t)q * p.N, have, d[u]);
+        for (int v = 0; v < V; ++v) sum[v] += d[v];
+        if (p.dpre != nullptr && q < r1) Wide<T>::store(dpre + q * p.ldp, min(V, (int)p.ldp - j), d);
       }
     }
   }
@@ -132,6 +132,46 @@ __global__ __launch_bounds__(kThreads) void dpre_kernel(DpreArgs p) {
 #pragma unroll
     for (int k = 1; k < 16; ++k) s += red[k][c];
     p.part[(int64_t)blockIdx.y * p.N + col] = s;
+  }
+}
+
+// Rows of bf16 operands copied to rows of whole 16-byte granules, zeros from `cols` on,
+// so that the product can take them straight to LDS.
+struct PadJob {
+  const __bf16* src;
+  __bf16* dst;
+  int64_t ld, octets;  // octets: rows * ldp / 8; 0: no job
+  int cols, ldp;
+};
+__global__ __launch_bounds__(kThreads) void pad_kernel(PadJob a, PadJob b) {
+  const int64_t all = a.octets + b.octets, step = (int64_t)gridDim.x * kThreads;
+  constexpr int kAhead = 4;
+  for (int64_t q0 = blockIdx.x * (int64_t)kThreads + threadIdx.x; q0 < all; q0 += kAhead * step) {
+    Granule w[kAhead];
+    int have[kAhead];
+    auto at = [&](int u, const PadJob** p) {  // the granule's job and its place there
+      const int64_t q = q0 + u * step;
+      *p = q < a.octets ? &a : &b;
+      return q < a.octets ? q : q - a.octets;
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (q0 + u * step >= all) continue;
+      const PadJob* p;
+      const int64_t o = at(u, &p);
+      const int per = p->ldp / 8;
+      const int64_t row = o / per;
+      const int c = (int)(o - row * per) * 8;
+      have[u] = p->cols - c;
+      w[u] = granule_load(p->src + row * p->ld + c, have[u], c);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (q0 + u * step >= all) continue;
+      const PadJob* p;
+      const int64_t o = at(u, &p);
+      *reinterpret_cast<Granule*>(p->dst + o * 8) = granule_settle(w[u], have[u]);
+    }
   }
 }
 
@@ -215,40 +255,90 @@ int check_bwd(const gs_linear_bwd_args* a, const char* who) {
   return GS_OK;
 }
 
-int fwd_split(const gs_linear_args* a) {
-  return a->dtype == GS_DTYPE_BF16 ? gemm_bf16_pick_split((int)a->M, (int)a->N, (int)a->K) : 1;
+// bf16 products of this many operations and more copy operands whose rows are not whole
+// 16-byte granules. x w^T and dpre w go well through registers (M = 10000, N = 501,
+// K = 333, 3.3 GFLOP: 19.5 us, 23.0 with copies; 13977 x 3171 x 694, 62 GFLOP: 141 and
+// 102). dpre^T x, whose rows all start at another alignment and which is split, does not
+// (M = 600, N = 501, K = 333, 0.2 GFLOP: 16.6 and 13.6 us; 20000 x 1021 x 515: 212 and 70);
+// its copy of dpre then serves dx too.
+constexpr double kPadFlops = 8e9, kPadFlopsDw = 0.2e9;
+
+int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
+
+// Rows of `n` bf16 that a product could take straight to LDS.
+bool granular(const void* p, int64_t ld, int64_t n) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0 && n % 8 == 0;
 }
 
-int64_t fwd_scratch(const gs_linear_args* a) {
-  const int s = fwd_split(a);
-  return s > 1 ? align256(s * a->M * a->N * 4) : 0;
-}
-
-// The backward's scratch: dpre, the column sums' parts, the splits of dx and of dw.
-struct BwdPlan {
-  int split_x, split_w;
-  int64_t dpre, cols, dx, dw, total;  // byte offsets; -1: not used
+// Scratch laid out in 256-byte steps.
+struct Layout {
+  int64_t total = 0;
+  int64_t take(bool used, int64_t bytes) {
+    if (!used) return -1;
+    const int64_t r = total;
+    total += align256(bytes);
+    return r;
+  }
 };
 
-BwdPlan bwd_plan(const gs_linear_bwd_args* a) {
+// The forward's splits and scratch: copies of x and w, the splits' sums (byte offsets, -1: none).
+struct FwdPlan {
+  int split = 1;
+  int64_t x = -1, w = -1, part = -1, total = 0;
+};
+
+// `any`: what any pointers and strides may need.
+FwdPlan fwd_plan(const gs_linear_args* a, bool any) {
+  FwdPlan p;
+  if (a->dtype != GS_DTYPE_BF16) return p;
+  p.split = gemm_bf16_pick_split((int)a->M, (int)a->N, (int)a->K);
+  Layout l;
+  const bool pays = 2.0 * a->M * a->N * a->K >= kPadFlops;
+  p.x = l.take(pays && (any || !granular(a->x, a->sx, a->K)), a->M * up8(a->K) * 2);
+  p.w = l.take(pays && (any || !granular(a->w, a->K, a->K)), a->N * up8(a->K) * 2);
+  p.part = l.take(p.split > 1, p.split * a->M * a->N * 4);
+  p.total = l.total;
+  return p;
+}
+
+// The backward's: dpre (rows of ldp), the column sums' parts, copies of x and w, the
+// splits' sums of dx and of dw.
+struct BwdPlan {
+  int split_x, split_w;
+  int64_t ldp, dpre, cols, x, w, dx, dw, total;
+};
+
+BwdPlan bwd_plan(const gs_linear_bwd_args* a, bool any) {
   BwdPlan p{};
-  const bool bf16 = a->dtype == GS_DTYPE_BF16;
+  const bool bf16 = a->dtype == GS_DTYPE_BF16, products = a->dx || a->dw;
   const int64_t size = bf16 ? 2 : 4;
   p.split_x = bf16 ? gemm_bf16_pick_split((int)a->M, (int)a->K, (int)a->N) : 1;
   p.split_w = bf16 ? gemm_bf16_pick_split((int)a->N, (int)a->K, (int)a->M) : gemm_pick_split((int)a->N, (int)a->K, (int)a->M);
-  int64_t at = 0;
-  auto take = [&](bool used, int64_t bytes) {
-    if (!used) return int64_t(-1);
-    const int64_t r = at;
-    at += align256(bytes);
-    return r;
-  };
-  p.dpre = take(a->activation != GS_ACT_NONE && (a->dx || a->dw), a->M * a->N * size);
-  p.cols = take(a->dbias != nullptr, (a->M + kRows - 1) / kRows * a->N * 4);
-  p.dx = take(a->dx != nullptr && p.split_x > 1, p.split_x * a->M * a->K * 4);
-  p.dw = take(a->dw != nullptr && p.split_w > 1, p.split_w * a->N * a->K * 4);
-  p.total = at;
+  const bool pays = bf16 && 2.0 * a->M * a->N * a->K >= (a->dw ? kPadFlopsDw : kPadFlops);
+  Layout l;
+  p.ldp = pays ? up8(a->N) : a->N;
+  p.dpre = l.take(products && (a->activation != GS_ACT_NONE || (pays && (any || !granular(a->dy, a->sdy, a->N)))),
+                  a->M * p.ldp * size);
+  p.cols = l.take(a->dbias != nullptr, (a->M + kRows - 1) / kRows * a->N * 4);
+  p.x = l.take(pays && a->dw && (any || !granular(a->x, a->sx, a->K)), a->M * up8(a->K) * 2);
+  p.w = l.take(pays && a->dx && (any || !granular(a->w, a->K, a->K)), a->N * up8(a->K) * 2);
+  p.dx = l.take(a->dx && p.split_x > 1, p.split_x * a->M * a->K * 4);
+  p.dw = l.take(a->dw && p.split_w > 1, p.split_w * a->N * a->K * 4);
+  p.total = l.total;
   return p;
+}
+
+// Copies x [M, K] and w [N, K] (either may stay: offset -1) to rows of up8(K).
+int pad(const void* x, int64_t sx, int64_t M, void* xp, const void* w, int64_t N, void* wp, int64_t K,
+        hipStream_t stream) {
+  if (xp == nullptr && wp == nullptr) return GS_OK;
+  const int kp = (int)up8(K);
+  PadJob a{static_cast<const __bf16*>(x), static_cast<__bf16*>(xp), sx, xp ? M * (kp / 8) : 0, (int)K, kp};
+  PadJob b{static_cast<const __bf16*>(w), static_cast<__bf16*>(wp), K, wp ? N * (kp / 8) : 0, (int)K, kp};
+  const int64_t groups = (a.octets + b.octets + kThreads - 1) / kThreads;
+  hipLaunchKernelGGL(pad_kernel, dim3((unsigned)std::min<int64_t>(groups, 8192)), dim3(kThreads), 0, stream, a, b);
+  GS_CHECK_HIP(hipGetLastError());
+  return GS_OK;
 }
 
 }  // namespace
@@ -259,7 +349,7 @@ using namespace gs;
 extern "C" int64_t gs_linear_scratch_bytes(const gs_linear_args* a) {
   clear_error();
   const int rc = check_fwd(a, "gs_linear_scratch_bytes");
-  return rc ? rc : fwd_scratch(a);
+  return rc ? rc : fwd_plan(a, true).total;
 }
 
 extern "C" int gs_linear_fwd(const gs_linear_args* a, hipStream_t stream) {
@@ -268,7 +358,10 @@ extern "C" int gs_linear_fwd(const gs_linear_args* a, hipStream_t stream) {
   int rc = check_fwd(a, who);
   if (rc) return rc;
   if (!a->x || !a->w || !a->y) return set_error(GS_ERR_INVALID, "%s: x, w and y must be non-NULL device pointers", who);
-  if ((rc = check_scratch(who, a->scratch, a->scratch_bytes, fwd_scratch(a)))) return rc;
+  const FwdPlan plan = fwd_plan(a, false);
+  if ((rc = check_scratch(who, a->scratch, a->scratch_bytes, plan.total))) return rc;
+  char* scratch = static_cast<char*>(a->scratch);
+  auto at = [&](int64_t off) -> void* { return off < 0 ? nullptr : scratch + off; };
   LinearEpilogue e;
   e.bias = a->bias;
   e.residual = a->residual;
@@ -276,19 +369,22 @@ extern "C" int gs_linear_fwd(const gs_linear_args* a, hipStream_t stream) {
   e.ldr = a->sr;
   e.act = a->activation;
   if (a->dtype == GS_DTYPE_BF16) {
+    if ((rc = pad(a->x, a->sx, a->M, at(plan.x), a->w, a->N, at(plan.w), a->K, stream))) return rc;
     GemmBf16Args g;
-    g.a = static_cast<const __bf16*>(a->x);
-    g.lda = a->sx;
-    g.b = static_cast<const __bf16*>(a->w);
-    g.ldb = a->K;
+    g.a = static_cast<const __bf16*>(plan.x < 0 ? a->x : at(plan.x));
+    g.lda = plan.x < 0 ? a->sx : up8(a->K);
+    g.b = static_cast<const __bf16*>(plan.w < 0 ? a->w : at(plan.w));
+    g.ldb = plan.w < 0 ? a->K : up8(a->K);
     g.y = static_cast<__bf16*>(a->y);
     g.ldy = a->sy;
-    g.part = static_cast<float*>(a->scratch);
+    g.part = static_cast<float*>(at(plan.part));
     g.epi = e;
     g.M = (int)a->M;
     g.N = (int)a->N;
+    g.a_pads = plan.x >= 0;
+    g.b_pads = plan.w >= 0;
     g.K = (int)a->K;
-    g.ksplit = fwd_split(a);
+    g.ksplit = plan.split;
     return gemm_bf16(g, stream, who);
   }
   GemmArgs g;
@@ -314,7 +410,7 @@ extern "C" int gs_linear_fwd(const gs_linear_args* a, hipStream_t stream) {
 extern "C" int64_t gs_linear_bwd_scratch_bytes(const gs_linear_bwd_args* a) {
   clear_error();
   const int rc = check_bwd(a, "gs_linear_bwd_scratch_bytes");
-  return rc ? rc : bwd_plan(a).total;
+  return rc ? rc : bwd_plan(a, true).total;
 }
 
 extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {
@@ -326,15 +422,15 @@ extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {
   if (!a->dy || (a->dx && !a->w) || (a->dw && !a->x) || (act && !a->pre))
     return set_error(GS_ERR_INVALID, "%s: dy, w (for dx), x (for dw) and pre (with an activation) must be non-NULL device pointers",
                      who);
-  const BwdPlan plan = bwd_plan(a);
+  const BwdPlan plan = bwd_plan(a, false);
   if ((rc = check_scratch(who, a->scratch, a->scratch_bytes, plan.total))) return rc;
   char* scratch = static_cast<char*>(a->scratch);
   auto at = [&](int64_t off) -> void* { return off < 0 ? nullptr : scratch + off; };
   const bool bf16 = a->dtype == GS_DTYPE_BF16;
   const int chunks = (int)((a->M + kRows - 1) / kRows);
   if (plan.dpre >= 0 || plan.cols >= 0) {
-    DpreArgs p{act ? a->pre : nullptr, a->dy, at(plan.dpre), static_cast<float*>(at(plan.cols)), a->sdy, (int)a->M,
-               (int)a->N, a->activation};
+    DpreArgs p{act ? a->pre : nullptr, a->dy, at(plan.dpre), static_cast<float*>(at(plan.cols)), a->sdy, plan.ldp,
+               (int)a->M, (int)a->N, a->activation};
     for (int first = 0; first < chunks; first += 65535) {  // grid.y
       DpreArgs q = p;
       const int64_t r = (int64_t)first * kRows;
@@ -342,7 +438,7 @@ extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {
       q.M = (int)std::min<int64_t>(a->M - r, 65535ll * kRows);
       if (q.pre) q.pre = static_cast<const char*>(q.pre) + r * a->N * size;
       q.dy = static_cast<const char*>(q.dy) + r * a->sdy * size;
-      if (q.dpre) q.dpre = static_cast<char*>(q.dpre) + r * a->N * size;
+      if (q.dpre) q.dpre = static_cast<char*>(q.dpre) + r * plan.ldp * size;
       if (q.part) q.part += (int64_t)first * a->N;
       auto fn = bf16 ? dpre_kernel<__bf16> : dpre_kernel<float>;
       const int cols = bf16 ? 128 : 64;
@@ -352,20 +448,24 @@ extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {
     }
   }
   const void* dpre = plan.dpre >= 0 ? at(plan.dpre) : a->dy;
-  const int64_t sd = plan.dpre >= 0 ? a->N : a->sdy;
+  const int64_t sd = plan.dpre >= 0 ? plan.ldp : a->sdy;
+  const bool dpre_pads = plan.dpre >= 0 && plan.ldp == up8(a->N);
+  if ((rc = pad(a->x, a->sx, a->M, at(plan.x), a->w, a->N, at(plan.w), a->K, stream))) return rc;
   if (a->dx != nullptr) {
     if (bf16) {
       GemmBf16Args g;
       g.a = static_cast<const __bf16*>(dpre);
       g.lda = sd;
-      g.b = static_cast<const __bf16*>(a->w);
-      g.ldb = a->K;
+      g.b = static_cast<const __bf16*>(plan.w < 0 ? a->w : at(plan.w));
+      g.ldb = plan.w < 0 ? a->K : up8(a->K);
       g.y = static_cast<__bf16*>(a->dx);
       g.ldy = a->K;
       g.part = static_cast<float*>(at(plan.dx));
       g.M = (int)a->M;
       g.N = (int)a->K;
       g.K = (int)a->N;
+      g.a_pads = dpre_pads;
+      g.b_pads = plan.w >= 0;
       g.ksplit = plan.split_x;
       g.layout = kGemmNN;
       rc = gemm_bf16(g, stream, who);
@@ -390,14 +490,16 @@ extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {
       GemmBf16Args g;
       g.a = static_cast<const __bf16*>(dpre);
       g.lda = sd;
-      g.b = static_cast<const __bf16*>(a->x);
-      g.ldb = a->sx;
+      g.b = static_cast<const __bf16*>(plan.x < 0 ? a->x : at(plan.x));
+      g.ldb = plan.x < 0 ? a->sx : up8(a->K);
       g.y = static_cast<__bf16*>(a->dw);
       g.ldy = a->K;
       g.part = static_cast<float*>(at(plan.dw));
       g.M = (int)a->N;
       g.N = (int)a->K;
       g.K = (int)a->M;
+      g.a_pads = dpre_pads;
+      g.b_pads = plan.x >= 0;
       g.ksplit = plan.split_w;
       g.layout = kGemmTN;
       rc = gemm_bf16(g, stream, who);
