@@ -661,6 +661,11 @@ int64_t scratch_of(const Plan& plan, int64_t B, int64_t H) {
   return plan.segments > 1 ? (int64_t)(plan.segments - 1) * B * H * (int64_t)sizeof(f2v) : 0;
 }
 
+// What a call of these sizes may need, whatever its pointers and strides.
+int64_t scratch_most(int64_t T, int64_t B, int64_t H) {
+  return std::max(scratch_of(make_plan(T, B, H, 1, true), B, H), scratch_of(make_plan(T, B, H, 2, true), B, H));
+}
+
 int launch(const char* who, int dtype, const Plan& plan, GlrParams& p, bool back, bool tanh, void* scratch,
            int64_t scratch_bytes, hipStream_t stream) {
   const int64_t need = scratch_of(plan, p.B, p.H);
@@ -729,7 +734,7 @@ using namespace gs;
 extern "C" int64_t gs_glr_scratch_bytes(const gs_glr_args* a) {
   clear_error();
   const int rc = check_fwd(a, "gs_glr_scratch_bytes");
-  return rc ? rc : scratch_of(plan_fwd(a), a->B, a->H);
+  return rc ? rc : scratch_most(a->T, a->B, a->H);
 }
 
 extern "C" int gs_glr_fwd(const gs_glr_args* a, hipStream_t stream) {
@@ -760,7 +765,7 @@ extern "C" int gs_glr_fwd(const gs_glr_args* a, hipStream_t stream) {
 extern "C" int64_t gs_glr_bwd_scratch_bytes(const gs_glr_bwd_args* a) {
   clear_error();
   const int rc = check_bwd(a, "gs_glr_bwd_scratch_bytes");
-  return rc ? rc : scratch_of(plan_bwd(a), a->B, a->H);
+  return rc ? rc : scratch_most(a->T, a->B, a->H);
 }
 
 extern "C" int gs_glr_bwd(const gs_glr_bwd_args* a, hipStream_t stream) {

@@ -761,6 +761,17 @@ def raw_size(lib: ctypes.CDLL, fn_name: str, packed: bytes) -> int:
     return n
 
 
+def call_on(fn_name: str, packed: bytes, ordinal: int) -> None:
+    """``raw_call`` by device ordinal, short on the host where that device is current (the common case)."""
+    fn = _RAW_FN.get(fn_name)
+    if fn is None or _raw_stream is None or ordinal != torch.cuda.current_device():
+        raw_call(load(), fn_name, packed, torch.device("cuda", ordinal))
+        return
+    rc = fn(packed, _raw_stream(ordinal))
+    if rc:
+        raise_for(rc, load())
+
+
 def raw_call(lib: ctypes.CDLL, fn_name: str, packed: bytes, dev: torch.device) -> None:
     """Calls ``fn_name`` on the current torch stream of ``dev``."""
     with on_device(dev):

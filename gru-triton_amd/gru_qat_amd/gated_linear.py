@@ -18,7 +18,8 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 _ACTIVATIONS = {"identity": _lib.ACT_NONE, "tanh": _lib.ACT_TANH}
-_SCRATCH: dict = {}  # scratch bytes per entry point, sizes, strides and alignment
+_SCRATCH: dict = {}  # scratch bytes per size query, sizes and strides
+_F32 = torch.float32
 
 
 def _activation(who: str, activation: str) -> int:
@@ -26,6 +27,17 @@ def _activation(who: str, activation: str) -> int:
         return _ACTIVATIONS[activation]
     except (KeyError, TypeError):
         raise ValueError(f"{who}: activation must be 'tanh' or 'identity'; got {activation!r}") from None
+
+
+def _ready(gi: torch.Tensor, a: Optional[torch.Tensor], b: Optional[torch.Tensor]) -> bool:
+    """Whether gi is of a supported type and all are on its GPU: the common case, in few calls. The
+    callers run _require where not, for its messages."""
+    try:
+        d = gi.get_device()
+        return (d >= 0 and gi.dtype in _DTYPES and (a is None or a.get_device() == d)
+                and (b is None or b.get_device() == d))
+    except AttributeError:
+        return False
 
 
 def _require(who: str, ref: torch.Tensor, **tensors: Any) -> None:
@@ -44,14 +56,13 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _scratch(lib: Any, query: str, pack: Any, pointers: tuple, sizes: tuple, aligned: tuple,
-             device: torch.device) -> Tuple[Optional[torch.Tensor], int, int]:
-    key = (query, sizes, sum(p & 3 for p in aligned) == 0)
-    need = _SCRATCH.get(key)
+def _scratch(query: str, pack: Any, pointers: int, sizes: tuple, device: torch.device) -> Tuple[Any, int, int]:
+    """The scratch tensor (None when none is needed), its address and its bytes, by the sizes alone."""
+    need = _SCRATCH.get((query, sizes))
     if need is None:
         if len(_SCRATCH) > 4096:
             _SCRATCH.clear()
-        need = _SCRATCH[key] = _lib.raw_size(lib, query, pack(*pointers, 0, 0, *sizes))
+        need = _SCRATCH[query, sizes] = _lib.raw_size(_lib.load(), query, pack(*[0] * pointers, 0, 0, *sizes))
     if need == 0:
         return None, 0, 0
     t = torch.empty(need, dtype=torch.uint8, device=device)
@@ -62,25 +73,21 @@ def _forward(gi: torch.Tensor, h0: Optional[torch.Tensor], reset: Optional[torch
              batch_first: bool) -> Tuple[torch.Tensor, torch.Tensor]:
     """gi [T, B, 2H] with unit last stride, already checked; out as [T, B, H] (batch rows outermost in
     memory when batch_first) and h_T [B, H] in float32."""
-    lib = _lib.load()
-    T, B, H2 = gi.shape
-    H = H2 // 2
-    dev = gi.device
+    T, B, H = gi.shape
+    H //= 2
+    dtype = gi.dtype
     if batch_first:
-        out = torch.empty((B, T, H), dtype=gi.dtype, device=dev).transpose(0, 1)
+        out = gi.new_empty((B, T, H)).transpose(0, 1)
     else:
-        out = torch.empty((T, B, H), dtype=gi.dtype, device=dev)
-    h_last = torch.empty((B, H), dtype=torch.float32, device=dev)
-    sg, so = gi.stride(), out.stride()
+        out = gi.new_empty((T, B, H))
+    h_last = gi.new_empty((B, H)) if dtype is _F32 else gi.new_empty((B, H), dtype=_F32)
     sr = reset.stride() if reset is not None else (0, 0)
-    pointers = (gi.data_ptr(), _lib.ptr(h0), _lib.ptr(reset), out.data_ptr(), h_last.data_ptr())
-    sizes = (T, B, H, sg[0], sg[1], h0.stride(0) if h0 is not None else 0, sr[0], sr[1], so[0], so[1],
-             _DTYPES[gi.dtype], act)
-    keep, scratch, nbytes = _scratch(lib, "gs_glr_scratch_bytes", _lib.GLR_ARGS.pack, pointers, sizes,
-                                     (pointers[0], pointers[3]), dev)
-    _lib.raw_call(lib, "gs_glr_fwd", _lib.GLR_ARGS.pack(*pointers, scratch, nbytes, *sizes), dev)
-    del keep  # the caching allocator keeps it until the stream's work is done
-    return out, h_last
+    sizes = (T, B, H, *gi.stride()[:2], h0.stride(0) if h0 is not None else 0, *sr, *out.stride()[:2], _DTYPES[dtype], act)
+    keep, scratch, nbytes = _scratch("gs_glr_scratch_bytes", _lib.GLR_ARGS.pack, 5, sizes, gi.device)
+    _lib.call_on("gs_glr_fwd", _lib.GLR_ARGS.pack(
+        gi.data_ptr(), 0 if h0 is None else h0.data_ptr(), 0 if reset is None else reset.data_ptr(), out.data_ptr(),
+        h_last.data_ptr(), scratch, nbytes, *sizes), gi.get_device())
+    return out, h_last  # the caching allocator keeps the scratch until the stream's work is done
 
 
 class GatedLinearScanFunction(torch.autograd.Function):
@@ -96,30 +103,24 @@ class GatedLinearScanFunction(torch.autograd.Function):
     def backward(ctx: Any, dout, dh_last):  # type: ignore[override]
         gi, h0, reset, out = ctx.saved_tensors
         T, B, H = out.shape
-        dev = gi.device
         if dout is None:
             if dh_last is None:
                 return None, None, None, None, None
-            dout = torch.zeros(H, dtype=out.dtype, device=dev).expand(T, B, H)
-        dout = _unit(dout)
-        if dh_last is not None:
+            dout = out.new_zeros(H).expand(T, B, H)
+        elif dout.stride(2) != 1 and H > 1:
+            dout = dout.contiguous()
+        if dh_last is not None and not dh_last.is_contiguous():
             dh_last = dh_last.contiguous()
-        lib = _lib.load()
-        if out.stride(0) >= out.stride(1):
-            dgi = torch.empty((T, B, 2 * H), dtype=gi.dtype, device=dev)
-        else:
-            dgi = torch.empty((B, T, 2 * H), dtype=gi.dtype, device=dev).transpose(0, 1)
-        dh0 = torch.empty((B, H), dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
-        sg, so, sd, sdg = gi.stride(), out.stride(), dout.stride(), dgi.stride()
+        so = out.stride()
+        dgi = gi.new_empty((T, B, 2 * H)) if so[0] >= so[1] else gi.new_empty((B, T, 2 * H)).transpose(0, 1)
+        dh0 = out.new_empty((B, H), dtype=_F32) if ctx.needs_input_grad[1] else None
         sr = reset.stride() if reset is not None else (0, 0)
-        pointers = (gi.data_ptr(), _lib.ptr(h0), _lib.ptr(reset), out.data_ptr(), dout.data_ptr(), _lib.ptr(dh_last),
-                    dgi.data_ptr(), _lib.ptr(dh0))
-        sizes = (T, B, H, sg[0], sg[1], h0.stride(0) if h0 is not None else 0, sr[0], sr[1], so[0], so[1],
-                 sd[0], sd[1], sdg[0], sdg[1], _DTYPES[gi.dtype], ctx.act)
-        keep, scratch, nbytes = _scratch(lib, "gs_glr_bwd_scratch_bytes", _lib.GLR_BWD_ARGS.pack, pointers, sizes,
-                                         (pointers[0], pointers[3], pointers[4], pointers[6]), dev)
-        _lib.raw_call(lib, "gs_glr_bwd", _lib.GLR_BWD_ARGS.pack(*pointers, scratch, nbytes, *sizes), dev)
-        del keep
+        sizes = (T, B, H, *gi.stride()[:2], h0.stride(0) if h0 is not None else 0, *sr, so[0], so[1], *dout.stride()[:2],
+                 *dgi.stride()[:2], _DTYPES[gi.dtype], ctx.act)
+        keep, scratch, nbytes = _scratch("gs_glr_bwd_scratch_bytes", _lib.GLR_BWD_ARGS.pack, 8, sizes, gi.device)
+        _lib.call_on("gs_glr_bwd", _lib.GLR_BWD_ARGS.pack(
+            gi.data_ptr(), _lib.ptr(h0), _lib.ptr(reset), out.data_ptr(), dout.data_ptr(), _lib.ptr(dh_last),
+            dgi.data_ptr(), _lib.ptr(dh0), scratch, nbytes, *sizes), gi.get_device())
         return dgi, dh0, None, None, None
 
 
@@ -138,8 +139,8 @@ def gated_linear_scan(
     taken as zero, whatever it is. Differentiable in gi and h0."""
     who = "gated_linear_scan"
     act = _activation(who, activation)
-    given = {k: t for k, t in (("h0", h0), ("reset", reset)) if t is not None}
-    _require(who, gi, **given)
+    if not _ready(gi, h0, reset):
+        _require(who, gi, **{k: t for k, t in (("h0", h0), ("reset", reset)) if t is not None})
     if gi.dim() != 3 or gi.shape[2] % 2 or gi.shape[2] == 0:
         raise ValueError(f"{who}: gi must be [T, B, 2H] with H > 0; got shape {tuple(gi.shape)}")
     if batch_first:
@@ -180,10 +181,8 @@ def gated_linear_step(
     touches no state. No autograd."""
     who = "gated_linear_step"
     act = _activation(who, activation)
-    if slots is None:
-        _require(who, gi, state=state)
-    else:
-        _require(who, gi, state=state, slots=slots)
+    if not _ready(gi, state, slots):
+        _require(who, gi, state=state, **({} if slots is None else {"slots": slots}))
     if gi.dim() != 2 or gi.shape[1] % 2 or gi.shape[1] == 0 or gi.shape[0] == 0:
         raise ValueError(f"{who}: gi must be [B, 2H] with B, H > 0; got shape {tuple(gi.shape)}")
     B, H = gi.shape[0], gi.shape[1] // 2
@@ -200,9 +199,8 @@ def gated_linear_step(
     else:
         slots = slots.contiguous()
     gi = _unit(gi)
-    out = torch.empty((B, H), dtype=gi.dtype, device=gi.device)
-    lib = _lib.load()
-    a = _lib.GLR_STEP_ARGS.pack(gi.data_ptr(), state.data_ptr(), _lib.ptr(slots), out.data_ptr(), B, H, state.shape[0],
-                                gi.stride(0), state.stride(0), H, _DTYPES[gi.dtype], act)
-    _lib.raw_call(lib, "gs_glr_step", a, gi.device)
+    out = gi.new_empty((B, H))
+    _lib.call_on("gs_glr_step", _lib.GLR_STEP_ARGS.pack(
+        gi.data_ptr(), state.data_ptr(), 0 if slots is None else slots.data_ptr(), out.data_ptr(), B, H, state.shape[0],
+        gi.stride(0), state.stride(0), H, _DTYPES[gi.dtype], act), gi.get_device())
     return out

@@ -31,30 +31,25 @@ def _bwd_scratch(M: int, N: int, K: int, dtype: int, act: int, dx: bool, dw: boo
                          _lib.LINEAR_BWD_ARGS.pack(0, 0, 0, 0, dx, dw, dbias, 0, 0, M, N, K, K, N, dtype, act))
 
 
-def _buffer(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
 def _forward(x2: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], res2: Optional[torch.Tensor], act: int,
              pre: Optional[torch.Tensor]) -> torch.Tensor:
-    lib = _lib.load()
     M, K = x2.shape
     N = w.shape[0]
-    y = torch.empty((M, N), dtype=x2.dtype, device=x2.device)
+    y = x2.new_empty((M, N))
     dtype = _DTYPES[x2.dtype]
     nbytes = _fwd_scratch(M, N, K, dtype)
-    buf = _buffer(nbytes, x2.device)
-    a = _lib.LINEAR_ARGS.pack(x2.data_ptr(), w.data_ptr(), _lib.ptr(bias), _lib.ptr(res2), y.data_ptr(), _lib.ptr(pre),
-                              _lib.ptr(buf), nbytes, M, N, K, x2.stride(0), res2.stride(0) if res2 is not None else 0, N,
-                              dtype, act)
-    _lib.raw_call(lib, "gs_linear_fwd", a, x2.device)
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=x2.device) if nbytes else None
+    _lib.call_on("gs_linear_fwd", _lib.LINEAR_ARGS.pack(
+        x2.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if res2 is None else res2.data_ptr(),
+        y.data_ptr(), 0 if pre is None else pre.data_ptr(), 0 if buf is None else buf.data_ptr(), nbytes, M, N, K,
+        x2.stride(0), 0 if res2 is None else res2.stride(0), N, dtype, act), x2.get_device())
     return y  # buf goes back to the caching allocator, which keeps it until the stream's work is done
 
 
 class LinearActFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x2, w, bias, res2, act):  # type: ignore[override]
-        pre = torch.empty((x2.shape[0], w.shape[0]), dtype=x2.dtype, device=x2.device) if act else None
+        pre = x2.new_empty((x2.shape[0], w.shape[0])) if act else None
         y = _forward(x2, w, bias, res2, act, pre)
         ctx.save_for_backward(x2, w, pre)
         ctx.act = act
@@ -71,22 +66,32 @@ class LinearActFunction(torch.autograd.Function):
             return None, None, None, dres, None
         if dy.stride(1) != 1 and N > 1:
             dy = dy.contiguous()
-        dev, kind = x2.device, x2.dtype
-        dx = torch.empty((M, K), dtype=kind, device=dev) if need[0] else None
-        dw = torch.empty((N, K), dtype=kind, device=dev) if need[1] else None
-        dbias = torch.empty(N, dtype=kind, device=dev) if need[2] else None
-        dtype = _DTYPES[kind]
+        dx = x2.new_empty((M, K)) if need[0] else None
+        dw = x2.new_empty((N, K)) if need[1] else None
+        dbias = x2.new_empty((N,)) if need[2] else None
+        dtype = _DTYPES[x2.dtype]
         nbytes = _bwd_scratch(M, N, K, dtype, ctx.act, *need[:3])
-        buf = _buffer(nbytes, dev)
-        a = _lib.LINEAR_BWD_ARGS.pack(x2.data_ptr(), w.data_ptr(), _lib.ptr(pre), dy.data_ptr(), _lib.ptr(dx),
-                                      _lib.ptr(dw), _lib.ptr(dbias), _lib.ptr(buf), nbytes, M, N, K, x2.stride(0),
-                                      dy.stride(0), dtype, ctx.act)
-        _lib.raw_call(_lib.load(), "gs_linear_bwd", a, dev)
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=x2.device) if nbytes else None
+        _lib.call_on("gs_linear_bwd", _lib.LINEAR_BWD_ARGS.pack(
+            x2.data_ptr(), w.data_ptr(), _lib.ptr(pre), dy.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(dbias),
+            _lib.ptr(buf), nbytes, M, N, K, x2.stride(0), dy.stride(0), dtype, ctx.act), x2.get_device())
         return dx, dw, dbias, dres, None
 
 
+def _require(who: str, x: torch.Tensor, **tensors: Any) -> None:
+    for k, t in dict(x=x, **tensors).items():
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"{who}: {k} must be a CUDA (HIP) tensor; got "
+                             f"{t.device if isinstance(t, torch.Tensor) else type(t).__name__}")
+        if t.get_device() != x.get_device():
+            raise ValueError(f"{who}: all tensors must be on {x.device}; {k} is on {t.device}")
+        if t.dtype != x.dtype or t.dtype not in _DTYPES:
+            raise ValueError(f"{who}: all tensors must be float32 or all bfloat16; {k} is {t.dtype}, x {x.dtype}")
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -108,19 +113,15 @@ def linear_act(
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):
         raise ValueError(f"{who}: activation must be one of {', '.join(_ACTIVATIONS)}; got {activation!r}") from None
-    given = [("x", x), ("weight", weight)]
-    if bias is not None:
-        given.append(("bias", bias))
-    if residual is not None:
-        given.append(("residual", residual))
-    for k, t in given:
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError(f"{who}: {k} must be a CUDA (HIP) tensor; got "
-                             f"{t.device if isinstance(t, torch.Tensor) else type(t).__name__}")
-        if t.get_device() != x.get_device():
-            raise ValueError(f"{who}: all tensors must be on {x.device}; {k} is on {t.device}")
-        if t.dtype != x.dtype or t.dtype not in _DTYPES:
-            raise ValueError(f"{who}: all tensors must be float32 or all bfloat16; {k} is {t.dtype}, x {x.dtype}")
+    try:
+        d, kind = x.get_device(), x.dtype
+        ready = (d >= 0 and kind in _DTYPES and weight.get_device() == d and weight.dtype is kind
+                 and (bias is None or (bias.get_device() == d and bias.dtype is kind))
+                 and (residual is None or (residual.get_device() == d and residual.dtype is kind)))
+    except AttributeError:
+        ready = False
+    if not ready:
+        _require(who, x, weight=weight, **{k: t for k, t in (("bias", bias), ("residual", residual)) if t is not None})
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"{who}: weight must be [N, K] with K = x.shape[-1]; got x {tuple(x.shape)}, weight "
                          f"{tuple(weight.shape)}")
@@ -132,11 +133,13 @@ def linear_act(
     shape = (*x.shape[:-1], N)
     if residual is not None and residual.shape != shape:
         raise ValueError(f"{who}: residual must be {shape}; got {tuple(residual.shape)}")
-    x2, w = _rows(x), weight.contiguous()
-    bias = bias.contiguous() if bias is not None else None
+    x2, w = _rows(x), weight if weight.is_contiguous() else weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     res2 = _rows(residual) if residual is not None else None
-    if torch.is_grad_enabled() and any([t.requires_grad for _, t in given]):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         y = LinearActFunction.apply(x2, w, bias, res2, act)
     else:
         y = _forward(x2, w, bias, res2, act, None)
-    return cast(torch.Tensor, y.view(shape))
+    return cast(torch.Tensor, y if len(shape) == 2 else y.view(shape))

@@ -7,6 +7,7 @@
 from __future__ import annotations
 
 import ctypes
+import operator
 import struct
 from typing import Any, Callable, Iterable, List, Optional, Sequence, Tuple
 
@@ -18,6 +19,11 @@ STATE_BLOCK = 256  # elements of a tensor that share a scale where moments are h
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 _F32 = {torch.float32}
+# over lists of tensors, in C: these calls are most of a small step's time
+_NUMEL, _PTR, _ORDINAL, _CONTIGUOUS = (torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.get_device,
+                                       torch.Tensor.is_contiguous)
+_DTYPE = operator.attrgetter("dtype")
+_ONLY = [{i} for i in range(64)]
 
 
 def _blocks(n: int) -> int:
@@ -29,8 +35,8 @@ def _check_list(who: str, name: str, tensors: Sequence[torch.Tensor], counts: Li
     """One contiguous tensor of counts[i] elements for each parameter, of one of the dtypes, on the device."""
     if len(tensors) != len(counts):
         raise ValueError(f"{who}: {len(tensors)} tensors in {name} for {len(counts)} parameters")
-    if ([t.numel() for t in tensors] == counts and {t.dtype for t in tensors} <= dtypes
-            and all([t.get_device() == device and t.is_contiguous() for t in tensors])):
+    if (list(map(_NUMEL, tensors)) == counts and dtypes.issuperset(map(_DTYPE, tensors))
+            and _ONLY[device] == set(map(_ORDINAL, tensors)) and all(map(_CONTIGUOUS, tensors))):
         return
     for i, (t, n) in enumerate(zip(tensors, counts)):
         if t.get_device() != device:
@@ -70,10 +76,10 @@ def adamw_step(
     who = "adamw_step"
     if not len(params):
         return
-    if not all(isinstance(t, torch.Tensor) for t in params) or not params[0].is_cuda:
+    if not isinstance(params[0], torch.Tensor) or not params[0].is_cuda:
         raise ValueError(f"{who}: params must be CUDA (HIP) tensors")
     dev = params[0].get_device()
-    counts = [p.numel() for p in params]
+    counts = list(map(_NUMEL, params))
     bits = 32 if exp_avg_scales is None else 8
     if (exp_avg_sq_scales is None) != (exp_avg_scales is None):
         raise ValueError(f"{who}: exp_avg_scales and exp_avg_sq_scales belong together")
@@ -81,35 +87,36 @@ def adamw_step(
         if len(ts) and ts[0].dtype not in _DTYPES:
             raise ValueError(f"{who}: {name} must be float32 or bfloat16; got {ts[0].dtype}")
     _check_list(who, "params", params, counts, {params[0].dtype}, dev)
-    if len(grads) == len(params) and not all([g.is_contiguous() for g in grads]):
+    if len(grads) == len(params) and not all(map(_CONTIGUOUS, grads)):
         grads = [g.contiguous() for g in grads]
     _check_list(who, "grads", grads, counts, {grads[0].dtype} if len(grads) else set(), dev)
     _check_list(who, "exp_avgs", exp_avgs, counts, _F32 if bits == 32 else {torch.int8}, dev)
     _check_list(who, "exp_avg_sqs", exp_avg_sqs, counts, _F32 if bits == 32 else {torch.uint8}, dev)
-    zeros: Any = [0] * len(counts)
-    scale_ptrs = master_ptrs = (zeros, zeros)
     if exp_avg_scales is not None and exp_avg_sq_scales is not None:
         blocks = [_blocks(n) for n in counts]
         _check_list(who, "exp_avg_scales", exp_avg_scales, blocks, _F32, dev)
         _check_list(who, "exp_avg_sq_scales", exp_avg_sq_scales, blocks, _F32, dev)
-        scale_ptrs = ([t.data_ptr() for t in exp_avg_scales], [t.data_ptr() for t in exp_avg_sq_scales])
     if masters is not None:
         if params[0].dtype != torch.bfloat16:
             raise ValueError(f"{who}: masters belong to bfloat16 parameters; got {params[0].dtype}")
         _check_list(who, "masters", masters, counts, _F32, dev)
-        master_ptrs = ([t.data_ptr() for t in masters], zeros)
     if grad_scale is not None and (grad_scale.get_device() != dev or grad_scale.dtype != torch.float32
                                    or grad_scale.numel() != 1):
         raise ValueError(f"{who}: grad_scale must be one float32 number on the parameters' device; got "
                          f"{grad_scale.dtype} {tuple(grad_scale.shape)} on {grad_scale.device}")
-    rows = zip([t.data_ptr() for t in params], [t.data_ptr() for t in grads], [t.data_ptr() for t in exp_avgs],
-               [t.data_ptr() for t in exp_avg_sqs], scale_ptrs[0], scale_ptrs[1], master_ptrs[0], counts)
-    table = struct.pack(f"<{8 * len(counts)}Q", *[x for r in rows for x in r])
-    lib = _lib.load()
+    # one row of eight words a tensor (GsAdamwTensor), column by column
+    words = [0] * (8 * len(counts))
+    words[0::8], words[1::8], words[2::8], words[3::8], words[7::8] = (
+        map(_PTR, params), map(_PTR, grads), map(_PTR, exp_avgs), map(_PTR, exp_avg_sqs), counts)
+    if bits == 8:
+        words[4::8], words[5::8] = map(_PTR, exp_avg_scales), map(_PTR, exp_avg_sq_scales)  # type: ignore[arg-type]
+    if masters is not None:
+        words[6::8] = map(_PTR, masters)
+    table = struct.pack(f"<{len(words)}Q", *words)
     a = _lib.ADAMW_ARGS.pack(ctypes.cast(ctypes.c_char_p(table), ctypes.c_void_p).value, len(counts), lr, betas[0],
                              betas[1], eps, weight_decay, step, _lib.ptr(grad_scale), _DTYPES[params[0].dtype],
                              _DTYPES[grads[0].dtype], bits, masters is not None)
-    _lib.raw_call(lib, "gs_adamw_step", a, params[0].device)  # `table` is read during the call
+    _lib.call_on("gs_adamw_step", a, dev)  # `table` is read during the call
 
 
 def adamw_dequantize_state(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
@@ -125,8 +132,8 @@ def adamw_dequantize_state(codes: torch.Tensor, scales: torch.Tensor) -> torch.T
     out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
     lib = _lib.load()
     with _lib.on_device(codes.device):
-        rc = lib.gs_adamw_dequantize(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), n,
-                                     int(codes.dtype == torch.uint8), _lib.current_stream_handle(codes.device))
+        rc = lib.gs_adamw_dequantize(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), n, codes.dtype is torch.uint8,
+                                     _lib.current_stream_handle(codes.device))
     _lib.raise_for(rc, lib)
     return out
 
