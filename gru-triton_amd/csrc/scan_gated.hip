@@ -134,15 +134,18 @@ template <int V, int LC, int NW>
 struct Place {
   static constexpr int NG = 64 / LC;
   int b, j, lc, lg, wave;
-  bool ok;
+  bool ok, any;  // the lane's channels exist; the workgroup's do
   __device__ __forceinline__ Place(const GlrParams& p) {
     const int lane = threadIdx.x & 63;
     wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     lc = lane % LC;
     lg = lane / LC;
-    b = blockIdx.x / p.blocks;
-    j = ((blockIdx.x - b * p.blocks) * LC + lc) * V;
-    ok = j < p.H;
+    // neighbours in a row, which share cache lines, on one XCD (workgroup mod 8)
+    const int per = gridDim.x >> 3, group = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    b = group / p.blocks;
+    any = b < p.B;
+    j = ((group - b * p.blocks) * LC + lc) * V;
+    ok = any && j < p.H;
   }
 };
 
@@ -232,6 +235,7 @@ __global__ __launch_bounds__(64 * NW) void glr_fwd_kernel(GlrParams p) {
   constexpr int NG = 64 / LC, kTile = NG * NW * U;
   __shared__ Map lds[2][NW > 1 ? NW : 1][LC * V];
   const Place<V, LC, NW> at(p);
+  if (!at.any) return;  // uniform
   const int tbeg = blockIdx.y * p.seg, tend = min(p.T, tbeg + p.seg);
   float carry[V];
   segment_carry<V, RESET>(p, p.h0, p.sh0_b, at.b, at.j, at.ok, carry);
@@ -311,6 +315,7 @@ __global__ __launch_bounds__(64 * NW) void glr_bwd_kernel(GlrParams p) {
   constexpr int NG = 64 / LC, kTile = NG * NW * U;
   __shared__ Map lds[2][NW > 1 ? NW : 1][LC * V];
   const Place<V, LC, NW> at(p);
+  if (!at.any) return;  // uniform
   const int tbeg = blockIdx.y * p.seg, tend = min(p.T, tbeg + p.seg);  // in tau
   float carry[V];
   segment_carry<V, RESET>(p, p.dh_last, p.H, at.b, at.j, at.ok, carry);
@@ -422,6 +427,7 @@ __global__ __launch_bounds__(64 * NW) void glr_segment_kernel(GlrParams p) {
   constexpr int NG = 64 / LC;
   __shared__ Map lds[NW][LC * V];
   const Place<V, LC, NW> at(p);
+  if (!at.any) return;  // uniform
   const int tbeg = blockIdx.y * p.seg, share = p.seg / (NG * NW);  // a multiple of U
   const int first = tbeg + (at.wave * NG + at.lg) * share;         // every step < T: not the last segment
   const T* gi = static_cast<const T*>(p.gi) + at.b * p.sg_b;
@@ -675,7 +681,7 @@ int launch(const char* who, int dtype, const Plan& plan, GlrParams& p, bool back
   p.agg = static_cast<f2v*>(scratch);
   p.blocks = plan.blocks;
   p.seg = plan.seg;
-  const int64_t groups = (int64_t)p.B * plan.blocks;
+  const int64_t groups = ((int64_t)p.B * plan.blocks + 7) / 8 * 8;
   if (groups * (plan.narrow ? 512 : 64) > UINT32_MAX)
     return set_error(GS_ERR_INVALID, "%s: too many channels (B=%d, H=%d)", who, p.B, p.H);
   const dim3 threads(plan.narrow ? 512 : 64);
