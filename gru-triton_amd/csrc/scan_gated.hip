@@ -39,11 +39,13 @@ struct GlrParams {
   const float* dh_last;
   void* dgi;
   float* dh0;
-  f2v* agg;            // [segments - 1][B][H] maps of whole segments, or NULL
+  uint64_t* maps;      // chained layout only: see Chain
+  uint32_t* states;
+  uint32_t* tickets;
   int64_t sg_t, sg_b, sh0_b, sr_t, sr_b, so_t, so_b, sd_t, sd_b, sdg_t, sdg_b;
   int T, B, H;
   int blocks;          // channel blocks per batch row
-  int seg;             // steps per segment (a multiple of the tile)
+  int tiles;           // chained layout: tiles of the time axis
 };
 
 // The map h -> a h + b. A reset is a = -0 (a is never negative otherwise; a NaN
@@ -134,28 +136,126 @@ template <int V, int LC, int NW>
 struct Place {
   static constexpr int NG = 64 / LC;
   int b, j, lc, lg, wave;
+  int tile;      // chained layout: the workgroup's tile of the time axis
   bool ok, any;  // the lane's channels exist; the workgroup's do
-  __device__ __forceinline__ Place(const GlrParams& p) {
-    const int lane = threadIdx.x & 63;
-    wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-    lc = lane % LC;
-    lg = lane / LC;
-    // neighbours in a row, which share cache lines, on one XCD (workgroup mod 8)
-    const int per = gridDim.x >> 3, group = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  __device__ __forceinline__ void at_group(const GlrParams& p, int group) {
     b = group / p.blocks;
     any = b < p.B;
     j = ((group - b * p.blocks) * LC + lc) * V;
     ok = any && j < p.H;
   }
+  // CHAIN: workgroups of one XCD (workgroup mod 8) draw their places in order, all its
+  // channel blocks of a tile before those of the next, so that whatever a workgroup waits
+  // for belongs to one that has started before it.
+  template <bool CHAIN>
+  __device__ __forceinline__ void init(const GlrParams& p, int* shared) {
+    const int lane = threadIdx.x & 63;
+    wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+    lc = lane % LC;
+    lg = lane / LC;
+    tile = 0;
+    // neighbours in a row, which share cache lines, on one XCD
+    const int xcd = blockIdx.x & 7;
+    if constexpr (CHAIN) {
+      if (threadIdx.x == 0)
+        *shared = (int)__hip_atomic_fetch_add(p.tickets + 32 * xcd, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      const int ticket = __builtin_amdgcn_readfirstlane(*shared + 1);  // the counters start at -1
+      const int per = gridDim.x / p.tiles >> 3;
+      tile = ticket / per;
+      at_group(p, xcd * per + ticket - tile * per);
+    } else {
+      at_group(p, xcd * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3));
+    }
+  }
 };
+
+// Chained layout, for few channels and a long axis: a workgroup takes one tile, and the
+// state with which it starts comes from the workgroups before it in time. Each publishes
+// its tile's map as soon as it has it; every 16th publishes the state after its tile.
+// A tile's carry is then the last such state taken through at most 15 maps in order, so
+// that results do not depend on timing, and the chain of waits along the axis has one
+// link in 16 tiles. Words are published with one 64-bit (map) or 32-bit (state) store and
+// are all ones before that; NaNs are stored in one form, which is not all ones.
+constexpr int kLink = 16;
+constexpr uint32_t kNaN = 0x7fc00000u, kNone32 = 0xffffffffu;
+constexpr uint64_t kNone64 = ~uint64_t(0);
+constexpr int kMostPolls = 1 << 22;  // seconds; then NaN, so that a launch ends whatever happens
+
+__device__ __forceinline__ uint32_t word_of(float x) { return x != x ? kNaN : __float_as_uint(x); }
+
+// wave 0 of a workgroup: the carry of its tile, from the map `m` of the tile (every lane of
+// a channel holds it). Lane group g of a channel gathers maps 4 g .. 4 g + 3.
+template <int V, int LC, int NW, bool RESET>
+__device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>& at, const float* first, int64_t ld,
+                                      const Map (&m)[V], float (&carry)[V], float (&last)[V]) {
+  static_assert(64 / LC == 4, "four lane groups share the maps");
+  const int64_t row = (int64_t)p.blocks * LC * V, plane = (int64_t)p.B * row;
+  const int s = at.tile, from = s & ~(kLink - 1), count = s - from;
+  const int64_t c0 = (int64_t)at.b * row + (int64_t)at.j;
+  const bool link = count == kLink - 1;
+  if (at.lg == 0 && !link && s + 1 < p.tiles) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      __hip_atomic_store(p.maps + s * plane + c0 + v, (uint64_t)word_of(m[v].a) | (uint64_t)word_of(m[v].b) << 32,
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  uint64_t w[4][V];
+  uint32_t h[V];
+  const uint64_t* src = p.maps + (from + 4 * at.lg) * plane + c0;
+  const uint32_t* state = p.states + (s / kLink) * plane + c0;
+  const int mine = min(4, count - 4 * at.lg);  // maps of this lane group
+  for (int polls = 0;; ++polls) {
+    bool ready = true;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      h[v] = from ? __hip_atomic_load(state + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k][v] = k < mine ? __hip_atomic_load(src + k * plane + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      ready = ready && h[v] != kNone32;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ready = ready && w[k][v] != kNone64;
+    }
+    if (__builtin_amdgcn_ballot_w64(!ready) == 0 || polls == kMostPolls) break;
+    __builtin_amdgcn_s_sleep(1);
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    Map f{1.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (w[k][v] == kNone64) w[k][v] = (uint64_t)kNaN << 32 | kNaN;
+      const Map x{__uint_as_float((uint32_t)w[k][v]), __uint_as_float((uint32_t)(w[k][v] >> 32))};
+      if (k < mine) f = then<RESET>(f, x);
+    }
+    float c;
+    if (from)
+      c = __uint_as_float(h[v] == kNone32 ? kNaN : h[v]);
+    else
+      c = first != nullptr && at.ok ? first[(int64_t)at.b * ld + at.j + v] : 0.0f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) c = apply<RESET>(Map{__shfl(f.a, g * LC + at.lc), __shfl(f.b, g * LC + at.lc)}, c);
+    carry[v] = c;
+    last[v] = apply<RESET>(m[v], c);
+    if (link && s + 1 < p.tiles && at.lg == 0)
+      __hip_atomic_store(p.states + (s / kLink + 1) * plane + c0 + v, word_of(last[v]), __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+  }
+}
 
 // The maps before a lane's own steps: given each lane's map of its U steps,
 // returns the state at the lane's first step and advances `carry` past the tile.
 // `lds` is one of two buffers used in turn: a wave writes a buffer again only
 // after a barrier that every wave reaches when it has read it.
-template <int V, int LC, int NW, bool RESET>
-__device__ __forceinline__ void enter(const Place<V, LC, NW>& at, Map (&m)[V], float (&carry)[V], float (&h)[V],
-                                      Map (*lds)[LC * V]) {
+// CHAIN: the carry comes from the workgroups of the tiles before (`first`, rows of ld: the
+// state with which the axis starts); `carry` is left as the state after the tile in wave 0.
+template <int V, int LC, int NW, bool RESET, bool CHAIN>
+__device__ __forceinline__ void enter(const GlrParams& p, const Place<V, LC, NW>& at, Map (&m)[V], float (&carry)[V],
+                                      float (&h)[V], Map (*lds)[LC * V], const float* first, int64_t ld) {
   constexpr int NG = 64 / LC;
   Map before[V];
   if constexpr (NG > 1) {
@@ -184,61 +284,74 @@ __device__ __forceinline__ void enter(const Place<V, LC, NW>& at, Map (&m)[V], f
       for (int v = 0; v < V; ++v) lds[at.wave][at.lc * V + v] = m[v];
     }
     lds_barrier();
+    float start[V];
+    if constexpr (CHAIN) {
+      if (at.wave == 0) {
+        Map whole[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          whole[v] = lds[0][at.lc * V + v];
+#pragma unroll
+          for (int w = 1; w < NW; ++w) whole[v] = then<RESET>(whole[v], lds[w][at.lc * V + v]);
+        }
+        chain<V, LC, NW, RESET>(p, at, first, ld, whole, start, carry);
+        if (at.lg == 0) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) lds[NW][at.lc * V + v].b = start[v];
+        }
+      }
+      lds_barrier();
+#pragma unroll
+      for (int v = 0; v < V; ++v) start[v] = lds[NW][at.lc * V + v].b;
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) start[v] = carry[v];
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float c = carry[v], mine = c;
+      float c = start[v], mine = c;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         if (w == at.wave) mine = c;
         c = apply<RESET>(lds[w][at.lc * V + v], c);
       }
-      carry[v] = c;
+      if constexpr (!CHAIN) carry[v] = c;
       h[v] = NG > 1 ? apply<RESET>(before[v], mine) : mine;
     }
   }
 }
 
-// The state with which a segment starts: the first one's, taken through the maps
-// of the segments before it.
-template <int V, bool RESET>
-__device__ __forceinline__ void segment_carry(const GlrParams& p, const float* first, int64_t ld, int b, int j, bool ok,
-                                              float (&carry)[V]) {
+template <int V>
+__device__ __forceinline__ void first_carry(const float* first, int64_t ld, int b, int j, bool ok, float (&carry)[V]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float c = first != nullptr && ok ? first[(int64_t)b * ld + j + v] : 0.0f;
-    const f2v* a = p.agg + (int64_t)b * p.H + j + v;
-    for (int s = 0; s < (int)blockIdx.y; ++s) {
-      const f2v x = ok ? a[(int64_t)s * p.B * p.H] : f2v{1.0f, 0.0f};
-      c = apply<RESET>(Map{x[0], x[1]}, c);
-    }
-    carry[v] = c;
-  }
+  for (int v = 0; v < V; ++v) carry[v] = first != nullptr && ok ? first[(int64_t)b * ld + j + v] : 0.0f;
 }
 
 // Loads of U steps. Step i of a lane is t0 + lg U + i forwards, and t0 - lg U - i
 // backwards (BACK); rem is how many of its steps exist. Offsets are the lane's
 // part only (its channel and its group's distance from the wave's base); the
 // base moves with i and the wave, in scalar registers.
-template <typename T, int V, int U, bool BACK, bool FULL>
+template <typename T, int V, int U, bool BACK>
 __device__ __forceinline__ void load_steps(const void* base, int64_t st, uint32_t off, int rem,
                                            typename Pack<T, V>::Raw (&x)[U]) {
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const T* q = static_cast<const T*>(base) + (BACK ? -i : i) * st;
-    x[i] = Pack<T, V>::load(q, FULL || i < rem ? off : kOffNone);
+    x[i] = Pack<T, V>::load(q, i < rem ? off : kOffNone);
   }
 }
 
-template <typename T, int V, int LC, int NW, int U, bool TANH, bool RESET>
+template <typename T, int V, int LC, int NW, int U, bool TANH, bool RESET, bool CHAIN>
 __global__ __launch_bounds__(64 * NW) void glr_fwd_kernel(GlrParams p) {
   typedef Pack<T, V> P;
   constexpr int NG = 64 / LC, kTile = NG * NW * U;
-  __shared__ Map lds[2][NW > 1 ? NW : 1][LC * V];
-  const Place<V, LC, NW> at(p);
+  __shared__ Map lds[CHAIN ? 1 : 2][NW > 1 ? NW + CHAIN : 1][LC * V];
+  __shared__ int ticket;
+  Place<V, LC, NW> at;
+  at.template init<CHAIN>(p, &ticket);
   if (!at.any) return;  // uniform
-  const int tbeg = blockIdx.y * p.seg, tend = min(p.T, tbeg + p.seg);
   float carry[V];
-  segment_carry<V, RESET>(p, p.h0, p.sh0_b, at.b, at.j, at.ok, carry);
+  if constexpr (!CHAIN) first_carry<V>(p.h0, p.sh0_b, at.b, at.j, at.ok, carry);
 
   const T* gi = static_cast<const T*>(p.gi) + at.b * p.sg_b;
   T* out = static_cast<T*>(p.out) + at.b * p.so_b;
@@ -254,9 +367,9 @@ __global__ __launch_bounds__(64 * NW) void glr_fwd_kernel(GlrParams p) {
   auto load = [&](int t0, Set& s) __attribute__((always_inline)) {
     const int tw = t0 + at.wave * NG * U;  // the wave's first step
     const T* g = gi + tw * p.sg_t;
-    const int rem = tend - tw - at.lg * U;
-    load_steps<T, V, U, false, false>(g, p.sg_t, off_z, rem, s.z);
-    load_steps<T, V, U, false, false>(g, p.sg_t, off_n, rem, s.n);
+    const int rem = p.T - tw - at.lg * U;
+    load_steps<T, V, U, false>(g, p.sg_t, off_z, rem, s.z);
+    load_steps<T, V, U, false>(g, p.sg_t, off_n, rem, s.n);
     if constexpr (RESET) {
 #pragma unroll
       for (int i = 0; i < U; ++i) s.r[i] = i < rem ? rs[(tw + at.lg * U + i) * p.sr_t] : 0u;
@@ -264,7 +377,7 @@ __global__ __launch_bounds__(64 * NW) void glr_fwd_kernel(GlrParams p) {
   };
   auto tile = [&](int t0, const Set& s, Map (*buf)[LC * V]) __attribute__((always_inline)) {
     const int tw = t0 + at.wave * NG * U;
-    const int rem = tend - tw - at.lg * U;
+    const int rem = p.T - tw - at.lg * U;
     Map m[V], e[U][V];
 #pragma unroll
     for (int v = 0; v < V; ++v) m[v] = Map{1.0f, 0.0f};
@@ -284,7 +397,7 @@ __global__ __launch_bounds__(64 * NW) void glr_fwd_kernel(GlrParams p) {
       }
     }
     float h[V];
-    enter<V, LC, NW, RESET>(at, m, carry, h, buf);
+    enter<V, LC, NW, RESET, CHAIN>(p, at, m, carry, h, buf, p.h0, p.sh0_b);
     T* o = out + tw * p.so_t;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -293,32 +406,39 @@ __global__ __launch_bounds__(64 * NW) void glr_fwd_kernel(GlrParams p) {
       P::store(o + i * p.so_t, i < rem ? off_o : kOffNone, h);
     }
   };
-  Set s0, s1;
-  load(tbeg, s0);
-  for (int t0 = tbeg; t0 < tend; t0 += 2 * kTile) {  // tend - tbeg >= 1
-    load(t0 + kTile, s1);
-    tile(t0, s0, lds[0]);
-    if (t0 + kTile >= tend) break;
-    load(t0 + 2 * kTile, s0);
-    tile(t0 + kTile, s1, lds[1]);
+  Set s0;
+  if constexpr (CHAIN) {
+    load(at.tile * kTile, s0);
+    tile(at.tile * kTile, s0, lds[0]);
+  } else {
+    Set s1;
+    load(0, s0);
+    for (int t0 = 0; t0 < p.T; t0 += 2 * kTile) {
+      load(t0 + kTile, s1);
+      tile(t0, s0, lds[0]);
+      if (t0 + kTile >= p.T) break;
+      load(t0 + 2 * kTile, s0);
+      tile(t0 + kTile, s1, lds[1]);
+    }
   }
-  if (p.h_last != nullptr && tend == p.T && at.ok && at.lg == 0 && at.wave == 0) {
+  if (p.h_last != nullptr && (!CHAIN || at.tile == p.tiles - 1) && at.ok && at.lg == 0 && at.wave == 0) {
 #pragma unroll
     for (int v = 0; v < V; ++v) p.h_last[(int64_t)at.b * p.H + at.j + v] = carry[v];
   }
 }
 
 // The same walk from the last step to the first: tau = T - 1 - t counts up.
-template <typename T, int V, int LC, int NW, int U, bool TANH, bool RESET>
+template <typename T, int V, int LC, int NW, int U, bool TANH, bool RESET, bool CHAIN>
 __global__ __launch_bounds__(64 * NW) void glr_bwd_kernel(GlrParams p) {
   typedef Pack<T, V> P;
   constexpr int NG = 64 / LC, kTile = NG * NW * U;
-  __shared__ Map lds[2][NW > 1 ? NW : 1][LC * V];
-  const Place<V, LC, NW> at(p);
+  __shared__ Map lds[CHAIN ? 1 : 2][NW > 1 ? NW + CHAIN : 1][LC * V];
+  __shared__ int ticket;
+  Place<V, LC, NW> at;
+  at.template init<CHAIN>(p, &ticket);
   if (!at.any) return;  // uniform
-  const int tbeg = blockIdx.y * p.seg, tend = min(p.T, tbeg + p.seg);  // in tau
   float carry[V];
-  segment_carry<V, RESET>(p, p.dh_last, p.H, at.b, at.j, at.ok, carry);
+  if constexpr (!CHAIN) first_carry<V>(p.dh_last, p.H, at.b, at.j, at.ok, carry);
 
   const T* gi = static_cast<const T*>(p.gi) + at.b * p.sg_b;
   const T* out = static_cast<const T*>(p.out) + at.b * p.so_b;
@@ -339,12 +459,12 @@ __global__ __launch_bounds__(64 * NW) void glr_bwd_kernel(GlrParams p) {
   auto load = [&](int t0, Set& s) __attribute__((always_inline)) {
     const int tw = t0 + at.wave * NG * U;  // the wave's first tau
     const int64_t t = p.T - 1 - tw - (NG - 1) * U;
-    const int rem = tend - tw - at.lg * U;
+    const int rem = p.T - tw - at.lg * U;
     const int before = p.T - 1 - tw - at.lg * U;  // steps before the lane's first: step i has h_{t-1} in `out` if i < before
-    load_steps<T, V, U, true, false>(gi + t * p.sg_t, p.sg_t, off_z, rem, s.z);
-    load_steps<T, V, U, true, false>(gi + t * p.sg_t, p.sg_t, off_n, rem, s.n);
-    load_steps<T, V, U, true, false>(dout + t * p.sd_t, p.sd_t, off_d, rem, s.d);
-    load_steps<T, V, U, true, false>(out + (t - 1) * p.so_t, p.so_t, off_o, min(rem, before), s.h);
+    load_steps<T, V, U, true>(gi + t * p.sg_t, p.sg_t, off_z, rem, s.z);
+    load_steps<T, V, U, true>(gi + t * p.sg_t, p.sg_t, off_n, rem, s.n);
+    load_steps<T, V, U, true>(dout + t * p.sd_t, p.sd_t, off_d, rem, s.d);
+    load_steps<T, V, U, true>(out + (t - 1) * p.so_t, p.so_t, off_o, min(rem, before), s.h);
     if constexpr (RESET) {
 #pragma unroll
       for (int i = 0; i < U; ++i) s.r[i] = i < rem ? rs[(int64_t)(before - i) * p.sr_t] : 0u;
@@ -352,7 +472,7 @@ __global__ __launch_bounds__(64 * NW) void glr_bwd_kernel(GlrParams p) {
   };
   auto tile = [&](int t0, const Set& s, Map (*buf)[LC * V]) __attribute__((always_inline)) {
     const int tw = t0 + at.wave * NG * U;
-    const int rem = tend - tw - at.lg * U;
+    const int rem = p.T - tw - at.lg * U;
     const int before = p.T - 1 - tw - at.lg * U;
     Map m[V];
     float z[U][V], n[U][V], d[U][V], hp[U][V];
@@ -384,7 +504,7 @@ __global__ __launch_bounds__(64 * NW) void glr_bwd_kernel(GlrParams p) {
         }
     }
     float E[V];
-    enter<V, LC, NW, RESET>(at, m, carry, E, buf);
+    enter<V, LC, NW, RESET, CHAIN>(p, at, m, carry, E, buf, p.dh_last, p.H);
     const int64_t t = p.T - 1 - tw - (NG - 1) * U;
     T* o = dgi + t * p.sdg_t;
 #pragma unroll
@@ -403,114 +523,31 @@ __global__ __launch_bounds__(64 * NW) void glr_bwd_kernel(GlrParams p) {
       P::store(o - i * p.sdg_t, i < rem ? off_dn : kOffNone, dn);
     }
   };
-  Set s0, s1;
-  load(tbeg, s0);
-  for (int t0 = tbeg; t0 < tend; t0 += 2 * kTile) {
-    load(t0 + kTile, s1);
-    tile(t0, s0, lds[0]);
-    if (t0 + kTile >= tend) break;
-    load(t0 + 2 * kTile, s0);
-    tile(t0 + kTile, s1, lds[1]);
+  Set s0;
+  if constexpr (CHAIN) {
+    load(at.tile * kTile, s0);
+    tile(at.tile * kTile, s0, lds[0]);
+  } else {
+    Set s1;
+    load(0, s0);
+    for (int t0 = 0; t0 < p.T; t0 += 2 * kTile) {
+      load(t0 + kTile, s1);
+      tile(t0, s0, lds[0]);
+      if (t0 + kTile >= p.T) break;
+      load(t0 + 2 * kTile, s0);
+      tile(t0 + kTile, s1, lds[1]);
+    }
   }
-  if (p.dh0 != nullptr && tend == p.T && at.ok && at.lg == 0 && at.wave == 0) {
+  if (p.dh0 != nullptr && (!CHAIN || at.tile == p.tiles - 1) && at.ok && at.lg == 0 && at.wave == 0) {
 #pragma unroll
     for (int v = 0; v < V; ++v) p.dh0[(int64_t)at.b * p.H + at.j + v] = carry[v];
   }
 }
 
-// The map of a whole segment, for axes so long that they are walked in several
-// segments at once: each step group folds its own share of the segment's steps,
-// then the shares are joined in order. The last segment's map is not needed.
-template <typename T, int V, int LC, int NW, int U, bool TANH, bool RESET, bool BACK>
-__global__ __launch_bounds__(64 * NW) void glr_segment_kernel(GlrParams p) {
-  typedef Pack<T, V> P;
-  constexpr int NG = 64 / LC;
-  __shared__ Map lds[NW][LC * V];
-  const Place<V, LC, NW> at(p);
-  if (!at.any) return;  // uniform
-  const int tbeg = blockIdx.y * p.seg, share = p.seg / (NG * NW);  // a multiple of U
-  const int first = tbeg + (at.wave * NG + at.lg) * share;         // every step < T: not the last segment
-  const T* gi = static_cast<const T*>(p.gi) + at.b * p.sg_b;
-  const T* dout = BACK ? static_cast<const T*>(p.dout) + at.b * p.sd_b : nullptr;
-  const uint8_t* rs = RESET ? p.reset + at.b * p.sr_b : nullptr;
-  const int groups = NG - 1 - at.lg;
-  // uniform base: the wave's first group forwards, its last one backwards
-  const int wave0 = tbeg + at.wave * NG * share;
-  const int64_t t0 = BACK ? (int64_t)p.T - 1 - wave0 - (NG - 1) * (int64_t)share : wave0;
-  const int64_t lane_t = (BACK ? groups : at.lg) * (int64_t)share;
-  const uint32_t off_z = at.ok ? (uint32_t)((lane_t * p.sg_t + at.j) * sizeof(T)) : kOffNone;
-  const uint32_t off_n = at.ok ? off_z + (uint32_t)(p.H * sizeof(T)) : kOffNone;
-  const uint32_t off_d = BACK && at.ok ? (uint32_t)((lane_t * p.sd_t + at.j) * sizeof(T)) : kOffNone;
-  struct Set {
-    typename P::Raw z[U], x[U];
-    unsigned int r[U];
-  };
-  auto load = [&](int i0, Set& s) __attribute__((always_inline)) {
-    const int rem = share - i0;
-    const int64_t t = BACK ? t0 - i0 : t0 + i0;
-    load_steps<T, V, U, BACK, false>(gi + t * p.sg_t, p.sg_t, off_z, rem, s.z);
-    if constexpr (BACK)
-      load_steps<T, V, U, BACK, false>(dout + t * p.sd_t, p.sd_t, off_d, rem, s.x);
-    else
-      load_steps<T, V, U, BACK, false>(gi + t * p.sg_t, p.sg_t, off_n, rem, s.x);
-    if constexpr (RESET) {
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int64_t step = BACK ? (int64_t)p.T - 1 - first - i0 - i : (int64_t)first + i0 + i;
-        s.r[i] = i < rem ? rs[step * p.sr_t] : 0u;
-      }
-    }
-  };
-  Map m[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) m[v] = Map{1.0f, 0.0f};
-  auto fold = [&](const Set& s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      float gz[V], x[V];
-      P::unpack(s.z[i], gz);
-      P::unpack(s.x[i], x);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float z, n;
-        gates<TANH && !BACK>(gz[v], x[v], z, n);
-        Map e{z, BACK ? z * n : __builtin_fmaf(-z, n, n)};
-        if (RESET && s.r[i]) e = Map{-0.0f, BACK ? 0.0f : e.b};
-        m[v] = then<RESET>(m[v], e);
-      }
-    }
-  };
-  Set s0, s1;
-  load(0, s0);
-  for (int i0 = 0; i0 < share; i0 += 2 * U) {
-    load(i0 + U, s1);
-    fold(s0);
-    if (i0 + U >= share) break;
-    load(i0 + 2 * U, s0);
-    fold(s1);
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-#pragma unroll
-    for (int d = 1; d < NG; d *= 2) {
-      const Map o{__shfl_up(m[v].a, d * LC), __shfl_up(m[v].b, d * LC)};
-      if (at.lg >= d) m[v] = then<RESET>(o, m[v]);
-    }
-  }
-  if (at.lg == NG - 1) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) lds[at.wave][at.lc * V + v] = m[v];
-  }
-  __syncthreads();
-  if (at.wave == 0 && at.lg == 0 && at.ok) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      Map r = lds[0][at.lc * V + v];
-#pragma unroll
-      for (int w = 1; w < NW; ++w) r = then<RESET>(r, lds[w][at.lc * V + v]);
-      p.agg[((int64_t)blockIdx.y * p.B + at.b) * p.H + at.j + v] = f2v{r.a, r.b};
-    }
-  }
+// All ones over the chain's words and counters.
+__global__ __launch_bounds__(256) void glr_fill_kernel(u4v* p, int64_t n) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e < n) p[e] = u4v{kNone32, kNone32, kNone32, kNone32};
 }
 
 // One step for each row of a batch of requests, whose states are rows of a cache.
@@ -544,38 +581,32 @@ __global__ __launch_bounds__(256) void glr_step_kernel(StepParams p) {
 
 // ---- host ---------------------------------------------------------------------------
 
-constexpr int kMaxSegments = 64;
+// The layouts: lanes of channels, waves, and whether tiles are chained. A lane holds
+// kSteps steps of v channels, so a tile is kSteps x 64 / lanes x waves steps.
+constexpr int kSteps = 8;
+struct LayoutOf {
+  int lanes, waves;
+  bool chain;
+};
+constexpr LayoutOf kLayouts[] = {{64, 1, false}, {64, 4, false}, {32, 8, false}, {16, 8, false}, {16, 8, true}};
+constexpr int kChain = 4;
+constexpr int tile_of(int layout) { return kSteps * (64 / kLayouts[layout].lanes) * kLayouts[layout].waves; }
 
-// How a call is laid out. V channels a lane; `narrow`: 16 lanes of channels by 4
-// step groups in 8 waves, tiles of 256 steps; otherwise 64 lanes of channels in
-// one wave, tiles of 8 steps. `segments` walk the axis at once.
 struct Plan {
-  int v;
-  bool narrow;
-  int blocks, segments, seg;
+  int v, layout, blocks, tiles;
 };
 
-constexpr int kNarrowTile = 4 * 8 * 8;
-
-Plan make_plan(int64_t T, int64_t B, int64_t H, int v, bool can_narrow) {
-  Plan r;
-  r.v = v;
-  r.narrow = can_narrow && T > 16 && B * ((H + 64 * v - 1) / (64 * v)) < 4096;
-  const int lanes = r.narrow ? 16 : 64;
+Plan make_plan(int64_t T, int64_t B, int64_t H, int v, bool near) {
+  // step groups side by side that give each CU eight waves
+  const double want = 131072.0 / (double)(B * ((H + v - 1) / v));
+  int l = want <= 1.5 ? 0 : want <= 6 ? 1 : want <= 20 ? 2 : 3;
+  while (l > 0 && tile_of(l) >= 4 * T) --l;
+  if (l == 3 && want > 48 && T >= 4 * tile_of(kChain)) l = kChain;
+  if (!near) l = l > 1 ? 1 : l;
+  Plan r{v, l, 0, 0};
+  const int lanes = kLayouts[l].lanes;
   r.blocks = (int)((H + lanes * v - 1) / (lanes * v));
-  const int64_t groups = B * r.blocks;
-  r.segments = 1;
-  r.seg = (int)T;
-  if (r.narrow) {
-    const int64_t tiles = (T + kNarrowTile - 1) / kNarrowTile;
-    int64_t want = std::min<int64_t>({(512 + groups - 1) / groups, tiles / 2, kMaxSegments});
-    if (groups >= 192) want = 1;
-    if (want > 1) {
-      const int64_t per = (tiles + want - 1) / want;
-      r.seg = (int)(per * kNarrowTile);
-      r.segments = (int)((T + r.seg - 1) / r.seg);
-    }
-  }
+  r.tiles = (int)((T + tile_of(l) - 1) / tile_of(l));
   return r;
 }
 
@@ -607,38 +638,40 @@ int check_rows(const char* who, const char* name, int64_t T, int64_t B, int64_t 
   return GS_OK;
 }
 
-// The largest lane offset of the narrow layout has to stay below 2^31 bytes: three
-// groups of 8 steps apart, or of a share of a segment.
-bool narrow_reach(int64_t st, int64_t groups_apart, int64_t H, int size) {
-  return st < (int64_t(1) << 40) && (3 * groups_apart * st + 2 * H + 64) * size < (int64_t(1) << 31);
+// Where a wave's lanes hold several step groups, a lane's offset from the wave's base has
+// to stay below 2^31 bytes.
+bool lanes_reach(int64_t st, int64_t H, int size) {
+  return st < (int64_t(1) << 40) && (3 * kSteps * st + 2 * H + 64) * size < (int64_t(1) << 31);
 }
 
 typedef void (*GlrFn)(GlrParams);
-template <typename T, int V, bool NARROW>
-struct Kernels {
-  static constexpr int LC = NARROW ? 16 : 64, NW = NARROW ? 8 : 1, U = 8;
-  template <bool TANH, bool RESET>
-  static GlrFn pick(int what) {
-    if (what == 0) return glr_fwd_kernel<T, V, LC, NW, U, TANH, RESET>;
-    if (what == 1) return glr_bwd_kernel<T, V, LC, NW, U, TANH, RESET>;
-    if constexpr (NARROW) {
-      if (what == 2) return glr_segment_kernel<T, V, LC, NW, U, TANH, RESET, false>;
-      if (what == 3) return glr_segment_kernel<T, V, LC, NW, U, false, RESET, true>;
-    }
-    return nullptr;
+template <typename T, int V, int L, bool BACK, bool TANH>
+GlrFn kernel_at(bool reset) {
+  constexpr int LC = kLayouts[L].lanes, NW = kLayouts[L].waves;
+  constexpr bool CHAIN = kLayouts[L].chain;
+  if constexpr (BACK)
+    return reset ? glr_bwd_kernel<T, V, LC, NW, kSteps, TANH, true, CHAIN> : glr_bwd_kernel<T, V, LC, NW, kSteps, TANH, false, CHAIN>;
+  else
+    return reset ? glr_fwd_kernel<T, V, LC, NW, kSteps, TANH, true, CHAIN> : glr_fwd_kernel<T, V, LC, NW, kSteps, TANH, false, CHAIN>;
+}
+template <typename T, int V, bool BACK, bool TANH>
+GlrFn kernel_in(int layout, bool reset) {
+  switch (layout) {
+    case 0: return kernel_at<T, V, 0, BACK, TANH>(reset);
+    case 1: return kernel_at<T, V, 1, BACK, TANH>(reset);
+    case 2: return kernel_at<T, V, 2, BACK, TANH>(reset);
+    case 3: return kernel_at<T, V, 3, BACK, TANH>(reset);
+    default: return kernel_at<T, V, 4, BACK, TANH>(reset);
   }
-  static GlrFn get(int what, bool tanh, bool reset) {
-    return tanh ? (reset ? pick<true, true>(what) : pick<true, false>(what))
-                : (reset ? pick<false, true>(what) : pick<false, false>(what));
-  }
-};
-
-GlrFn kernel_of(int dtype, const Plan& plan, int what, bool tanh, bool reset) {
-  if (dtype == GS_DTYPE_F32)
-    return plan.narrow ? Kernels<float, 1, true>::get(what, tanh, reset) : Kernels<float, 1, false>::get(what, tanh, reset);
-  if (plan.v == 2)
-    return plan.narrow ? Kernels<__bf16, 2, true>::get(what, tanh, reset) : Kernels<__bf16, 2, false>::get(what, tanh, reset);
-  return plan.narrow ? Kernels<__bf16, 1, true>::get(what, tanh, reset) : Kernels<__bf16, 1, false>::get(what, tanh, reset);
+}
+template <typename T, int V>
+GlrFn kernel_for(const Plan& plan, bool back, bool tanh, bool reset) {
+  return back ? (tanh ? kernel_in<T, V, true, true>(plan.layout, reset) : kernel_in<T, V, true, false>(plan.layout, reset))
+              : (tanh ? kernel_in<T, V, false, true>(plan.layout, reset) : kernel_in<T, V, false, false>(plan.layout, reset));
+}
+GlrFn kernel_of(int dtype, const Plan& plan, bool back, bool tanh, bool reset) {
+  if (dtype == GS_DTYPE_F32) return kernel_for<float, 1>(plan, back, tanh, reset);
+  return plan.v == 2 ? kernel_for<__bf16, 2>(plan, back, tanh, reset) : kernel_for<__bf16, 1>(plan, back, tanh, reset);
 }
 
 struct Strided {
@@ -649,50 +682,58 @@ struct Strided {
 Plan plan_of(int dtype, int64_t T, int64_t B, int64_t H, const Strided* t, int count) {
   const int size = dtype == GS_DTYPE_F32 ? 4 : 2;
   int v = dtype == GS_DTYPE_F32 || H % 2 ? 1 : 2;
-  bool narrow = true;
+  bool near = true;
   for (int i = 0; i < count; ++i) {
     if (v == 2 && (!unit_aligned(t[i].p, 4) || t[i].st % 2 || t[i].sb % 2)) v = 1;
-    narrow = narrow && narrow_reach(t[i].st, 8, H, size);
+    near = near && lanes_reach(t[i].st, H, size);
   }
-  Plan plan = make_plan(T, B, H, v, narrow);
-  for (int i = 0; i < count && plan.segments > 1; ++i)
-    if (!narrow_reach(t[i].st, plan.seg / 32, H, size)) {
-      plan.segments = 1;
-      plan.seg = (int)T;
-    }
-  return plan;
+  return make_plan(T, B, H, v, near);
 }
 
-int64_t scratch_of(const Plan& plan, int64_t B, int64_t H) {
-  return plan.segments > 1 ? (int64_t)(plan.segments - 1) * B * H * (int64_t)sizeof(f2v) : 0;
+// The chain's scratch: eight counters on lines of their own, the maps, the states.
+constexpr int64_t kTicketBytes = 8 * 32 * 4;
+struct ChainBytes {
+  int64_t maps = 0, states = 0, total = 0;  // offsets
+};
+ChainBytes chain_bytes(const Plan& plan, int64_t B) {
+  ChainBytes c;
+  if (plan.layout != kChain) return c;
+  const int64_t plane = B * plan.blocks * kLayouts[kChain].lanes * plan.v;
+  c.maps = kTicketBytes;
+  c.states = c.maps + align256(plan.tiles * plane * 8);
+  c.total = c.states + align256((plan.tiles / kLink + 1) * plane * 4);
+  return c;
 }
 
 // What a call of these sizes may need, whatever its pointers and strides.
 int64_t scratch_most(int64_t T, int64_t B, int64_t H) {
-  return std::max(scratch_of(make_plan(T, B, H, 1, true), B, H), scratch_of(make_plan(T, B, H, 2, true), B, H));
+  return std::max(chain_bytes(make_plan(T, B, H, 1, true), B).total, chain_bytes(make_plan(T, B, H, 2, true), B).total);
 }
 
 int launch(const char* who, int dtype, const Plan& plan, GlrParams& p, bool back, bool tanh, void* scratch,
            int64_t scratch_bytes, hipStream_t stream) {
-  const int64_t need = scratch_of(plan, p.B, p.H);
-  if (need > 0 && (scratch == nullptr || scratch_bytes < need || !unit_aligned(scratch, 256)))
+  const ChainBytes c = chain_bytes(plan, p.B);
+  if (c.total > 0 && (scratch == nullptr || scratch_bytes < c.total || !unit_aligned(scratch, 256)))
     return set_error(GS_ERR_INVALID, "%s: scratch of %lld bytes, 256-byte aligned, required; got %lld at %p", who,
-                     (long long)need, (long long)scratch_bytes, scratch);
-  p.agg = static_cast<f2v*>(scratch);
+                     (long long)c.total, (long long)scratch_bytes, scratch);
   p.blocks = plan.blocks;
-  p.seg = plan.seg;
-  const int64_t groups = ((int64_t)p.B * plan.blocks + 7) / 8 * 8;
-  if (groups * (plan.narrow ? 512 : 64) > UINT32_MAX)
-    return set_error(GS_ERR_INVALID, "%s: too many channels (B=%d, H=%d)", who, p.B, p.H);
-  const dim3 threads(plan.narrow ? 512 : 64);
-  const bool reset = p.reset != nullptr;
-  if (plan.segments > 1) {
-    GlrFn fn = kernel_of(dtype, plan, back ? 3 : 2, tanh, reset);
-    hipLaunchKernelGGL(fn, dim3((unsigned)groups, (unsigned)(plan.segments - 1)), threads, 0, stream, p);
+  p.tiles = plan.tiles;
+  const int threads = 64 * kLayouts[plan.layout].waves;
+  int64_t groups = ((int64_t)p.B * plan.blocks + 7) / 8 * 8;
+  if (c.total > 0) {
+    groups *= plan.tiles;
+    p.tickets = static_cast<uint32_t*>(scratch);
+    p.maps = reinterpret_cast<uint64_t*>(static_cast<char*>(scratch) + c.maps);
+    p.states = reinterpret_cast<uint32_t*>(static_cast<char*>(scratch) + c.states);
+    const int64_t n = c.total / 16;
+    hipLaunchKernelGGL(glr_fill_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream,
+                       static_cast<u4v*>(scratch), n);
     GS_CHECK_HIP(hipGetLastError());
   }
-  GlrFn fn = kernel_of(dtype, plan, back ? 1 : 0, tanh, reset);
-  hipLaunchKernelGGL(fn, dim3((unsigned)groups, (unsigned)plan.segments), threads, 0, stream, p);
+  if (groups * threads > UINT32_MAX)
+    return set_error(GS_ERR_INVALID, "%s: too many channels (B=%d, H=%d)", who, p.B, p.H);
+  hipLaunchKernelGGL(kernel_of(dtype, plan, back, tanh, p.reset != nullptr), dim3((unsigned)groups), dim3(threads), 0,
+                     stream, p);
   GS_CHECK_HIP(hipGetLastError());
   return GS_OK;
 }
