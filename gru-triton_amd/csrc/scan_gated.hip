@@ -172,10 +172,10 @@ struct Place {
 
 // Chained layout, for few channels and a long axis: a workgroup takes one tile, and the
 // state with which it starts comes from the workgroups before it in time. Each publishes
-// its tile's map as soon as it has it; every 16th publishes the state after its tile.
-// A tile's carry is then the last such state taken through at most 15 maps in order, so
-// that results do not depend on timing, and the chain of waits along the axis has one
-// link in 16 tiles. Words are published with one 64-bit (map) or 32-bit (state) store and
+// its tile's map as soon as it has it; every kLink-th publishes the state after its tile.
+// A tile's carry is then the last such state taken through the maps since, joined in order
+// before the state is there, so that results do not depend on timing, and the chain of
+// waits along the axis has one link in kLink tiles. Words are published with one 64-bit (map) or 32-bit (state) store and
 // are all ones before that; NaNs are stored in one form, which is not all ones.
 constexpr int kLink = 16;
 constexpr uint32_t kNaN = 0x7fc00000u, kNone32 = 0xffffffffu;
@@ -185,7 +185,7 @@ constexpr int kMostPolls = 1 << 22;  // seconds; then NaN, so that a launch ends
 __device__ __forceinline__ uint32_t word_of(float x) { return x != x ? kNaN : __float_as_uint(x); }
 
 // wave 0 of a workgroup: the carry of its tile, from the map `m` of the tile (every lane of
-// a channel holds it). Lane group g of a channel gathers maps 4 g .. 4 g + 3.
+// a channel holds it). The lane groups of a channel gather a quarter of the maps each.
 template <int V, int LC, int NW, bool RESET>
 __device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>& at, const float* first, int64_t ld,
                                       const Map (&m)[V], float (&carry)[V], float (&last)[V]) {
@@ -200,50 +200,75 @@ __device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>
       __hip_atomic_store(p.maps + s * plane + c0 + v, (uint64_t)word_of(m[v].a) | (uint64_t)word_of(m[v].b) << 32,
                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  uint64_t w[4][V];
+  // the maps of this lane group, four at a time
+  constexpr int kShare = kLink / 4;
+  const uint64_t* src = p.maps + (from + kShare * at.lg) * plane + c0;
+  const int mine = count - kShare * at.lg;
+  Map f[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) f[v] = Map{1.0f, 0.0f};
+  int polls = 0;
+  for (int k0 = 0; k0 < kShare && k0 < count; k0 += 4) {
+    uint64_t w[4][V];
+    for (;; ++polls) {
+      bool ready = true;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          w[k][v] = 0u;
+          if (k0 + k < mine)
+            w[k][v] = __hip_atomic_load(src + (k0 + k) * plane + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          ready = ready && w[k][v] != kNone64;
+        }
+      if (__builtin_amdgcn_ballot_w64(!ready) == 0 || polls >= kMostPolls) break;
+      __builtin_amdgcn_s_sleep(1);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (w[k][v] == kNone64) w[k][v] = (uint64_t)kNaN << 32 | kNaN;
+        const Map x{__uint_as_float((uint32_t)w[k][v]), __uint_as_float((uint32_t)(w[k][v] >> 32))};
+        if (k0 + k < mine) f[v] = then<RESET>(f[v], x);
+      }
+  }
+  // all of them in order, and this tile's: what is left once the state is there is one step
+  Map all[V], past[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    all[v] = Map{__shfl(f[v].a, at.lc), __shfl(f[v].b, at.lc)};
+#pragma unroll
+    for (int g = 1; g < 4; ++g) all[v] = then<RESET>(all[v], Map{__shfl(f[v].a, g * LC + at.lc), __shfl(f[v].b, g * LC + at.lc)});
+    past[v] = then<RESET>(all[v], m[v]);
+  }
   uint32_t h[V];
-  const uint64_t* src = p.maps + (from + 4 * at.lg) * plane + c0;
-  const uint32_t* state = p.states + (s / kLink) * plane + c0;
-  const int mine = min(4, count - 4 * at.lg);  // maps of this lane group
-  for (int polls = 0;; ++polls) {
-    bool ready = true;
+  if (from) {
+    const uint32_t* state = p.states + (s / kLink) * plane + c0;
+    for (;; ++polls) {
+      bool ready = true;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        h[v] = __hip_atomic_load(state + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        ready = ready && h[v] != kNone32;
+      }
+      if (__builtin_amdgcn_ballot_w64(!ready) == 0 || polls >= kMostPolls) break;
+    }
+  } else {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      h[v] = from ? __hip_atomic_load(state + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        w[k][v] = k < mine ? __hip_atomic_load(src + k * plane + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
+      const float c = first != nullptr && at.ok ? first[(int64_t)at.b * ld + at.j + v] : 0.0f;
+      h[v] = word_of(c);
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      ready = ready && h[v] != kNone32;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) ready = ready && w[k][v] != kNone64;
-    }
-    if (__builtin_amdgcn_ballot_w64(!ready) == 0 || polls == kMostPolls) break;
-    __builtin_amdgcn_s_sleep(1);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    Map f{1.0f, 0.0f};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (w[k][v] == kNone64) w[k][v] = (uint64_t)kNaN << 32 | kNaN;
-      const Map x{__uint_as_float((uint32_t)w[k][v]), __uint_as_float((uint32_t)(w[k][v] >> 32))};
-      if (k < mine) f = then<RESET>(f, x);
-    }
-    float c;
-    if (from)
-      c = __uint_as_float(h[v] == kNone32 ? kNaN : h[v]);
-    else
-      c = first != nullptr && at.ok ? first[(int64_t)at.b * ld + at.j + v] : 0.0f;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) c = apply<RESET>(Map{__shfl(f.a, g * LC + at.lc), __shfl(f.b, g * LC + at.lc)}, c);
-    carry[v] = c;
-    last[v] = apply<RESET>(m[v], c);
+    const float c = __uint_as_float(h[v] == kNone32 ? kNaN : h[v]);
+    last[v] = apply<RESET>(past[v], c);
     if (link && s + 1 < p.tiles && at.lg == 0)
       __hip_atomic_store(p.states + (s / kLink + 1) * plane + c0 + v, word_of(last[v]), __ATOMIC_RELAXED,
                          __HIP_MEMORY_SCOPE_AGENT);
+    carry[v] = apply<RESET>(all[v], c);
   }
 }
 
@@ -341,8 +366,12 @@ __device__ __forceinline__ void load_steps(const void* base, int64_t st, uint32_
   }
 }
 
+__device__ __forceinline__ unsigned int load_flag(const uint8_t* base, uint32_t off) {
+  return (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(bounded_rsrc(base, 0x7fffffffu), (int)off, 0, 0);
+}
+
 template <typename T, int V, int LC, int NW, int U, bool TANH, bool RESET, bool CHAIN>
-__global__ __launch_bounds__(64 * NW) void glr_fwd_kernel(GlrParams p) {
+__global__ __launch_bounds__(64 * NW, CHAIN ? 6 : 1) void glr_fwd_kernel(GlrParams p) {
   typedef Pack<T, V> P;
   constexpr int NG = 64 / LC, kTile = NG * NW * U;
   __shared__ Map lds[CHAIN ? 1 : 2][NW > 1 ? NW + CHAIN : 1][LC * V];
@@ -360,6 +389,7 @@ __global__ __launch_bounds__(64 * NW) void glr_fwd_kernel(GlrParams p) {
   const uint32_t off_z = at.ok ? lane_g : kOffNone;
   const uint32_t off_n = at.ok ? lane_g + (uint32_t)(p.H * sizeof(T)) : kOffNone;
   const uint32_t off_o = at.ok ? (uint32_t)((at.lg * U * p.so_t + at.j) * sizeof(T)) : kOffNone;
+  const uint32_t off_r = (uint32_t)(at.lg * U * p.sr_t);
   struct Set {
     typename P::Raw z[U], n[U];
     unsigned int r[U];
@@ -372,7 +402,7 @@ __global__ __launch_bounds__(64 * NW) void glr_fwd_kernel(GlrParams p) {
     load_steps<T, V, U, false>(g, p.sg_t, off_n, rem, s.n);
     if constexpr (RESET) {
 #pragma unroll
-      for (int i = 0; i < U; ++i) s.r[i] = i < rem ? rs[(tw + at.lg * U + i) * p.sr_t] : 0u;
+      for (int i = 0; i < U; ++i) s.r[i] = load_flag(rs + (tw + i) * p.sr_t, i < rem ? off_r : kOffNone);
     }
   };
   auto tile = [&](int t0, const Set& s, Map (*buf)[LC * V]) __attribute__((always_inline)) {
@@ -451,6 +481,7 @@ __global__ __launch_bounds__(64 * NW) void glr_bwd_kernel(GlrParams p) {
   const uint32_t off_h = (uint32_t)(p.H * sizeof(T));
   const uint32_t off_z = at.ok ? lane_off(p.sg_t) : kOffNone, off_n = at.ok ? off_z + off_h : kOffNone;
   const uint32_t off_o = at.ok ? lane_off(p.so_t) : kOffNone, off_d = at.ok ? lane_off(p.sd_t) : kOffNone;
+  const uint32_t off_r = (uint32_t)(back * p.sr_t);
   const uint32_t off_dz = at.ok ? lane_off(p.sdg_t) : kOffNone, off_dn = at.ok ? off_dz + off_h : kOffNone;
   struct Set {
     typename P::Raw z[U], n[U], h[U], d[U];
@@ -467,7 +498,7 @@ __global__ __launch_bounds__(64 * NW) void glr_bwd_kernel(GlrParams p) {
     load_steps<T, V, U, true>(out + (t - 1) * p.so_t, p.so_t, off_o, min(rem, before), s.h);
     if constexpr (RESET) {
 #pragma unroll
-      for (int i = 0; i < U; ++i) s.r[i] = i < rem ? rs[(int64_t)(before - i) * p.sr_t] : 0u;
+      for (int i = 0; i < U; ++i) s.r[i] = load_flag(rs + (t - i) * p.sr_t, i < rem ? off_r : kOffNone);
     }
   };
   auto tile = [&](int t0, const Set& s, Map (*buf)[LC * V]) __attribute__((always_inline)) {
@@ -601,7 +632,7 @@ Plan make_plan(int64_t T, int64_t B, int64_t H, int v, bool near) {
   const double want = 131072.0 / (double)(B * ((H + v - 1) / v));
   int l = want <= 1.5 ? 0 : want <= 6 ? 1 : want <= 20 ? 2 : 3;
   while (l > 0 && tile_of(l) >= 4 * T) --l;
-  if (l == 3 && want > 48 && T >= 4 * tile_of(kChain)) l = kChain;
+  if (l == 3 && want > 24 && T > 2 * tile_of(kChain)) l = kChain;
   if (!near) l = l > 1 ? 1 : l;
   Plan r{v, l, 0, 0};
   const int lanes = kLayouts[l].lanes;
@@ -679,7 +710,7 @@ struct Strided {
   int64_t st, sb;
 };
 
-Plan plan_of(int dtype, int64_t T, int64_t B, int64_t H, const Strided* t, int count) {
+Plan plan_of(int dtype, int64_t T, int64_t B, int64_t H, const Strided* t, int count, int64_t sr_t) {
   const int size = dtype == GS_DTYPE_F32 ? 4 : 2;
   int v = dtype == GS_DTYPE_F32 || H % 2 ? 1 : 2;
   bool near = true;
@@ -687,7 +718,7 @@ Plan plan_of(int dtype, int64_t T, int64_t B, int64_t H, const Strided* t, int c
     if (v == 2 && (!unit_aligned(t[i].p, 4) || t[i].st % 2 || t[i].sb % 2)) v = 1;
     near = near && lanes_reach(t[i].st, H, size);
   }
-  return make_plan(T, B, H, v, near);
+  return make_plan(T, B, H, v, near && lanes_reach(sr_t, 0, 1));
 }
 
 // The chain's scratch: eight counters on lines of their own, the maps, the states.
@@ -764,13 +795,13 @@ int check_bwd(const gs_glr_bwd_args* a, const char* who) {
 
 Plan plan_fwd(const gs_glr_args* a) {
   const Strided t[2] = {{a->gi, a->sg_t, a->sg_b}, {a->out, a->so_t, a->so_b}};
-  return plan_of(a->dtype, a->T, a->B, a->H, t, 2);
+  return plan_of(a->dtype, a->T, a->B, a->H, t, 2, a->sr_t);
 }
 
 Plan plan_bwd(const gs_glr_bwd_args* a) {
   const Strided t[4] = {{a->gi, a->sg_t, a->sg_b}, {a->out, a->so_t, a->so_b}, {a->dout, a->sd_t, a->sd_b},
                         {a->dgi, a->sdg_t, a->sdg_b}};
-  return plan_of(a->dtype, a->T, a->B, a->H, t, 4);
+  return plan_of(a->dtype, a->T, a->B, a->H, t, 4, a->sr_t);
 }
 
 }  // namespace
