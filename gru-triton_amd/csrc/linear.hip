@@ -349,7 +349,7 @@ using namespace gs;
 extern "C" int64_t gs_linear_scratch_bytes(const gs_linear_args* a) {
   clear_error();
   const int rc = check_fwd(a, "gs_linear_scratch_bytes");
-  return rc ? rc : fwd_plan(a, true).total;
+  return rc ? rc : fwd_plan(a, !a->x || !a->w).total;
 }
 
 extern "C" int gs_linear_fwd(const gs_linear_args* a, hipStream_t stream) {
@@ -410,7 +410,7 @@ extern "C" int gs_linear_fwd(const gs_linear_args* a, hipStream_t stream) {
 extern "C" int64_t gs_linear_bwd_scratch_bytes(const gs_linear_bwd_args* a) {
   clear_error();
   const int rc = check_bwd(a, "gs_linear_bwd_scratch_bytes");
-  return rc ? rc : bwd_plan(a, true).total;
+  return rc ? rc : bwd_plan(a, !a->x || !a->w || !a->dy).total;
 }
 
 extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {

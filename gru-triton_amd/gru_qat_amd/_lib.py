@@ -13,7 +13,7 @@ import os
 import struct
 import threading
 import weakref
-from typing import Callable, Optional, Tuple
+from typing import Any, Callable, Optional, Tuple
 
 import torch
 
@@ -520,6 +520,26 @@ def load() -> ctypes.CDLL:
         return lib
 
 
+_ops: Any = None
+
+
+def ops() -> Any:
+    """The C++ side of the operators that do their checks, allocations and autograd there
+    (csrc/torch_ops.cpp, built next to libgruscan.so). Loaded once, like the library."""
+    global _ops
+    if _ops is None:
+        load()
+        try:
+            from . import _ops as module  # type: ignore[attr-defined]
+        except ImportError as e:
+            raise RuntimeError(f"_ops.so cannot be loaded ({e}); build it with `make -C gru-triton_amd/csrc` or "
+                               "__graft_entry__.build()") from e
+        if module.abi_version() != ABI_VERSION:
+            raise RuntimeError(f"_ops.so ABI version {module.abi_version()} != expected {ABI_VERSION}; rebuild it")
+        _ops = module
+    return _ops
+
+
 _QUANT_OFF = GsQuant(0, 1.0, -(2**31), 2**31 - 1)
 
 
@@ -737,15 +757,6 @@ PROJ_BWD_ARGS = struct.Struct("<8Q7q" "ifii" "2Q" "ifii")
 SPROJ_ARGS = struct.Struct("<i4x8Q9q" "ifii" "ifii" "ifii" "ifii")
 SPROJ_BWD_ARGS = struct.Struct("<i4x10Q10q" "ifii" "ifii" "ifii" "ifii")
 
-# Those of the gated linear recurrence (GsGlrArgs, GsGlrBwdArgs, GsGlrStepArgs) and of the linear operator.
-GLR_ARGS = struct.Struct("<6Q11q2i")
-GLR_BWD_ARGS = struct.Struct("<9Q15q2i")
-GLR_STEP_ARGS = struct.Struct("<4Q6q2i")
-LINEAR_ARGS = struct.Struct("<7Q7q2i")
-LINEAR_BWD_ARGS = struct.Struct("<8Q6q2i")
-# gs_adamw_args; its tensor array (GsAdamwTensor) is packed as 8 words a tensor.
-ADAMW_ARGS = struct.Struct("<Qq5dqQ4i")
-
 
 def raw_size(lib: ctypes.CDLL, fn_name: str, packed: bytes) -> int:
     """What the size query ``fn_name`` says for packed arguments."""
@@ -759,17 +770,6 @@ def raw_size(lib: ctypes.CDLL, fn_name: str, packed: bytes) -> int:
     if n < 0:
         raise_for(n, lib)
     return n
-
-
-def call_on(fn_name: str, packed: bytes, ordinal: int) -> None:
-    """``raw_call`` by device ordinal, short on the host where that device is current (the common case)."""
-    fn = _RAW_FN.get(fn_name)
-    if fn is None or _raw_stream is None or ordinal != torch.cuda.current_device():
-        raw_call(load(), fn_name, packed, torch.device("cuda", ordinal))
-        return
-    rc = fn(packed, _raw_stream(ordinal))
-    if rc:
-        raise_for(rc, load())
 
 
 def raw_call(lib: ctypes.CDLL, fn_name: str, packed: bytes, dev: torch.device) -> None:

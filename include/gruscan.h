@@ -681,6 +681,8 @@ typedef struct gs_linear_args {
   int32_t dtype, activation;
 } gs_linear_args;
 
+/* With x and w set, what a call with these arguments needs; with either NULL, what any
+ * call of these sizes may need. (gs_linear_bwd_scratch_bytes: x, w and dy.) */
 int64_t gs_linear_scratch_bytes(const gs_linear_args* args);
 int gs_linear_fwd(const gs_linear_args* args, hipStream_t stream);
 
