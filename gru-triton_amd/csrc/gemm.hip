@@ -174,11 +174,11 @@ __device__ __forceinline__ void interleave() {
   });
 }
 
-// Q: fake-quantizes A (NT) or B (TN) on its way to LDS.
+// Q: fake-quantizes A (NT) or B (TN) on its way to LDS. EPI: GemmArgs::epi follows.
 // Four workgroups of NT's small tiles fit a CU, which short products, bound by
 // their stores, are the faster for (M = 16384, N = 1536, K = 64: 60 -> 53 us);
 // NN and TN lose more to the registers (their backward 112 -> 116 us).
-template <int LAYOUT, int T, int LOAD, bool Q>
+template <int LAYOUT, int T, int LOAD, bool Q, bool EPI = false>
 __global__ __launch_bounds__(kGemmThreads, T == kBigT || LOAD == kLoadFar                ? 2
                                            : LAYOUT == kGemmNT && LOAD == kLoadVec ? 4
                                                                                    : 3) void gemm_kernel(GemmArgs g) {
@@ -285,7 +285,16 @@ __global__ __launch_bounds__(kGemmThreads, T == kBigT || LOAD == kLoadFar       
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int i = i0 + 16 * (MT * wy + ti) + 4 * kq + v;
-        if (i < g.M) c[(int64_t)i * g.ldc + j] = acc[ti][tj][v] + bias;
+        if constexpr (EPI) {
+          if (i >= g.M) continue;
+          float x[1] = {acc[ti][tj][v] + bias};
+          if (g.epi.pre != nullptr) static_cast<float*>(g.epi.pre)[(int64_t)i * g.N + j] = x[0];
+          act_values(x, g.epi.act);
+          if (g.epi.residual != nullptr) x[0] += static_cast<const float*>(g.epi.residual)[i * g.epi.ldr + j];
+          c[(int64_t)i * g.ldc + j] = x[0];
+        } else {
+          if (i < g.M) c[(int64_t)i * g.ldc + j] = acc[ti][tj][v] + bias;
+        }
       }
   }
 }
@@ -552,6 +561,14 @@ int gemm_f32(const GemmArgs& g, hipStream_t stream, const char* who) {
   if ((g.qa.on || g.qb.on) && (!quant || g.layout == kGemmNN || (g.qa.on && g.qb.on)))
     return set_error(GS_ERR_INVALID, "%s: GEMM layout %d quantizes no such operand", who, g.layout);
   GemmFn fn = table[g.layout][big ? 3 + load : load][quant ? 1 : 0];
+  if (g.has_epi) {
+    if (g.layout != kGemmNT || quant || g.ksplit != 1 || g.batch != 1)
+      return set_error(GS_ERR_INVALID, "%s: an epilogue follows a plain NT product only", who);
+    static const GemmFn with[5] = {gemm_kernel<kGemmNT, kSmallT, kLoadVec, false, true>, gemm_kernel<kGemmNT, kSmallT, kLoadWord, false, true>,
+                                   gemm_kernel<kGemmNT, kSmallT, kLoadFar, false, true>, gemm_kernel<kGemmNT, kBigT, kLoadVec, false, true>,
+                                   gemm_kernel<kGemmNT, kBigT, kLoadWord, false, true>};
+    fn = with[big ? 3 + load : load];
+  }
   int64_t tiles = tile_count(g.M, g.N, big ? kBigT : kSmallT);
   if (big) tiles = 8 * ((tiles + 7) / 8);
   const int64_t gx = std::min<int64_t>(tiles, 1 << 20);  // for big tiles a multiple of 8

@@ -8,6 +8,7 @@
 // loaded.
 #pragma once
 
+#include "gs_act.h"
 #include "gs_host.h"
 
 namespace gs {
@@ -32,6 +33,10 @@ struct GemmArgs {
   // product z still step by split_stride from there).
   int batch = 1, a_mod = 1, b_mod = 1;
   int64_t a_bs = 0, b_bs = 0, c_bs = 0, bias_bs = 0;
+  // NT without quants, splits and batch: `epi` (its bias unused: `bias` above) follows the
+  // sums where `has_epi`.
+  bool has_epi = false;
+  LinearEpilogue epi;
 };
 
 // Launches the product on `stream`. Every element of C (of every split) is written.

@@ -12,7 +12,16 @@ namespace gs {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 128;  // rows of one workgroup of the dpre pass
+
+// Rows of one workgroup of the dpre pass: as many workgroups as fill the device several
+// times over, from 16 rows (a row for each of its lanes) to 128 (M = 2048, N = 1024 in
+// bf16: 13.5 us in 128 workgroups of 128 rows, 5 in 1024 of 16).
+int64_t dpre_rows(int64_t M, int64_t N, bool bf16) {
+  const int64_t across = (N + (bf16 ? 127 : 63)) / (bf16 ? 128 : 64);
+  int64_t rows = 16;
+  while (rows < 128 && (M + rows - 1) / rows * across > 2048) rows *= 2;
+  return rows;
+}
 
 typedef float f2v __attribute__((ext_vector_type(2)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -77,19 +86,19 @@ struct DpreArgs {
   const void* pre;  // NULL: no activation, only the column sums
   const void* dy;
   void* dpre;       // row stride ldp >= N, zeros from column N on; or NULL (column sums only)
-  float* part;      // [ceil(M / kRows)][N], or NULL
+  float* part;      // [ceil(M / rows)][N], or NULL
   int64_t sdy, ldp;
-  int M, N, act;
+  int M, N, act, rows;
 };
 
-// A workgroup takes 16 lanes of columns (16 bytes each) by kRows rows; its 16 row lanes
+// A workgroup takes 16 lanes of columns (16 bytes each) by `rows` rows; its 16 row lanes
 // take every 16th row, four at a time, and their sums are joined through LDS in order.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void dpre_kernel(DpreArgs p) {
   constexpr int V = Wide<T>::V, kAhead = 4;
   __shared__ float red[16][16 * V + 1];
   const int jl = threadIdx.x & 15, rl = threadIdx.x >> 4, j = (blockIdx.x * 16 + jl) * V;
-  const int r0 = blockIdx.y * kRows, r1 = min(p.M, r0 + kRows), have = p.N - j;
+  const int r0 = blockIdx.y * p.rows, r1 = min(p.M, r0 + p.rows), have = p.N - j;
   float sum[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[v] = 0.0f;
@@ -182,36 +191,21 @@ __global__ __launch_bounds__(kThreads) void sum_columns_kernel(T* dst, const flo
   __shared__ float red[16][17];
   const int c = threadIdx.x & 15, l = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
   float s = 0.0f;
-  if (e < n)
-    for (int k = l; k < parts; k += 16) s += src[(int64_t)k * n + e];
+  if (e < n) {
+    for (int k0 = l; k0 < parts; k0 += 16 * 8) {  // eight loads in flight
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = k0 + 16 * u < parts ? src[(int64_t)(k0 + 16 * u) * n + e] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += x[u];
+    }
+  }
   red[l][c] = s;
   __syncthreads();
   if (l == 0 && e < n) {
 #pragma unroll
     for (int k = 1; k < 16; ++k) s += red[k][c];
     dst[e] = (T)s;
-  }
-}
-
-// fp32: what follows the product's sums (with the bias already added), in place in y.
-struct PostArgs {
-  float* y;
-  int64_t ldy;
-  LinearEpilogue e;
-  int64_t n;
-  int N;
-};
-__global__ __launch_bounds__(kThreads) void post_kernel(PostArgs p) {
-  for (int64_t e = blockIdx.x * (int64_t)kThreads + threadIdx.x; e < p.n; e += (int64_t)gridDim.x * kThreads) {
-    const int64_t i = e / p.N;
-    const int j = (int)(e - i * p.N);
-    float x = p.y[i * p.ldy + j];
-    if (p.e.pre != nullptr) static_cast<float*>(p.e.pre)[e] = x;
-    float v[1] = {x};
-    act_values(v, p.e.act);
-    x = v[0];
-    if (p.e.residual != nullptr) x += static_cast<const float*>(p.e.residual)[i * p.e.ldr + j];
-    p.y[i * p.ldy + j] = x;
   }
 }
 
@@ -305,7 +299,7 @@ FwdPlan fwd_plan(const gs_linear_args* a, bool any) {
 // splits' sums of dx and of dw.
 struct BwdPlan {
   int split_x, split_w;
-  int64_t ldp, dpre, cols, x, w, dx, dw, total;
+  int64_t rows, ldp, dpre, cols, x, w, dx, dw, total;
 };
 
 BwdPlan bwd_plan(const gs_linear_bwd_args* a, bool any) {
@@ -319,7 +313,8 @@ BwdPlan bwd_plan(const gs_linear_bwd_args* a, bool any) {
   p.ldp = pays ? up8(a->N) : a->N;
   p.dpre = l.take(products && (a->activation != GS_ACT_NONE || (pays && (any || !granular(a->dy, a->sdy, a->N)))),
                   a->M * p.ldp * size);
-  p.cols = l.take(a->dbias != nullptr, (a->M + kRows - 1) / kRows * a->N * 4);
+  p.rows = dpre_rows(a->M, a->N, bf16);
+  p.cols = l.take(a->dbias != nullptr, (a->M + p.rows - 1) / p.rows * a->N * 4);
   p.x = l.take(pays && a->dw && (any || !granular(a->x, a->sx, a->K)), a->M * up8(a->K) * 2);
   p.w = l.take(pays && a->dx && (any || !granular(a->w, a->K, a->K)), a->N * up8(a->K) * 2);
   p.dx = l.take(a->dx && p.split_x > 1, p.split_x * a->M * a->K * 4);
@@ -398,13 +393,9 @@ extern "C" int gs_linear_fwd(const gs_linear_args* a, hipStream_t stream) {
   g.M = (int)a->M;
   g.N = (int)a->N;
   g.K = (int)a->K;
-  if ((rc = gemm_f32(g, stream, who))) return rc;
-  if (e.act == GS_ACT_NONE && e.residual == nullptr && e.pre == nullptr) return GS_OK;
-  PostArgs p{static_cast<float*>(a->y), a->sy, e, a->M * a->N, (int)a->N};
-  hipLaunchKernelGGL(post_kernel, dim3((unsigned)std::min<int64_t>((p.n + kThreads - 1) / kThreads, 8192)),
-                     dim3(kThreads), 0, stream, p);
-  GS_CHECK_HIP(hipGetLastError());
-  return GS_OK;
+  g.has_epi = e.act != GS_ACT_NONE || e.residual != nullptr || e.pre != nullptr;
+  g.epi = e;
+  return gemm_f32(g, stream, who);
 }
 
 extern "C" int64_t gs_linear_bwd_scratch_bytes(const gs_linear_bwd_args* a) {
@@ -427,22 +418,22 @@ extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {
   char* scratch = static_cast<char*>(a->scratch);
   auto at = [&](int64_t off) -> void* { return off < 0 ? nullptr : scratch + off; };
   const bool bf16 = a->dtype == GS_DTYPE_BF16;
-  const int chunks = (int)((a->M + kRows - 1) / kRows);
+  const int chunks = (int)((a->M + plan.rows - 1) / plan.rows);
   if (plan.dpre >= 0 || plan.cols >= 0) {
     DpreArgs p{act ? a->pre : nullptr, a->dy, at(plan.dpre), static_cast<float*>(at(plan.cols)), a->sdy, plan.ldp,
-               (int)a->M, (int)a->N, a->activation};
+               (int)a->M, (int)a->N, a->activation, (int)plan.rows};
     for (int first = 0; first < chunks; first += 65535) {  // grid.y
       DpreArgs q = p;
-      const int64_t r = (int64_t)first * kRows;
+      const int64_t r = (int64_t)first * plan.rows;
       const int64_t size = bf16 ? 2 : 4;
-      q.M = (int)std::min<int64_t>(a->M - r, 65535ll * kRows);
+      q.M = (int)std::min<int64_t>(a->M - r, 65535 * plan.rows);
       if (q.pre) q.pre = static_cast<const char*>(q.pre) + r * a->N * size;
       q.dy = static_cast<const char*>(q.dy) + r * a->sdy * size;
       if (q.dpre) q.dpre = static_cast<char*>(q.dpre) + r * plan.ldp * size;
       if (q.part) q.part += (int64_t)first * a->N;
       auto fn = bf16 ? dpre_kernel<__bf16> : dpre_kernel<float>;
       const int cols = bf16 ? 128 : 64;
-      hipLaunchKernelGGL(fn, dim3((unsigned)((a->N + cols - 1) / cols), (unsigned)((q.M + kRows - 1) / kRows)), dim3(kThreads),
+      hipLaunchKernelGGL(fn, dim3((unsigned)((a->N + cols - 1) / cols), (unsigned)((q.M + plan.rows - 1) / plan.rows)), dim3(kThreads),
                          0, stream, q);
       GS_CHECK_HIP(hipGetLastError());
     }
