@@ -106,30 +106,41 @@ __global__ __launch_bounds__(kThreads) void dpre_kernel(DpreArgs p) {
     const T* dy = static_cast<const T*>(p.dy) + j;
     const T* pre = static_cast<const T*>(p.pre) + j;
     T* dpre = static_cast<T*>(p.dpre) + j;
-    for (int r = r0 + rl; r < r1; r += 16 * kAhead) {
-      typename Wide<T>::Raw rd[kAhead], rx[kAhead];
+    // INSIDE: whole columns and rows, no load under a mask
+    auto run = [&](auto INSIDE) __attribute__((always_inline)) {
+      constexpr bool in = decltype(INSIDE)::value;
+      for (int r = r0 + rl; r < r1; r += 16 * kAhead) {
+        typename Wide<T>::Raw rd[kAhead], rx[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int q = r + 16 * u;
-        rd[u] = Wide<T>::load(dy + q * p.sdy, q < r1 ? have : 0, j);
-        if (p.pre != nullptr) rx[u] = Wide<T>::load(pre + (int64_t)q * p.N, q < r1 ? have : 0, j);
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int q = r + 16 * u;
-        float d[V], x[V];
-        Wide<T>::values(rd[u], q < r1 ? have : 0, d);
-        if (p.pre != nullptr) {
-          Wide<T>::values(rx[u], q < r1 ? have : 0, x);
-          act_slopes(x, p.act);
-#pragma unroll
-          for (int v = 0; v < V; ++v) d[v] *= x[v];
+        for (int u = 0; u < kAhead; ++u) {
+          const int q = min(r + 16 * u, r1 - 1);  // past the end: a row of its own again, not used
+          const int h = in ? V : have;
+          rd[u] = Wide<T>::load(dy + q * p.sdy, h, in ? 0 : j);
+          if (p.pre != nullptr) rx[u] = Wide<T>::load(pre + (int64_t)q * p.N, h, in ? 0 : j);
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] += d[v];
-        if (p.dpre != nullptr && q < r1) Wide<T>::store(dpre + q * p.ldp, min(V, (int)p.ldp - j), d);
+        for (int u = 0; u < kAhead; ++u) {
+          const int q = r + 16 * u;
+          if (q >= r1) break;
+          const int h = in ? V : have;
+          float d[V], x[V];
+          Wide<T>::values(rd[u], h, d);
+          if (p.pre != nullptr) {
+            Wide<T>::values(rx[u], h, x);
+            act_slopes(x, p.act);
+#pragma unroll
+            for (int v = 0; v < V; ++v) d[v] *= x[v];
+          }
+#pragma unroll
+          for (int v = 0; v < V; ++v) sum[v] += d[v];
+          if (p.dpre != nullptr) Wide<T>::store(dpre + q * p.ldp, in ? V : min(V, (int)p.ldp - j), d);
+        }
       }
-    }
+    };
+    if ((int)(blockIdx.x + 1) * 16 * V <= p.N)  // uniform
+      run(std::true_type{});
+    else
+      run(std::false_type{});
   }
   if (p.part == nullptr) return;
 #pragma unroll
