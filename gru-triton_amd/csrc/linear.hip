@@ -295,7 +295,7 @@ struct FwdPlan {
 // `any`: what any pointers and strides may need.
 FwdPlan fwd_plan(const gs_linear_args* a, bool any) {
   FwdPlan p;
-  if (a->dtype != GS_DTYPE_BF16) return p;
+  if (a->dtype != GS_DTYPE_BF16 || gemm_bf16_few_rows((int)a->M)) return p;
   p.split = gemm_bf16_pick_split((int)a->M, (int)a->N, (int)a->K);
   Layout l;
   const bool pays = 2.0 * a->M * a->N * a->K >= kPadFlops;

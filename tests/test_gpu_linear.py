@@ -95,7 +95,7 @@ def _call(x, w, bias, res, dy, act):
 
 # around the tiles of 64 and 128, slices of 64 k, 16-byte rows and splits of K
 SHAPES = [(1, 1, 1), (1, 5, 3), (3, 17, 8), (8, 64, 64), (16, 130, 33), (65, 64, 65), (64, 128, 128), (129, 136, 127),
-          (200, 96, 1000), (333, 257, 301), (7, 2048, 1024), (17, 515, 2050), (700, 520, 264), (2100, 40, 24)]
+          (200, 96, 1000), (31, 47, 1030), (32, 96, 4096), (33, 33, 256), (333, 257, 301), (7, 2048, 1024), (17, 515, 2050), (700, 520, 264), (2100, 40, 24)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
