@@ -212,25 +212,30 @@ __device__ __forceinline__ void interleave() {
   });
 }
 
-// A workgroup's waves are 2 along the rows by WJ along the columns.
+// LDS of a product's tiles: four slices of each operand (two where they come through
+// registers), as arrays of their own, so that the compiler knows which loads to LDS a read
+// has to wait for.
+#define GS_TILE_LDS(BT)                                                                            \
+  __shared__ __attribute__((aligned(1024))) char A0[(BT)*BK * 2], A1[(BT)*BK * 2], A2[(BT)*BK * 2], \
+      A3[(BT)*BK * 2], B0[(BT)*BK * 2], B1[(BT)*BK * 2], B2[(BT)*BK * 2], B3[(BT)*BK * 2]
+#define GS_TILE_ARRAYS A0, A1, A2, A3, B0, B1, B2, B3
+
+// Workgroup `group` of a product. Its waves are 2 along the rows by WJ along the columns.
 template <int BT, int WJ, int LAYOUT, bool DIRECT, bool PART>
-__global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) {
+__device__ __forceinline__ void gemm_bf16_group(const GemmBf16Args& g, int group, char* A0, char* A1, char* A2, char* A3,
+                                                char* B0, char* B1, char* B2, char* B3) {
   constexpr int THREADS = 128 * WJ, TI = BT / 32, TJ = BT / WJ / 16;  // a wave's fragments
   constexpr bool A_KC = LAYOUT != kGemmTN, B_KC = LAYOUT == kGemmNT;
   typedef typename std::conditional<DIRECT, Direct<BT, A_KC, THREADS>, Staged<BT, A_KC, THREADS>>::type LA;
   typedef typename std::conditional<DIRECT, Direct<BT, B_KC, THREADS>, Staged<BT, B_KC, THREADS>>::type LB;
   constexpr int kLoads = LA::kLoads + LB::kLoads;
-  __shared__ __attribute__((aligned(1024))) char A0[LA::kBytes];
-  __shared__ __attribute__((aligned(1024))) char A1[LA::kBytes];
-  __shared__ __attribute__((aligned(1024))) char B0[LB::kBytes];
-  __shared__ __attribute__((aligned(1024))) char B1[LB::kBytes];
   // Each XCD (workgroup mod 8) takes one split, or as few as there are, and of its tiles a
   // run, in patches of 1024 rows: its L2 then holds what its workgroups share. (With the
   // tiles of every split spread over all XCDs, dw of M = 32768, N = 2048, K = 1024 read
   // 670 MB instead of 200.)
   const int mt = (g.M + BT - 1) / BT, nt = (g.N + BT - 1) / BT, total = mt * nt;
-  const int xcd = blockIdx.x & 7, spread = g.ksplit < 8 ? 8 / g.ksplit : 1;  // XCDs of a split
-  const int per = (total + spread - 1) / spread, slot = blockIdx.x >> 3;
+  const int xcd = group & 7, spread = g.ksplit < 8 ? 8 / g.ksplit : 1;  // XCDs of a split
+  const int per = (total + spread - 1) / spread, slot = group >> 3;
   const int split = g.ksplit < 8 ? xcd % g.ksplit : xcd + 8 * (slot / per);
   const int tile = g.ksplit < 8 ? xcd / g.ksplit * per + slot : slot % per;
   if ((g.ksplit < 8 && slot >= per) || split >= g.ksplit || tile >= total) return;  // uniform
@@ -273,10 +278,6 @@ __global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) 
   };
   constexpr int kReads = TI * LA::kReads + TJ * LB::kReads;
   if constexpr (DIRECT) {
-    __shared__ __attribute__((aligned(1024))) char A2[LA::kBytes];
-    __shared__ __attribute__((aligned(1024))) char A3[LA::kBytes];
-    __shared__ __attribute__((aligned(1024))) char B2[LB::kBytes];
-    __shared__ __attribute__((aligned(1024))) char B3[LB::kBytes];
     auto load = [&](int s, char* A, char* B) __attribute__((always_inline)) {
       la.load(s, n, A);
       lb.load(s, n, B);
@@ -397,6 +398,41 @@ __global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) 
       }
     }
     __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int BT, int WJ, int LAYOUT, bool DIRECT, bool PART>
+__global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) {
+  if constexpr (DIRECT) {
+    GS_TILE_LDS(BT);
+    gemm_bf16_group<BT, WJ, LAYOUT, DIRECT, PART>(g, blockIdx.x, GS_TILE_ARRAYS);
+  } else {
+    __shared__ __attribute__((aligned(1024))) char A0[BT * BK * 2], A1[BT * BK * 2], B0[BT * BK * 2], B1[BT * BK * 2];
+    gemm_bf16_group<BT, WJ, LAYOUT, DIRECT, PART>(g, blockIdx.x, A0, A1, nullptr, nullptr, B0, B1, nullptr, nullptr);
+  }
+}
+
+// The products of a small backward in one launch, side by side on the device: dx (NN),
+// dw (TN) and the column sums' end (sum_columns) have no part in each other.
+template <bool DIRECT, bool PART>
+__global__ __launch_bounds__(256, 2) void gemm_bf16_pair_kernel(GemmBf16Args x, GemmBf16Args w, ColumnSums c, int nx, int nw) {
+  const int group = blockIdx.x;
+  if constexpr (DIRECT) {
+    GS_TILE_LDS(64);
+    if (group < nw)
+      gemm_bf16_group<64, 2, kGemmTN, DIRECT, PART>(w, group, GS_TILE_ARRAYS);
+    else if (group < nw + nx)
+      gemm_bf16_group<64, 2, kGemmNN, DIRECT, false>(x, group - nw, GS_TILE_ARRAYS);
+    else
+      sum_columns<__bf16>(c, group - nw - nx, reinterpret_cast<float(*)[17]>(A0));
+  } else {
+    __shared__ __attribute__((aligned(1024))) char A0[64 * BK * 2], A1[64 * BK * 2], B0[64 * BK * 2], B1[64 * BK * 2];
+    if (group < nw)
+      gemm_bf16_group<64, 2, kGemmTN, DIRECT, PART>(w, group, A0, A1, nullptr, nullptr, B0, B1, nullptr, nullptr);
+    else if (group < nw + nx)
+      gemm_bf16_group<64, 2, kGemmNN, DIRECT, false>(x, group - nw, A0, A1, nullptr, nullptr, B0, B1, nullptr, nullptr);
+    else
+      sum_columns<__bf16>(c, group - nw - nx, reinterpret_cast<float(*)[17]>(A0));
   }
 }
 
@@ -575,36 +611,76 @@ int gemm_bf16_pick_split(int M, int N, int K) {
   return best;
 }
 
+namespace {
+
+int check(const GemmBf16Args& g, const char* who) {
+  if (g.M < 1 || g.N < 1 || g.K < 1 || g.ksplit < 1 || g.ksplit > 32 || (g.ksplit & (g.ksplit - 1)) != 0)
+    return set_error(GS_ERR_INVALID, "%s: GEMM dims must be positive and ksplit a power of 2 (M=%d, N=%d, K=%d, ksplit=%d)",
+                     who, g.M, g.N, g.K, g.ksplit);
+  return GS_OK;
+}
+
+bool direct_of(const GemmBf16Args& g) {
+  const bool a_kc = g.layout != kGemmTN, b_kc = g.layout == kGemmNT;
+  return direct_ok(g.a, g.lda, a_kc ? g.K : g.M, a_kc, g.a_pads) && direct_ok(g.b, g.ldb, b_kc ? g.K : g.N, b_kc, g.b_pads);
+}
+
+// Workgroups of a product in tiles of T: a multiple of 8.
+int64_t groups_of(const GemmBf16Args& g, int T) {
+  const int64_t tiles = tiles_of(g.M, g.N, T), spread = g.ksplit < 8 ? 8 / g.ksplit : 1;
+  return 8 * ((tiles + spread - 1) / spread) * (g.ksplit < 8 ? 1 : (g.ksplit + 7) / 8);
+}
+
+int finish(const GemmBf16Args& g, hipStream_t stream) {
+  const int64_t octets = (int64_t)g.M * ((g.N + 7) / 8);
+  hipLaunchKernelGGL(gemm_bf16_finish_kernel, dim3((unsigned)std::min<int64_t>((octets + 255) / 256, 8192)), dim3(256), 0,
+                     stream, g);
+  GS_CHECK_HIP(hipGetLastError());
+  return GS_OK;
+}
+
+constexpr int64_t kMostGroups = 1 << 22;
+
+}  // namespace
+
 int gemm_bf16(const GemmBf16Args& g, hipStream_t stream, const char* who) {
-  if (g.M < 1 || g.N < 1 || g.K < 1 || g.ksplit < 1 || g.ksplit > 32)
-    return set_error(GS_ERR_INVALID, "%s: GEMM dims must be positive (M=%d, N=%d, K=%d, ksplit=%d)", who, g.M, g.N,
-                     g.K, g.ksplit);
-  if ((g.ksplit & (g.ksplit - 1)) != 0) return set_error(GS_ERR_INVALID, "%s: ksplit must be a power of 2", who);
+  const int rc = check(g, who);
+  if (rc) return rc;
   if (g.layout == kGemmNT && g.ksplit == 1 && gemm_bf16_few_rows(g.M)) {
     hipLaunchKernelGGL(g.M <= 16 ? gemm_bf16_rows_kernel<1> : gemm_bf16_rows_kernel<2>, dim3((unsigned)((g.N + 15) / 16)),
                        dim3(64 * kRowWaves), 0, stream, g);
     GS_CHECK_HIP(hipGetLastError());
     return GS_OK;
   }
-  const bool a_kc = g.layout != kGemmTN, b_kc = g.layout == kGemmNT;
-  const bool direct = direct_ok(g.a, g.lda, a_kc ? g.K : g.M, a_kc, g.a_pads) && direct_ok(g.b, g.ldb, b_kc ? g.K : g.N, b_kc, g.b_pads);
+  const bool direct = direct_of(g), part = g.ksplit > 1;
   const int T = pick_tile(g.M, g.N, g.K, g.ksplit, direct);
-  const bool part = g.ksplit > 1;
   GemmBf16Fn fn = g.layout == kGemmNT   ? kernel_of<kGemmNT>(T, direct, part)
                   : g.layout == kGemmNN ? kernel_of<kGemmNN>(T, direct, part)
                                         : kernel_of<kGemmTN>(T, direct, part);
-  const int64_t tiles = tiles_of(g.M, g.N, T), spread = g.ksplit < 8 ? 8 / g.ksplit : 1;
-  const int64_t groups = 8 * ((tiles + spread - 1) / spread) * (g.ksplit < 8 ? 1 : (g.ksplit + 7) / 8);
-  if (groups > (1 << 22)) return set_error(GS_ERR_INVALID, "%s: GEMM of too many tiles (M=%d, N=%d)", who, g.M, g.N);
+  const int64_t groups = groups_of(g, T);
+  if (groups > kMostGroups) return set_error(GS_ERR_INVALID, "%s: GEMM of too many tiles (M=%d, N=%d)", who, g.M, g.N);
   hipLaunchKernelGGL(fn, dim3((unsigned)groups), dim3(T == 256 ? 512 : 256), 0, stream, g);
   GS_CHECK_HIP(hipGetLastError());
-  if (part) {
-    const int64_t octets = (int64_t)g.M * ((g.N + 7) / 8);
-    hipLaunchKernelGGL(gemm_bf16_finish_kernel, dim3((unsigned)std::min<int64_t>((octets + 255) / 256, 8192)), dim3(256),
-                       0, stream, g);
-    GS_CHECK_HIP(hipGetLastError());
-  }
-  return GS_OK;
+  return part ? finish(g, stream) : GS_OK;
+}
+
+bool gemm_bf16_pair_applies(const GemmBf16Args& x, const GemmBf16Args& w) {
+  const bool direct = direct_of(x);
+  return x.ksplit == 1 && direct == direct_of(w) && pick_tile(x.M, x.N, x.K, x.ksplit, direct) == 64 &&
+         pick_tile(w.M, w.N, w.K, w.ksplit, direct) == 64 && groups_of(x, 64) + groups_of(w, 64) <= kMostGroups;
+}
+
+int gemm_bf16_pair(const GemmBf16Args& x, const GemmBf16Args& w, const ColumnSums& c, hipStream_t stream, const char* who) {
+  int rc = check(x, who);
+  if (!rc) rc = check(w, who);
+  if (rc) return rc;
+  const bool direct = direct_of(x), part = w.ksplit > 1;
+  const int nx = (int)groups_of(x, 64), nw = (int)groups_of(w, 64), nc = c.dst ? (c.n + 15) / 16 : 0;
+  auto fn = direct ? (part ? gemm_bf16_pair_kernel<true, true> : gemm_bf16_pair_kernel<true, false>)
+                   : (part ? gemm_bf16_pair_kernel<false, true> : gemm_bf16_pair_kernel<false, false>);
+  hipLaunchKernelGGL(fn, dim3((unsigned)(nx + nw + nc)), dim3(256), 0, stream, x, w, c, nx, nw);
+  GS_CHECK_HIP(hipGetLastError());
+  return part ? finish(w, stream) : GS_OK;
 }
 
 }  // namespace gs

@@ -195,29 +195,10 @@ __global__ __launch_bounds__(kThreads) void pad_kernel(PadJob a, PadJob b) {
   }
 }
 
-// dst[e] = sum over parts of src[part * n + e], rounded to the tensor's type: a workgroup
-// takes 16 columns, its 16 part lanes every 16th part, joined through LDS in order.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sum_columns_kernel(T* dst, const float* src, int n, int parts) {
+__global__ __launch_bounds__(kThreads) void sum_columns_kernel(ColumnSums c) {
   __shared__ float red[16][17];
-  const int c = threadIdx.x & 15, l = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
-  float s = 0.0f;
-  if (e < n) {
-    for (int k0 = l; k0 < parts; k0 += 16 * 8) {  // eight loads in flight
-      float x[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] = k0 + 16 * u < parts ? src[(int64_t)(k0 + 16 * u) * n + e] : 0.0f;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) s += x[u];
-    }
-  }
-  red[l][c] = s;
-  __syncthreads();
-  if (l == 0 && e < n) {
-#pragma unroll
-    for (int k = 1; k < 16; ++k) s += red[k][c];
-    dst[e] = (T)s;
-  }
+  sum_columns<T>(c, blockIdx.x, red);
 }
 
 int check_linear(const char* who, int64_t M, int64_t N, int64_t K, int dtype, int act) {
@@ -453,88 +434,74 @@ extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {
   const int64_t sd = plan.dpre >= 0 ? plan.ldp : a->sdy;
   const bool dpre_pads = plan.dpre >= 0 && plan.ldp == up8(a->N);
   if ((rc = pad(a->x, a->sx, a->M, at(plan.x), a->w, a->N, at(plan.w), a->K, stream))) return rc;
-  if (a->dx != nullptr) {
-    if (bf16) {
-      GemmBf16Args g;
-      g.a = static_cast<const __bf16*>(dpre);
-      g.lda = sd;
-      g.b = static_cast<const __bf16*>(plan.w < 0 ? a->w : at(plan.w));
-      g.ldb = plan.w < 0 ? a->K : up8(a->K);
-      g.y = static_cast<__bf16*>(a->dx);
-      g.ldy = a->K;
-      g.part = static_cast<float*>(at(plan.dx));
-      g.M = (int)a->M;
-      g.N = (int)a->K;
-      g.K = (int)a->N;
-      g.a_pads = dpre_pads;
-      g.b_pads = plan.w >= 0;
-      g.ksplit = plan.split_x;
-      g.layout = kGemmNN;
-      rc = gemm_bf16(g, stream, who);
-    } else {
-      GemmArgs g;
-      g.a = static_cast<const float*>(dpre);
-      g.lda = sd;
-      g.b = static_cast<const float*>(a->w);
-      g.ldb = a->K;
-      g.c = static_cast<float*>(a->dx);
-      g.ldc = a->K;
-      g.M = (int)a->M;
-      g.N = (int)a->K;
-      g.K = (int)a->N;
-      g.layout = kGemmNN;
-      rc = gemm_f32(g, stream, who);
-    }
-    if (rc) return rc;
-  }
-  if (a->dw != nullptr) {
-    if (bf16) {
-      GemmBf16Args g;
-      g.a = static_cast<const __bf16*>(dpre);
-      g.lda = sd;
-      g.b = static_cast<const __bf16*>(plan.x < 0 ? a->x : at(plan.x));
-      g.ldb = plan.x < 0 ? a->sx : up8(a->K);
-      g.y = static_cast<__bf16*>(a->dw);
-      g.ldy = a->K;
-      g.part = static_cast<float*>(at(plan.dw));
-      g.M = (int)a->N;
-      g.N = (int)a->K;
-      g.K = (int)a->M;
-      g.a_pads = dpre_pads;
-      g.b_pads = plan.x >= 0;
-      g.ksplit = plan.split_w;
-      g.layout = kGemmTN;
-      rc = gemm_bf16(g, stream, who);
-    } else {
-      GemmArgs g;
-      g.a = static_cast<const float*>(dpre);
-      g.lda = sd;
-      g.b = static_cast<const float*>(a->x);
-      g.ldb = a->sx;
-      g.c = plan.dw >= 0 ? static_cast<float*>(at(plan.dw)) : static_cast<float*>(a->dw);
-      g.ldc = a->K;
-      g.split_stride = a->N * a->K;
-      g.M = (int)a->N;
-      g.N = (int)a->K;
-      g.K = (int)a->M;
-      g.ksplit = plan.split_w;
-      g.layout = kGemmTN;
-      rc = gemm_f32(g, stream, who);
-      if (!rc && plan.dw >= 0)
-        rc = sum_partials(static_cast<float*>(a->dw), g.c, a->N * a->K, plan.split_w, a->N * a->K, stream, who);
-    }
-    if (rc) return rc;
-  }
+  ColumnSums sums;
   if (a->dbias != nullptr) {
-    const float* part = static_cast<const float*>(at(plan.cols));
-    const dim3 grid((unsigned)((a->N + 15) / 16));
-    if (bf16)
-      hipLaunchKernelGGL(sum_columns_kernel<__bf16>, grid, dim3(kThreads), 0, stream, static_cast<__bf16*>(a->dbias),
-                         part, (int)a->N, chunks);
-    else
-      hipLaunchKernelGGL(sum_columns_kernel<float>, grid, dim3(kThreads), 0, stream, static_cast<float*>(a->dbias),
-                         part, (int)a->N, chunks);
+    sums.dst = a->dbias;
+    sums.src = static_cast<const float*>(at(plan.cols));
+    sums.n = (int)a->N;
+    sums.parts = chunks;
+  }
+  if (bf16) {
+    GemmBf16Args x, w;
+    x.a = w.a = static_cast<const __bf16*>(dpre);
+    x.lda = w.lda = sd;
+    x.a_pads = w.a_pads = dpre_pads;
+    x.b = static_cast<const __bf16*>(plan.w < 0 ? a->w : at(plan.w));
+    x.ldb = plan.w < 0 ? a->K : up8(a->K);
+    x.b_pads = plan.w >= 0;
+    x.y = static_cast<__bf16*>(a->dx);
+    x.ldy = w.ldy = a->K;
+    x.part = static_cast<float*>(at(plan.dx));
+    x.M = (int)a->M;
+    x.N = (int)a->K;
+    x.K = (int)a->N;
+    x.ksplit = plan.split_x;
+    x.layout = kGemmNN;
+    w.b = static_cast<const __bf16*>(plan.x < 0 ? a->x : at(plan.x));
+    w.ldb = plan.x < 0 ? a->sx : up8(a->K);
+    w.b_pads = plan.x >= 0;
+    w.y = static_cast<__bf16*>(a->dw);
+    w.part = static_cast<float*>(at(plan.dw));
+    w.M = (int)a->N;
+    w.N = (int)a->K;
+    w.K = (int)a->M;
+    w.ksplit = plan.split_w;
+    w.layout = kGemmTN;
+    if (a->dx && a->dw && gemm_bf16_pair_applies(x, w)) return gemm_bf16_pair(x, w, sums, stream, who);
+    if (a->dx && (rc = gemm_bf16(x, stream, who))) return rc;
+    if (a->dw && (rc = gemm_bf16(w, stream, who))) return rc;
+  } else {
+    GemmArgs x, w;
+    x.a = w.a = static_cast<const float*>(dpre);
+    x.lda = w.lda = sd;
+    x.b = static_cast<const float*>(a->w);
+    x.ldb = a->K;
+    x.c = static_cast<float*>(a->dx);
+    x.ldc = w.ldc = a->K;
+    x.M = (int)a->M;
+    x.N = (int)a->K;
+    x.K = (int)a->N;
+    x.layout = kGemmNN;
+    w.b = static_cast<const float*>(a->x);
+    w.ldb = a->sx;
+    w.c = static_cast<float*>(plan.dw >= 0 ? at(plan.dw) : a->dw);
+    w.split_stride = a->N * a->K;
+    w.M = (int)a->N;
+    w.N = (int)a->K;
+    w.K = (int)a->M;
+    w.ksplit = plan.split_w;
+    w.layout = kGemmTN;
+    if (a->dx && (rc = gemm_f32(x, stream, who))) return rc;
+    if (a->dw) {
+      if ((rc = gemm_f32(w, stream, who))) return rc;
+      if (plan.dw >= 0 && (rc = sum_partials(static_cast<float*>(a->dw), w.c, a->N * a->K, plan.split_w, a->N * a->K, stream, who)))
+        return rc;
+    }
+  }
+  if (sums.dst != nullptr) {
+    hipLaunchKernelGGL(bf16 ? sum_columns_kernel<__bf16> : sum_columns_kernel<float>, dim3((unsigned)((a->N + 15) / 16)),
+                       dim3(kThreads), 0, stream, sums);
     GS_CHECK_HIP(hipGetLastError());
   }
-  return rc;
+  return GS_OK;
 }
