@@ -198,7 +198,7 @@ __device__ __forceinline__ void finish8(const LinearEpilogue& e, __bf16* y, int6
 // loads: the reads first, one per MFMA or two, then the others.
 template <int NM, int NR, int NW, int NV>
 __device__ __forceinline__ void interleave() {
-  constexpr int kPer = NR * 2 <= NM ? 1 : 2, kFirst = (NR + kPer - 1) / kPer;
+  constexpr int kPer = NR * 4 <= NM * 3 ? 1 : 2, kFirst = (NR + kPer - 1) / kPer;
   constexpr int kRest = NM - kFirst > 0 ? NM - kFirst : 1, kPut = (NW + NV + kRest - 1) / kRest;
   static_for<0, NM>([&](auto I) {
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
@@ -212,6 +212,12 @@ __device__ __forceinline__ void interleave() {
   });
 }
 
+// What a launch stores: finished outputs, a split's sums, or either as it is asked. TN
+// products take the last: with the first two apart, the instance of 256 x 256 tiles that
+// stores sums spilled inside its loop (128 slices in 166 us instead of 100); the others
+// store finished outputs faster alone (M = 32768, N = 2048, K = 1024: 136 us, not 147).
+enum { kOutputs = 0, kSums = 1, kEither = 2 };
+
 // LDS of a product's tiles: four slices of each operand (two where they come through
 // registers), as arrays of their own, so that the compiler knows which loads to LDS a read
 // has to wait for.
@@ -221,7 +227,7 @@ __device__ __forceinline__ void interleave() {
 #define GS_TILE_ARRAYS A0, A1, A2, A3, B0, B1, B2, B3
 
 // Workgroup `group` of a product. Its waves are 2 along the rows by WJ along the columns.
-template <int BT, int WJ, int LAYOUT, bool DIRECT, bool PART>
+template <int BT, int WJ, int LAYOUT, bool DIRECT, int PART>
 __device__ __forceinline__ void gemm_bf16_group(const GemmBf16Args& g, int group, char* A0, char* A1, char* A2, char* A3,
                                                 char* B0, char* B1, char* B2, char* B3) {
   constexpr int THREADS = 128 * WJ, TI = BT / 32, TJ = BT / WJ / 16;  // a wave's fragments
@@ -363,37 +369,43 @@ __device__ __forceinline__ void gemm_bf16_group(const GemmBf16Args& g, int group
   const int r16 = lane & 15, q4 = (lane >> 4) * 4;
   const int j = j0 + wj + 8 * (lane % kLanes);
   float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (!PART && g.epi.bias != nullptr && j < g.N) load_row8(g.epi.bias, j, g.N, bias);
+  if (PART != kSums && g.epi.bias != nullptr && j < g.N) load_row8(g.epi.bias, j, g.N, bias);
 #pragma unroll
   for (int a = 0; a < TI; ++a) {
 #pragma unroll
     for (int b = 0; b < TJ; ++b) *reinterpret_cast<f4v*>(mine + r16 * kStride + 16 * b + q4) = acc[a][b];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    if (PART == kSums || (PART == kEither && g.ksplit > 1)) {  // four columns a lane: a store covers whole lines
+      typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+      constexpr int kQuads = kCols / 4;
+      const int jq = j0 + wj + 4 * (lane % kQuads);
 #pragma unroll
-    for (int rr = 0; rr < 16; rr += 64 / kLanes) {
-      const int row = rr + lane / kLanes, i = i0 + wi + 16 * a + row;
-      float x[8];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const f4v w = *reinterpret_cast<const f4v*>(mine + row * kStride + 8 * (lane % kLanes) + 4 * h);
-#pragma unroll
-        for (int v = 0; v < 4; ++v) x[4 * h + v] = w[v];
-      }
-      if (i >= g.M || j >= g.N) continue;
-      if constexpr (PART) {
-        float* c = g.part + ((int64_t)split * g.M + i) * g.N + j;
-        typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
-        if (j + 8 <= g.N) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<f4u*>(c + 4 * h) = f4u{x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]};
+      for (int rr = 0; rr < 16; rr += 64 / kQuads) {
+        const int row = rr + lane / kQuads, i = i0 + wi + 16 * a + row;
+        const f4v w = *reinterpret_cast<const f4v*>(mine + row * kStride + 4 * (lane % kQuads));
+        if (i >= g.M || jq >= g.N) continue;
+        float* c = g.part + ((int64_t)split * g.M + i) * g.N + jq;
+        if (jq + 4 <= g.N) {
+          *reinterpret_cast<f4u*>(c) = w;
         } else {
 #pragma unroll
-          for (int v = 0; v < 8; ++v)
-            if (j + v < g.N) c[v] = x[v];
+          for (int v = 0; v < 3; ++v)
+            if (jq + v < g.N) c[v] = w[v];
         }
-      } else {
+      }
+    } else {
+#pragma unroll
+      for (int rr = 0; rr < 16; rr += 64 / kLanes) {
+        const int row = rr + lane / kLanes, i = i0 + wi + 16 * a + row;
+        float x[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f4v w = *reinterpret_cast<const f4v*>(mine + row * kStride + 8 * (lane % kLanes) + 4 * h);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) x[4 * h + v] = w[v];
+        }
+        if (i >= g.M || j >= g.N) continue;
         finish8(g.epi, g.y, g.ldy, i, j, g.N, bias, x);
       }
     }
@@ -401,7 +413,7 @@ __device__ __forceinline__ void gemm_bf16_group(const GemmBf16Args& g, int group
   }
 }
 
-template <int BT, int WJ, int LAYOUT, bool DIRECT, bool PART>
+template <int BT, int WJ, int LAYOUT, bool DIRECT, int PART>
 __global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) {
   if constexpr (DIRECT) {
     GS_TILE_LDS(BT);
@@ -414,23 +426,23 @@ __global__ __launch_bounds__(128 * WJ, 2) void gemm_bf16_kernel(GemmBf16Args g) 
 
 // The products of a small backward in one launch, side by side on the device: dx (NN),
 // dw (TN) and the column sums' end (sum_columns) have no part in each other.
-template <bool DIRECT, bool PART>
+template <bool DIRECT>
 __global__ __launch_bounds__(256, 2) void gemm_bf16_pair_kernel(GemmBf16Args x, GemmBf16Args w, ColumnSums c, int nx, int nw) {
   const int group = blockIdx.x;
   if constexpr (DIRECT) {
     GS_TILE_LDS(64);
     if (group < nw)
-      gemm_bf16_group<64, 2, kGemmTN, DIRECT, PART>(w, group, GS_TILE_ARRAYS);
+      gemm_bf16_group<64, 2, kGemmTN, DIRECT, kEither>(w, group, GS_TILE_ARRAYS);
     else if (group < nw + nx)
-      gemm_bf16_group<64, 2, kGemmNN, DIRECT, false>(x, group - nw, GS_TILE_ARRAYS);
+      gemm_bf16_group<64, 2, kGemmNN, DIRECT, kOutputs>(x, group - nw, GS_TILE_ARRAYS);
     else
       sum_columns<__bf16>(c, group - nw - nx, reinterpret_cast<float(*)[17]>(A0));
   } else {
     __shared__ __attribute__((aligned(1024))) char A0[64 * BK * 2], A1[64 * BK * 2], B0[64 * BK * 2], B1[64 * BK * 2];
     if (group < nw)
-      gemm_bf16_group<64, 2, kGemmTN, DIRECT, PART>(w, group, A0, A1, nullptr, nullptr, B0, B1, nullptr, nullptr);
+      gemm_bf16_group<64, 2, kGemmTN, DIRECT, kEither>(w, group, A0, A1, nullptr, nullptr, B0, B1, nullptr, nullptr);
     else if (group < nw + nx)
-      gemm_bf16_group<64, 2, kGemmNN, DIRECT, false>(x, group - nw, A0, A1, nullptr, nullptr, B0, B1, nullptr, nullptr);
+      gemm_bf16_group<64, 2, kGemmNN, DIRECT, kOutputs>(x, group - nw, A0, A1, nullptr, nullptr, B0, B1, nullptr, nullptr);
     else
       sum_columns<__bf16>(c, group - nw - nx, reinterpret_cast<float(*)[17]>(A0));
   }
@@ -560,9 +572,9 @@ constexpr int kTileSizes[3] = {256, 128, 64};
 // them. (M, N, K, layout; predicted and measured: 32768 x 2048 x 1024 NT T 256 138, 139;
 // 4096 x 1024 x 1024 NT T 128 13, 13; 2048 x 1024 x 512 NT T 64 7.3, 6.8, T 128 9.5, 8.8.)
 double tile_us(int M, int N, int K, int T, int split) {
-  const double slice = T == 256 ? 0.84 : T == 128 ? 0.235 : 0.1, ends = T == 256 ? 7.0 : T == 128 ? 2.7 : 0.55;
+  const double slice = T == 256 ? 0.76 : T == 128 ? 0.235 : 0.1, ends = T == 256 ? 7.0 : T == 128 ? 2.7 : 0.55;
   const int64_t slices = ((K + split - 1) / split + BK - 1) / BK, per_cu = (tiles_of(M, N, T) * split + 255) / 256;
-  return 3.0 + per_cu * (slices * slice + ends) + (split > 1 ? 5.0 + 8e-6 * split * M * N / 4.5 : 0.0);
+  return 3.0 + per_cu * (slices * slice + ends) + (split > 1 ? 3.0 + 8e-6 * split * M * N / 9.0 : 0.0);
 }
 
 int pick_tile(int M, int N, int K, int split, bool direct) {
@@ -583,7 +595,10 @@ typedef void (*GemmBf16Fn)(GemmBf16Args);
 
 template <int LAYOUT, int BT, int WJ, bool DIRECT>
 GemmBf16Fn pick(bool part) {
-  return part ? gemm_bf16_kernel<BT, WJ, LAYOUT, DIRECT, true> : gemm_bf16_kernel<BT, WJ, LAYOUT, DIRECT, false>;
+  if constexpr (LAYOUT == kGemmTN)
+    return gemm_bf16_kernel<BT, WJ, LAYOUT, DIRECT, kEither>;
+  else
+    return part ? gemm_bf16_kernel<BT, WJ, LAYOUT, DIRECT, kSums> : gemm_bf16_kernel<BT, WJ, LAYOUT, DIRECT, kOutputs>;
 }
 
 template <int LAYOUT>
@@ -676,8 +691,7 @@ int gemm_bf16_pair(const GemmBf16Args& x, const GemmBf16Args& w, const ColumnSum
   if (rc) return rc;
   const bool direct = direct_of(x), part = w.ksplit > 1;
   const int nx = (int)groups_of(x, 64), nw = (int)groups_of(w, 64), nc = c.dst ? (c.n + 15) / 16 : 0;
-  auto fn = direct ? (part ? gemm_bf16_pair_kernel<true, true> : gemm_bf16_pair_kernel<true, false>)
-                   : (part ? gemm_bf16_pair_kernel<false, true> : gemm_bf16_pair_kernel<false, false>);
+  auto fn = direct ? gemm_bf16_pair_kernel<true> : gemm_bf16_pair_kernel<false>;
   hipLaunchKernelGGL(fn, dim3((unsigned)(nx + nw + nc)), dim3(256), 0, stream, x, w, c, nx, nw);
   GS_CHECK_HIP(hipGetLastError());
   return part ? finish(w, stream) : GS_OK;
