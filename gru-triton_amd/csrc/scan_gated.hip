@@ -737,8 +737,9 @@ ChainBytes chain_bytes(const Plan& plan, int64_t B) {
 }
 
 // What a call of these sizes may need, whatever its pointers and strides.
-int64_t scratch_most(int64_t T, int64_t B, int64_t H) {
-  return std::max(chain_bytes(make_plan(T, B, H, 1, true), B).total, chain_bytes(make_plan(T, B, H, 2, true), B).total);
+int64_t scratch_most(int dtype, int64_t T, int64_t B, int64_t H) {
+  const int64_t one = chain_bytes(make_plan(T, B, H, 1, true), B).total;
+  return dtype == GS_DTYPE_F32 ? one : std::max(one, chain_bytes(make_plan(T, B, H, 2, true), B).total);
 }
 
 int launch(const char* who, int dtype, const Plan& plan, GlrParams& p, bool back, bool tanh, void* scratch,
@@ -812,7 +813,7 @@ using namespace gs;
 extern "C" int64_t gs_glr_scratch_bytes(const gs_glr_args* a) {
   clear_error();
   const int rc = check_fwd(a, "gs_glr_scratch_bytes");
-  return rc ? rc : scratch_most(a->T, a->B, a->H);
+  return rc ? rc : scratch_most(a->dtype, a->T, a->B, a->H);
 }
 
 extern "C" int gs_glr_fwd(const gs_glr_args* a, hipStream_t stream) {
@@ -843,7 +844,7 @@ extern "C" int gs_glr_fwd(const gs_glr_args* a, hipStream_t stream) {
 extern "C" int64_t gs_glr_bwd_scratch_bytes(const gs_glr_bwd_args* a) {
   clear_error();
   const int rc = check_bwd(a, "gs_glr_bwd_scratch_bytes");
-  return rc ? rc : scratch_most(a->T, a->B, a->H);
+  return rc ? rc : scratch_most(a->dtype, a->T, a->B, a->H);
 }
 
 extern "C" int gs_glr_bwd(const gs_glr_bwd_args* a, hipStream_t stream) {

@@ -32,6 +32,7 @@ from .quantizers import FakeQuantizePerTensor, QuantizerConfig
 from .observe import gru_scan_observe, hidden_map_dense
 from .calibration import calibrate, freeze_all
 from .gated_linear import gated_linear_scan, gated_linear_step
+from .gated_layer import GatedLinearLayer
 from .linear import linear_act
 from .optim import AdamW, adamw_dequantize_state, adamw_step
 from .export import dequantize_int_weights, export_int_weights, quantize_rows
@@ -41,6 +42,7 @@ __all__ = [
     "adamw_dequantize_state",
     "adamw_step",
     "FakeQuantizePerTensor",
+    "GatedLinearLayer",
     "GRUScanFunction",
     "GRUScanPersistentFunction",
     "QuantizerConfig",
