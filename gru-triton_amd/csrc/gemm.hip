@@ -178,22 +178,30 @@ __device__ __forceinline__ void interleave() {
 // Four workgroups of NT's small tiles fit a CU, which short products, bound by
 // their stores, are the faster for (M = 16384, N = 1536, K = 64: 60 -> 53 us);
 // NN and TN lose more to the registers (their backward 112 -> 116 us).
-template <int LAYOUT, int T, int LOAD, bool Q, bool EPI = false>
-__global__ __launch_bounds__(kGemmThreads, T == kBigT || LOAD == kLoadFar                ? 2
-                                           : LAYOUT == kGemmNT && LOAD == kLoadVec ? 4
-                                                                                   : 3) void gemm_kernel(GemmArgs g) {
+//
+// Workgroup (wg, z) of the product, wg over its tiles, z over batch and splits; `lds`
+// holds kGemmLds floats.
+constexpr int stage_floats(bool kc, int T, int layout) {
+  return kc ? T * (2048 / T + 8) : 2048 / T * (T + (layout == kGemmNN ? 4 : 16));
+}
+template <int LAYOUT, int T>
+constexpr int kGemmLds = 2 * (stage_floats(LAYOUT != kGemmTN, T, LAYOUT) + stage_floats(LAYOUT == kGemmNT, T, LAYOUT));
+
+template <int LAYOUT, int T, int LOAD, bool Q, bool EPI>
+__device__ __forceinline__ void gemm_group(const GemmArgs& g, int wg, int zz, float* lds) {
   constexpr bool A_KC = LAYOUT != kGemmTN, B_KC = LAYOUT == kGemmNT, TN = LAYOUT == kGemmTN;
   constexpr bool QA = Q && LAYOUT == kGemmNT, QB = Q && LAYOUT == kGemmTN;
   constexpr int RS = T + (LAYOUT == kGemmNN ? 4 : 16);
   typedef TileLoader<A_KC, T, LOAD, RS> LA;
   typedef TileLoader<B_KC, T, LOAD, RS> LB;
   constexpr int BK = LA::BK, MT = T / 32, KH = BK / 16;
-  __shared__ __attribute__((aligned(16))) float As[2][LA::kStage];
-  __shared__ __attribute__((aligned(16))) float Bs[2][LB::kStage];
+  static_assert(2 * (LA::kStage + LB::kStage) == kGemmLds<LAYOUT, T>, "the operands' stages");
+  float(*As)[LA::kStage] = reinterpret_cast<float(*)[LA::kStage]>(lds);
+  float(*Bs)[LB::kStage] = reinterpret_cast<float(*)[LB::kStage]>(lds + 2 * LA::kStage);
   // this workgroup's tile: patches of 1024 rows; of big tiles, each XCD
   // (workgroup mod 8) takes a run, whose operands its L2 then holds
   const int mt = (g.M + T - 1) / T, nt = (g.N + T - 1) / T, total = mt * nt;
-  const int wg = blockIdx.y * gridDim.x + blockIdx.x, per = (total + 7) / 8;
+  const int per = (total + 7) / 8;
   const int tile = T == kBigT ? (wg & 7) * per + (wg >> 3) : wg;
   if ((T == kBigT && (wg >> 3) >= per) || tile >= total) return;  // uniform
   constexpr int kPatch = 1024 / T;
@@ -204,7 +212,7 @@ __global__ __launch_bounds__(kGemmThreads, T == kBigT || LOAD == kLoadFar       
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wy = wave >> 1, wx = wave & 1;
   const int kper = ((g.K + g.ksplit - 1) / g.ksplit + kSplitK - 1) / kSplitK * kSplitK;
-  const int z = blockIdx.z / g.ksplit, split = blockIdx.z - z * g.ksplit;
+  const int z = zz / g.ksplit, split = zz - z * g.ksplit;
   const int kbeg = split * kper, kend = min(g.K, kbeg + kper);
   const int n = kend > kbeg ? (kend - kbeg + BK - 1) / BK : 0;
   const int klast = kbeg + (n - 1) * BK;
@@ -297,6 +305,32 @@ __global__ __launch_bounds__(kGemmThreads, T == kBigT || LOAD == kLoadFar       
         }
       }
   }
+}
+
+template <int LAYOUT, int T, int LOAD, bool Q, bool EPI = false>
+__global__ __launch_bounds__(kGemmThreads, T == kBigT || LOAD == kLoadFar                ? 2
+                                           : LAYOUT == kGemmNT && LOAD == kLoadVec ? 4
+                                                                                   : 3) void gemm_kernel(GemmArgs g) {
+  __shared__ __attribute__((aligned(16))) float lds[kGemmLds<LAYOUT, T>];
+  gemm_group<LAYOUT, T, LOAD, Q, EPI>(g, blockIdx.y * gridDim.x + blockIdx.x, blockIdx.z, lds);
+}
+
+// Two small products without quants and batch, NN and TN, and a sum of columns, side by
+// side in one launch: the linear operator's dx, dw and dbias, none of which alone has a
+// workgroup for every place on the device. The linear operator's backward at M 1650, N 1002,
+// K 301, on the GPU: 40 us, of 47 one after the other and 5 for the sums.
+template <int LOAD>
+__global__ __launch_bounds__(kGemmThreads, 3) void gemm_pair_kernel(GemmArgs x, GemmArgs w, ColumnSums c, int nx, int nw,
+                                                                    int tiles_w) {
+  constexpr int kLds = kGemmLds<kGemmTN, kSmallT> > kGemmLds<kGemmNN, kSmallT> ? kGemmLds<kGemmTN, kSmallT> : kGemmLds<kGemmNN, kSmallT>;
+  __shared__ __attribute__((aligned(16))) float lds[kLds];
+  const int group = blockIdx.x;
+  if (group < nw)
+    gemm_group<kGemmTN, kSmallT, LOAD, false, false>(w, group % tiles_w, group / tiles_w, lds);
+  else if (group < nw + nx)
+    gemm_group<kGemmNN, kSmallT, LOAD, false, false>(x, group - nw, 0, lds);
+  else
+    sum_columns<float>(c, group - nw - nx, reinterpret_cast<float(*)[17]>(lds));
 }
 
 // ---- int8 NT product (gemm_i8_nt) -----------------------------------------------
@@ -532,6 +566,40 @@ int gemm_pick_split(int M, int N, int K) {
   return best;
 }
 
+namespace {
+
+// How an operand pair is loaded, whether tiles of T lie within 32-bit offsets.
+bool near_tiles(const GemmArgs& g, int T) {
+  const bool a_kc = g.layout != kGemmTN, b_kc = g.layout == kGemmNT;
+  // the farthest float of a slice's tile from its first, for 32-bit byte offsets
+  auto reach = [&](bool kc, int64_t ld) { return (kc ? T : 2048 / T) * ld + (kc ? 2048 / T : T); };
+  return std::max(reach(a_kc, g.lda), reach(b_kc, g.ldb)) < (int64_t(1) << 29);
+}
+int load_of(const GemmArgs& g) {
+  const bool a_kc = g.layout != kGemmTN, b_kc = g.layout == kGemmNT;
+  const bool vec = (a_kc ? g.K % 4 == 0 : g.M % 4 == 0) && (b_kc ? g.K % 4 == 0 : g.N % 4 == 0);
+  return !near_tiles(g, kSmallT) ? kLoadFar : vec ? kLoadVec : kLoadWord;
+}
+
+}  // namespace
+
+bool gemm_pair_applies(const GemmArgs& x, const GemmArgs& w) {
+  const int load = load_of(x);
+  return load != kLoadFar && load == load_of(w) && !big_tiles(x) && !big_tiles(w) && x.ksplit == 1 &&
+         tile_count(x.M, x.N, kSmallT) + tile_count(w.M, w.N, kSmallT) * w.ksplit < (1 << 20);
+}
+
+int gemm_pair(const GemmArgs& x, const GemmArgs& w, const ColumnSums& c, hipStream_t stream, const char* who) {
+  if (x.M < 1 || x.N < 1 || x.K < 1 || w.ksplit < 1 || x.layout != kGemmNN || w.layout != kGemmTN || w.M < 1 || w.N < 1 || w.K < 1)
+    return set_error(GS_ERR_INVALID, "%s: bad pair of products", who);
+  const int tiles_w = (int)tile_count(w.M, w.N, kSmallT), nw = tiles_w * w.ksplit, nx = (int)tile_count(x.M, x.N, kSmallT);
+  const int nc = c.dst ? (c.n + 15) / 16 : 0;
+  auto fn = load_of(x) == kLoadVec ? gemm_pair_kernel<kLoadVec> : gemm_pair_kernel<kLoadWord>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)(nx + nw + nc)), dim3(kGemmThreads), 0, stream, x, w, c, nx, nw, tiles_w);
+  GS_CHECK_HIP(hipGetLastError());
+  return GS_OK;
+}
+
 int gemm_f32(const GemmArgs& g, hipStream_t stream, const char* who) {
   if (g.M < 1 || g.N < 1 || g.K < 1 || g.ksplit < 1)
     return set_error(GS_ERR_INVALID, "%s: GEMM dims must be positive (M=%d, N=%d, K=%d, ksplit=%d)", who, g.M, g.N,
@@ -541,15 +609,8 @@ int gemm_f32(const GemmArgs& g, hipStream_t stream, const char* who) {
                      g.a_mod, g.b_mod, g.ksplit);
   if (g.layout != kGemmNT && g.layout != kGemmTN && g.layout != kGemmNN)
     return set_error(GS_ERR_INVALID, "%s: unknown GEMM layout %d", who, g.layout);
-  const bool a_kc = g.layout != kGemmTN, b_kc = g.layout == kGemmNT;
-  const bool vec = (a_kc ? g.K % 4 == 0 : g.M % 4 == 0) && (b_kc ? g.K % 4 == 0 : g.N % 4 == 0);
-  // the farthest float of a slice's tile from its first, for 32-bit byte offsets
-  auto reach = [](bool kc, int64_t ld, int T) { return (kc ? T : 2048 / T) * ld + (kc ? 2048 / T : T); };
-  auto near = [&](int T) {
-    return std::max(reach(a_kc, g.lda, T), reach(b_kc, g.ldb, T)) < (int64_t(1) << 29);
-  };
-  const bool big = near(kBigT) && big_tiles(g);
-  const int load = !near(kSmallT) ? kLoadFar : vec ? kLoadVec : kLoadWord;
+  const bool big = near_tiles(g, kBigT) && big_tiles(g);
+  const int load = load_of(g);
 #define GS_GEMM_ROW(L, T, V) {gemm_kernel<L, T, V, false>, gemm_kernel<L, T, V, L != kGemmNN>}
 #define GS_GEMM_LAYOUT(L) \
   {GS_GEMM_ROW(L, kSmallT, kLoadVec), GS_GEMM_ROW(L, kSmallT, kLoadWord), GS_GEMM_ROW(L, kSmallT, kLoadFar), \

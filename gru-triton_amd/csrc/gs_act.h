@@ -1,4 +1,5 @@
-// The linear operator's activations, their derivatives, and what follows a product's sums.
+// The linear operator's activations, their derivatives, what follows a product's sums, and
+// sums over columns.
 #pragma once
 
 #include "gs_host.h"
@@ -92,6 +93,37 @@ __device__ __forceinline__ void act_slopes(float (&x)[N], int act) {
 #pragma unroll
     for (int v = 0; v < N; ++v) x[v] = act_slope<decltype(A)::value>(x[v]);
   });
+}
+
+// dst[e] = sum over parts of src[part * n + e], rounded to the tensor's type.
+struct ColumnSums {
+  void* dst = nullptr;
+  const float* src = nullptr;
+  int n = 0, parts = 0;
+};
+
+// Workgroup `group` of 256 threads takes 16 columns, its 16 part lanes every 16th part,
+// joined through LDS in order.
+template <typename T>
+__device__ __forceinline__ void sum_columns(const ColumnSums& p, int group, float (*red)[17]) {
+  const int c = threadIdx.x & 15, l = threadIdx.x >> 4, e = group * 16 + c;
+  float s = 0.0f;
+  if (e < p.n) {
+    for (int k0 = l; k0 < p.parts; k0 += 16 * 8) {  // eight loads in flight
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = k0 + 16 * u < p.parts ? p.src[(int64_t)(k0 + 16 * u) * p.n + e] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += x[u];
+    }
+  }
+  red[l][c] = s;
+  __syncthreads();
+  if (l == 0 && e < p.n) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += red[k][c];
+    static_cast<T*>(p.dst)[e] = (T)s;
+  }
 }
 
 }  // namespace gs

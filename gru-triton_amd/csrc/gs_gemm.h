@@ -42,6 +42,10 @@ struct GemmArgs {
 // Launches the product on `stream`. Every element of C (of every split) is written.
 int gemm_f32(const GemmArgs& g, hipStream_t stream, const char* who);
 
+// x (NN, unsplit) and w (TN) in small tiles, and the column sums (dst NULL: none), in one launch.
+bool gemm_pair_applies(const GemmArgs& x, const GemmArgs& w);
+int gemm_pair(const GemmArgs& x, const GemmArgs& w, const ColumnSums& c, hipStream_t stream, const char* who);
+
 // NT product of int8 operands on the int8 MFMA:
 //   C[i, j] = float(sum_k a[i lda + k] b[j ldb + k]) * (sa * b_scale[j]) (+ bias[j])
 // with a the levels of a per-tensor fake-quant of scale sa and b per-row codes

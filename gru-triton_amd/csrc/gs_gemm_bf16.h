@@ -71,37 +71,6 @@ __device__ __forceinline__ void granule_floats(const Granule& w, float (&x)[8]) 
   }
 }
 
-// dst[e] = sum over parts of src[part * n + e], rounded to the tensor's type.
-struct ColumnSums {
-  void* dst = nullptr;
-  const float* src = nullptr;
-  int n = 0, parts = 0;
-};
-
-// Workgroup `group` of 256 threads takes 16 columns, its 16 part lanes every 16th part,
-// joined through LDS in order.
-template <typename T>
-__device__ __forceinline__ void sum_columns(const ColumnSums& p, int group, float (*red)[17]) {
-  const int c = threadIdx.x & 15, l = threadIdx.x >> 4, e = group * 16 + c;
-  float s = 0.0f;
-  if (e < p.n) {
-    for (int k0 = l; k0 < p.parts; k0 += 16 * 8) {  // eight loads in flight
-      float x[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] = k0 + 16 * u < p.parts ? p.src[(int64_t)(k0 + 16 * u) * p.n + e] : 0.0f;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) s += x[u];
-    }
-  }
-  red[l][c] = s;
-  __syncthreads();
-  if (l == 0 && e < p.n) {
-#pragma unroll
-    for (int k = 1; k < 16; ++k) s += red[k][c];
-    static_cast<T*>(p.dst)[e] = (T)s;
-  }
-}
-
 // dx (NN) and dw (TN) of a backward whose tiles are all small, and the column sums, in one
 // launch (and the splits' sum of dw): M = 2048, N = 1024, K = 512 takes 12.6 + 9.3 + 3.9
 // us in three.

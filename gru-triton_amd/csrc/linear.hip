@@ -491,9 +491,14 @@ extern "C" int gs_linear_bwd(const gs_linear_bwd_args* a, hipStream_t stream) {
     w.K = (int)a->M;
     w.ksplit = plan.split_w;
     w.layout = kGemmTN;
-    if (a->dx && (rc = gemm_f32(x, stream, who))) return rc;
+    if (a->dx && a->dw && gemm_pair_applies(x, w)) {
+      if ((rc = gemm_pair(x, w, sums, stream, who))) return rc;
+      sums.dst = nullptr;
+    } else {
+      if (a->dx && (rc = gemm_f32(x, stream, who))) return rc;
+      if (a->dw && (rc = gemm_f32(w, stream, who))) return rc;
+    }
     if (a->dw) {
-      if ((rc = gemm_f32(w, stream, who))) return rc;
       if (plan.dw >= 0 && (rc = sum_partials(static_cast<float*>(a->dw), w.c, a->N * a->K, plan.split_w, a->N * a->K, stream, who)))
         return rc;
     }

@@ -627,12 +627,29 @@ struct Plan {
   int v, layout, blocks, tiles;
 };
 
+// Few channels leave the CUs with few waves, and a row's steps then go to more of them at
+// once; many channels have their waves without that, and each layer of it (LDS, barriers,
+// runs of 16 lanes in memory) costs. Measured in us, forward / backward, tanh, one layout
+// after the other on the same tensors:
+//   T, B, H            64 x 1       64 x 4       32 x 8       16 x 8       16 x 8 chained
+//   512, 128, 1024 f32 163 / 329    166 / 338    193 / 368    238 / 503
+//   256, 64, 2048 bf16 53 / 82      37 / 86      44 / 119     45 / 167
+//   8192, 32, 512 f32  687 / 1345   287 / 629    359 / 756    461 / 861    320 / 672
+//   512, 16, 512 f32   45 / 79      17 / 27      11 / 20      12 / 21
+//   1500, 11, 512 f32  125 / 226    42 / 69      21 / 37      25 / 46      23 / 37
+//   4096, 16, 512 f32  340 / 644    114 / 249    93 / 180     107 / 218    82 / 163
+//   4096, 4, 512 f32   335 / 607    109 / 181    46 / 75      30 / 51      22 / 37
+//   640, 8, 512 f32    54 / 98      20 / 32      11 / 17      8.3 / 16     11 / 16
+//   640, 4, 512 f32    55 / 98      20 / 31      9.8 / 15     7.2 / 11     9.3 / 10
+//   65536, 1, 1024 b.  11600/17400  3290 / 4960  1320 / 2080  781 / 1340   119 / 209
+//   8, 1024, 1024 bf16 12 / 21      29 / 54      115 / 298    232 / 611
+// The last row is the loop below: no layout whose tile is four times the row and more.
 Plan make_plan(int64_t T, int64_t B, int64_t H, int v, bool near) {
   // step groups side by side that give each CU eight waves
   const double want = 131072.0 / (double)(B * ((H + v - 1) / v));
-  int l = want <= 1.5 ? 0 : want <= 6 ? 1 : want <= 20 ? 2 : 3;
+  int l = want <= 1.5 ? 0 : want <= 10 ? 1 : want <= 28 ? 2 : 3;
   while (l > 0 && tile_of(l) >= 4 * T) --l;
-  if (l == 3 && want > 24 && T > 2 * tile_of(kChain)) l = kChain;
+  if (want > 12 && T > (want > 48 ? 2 : 4) * tile_of(kChain)) l = kChain;
   if (!near) l = l > 1 ? 1 : l;
   Plan r{v, l, 0, 0};
   const int lanes = kLayouts[l].lanes;
