@@ -3,11 +3,13 @@
 // forward in the epilogue.
 //
 // A workgroup computes a T x T tile of C, T = 256 with 8 waves (each 128 x 64 of it) or
-// 128 or 64 with 4 (each a quarter), K in slices of 32. The MFMA takes B's tile as its first operand, so that
-// a lane holds four consecutive columns of one row of C (D VGPR v of lane l:
-// C[l % 16][4 (l / 16) + v]) and stores them at once. While a slice's products run, the
-// next slice's operands are read from LDS into a second set of registers, so that after
-// the barrier that ends a slice the matrix pipe goes on at once.
+// 128 or 64 with 4 (each a quarter), K in slices of 32. The MFMA takes B's tile as its
+// first operand, so that a lane holds four consecutive columns of one row of C (D VGPR v
+// of lane l: C[l % 16][4 (l / 16) + v]) and stores them at once. While a slice's products
+// run, the next slice's operands are read from LDS into a second set of registers, so that
+// after the barrier that ends a slice the matrix pipe goes on at once. 8192 x 8192 x 8192
+// takes 840 us forward and 760 for either gradient (1.3 and 1.45 PFLOP/s), bound by the
+// matrix pipe.
 //
 // LDS layouts (16-byte granules, no padding):
 //   operand contiguous along k: row r is 4 granules of 8 k; granule c sits in slot
@@ -490,8 +492,8 @@ __global__ __launch_bounds__(256) void gemm_bf16_finish_kernel(GemmBf16Args g) {
 // x w^T for at most 16 MT rows of x, as in serving: what there is to do is to read w once.
 // A workgroup takes 16 columns; its 8 waves take K in turns of 32 and hold the operands
 // of kAhead turns straight from memory, without LDS; their sums are joined through LDS in
-// order. M = 8, N = 2048, K = 1024: 7.2 us in 64 x 64 tiles (32 workgroups, 32 slices one
-// after the other), 4.1 here.
+// order. M = 8, N = 2048, K = 1024: 4.1 us on the GPU, 1.0 TB/s of w, where an empty launch
+// takes 2.3; in 64 x 64 tiles (32 workgroups, 32 slices one after the other) 6.4.
 constexpr int kRowWaves = 8;
 template <int MT>
 __global__ __launch_bounds__(64 * kRowWaves) void gemm_bf16_rows_kernel(GemmBf16Args g) {
@@ -569,8 +571,17 @@ constexpr int kTileSizes[3] = {256, 128, 64};
 // Microseconds of a product with tile T and `split` splits of K, from runs on the chip:
 // a launch takes 3; a CU does a tile's slice in `slice` and its first loads and last
 // stores in `ends`, tile after tile; splits write their sums and a second launch reads
-// them. (M, N, K, layout; predicted and measured: 32768 x 2048 x 1024 NT T 256 138, 139;
-// 4096 x 1024 x 1024 NT T 128 13, 13; 2048 x 1024 x 512 NT T 64 7.3, 6.8, T 128 9.5, 8.8.)
+// them. Rows M, N, K of x w^T, dpre w and dpre^T x; measured (predicted) in us:
+//                         T = 256          T = 128       T = 64
+//   32768, 2048, 1024 fwd 141 (128)        162 (167)     241 (243)
+//   32768, 2048, 1024 dx  115 (114)        139 (145)     232 (225)
+//   32768, 2048, 1024 dw  118 (125), 8     127 (139), 4  241 (209)   and K in 8 or 4 splits
+//   4096, 1024, 1024 fwd  29 (34)          13.5 (13.2)   18 (18)
+//   2048, 1024, 512 fwd   18 (22)          9.0 (9.5)     7.3 (7.3)
+//   512, 4096, 4096 fwd   38 (45), 4       29 (28), 2    35 (30)
+// The largest tile runs x w^T of 32768 x 2048 x 1024 at 0.97 PFLOP/s with warm caches and at
+// 0.80 where y goes to memory (172 us): all CUs store their tiles at the same time, and no
+// registers are left to hold a tile back and store it during the next one's slices.
 double tile_us(int M, int N, int K, int T, int split) {
   const double slice = T == 256 ? 0.76 : T == 128 ? 0.235 : 0.1, ends = T == 256 ? 7.0 : T == 128 ? 2.7 : 0.55;
   const int64_t slices = ((K + split - 1) / split + BK - 1) / BK, per_cu = (tiles_of(M, N, T) * split + 255) / 256;
@@ -610,7 +621,15 @@ GemmBf16Fn kernel_of(int T, bool direct, bool part) {
 
 }  // namespace
 
-bool gemm_bf16_few_rows(int M) { return M <= 32; }
+// Rows of M at most 32 straight from memory, unless K is long (a wave's turns of it come one
+// after the other, where tiles split K) or w is wide (tiles read each of its lines once and
+// in order). Measured in us, straight and in tiles, w in cache:
+//   8, 2048, 1024    4.8  6.4   32, 2048, 1024  5.4  6.7   8, 1811, 1001  6.1 18.9
+//   8, 2048, 2048    5.4  7.1   32, 2048, 2048  7.7  8.0   32, 1001, 4003 31.0 17.8
+//   8, 2048, 4096    8.4  8.0   32, 2048, 4096 13.9  9.1
+//   8, 8192, 1024    5.4  6.4   32, 4096, 1024  5.2  6.7
+//   8, 16384, 1024   9.1  7.6   32, 8192, 1024  7.7  6.7
+bool gemm_bf16_few_rows(int M, int N, int K) { return M <= 32 && K <= 2048 && N <= (M <= 16 ? 8192 : 4096); }
 
 int gemm_bf16_pick_split(int M, int N, int K) {
   int best = 1;
@@ -661,7 +680,7 @@ constexpr int64_t kMostGroups = 1 << 22;
 int gemm_bf16(const GemmBf16Args& g, hipStream_t stream, const char* who) {
   const int rc = check(g, who);
   if (rc) return rc;
-  if (g.layout == kGemmNT && g.ksplit == 1 && gemm_bf16_few_rows(g.M)) {
+  if (g.layout == kGemmNT && g.ksplit == 1 && gemm_bf16_few_rows(g.M, g.N, g.K)) {
     hipLaunchKernelGGL(g.M <= 16 ? gemm_bf16_rows_kernel<1> : gemm_bf16_rows_kernel<2>, dim3((unsigned)((g.N + 15) / 16)),
                        dim3(64 * kRowWaves), 0, stream, g);
     GS_CHECK_HIP(hipGetLastError());

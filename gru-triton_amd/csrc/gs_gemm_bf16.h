@@ -25,7 +25,7 @@ struct GemmBf16Args {
 int gemm_bf16_pick_split(int M, int N, int K);
 // NT products of so few rows of A are read from memory straight into the matrix units: no
 // splits, no copies.
-bool gemm_bf16_few_rows(int M);
+bool gemm_bf16_few_rows(int M, int N, int K);
 int gemm_bf16(const GemmBf16Args& g, hipStream_t stream, const char* who);
 
 // Granules: eight consecutive bf16 of a row, at any alignment. Where a row ends inside

@@ -18,7 +18,15 @@
 // then runs its U steps from its own carry. Each input is read once, the state
 // between tiles stays in registers, and the next tile's loads are in flight
 // meanwhile. Sums and states are fp32; the order of every operation is fixed by
-// the sizes, so results are reproducible.
+// the sizes, so results are reproducible. With few channels and a long axis a workgroup
+// takes one tile instead, and tiles hand their states on through memory (see chain()).
+//
+// Bound by memory where there are enough waves: T 256, B 64, H 2048 in bf16 takes 37 us
+// forward and 86 backward, 5.4 and 4.7 TB/s where a copy reaches 5.2; T 512, B 16, H 512 in
+// fp32 11.4 and 19.5 (4.4, 5.2). The chained layout reaches 3.4 to 4.5: T 4096, B 8, H 1024
+// in bf16 44 and 92 us; T 65536, B 1, H 1024 117 and 209. What keeps it below a copy is the
+// start of each workgroup (its ticket, its loads and the wait for its carry, one after the
+// other), which six waves a SIMD only partly hide.
 #include "gs_mfma.h"
 
 namespace gs {
@@ -175,8 +183,9 @@ struct Place {
 // its tile's map as soon as it has it; every kLink-th publishes the state after its tile.
 // A tile's carry is then the last such state taken through the maps since, joined in order
 // before the state is there, so that results do not depend on timing, and the chain of
-// waits along the axis has one link in kLink tiles. Words are published with one 64-bit (map) or 32-bit (state) store and
-// are all ones before that; NaNs are stored in one form, which is not all ones.
+// waits along the axis has one link in kLink tiles. Words are published with one 64-bit
+// (map) or 32-bit (state) store and are all ones before that; NaNs are stored in one form,
+// which is not all ones.
 constexpr int kLink = 16;
 constexpr uint32_t kNaN = 0x7fc00000u, kNone32 = 0xffffffffu;
 constexpr uint64_t kNone64 = ~uint64_t(0);
@@ -581,7 +590,8 @@ __global__ __launch_bounds__(256) void glr_fill_kernel(u4v* p, int64_t n) {
   if (e < n) p[e] = u4v{kNone32, kNone32, kNone32, kNone32};
 }
 
-// One step for each row of a batch of requests, whose states are rows of a cache.
+// One step for each row of a batch of requests, whose states are rows of a cache: one lane a
+// channel, one launch. B 8, H 1024 in bf16 takes 2.3 us on the GPU, what an empty launch takes.
 struct StepParams {
   const void* gi;
   float* state;

@@ -125,6 +125,13 @@ def test_many_tiles(dev, shape, cut):
     _check(*args, "gelu", _call(*args, "gelu"))
 
 
+@pytest.mark.parametrize("shape", [(20, 4104, 33), (32, 4096, 40), (5, 8200, 16), (16, 8192, 16), (8, 40, 2056), (8, 40, 2048)],
+                         ids=str)
+def test_few_rows_of_wide_and_long_layers(dev, shape):
+    args = _inputs(dev, *shape, torch.bfloat16, seed=13)
+    _check(*args, "silu", _call(*args, "silu"))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_strides_and_alignment(dev, dtype):
     M, N, K = 70, 72, 64
