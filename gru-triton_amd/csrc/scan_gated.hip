@@ -18,7 +18,8 @@
 // then runs its U steps from its own carry. Each input is read once, the state
 // between tiles stays in registers, and the next tile's loads are in flight
 // meanwhile. Sums and states are fp32; the order of every operation is fixed by
-// the sizes, so results are reproducible. With few channels and a long axis a workgroup
+// the sizes, so results are reproducible. (An infinite state stays infinite step by step;
+// taken through a map whose a has underflowed to 0 it becomes NaN.) With few channels and a long axis a workgroup
 // takes one tile instead, and tiles hand their states on through memory (see chain()).
 //
 // Bound by memory where there are enough waves: T 256, B 64, H 2048 in bf16 takes 37 us
