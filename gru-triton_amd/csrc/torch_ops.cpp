@@ -8,8 +8,10 @@
 // the rest of the package.
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <string>
 #include <vector>
 
 #include "../../include/gruscan.h"
@@ -61,6 +63,23 @@ void check_on(const char* who, const char* name, const Tensor& t, const Tensor& 
 
 // Unit stride along the last dimension.
 Tensor unit(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+
+// A tensor written through its pointer counts as modified in place: autograd refuses graphs
+// that saved it before, and what the package keeps per version of a weight is found anew.
+void modified(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+
+// A backward's results. Where a graph of them is asked for (create_graph), it goes on to
+// `from`, which they were computed from, through an error for whoever asks for a second
+// derivative: without it that derivative would lack their terms and nobody would know.
+variable_list once(const char* who, variable_list grads, const variable_list& from) {
+  if (!torch::GradMode::is_enabled()) return grads;
+  const size_t n = grads.size();
+  grads.insert(grads.end(), from.begin(), from.end());
+  grads = torch::autograd::DelayedError(std::string(who) + ": second derivatives are not implemented",
+                                        (int64_t)grads.size())(std::move(grads));
+  grads.resize(n);
+  return grads;
+}
 
 Tensor scratch(int64_t bytes, const Tensor& like) {
   raise_for(bytes);
@@ -152,7 +171,7 @@ struct GlrFunction : torch::autograd::Function<GlrFunction> {
     a.scratch = ptr<void>(buf);
     a.scratch_bytes = buf.defined() ? buf.numel() : 0;
     raise_for(gs_glr_bwd(&a, on.stream));
-    return {dgi, dh0, Tensor(), Tensor(), Tensor()};
+    return once("gated_linear_scan", {dgi, dh0, Tensor(), Tensor(), Tensor()}, {gi, h0, grads[0], grads[1]});
   }
 };
 
@@ -230,6 +249,7 @@ Tensor gated_linear_step(const Tensor& gi_, const Tensor& state, const OptTensor
   a.activation = (int32_t)act;
   const On on(gi);
   raise_for(gs_glr_step(&a, on.stream));
+  modified(state);
   return out;
 }
 
@@ -305,7 +325,9 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     a.scratch = ptr<void>(buf);
     a.scratch_bytes = buf.defined() ? buf.numel() : 0;
     raise_for(gs_linear_bwd(&a, on.stream));
-    return {dx, dw, db, dres, Tensor()};
+    variable_list r = once("linear_act", {dx, dw, db, Tensor(), Tensor()}, {x, w, pre, grads[0]});
+    r[3] = dres;
+    return r;
   }
 };
 
@@ -352,6 +374,8 @@ Tensor linear_act(const Tensor& x, const Tensor& w, OptTensor bias, OptTensor re
 // ---- AdamW ---------------------------------------------------------------------------
 
 typedef std::vector<Tensor> Tensors;
+
+const Tensors* get(const std::optional<Tensors>& t) { return t.has_value() ? &*t : nullptr; }
 
 // One contiguous tensor of counts[i] elements for each parameter, of type `kind`, on ref's device.
 void check_list(const char* name, const Tensors& ts, const std::vector<int64_t>& counts, torch::ScalarType kind,
@@ -438,6 +462,9 @@ void adamw_step(const Tensors& params, Tensors grads, const Tensors& exp_avgs, c
   a.has_master = masters.has_value();
   const On on(ref);
   raise_for(gs_adamw_step(&a, on.stream));
+  for (const Tensors* ts : {&params, &exp_avgs, &exp_avg_sqs, get(masters), get(exp_avg_scales), get(exp_avg_sq_scales)})
+    if (ts != nullptr)
+      for (const Tensor& t : *ts) modified(t);
 }
 
 Tensor adamw_dequantize_state(const Tensor& codes, const Tensor& scales) {

@@ -29,7 +29,7 @@ def linear_act(
     """``act(x @ weight.T + bias) + residual`` for ``x`` [..., K], ``weight`` [N, K], ``bias``
     [N] and ``residual`` [..., N], all float32 or all bfloat16 on one GPU; returns [..., N] in
     that type, every sum in float32. ``activation``: "none", "relu", "gelu" (of erf), "silu",
-    "tanh" or "sigmoid". Differentiable in all four tensors; with an activation, a training
+    "tanh" or "sigmoid". Differentiable in all four tensors (once); with an activation, a training
     forward keeps its argument [..., N] in x's type."""
     try:
         act = _ACTIVATIONS[activation]

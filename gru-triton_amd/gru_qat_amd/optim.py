@@ -65,8 +65,11 @@ class AdamW(torch.optim.Optimizer):
     """AdamW whose step is ``adamw_step``: one launch for up to 48 parameters.
 
     ``state_bits`` 32 keeps float32 moments, 8 keeps codes of 8 bits with a float32 scale
-    per 256 elements (2 bytes an element instead of 8). bfloat16 parameters get float32
-    masters unless ``master_weights`` is off. ``step(grad_scale=...)`` multiplies the
+    per 256 elements (2 bytes an element instead of 8); an element whose gradients are
+    under four millionths of its block's largest keeps a second moment of 0 there, and an
+    ``eps`` of the size of such gradients keeps its updates small. bfloat16 parameters get float32
+    masters unless ``master_weights`` is off (taken at a parameter's first step; from then on
+    a parameter is its master's rounding, whatever else is written to it). ``step(grad_scale=...)`` multiplies the
     gradients by a device scalar (a clipping factor, an inverse loss scale); where that is
     not finite, parameters and moments stay as they are (the count of steps still advances:
     the host does not read the scalar)."""

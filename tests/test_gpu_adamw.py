@@ -13,6 +13,7 @@ import pytest
 import torch
 
 import gru_qat_amd as G
+from gru_qat_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -137,6 +138,34 @@ def test_many_tensors_and_steps(dev, bits):
         before = _clone(s)
         _run(s, step)
         _check(before, s, step)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_is_a_modification_in_place(dev, bits):
+    s = _make([300, 5], 6, pd=BF16, gd=BF16, bits=bits, master=True)
+    before = {k: [t._version for t in v] for k, v in s.items() if v is not None}
+    _run(s, 1)
+    for k, v in before.items():
+        assert all((t._version > was) == (k != "grads") for t, was in zip(s[k], v)), k
+
+    w = torch.nn.Parameter(torch.randn(4, 4, device=dev))
+    w.grad = torch.ones_like(w)
+    y = (w * w).sum()
+    G.AdamW([w], state_bits=bits).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_codes_of_a_weight_are_found_again_after_a_step(dev):
+    codes = torch.randint(-127, 128, (48, 16), device=dev)
+    codes[:, 0] = 127
+    w = torch.nn.Parameter(codes * (1 / 128))
+    first = _lib.weight_codes(w)
+    assert first is not None and torch.equal(first[0].float() * first[1][:, None], w.detach())
+    w.grad = torch.randn_like(w)
+    G.AdamW([w], lr=0.1).step()
+    after = _lib.weight_codes(w)
+    assert after is None or torch.equal(after[0].float() * after[1][:, None], w.detach())
 
 
 @pytest.mark.parametrize("bits", [32, 8])

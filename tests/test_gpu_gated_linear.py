@@ -266,8 +266,22 @@ def test_step_equals_a_scan_of_one(dev):
     gi = torch.randn(5, 80, device=dev)
     state = torch.randn(5, 40, device=dev)
     out, h = G.gated_linear_scan(gi[None], state)
+    version = state._version
     got = G.gated_linear_step(gi, state)
-    assert torch.equal(got, out[0]) and torch.equal(state, h)
+    assert torch.equal(got, out[0]) and torch.equal(state, h) and state._version > version
+
+
+def test_second_derivatives_are_refused(dev):
+    gi, h0, _, _, _ = _inputs(5, 2, 7, torch.float32, seed=31)
+    gi, h0 = gi.to(dev).requires_grad_(True), h0.to(dev).requires_grad_(True)
+    plain = torch.autograd.grad(G.gated_linear_scan(gi, h0)[0].sum(), (gi, h0))
+    graph = torch.autograd.grad(G.gated_linear_scan(gi, h0)[0].sum(), (gi, h0), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, graph))
+    with pytest.raises(RuntimeError, match="gated_linear_scan: second derivatives"):
+        torch.autograd.grad(graph[0].square().sum(), gi)
+    alone, = torch.autograd.grad(G.gated_linear_scan(gi)[1].sum(), gi, create_graph=True)
+    with pytest.raises(RuntimeError, match="gated_linear_scan: second derivatives"):
+        alone.sum().backward()
 
 
 def test_refusals(dev):

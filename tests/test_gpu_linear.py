@@ -206,6 +206,21 @@ def test_same_inputs_same_results(dev):
     assert all(torch.equal(s, t) for s, t in zip(a, b))
 
 
+def test_second_derivatives_are_refused(dev):
+    x, w, bias, res, _ = _inputs(dev, 6, 9, 5, torch.float32, seed=31)
+    leaves = [t.requires_grad_(True) for t in (x, w, bias, res)]
+    y = G.linear_act(x, w, bias, activation="silu", residual=res)
+    plain = torch.autograd.grad(y.sum(), leaves)
+    y = G.linear_act(x, w, bias, activation="silu", residual=res)
+    graph = torch.autograd.grad(y.sum(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, graph))
+    with pytest.raises(RuntimeError, match="linear_act: second derivatives"):
+        torch.autograd.grad(graph[0].square().sum(), w)
+    alone, = torch.autograd.grad(G.linear_act(x, w.detach()).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="linear_act: second derivatives"):
+        alone.sum().backward()
+
+
 def test_refusals(dev):
     x, w, bias, res, _ = _inputs(dev, 6, 5, 4, torch.float32, seed=16)
     f = G.linear_act
