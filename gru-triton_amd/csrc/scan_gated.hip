@@ -25,10 +25,10 @@
 //
 // Bound by memory where there are enough waves: T 256, B 64, H 2048 in bf16 takes 37 us
 // forward and 86 backward, 5.4 and 4.7 TB/s where a copy reaches 5.2; T 512, B 16, H 512 in
-// fp32 11.4 and 19.5 (4.4, 5.2). The chained layout reaches 3.4 to 4.5: T 4096, B 8, H 1024
-// in bf16 44 and 92 us; T 65536, B 1, H 1024 117 and 209. What keeps it below a copy is the
-// start of each workgroup (its ticket, its loads and the wait for its carry, one after the
-// other), which six waves a SIMD only partly hide.
+// fp32 11.4 and 19.5 (4.4, 5.2). The chained layouts reach 3.4 to 5.4: T 4096, B 8, H 1024
+// in bf16 44 and 85 us, T 65536, B 1, H 1024 113 and 191, in fp32 171 and 301. What keeps
+// them below a copy is the start of each workgroup (its ticket, its loads and the wait for
+// its carry, one after the other), which six waves a SIMD only partly hide.
 #include "gs_mfma.h"
 
 namespace gs {
@@ -196,11 +196,12 @@ constexpr int kMostPolls = 1 << 22;  // seconds; then NaN, so that a launch ends
 __device__ __forceinline__ uint32_t word_of(float x) { return x != x ? kNaN : __float_as_uint(x); }
 
 // wave 0 of a workgroup: the carry of its tile, from the map `m` of the tile (every lane of
-// a channel holds it). The lane groups of a channel gather a quarter of the maps each.
+// a channel holds it). The lane groups of a channel gather a share of the maps each.
 template <int V, int LC, int NW, bool RESET>
 __device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>& at, const float* first, int64_t ld,
                                       const Map (&m)[V], float (&carry)[V], float (&last)[V]) {
-  static_assert(64 / LC == 4, "four lane groups share the maps");
+  constexpr int NG = 64 / LC, kShare = kLink / NG;
+  static_assert(NG > 1 && kShare % 4 == 0, "a lane group's share of the maps, in fours");
   const int64_t row = (int64_t)p.blocks * LC * V, plane = (int64_t)p.B * row;
   const int s = at.tile, from = s & ~(kLink - 1), count = s - from;
   const int64_t c0 = (int64_t)at.b * row + (int64_t)at.j;
@@ -212,7 +213,6 @@ __device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>
                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   // the maps of this lane group, four at a time
-  constexpr int kShare = kLink / 4;
   const uint64_t* src = p.maps + (from + kShare * at.lg) * plane + c0;
   const int mine = count - kShare * at.lg;
   Map f[V];
@@ -250,7 +250,7 @@ __device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>
   for (int v = 0; v < V; ++v) {
     all[v] = Map{__shfl(f[v].a, at.lc), __shfl(f[v].b, at.lc)};
 #pragma unroll
-    for (int g = 1; g < 4; ++g) all[v] = then<RESET>(all[v], Map{__shfl(f[v].a, g * LC + at.lc), __shfl(f[v].b, g * LC + at.lc)});
+    for (int g = 1; g < NG; ++g) all[v] = then<RESET>(all[v], Map{__shfl(f[v].a, g * LC + at.lc), __shfl(f[v].b, g * LC + at.lc)});
     past[v] = then<RESET>(all[v], m[v]);
   }
   uint32_t h[V];
@@ -631,8 +631,8 @@ struct LayoutOf {
   int lanes, waves;
   bool chain;
 };
-constexpr LayoutOf kLayouts[] = {{64, 1, false}, {64, 4, false}, {32, 8, false}, {16, 8, false}, {16, 8, true}};
-constexpr int kChain = 4;
+constexpr LayoutOf kLayouts[] = {{64, 1, false}, {64, 4, false}, {32, 8, false}, {16, 8, false}, {16, 8, true}, {32, 8, true}};
+constexpr int kChain = 4, kWideChain = 5;
 constexpr int tile_of(int layout) { return kSteps * (64 / kLayouts[layout].lanes) * kLayouts[layout].waves; }
 
 struct Plan {
@@ -656,12 +656,20 @@ struct Plan {
 //   65536, 1, 1024 b.  11600/17400  3290 / 4960  1320 / 2080  781 / 1340   119 / 209
 //   8, 1024, 1024 bf16 12 / 21      29 / 54      115 / 298    232 / 611
 // The last row is the loop below: no layout whose tile is four times the row and more.
-Plan make_plan(int64_t T, int64_t B, int64_t H, int v, bool near) {
+// Chained tiles of 32 lanes have whole cache lines of a step but half as many steps; they
+// pay where the lines are many (backwards, and in fp32) and so are the channels:
+//   T, B, H                 16 x 8 chained   32 x 8 chained
+//   65536, 1, 1024 bf16     113 / 204        119 / 191
+//   4096, 8, 1024 bf16      44 / 93          48 / 86
+//   65536, 1, 1024 f32      178 / 357        171 / 303
+//   4096, 16, 512 f32       83 / 166         79 / 149
+//   40000, 1, 333 f32       49 / 106         54 / 108
+Plan make_plan(int64_t T, int64_t B, int64_t H, int v, bool near, bool lines) {
   // step groups side by side that give each CU eight waves
   const double want = 131072.0 / (double)(B * ((H + v - 1) / v));
   int l = want <= 1.5 ? 0 : want <= 10 ? 1 : want <= 28 ? 2 : 3;
   while (l > 0 && tile_of(l) >= 4 * T) --l;
-  if (want > 12 && T > (want > 48 ? 2 : 4) * tile_of(kChain)) l = kChain;
+  if (want > 12 && T > (want > 48 ? 2 : 4) * tile_of(kChain)) l = lines && want <= 256 ? kWideChain : kChain;
   if (!near) l = l > 1 ? 1 : l;
   Plan r{v, l, 0, 0};
   const int lanes = kLayouts[l].lanes;
@@ -704,6 +712,12 @@ bool lanes_reach(int64_t st, int64_t H, int size) {
   return st < (int64_t(1) << 40) && (3 * kSteps * st + 2 * H + 64) * size < (int64_t(1) << 31);
 }
 
+// Which scans the wide chain is for (make_plan's `lines`).
+template <typename T>
+constexpr bool many_lines(bool back) {
+  return back || sizeof(T) == 4;
+}
+
 typedef void (*GlrFn)(GlrParams);
 template <typename T, int V, int L, bool BACK, bool TANH>
 GlrFn kernel_at(bool reset) {
@@ -716,12 +730,14 @@ GlrFn kernel_at(bool reset) {
 }
 template <typename T, int V, bool BACK, bool TANH>
 GlrFn kernel_in(int layout, bool reset) {
+  if constexpr (many_lines<T>(BACK))
+    if (layout == kWideChain) return kernel_at<T, V, kWideChain, BACK, TANH>(reset);
   switch (layout) {
     case 0: return kernel_at<T, V, 0, BACK, TANH>(reset);
     case 1: return kernel_at<T, V, 1, BACK, TANH>(reset);
     case 2: return kernel_at<T, V, 2, BACK, TANH>(reset);
     case 3: return kernel_at<T, V, 3, BACK, TANH>(reset);
-    default: return kernel_at<T, V, 4, BACK, TANH>(reset);
+    default: return kernel_at<T, V, kChain, BACK, TANH>(reset);
   }
 }
 template <typename T, int V>
@@ -739,7 +755,9 @@ struct Strided {
   int64_t st, sb;
 };
 
-Plan plan_of(int dtype, int64_t T, int64_t B, int64_t H, const Strided* t, int count, int64_t sr_t) {
+bool lines_of(int dtype, bool back) { return dtype == GS_DTYPE_F32 ? many_lines<float>(back) : many_lines<__bf16>(back); }
+
+Plan plan_of(int dtype, bool back, int64_t T, int64_t B, int64_t H, const Strided* t, int count, int64_t sr_t) {
   const int size = dtype == GS_DTYPE_F32 ? 4 : 2;
   int v = dtype == GS_DTYPE_F32 || H % 2 ? 1 : 2;
   bool near = true;
@@ -747,7 +765,7 @@ Plan plan_of(int dtype, int64_t T, int64_t B, int64_t H, const Strided* t, int c
     if (v == 2 && (!unit_aligned(t[i].p, 4) || t[i].st % 2 || t[i].sb % 2)) v = 1;
     near = near && lanes_reach(t[i].st, H, size);
   }
-  return make_plan(T, B, H, v, near && lanes_reach(sr_t, 0, 1));
+  return make_plan(T, B, H, v, near && lanes_reach(sr_t, 0, 1), lines_of(dtype, back));
 }
 
 // The chain's scratch: eight counters on lines of their own, the maps, the states.
@@ -757,8 +775,8 @@ struct ChainBytes {
 };
 ChainBytes chain_bytes(const Plan& plan, int64_t B) {
   ChainBytes c;
-  if (plan.layout != kChain) return c;
-  const int64_t plane = B * plan.blocks * kLayouts[kChain].lanes * plan.v;
+  if (!kLayouts[plan.layout].chain) return c;
+  const int64_t plane = B * plan.blocks * kLayouts[plan.layout].lanes * plan.v;
   c.maps = kTicketBytes;
   c.states = c.maps + align256(plan.tiles * plane * 8);
   c.total = c.states + align256((plan.tiles / kLink + 1) * plane * 4);
@@ -766,9 +784,10 @@ ChainBytes chain_bytes(const Plan& plan, int64_t B) {
 }
 
 // What a call of these sizes may need, whatever its pointers and strides.
-int64_t scratch_most(int dtype, int64_t T, int64_t B, int64_t H) {
-  const int64_t one = chain_bytes(make_plan(T, B, H, 1, true), B).total;
-  return dtype == GS_DTYPE_F32 ? one : std::max(one, chain_bytes(make_plan(T, B, H, 2, true), B).total);
+int64_t scratch_most(int dtype, bool back, int64_t T, int64_t B, int64_t H) {
+  const bool lines = lines_of(dtype, back);
+  const int64_t one = chain_bytes(make_plan(T, B, H, 1, true, lines), B).total;
+  return dtype == GS_DTYPE_F32 ? one : std::max(one, chain_bytes(make_plan(T, B, H, 2, true, lines), B).total);
 }
 
 int launch(const char* who, int dtype, const Plan& plan, GlrParams& p, bool back, bool tanh, void* scratch,
@@ -825,13 +844,13 @@ int check_bwd(const gs_glr_bwd_args* a, const char* who) {
 
 Plan plan_fwd(const gs_glr_args* a) {
   const Strided t[2] = {{a->gi, a->sg_t, a->sg_b}, {a->out, a->so_t, a->so_b}};
-  return plan_of(a->dtype, a->T, a->B, a->H, t, 2, a->sr_t);
+  return plan_of(a->dtype, false, a->T, a->B, a->H, t, 2, a->sr_t);
 }
 
 Plan plan_bwd(const gs_glr_bwd_args* a) {
   const Strided t[4] = {{a->gi, a->sg_t, a->sg_b}, {a->out, a->so_t, a->so_b}, {a->dout, a->sd_t, a->sd_b},
                         {a->dgi, a->sdg_t, a->sdg_b}};
-  return plan_of(a->dtype, a->T, a->B, a->H, t, 4, a->sr_t);
+  return plan_of(a->dtype, true, a->T, a->B, a->H, t, 4, a->sr_t);
 }
 
 }  // namespace
@@ -842,7 +861,7 @@ using namespace gs;
 extern "C" int64_t gs_glr_scratch_bytes(const gs_glr_args* a) {
   clear_error();
   const int rc = check_fwd(a, "gs_glr_scratch_bytes");
-  return rc ? rc : scratch_most(a->dtype, a->T, a->B, a->H);
+  return rc ? rc : scratch_most(a->dtype, false, a->T, a->B, a->H);
 }
 
 extern "C" int gs_glr_fwd(const gs_glr_args* a, hipStream_t stream) {
@@ -873,7 +892,7 @@ extern "C" int gs_glr_fwd(const gs_glr_args* a, hipStream_t stream) {
 extern "C" int64_t gs_glr_bwd_scratch_bytes(const gs_glr_bwd_args* a) {
   clear_error();
   const int rc = check_bwd(a, "gs_glr_bwd_scratch_bytes");
-  return rc ? rc : scratch_most(a->dtype, a->T, a->B, a->H);
+  return rc ? rc : scratch_most(a->dtype, true, a->T, a->B, a->H);
 }
 
 extern "C" int gs_glr_bwd(const gs_glr_bwd_args* a, hipStream_t stream) {

@@ -262,6 +262,13 @@ def test_step(dev, H, act, dtype):
     assert torch.equal(cache[rest].cpu(), before[rest])
 
 
+# long axes of many channels: a tile of 128 steps by 32 lanes, the last one of each partly filled
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1025, 8, 65), (1100, 4, 258), (2100, 9, 130), (2200, 8, 135)], ids=str)
+def test_long_axes_of_many_channels(dev, shape, dtype):
+    _check(dev, *_inputs(*shape, dtype, seed=sum(shape), p_reset=0.01 if shape[0] % 2 else 0.0), "tanh")
+
+
 def test_step_equals_a_scan_of_one(dev):
     gi = torch.randn(5, 80, device=dev)
     state = torch.randn(5, 40, device=dev)
