@@ -18,10 +18,8 @@
 // then runs its U steps from its own carry. Each input is read once, the state
 // between tiles stays in registers, and the next tile's loads are in flight
 // meanwhile. Sums and states are fp32; the order of every operation is fixed by
-// the sizes, so results are reproducible. (An infinite state stays infinite step by step;
-// taken through a map whose a has underflowed to 0 it becomes NaN.) With few channels and
-// a long axis a workgroup takes one tile instead, and tiles hand their states on through
-// memory (see chain()).
+// the sizes, so results are reproducible. With few channels and a long axis a workgroup
+// takes one tile instead, and tiles hand their states on through memory (see chain()).
 //
 // Bound by memory where there are enough waves: T 256, B 64, H 2048 in bf16 takes 37 us
 // forward and 86 backward, 5.4 and 4.7 TB/s where a copy reaches 5.2; T 512, B 16, H 512 in
@@ -72,6 +70,16 @@ template <bool RESET>
 __device__ __forceinline__ Map then(const Map& first, const Map& second) {
   Map r{second.a * first.a, __builtin_fmaf(second.a, first.b, second.b)};
   if (RESET && (int)__float_as_uint(second.a) < 0) r = second;
+  return r;
+}
+// A map of many steps keeps a > 0: a product of z under the smallest float is held as that,
+// so that an infinite state, which no step takes away, does not become 0 x infinity (a finite
+// one moves by less than 1.5e-45 of its size). As unsigned words -0 and NaNs are above it.
+__device__ __forceinline__ float span_a(float a) { return __uint_as_float(max(__float_as_uint(a), 1u)); }
+template <bool RESET>
+__device__ __forceinline__ Map then_span(const Map& first, const Map& second) {
+  Map r = then<RESET>(first, second);
+  r.a = span_a(r.a);
   return r;
 }
 
@@ -139,6 +147,13 @@ template <bool TANH>
 __device__ __forceinline__ void gates(float gz, float gn, float& z, float& n) {
   z = sigmoid(gz);
   n = TANH ? tanh_near(gn) : gn;
+}
+// (1 - z) n in one rounding. The fma makes infinity - infinity of an infinite n (there is none
+// after tanh), which stays infinite, also where z has rounded to 1; a NaN in z passes.
+template <bool TANH>
+__device__ __forceinline__ float candidate(float z, float n) {
+  const float b = __builtin_fmaf(-z, n, n);
+  return !TANH && __builtin_isinf(n) ? (1.0f + z) * n : b;
 }
 
 // Where a lane is: its channels, its step group, and its wave (uniform).
@@ -241,7 +256,7 @@ __device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>
       for (int k = 0; k < 4; ++k) {
         if (w[k][v] == kNone64) w[k][v] = (uint64_t)kNaN << 32 | kNaN;
         const Map x{__uint_as_float((uint32_t)w[k][v]), __uint_as_float((uint32_t)(w[k][v] >> 32))};
-        if (k0 + k < mine) f[v] = then<RESET>(f[v], x);
+        if (k0 + k < mine) f[v] = then_span<RESET>(f[v], x);
       }
   }
   // all of them in order, and this tile's: what is left once the state is there is one step
@@ -250,8 +265,8 @@ __device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>
   for (int v = 0; v < V; ++v) {
     all[v] = Map{__shfl(f[v].a, at.lc), __shfl(f[v].b, at.lc)};
 #pragma unroll
-    for (int g = 1; g < NG; ++g) all[v] = then<RESET>(all[v], Map{__shfl(f[v].a, g * LC + at.lc), __shfl(f[v].b, g * LC + at.lc)});
-    past[v] = then<RESET>(all[v], m[v]);
+    for (int g = 1; g < NG; ++g) all[v] = then_span<RESET>(all[v], Map{__shfl(f[v].a, g * LC + at.lc), __shfl(f[v].b, g * LC + at.lc)});
+    past[v] = then_span<RESET>(all[v], m[v]);
   }
   uint32_t h[V];
   if (from) {
@@ -294,13 +309,15 @@ __device__ __forceinline__ void enter(const GlrParams& p, const Place<V, LC, NW>
                                       float (&h)[V], Map (*lds)[LC * V], const float* first, int64_t ld) {
   constexpr int NG = 64 / LC;
   Map before[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) m[v].a = span_a(m[v].a);
   if constexpr (NG > 1) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
 #pragma unroll
       for (int d = 1; d < NG; d *= 2) {
         const Map o{__shfl_up(m[v].a, d * LC), __shfl_up(m[v].b, d * LC)};
-        if (at.lg >= d) m[v] = then<RESET>(o, m[v]);
+        if (at.lg >= d) m[v] = then_span<RESET>(o, m[v]);
       }
       before[v] = Map{__shfl_up(m[v].a, LC), __shfl_up(m[v].b, LC)};
       if (at.lg == 0) before[v] = Map{1.0f, 0.0f};
@@ -328,7 +345,7 @@ __device__ __forceinline__ void enter(const GlrParams& p, const Place<V, LC, NW>
         for (int v = 0; v < V; ++v) {
           whole[v] = lds[0][at.lc * V + v];
 #pragma unroll
-          for (int w = 1; w < NW; ++w) whole[v] = then<RESET>(whole[v], lds[w][at.lc * V + v]);
+          for (int w = 1; w < NW; ++w) whole[v] = then_span<RESET>(whole[v], lds[w][at.lc * V + v]);
         }
         chain<V, LC, NW, RESET>(p, at, first, ld, whole, start, carry);
         if (at.lg == 0) {
@@ -431,7 +448,7 @@ __global__ __launch_bounds__(64 * NW, CHAIN ? 6 : 1) void glr_fwd_kernel(GlrPara
       for (int v = 0; v < V; ++v) {
         float z, n;
         gates<TANH>(gz[v], gn[v], z, n);
-        e[i][v] = Map{z, __builtin_fmaf(-z, n, n)};
+        e[i][v] = Map{z, candidate<TANH>(z, n)};
         if (RESET && s.r[i]) e[i][v].a = -0.0f;
         if (i >= rem) e[i][v] = Map{1.0f, 0.0f};
         m[v] = then<RESET>(m[v], e[i][v]);
@@ -617,7 +634,7 @@ __global__ __launch_bounds__(256) void glr_step_kernel(StepParams p) {
   float z, n;
   gates<TANH>((float)g[0], (float)g[p.H], z, n);
   float* s = p.state + slot * p.ss + j;
-  const float h = __builtin_fmaf(z, *s, __builtin_fmaf(-z, n, n));
+  const float h = __builtin_fmaf(z, *s, candidate<TANH>(z, n));
   *s = h;
   *o = (T)h;
 }

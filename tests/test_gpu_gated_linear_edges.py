@@ -1,0 +1,77 @@
+"""The gated linear recurrence where states, candidates or gradients are infinite, where
+tiles follow each other, and where chained tiles hand states on. Bounds are those of the
+operator's own tests."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import gru_qat_amd as G
+import test_gpu_gated_linear as scan
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+TYPES, IDS = [F32, BF16], ["f32", "bf16"]
+
+
+def _same_kind(got, want, what):
+    """NaN where the formula has NaN, each infinity where it has that one, finite elsewhere."""
+    got, want = got.detach().cpu().double(), want.double()
+    for name, f in (("NaN", torch.isnan), ("inf", torch.isposinf), ("-inf", torch.isneginf)):
+        assert torch.equal(f(got), f(want)), f"{what}: {name} at other places than in the formula"
+    return got.isfinite()
+
+
+# Each layout: a wave a row (float32), four waves, eight waves by 32 lanes (float32, bfloat16) and by 16, and
+# tiles chained in two widths.
+INFINITE = [(20, 700, 130), (100, 20, 701), (300, 20, 300), (150, 20, 601), (300, 2, 40), (1300, 1, 40), (1200, 8, 140)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("shape", INFINITE, ids=str)
+def test_infinite_candidates_and_states(dev, shape, dtype):
+    """(1 - z) n is infinite with n, and a state that is infinite stays so, also over spans of steps whose z
+    multiply to less than the smallest float."""
+    T, B, H = shape
+    gi, h0, _, dout, dh = scan._inputs(T, B, H, dtype, seed=T)
+    inf = float("inf")
+    gi[3, 0, H], gi[5, 0, H + 1], gi[T - 4, 0, H + 2], h0[1 % B, 0] = inf, -inf, inf, inf
+    gi[9, 0, H + 1] = -inf  # the same infinity again
+    gi[11, 0, H] = -inf     # the other one: NaN from here on
+    x, s = gi.to(dev).requires_grad_(True), h0.to(dev).requires_grad_(True)
+    out, last = G.gated_linear_scan(x, s, activation="identity")
+    dgi, dh0 = torch.autograd.grad((out, last), (x, s), (dout.to(dev), dh.to(dev)))
+    (o, e), (hl, _), (dg, _), (d0, _), _, _ = scan._oracle(gi, h0, None, "identity", dout, dh)
+    ok = _same_kind(out, o, "out")
+    _same_kind(last, hl, "h_T")
+    _same_kind(dgi, dg, "dgi")
+    _same_kind(dh0, d0, "dh0")
+    u = 2.0 ** -8 if dtype == BF16 else 0.0
+    assert ((out.detach().cpu().double() - o).abs()[ok] <= (e * (1 + u) + u * o.abs())[ok]).all()
+
+
+@pytest.mark.parametrize("shape", INFINITE, ids=str)
+def test_infinite_gradients(dev, shape):
+    T, B, H = shape
+    gi, h0, _, dout, dh = scan._inputs(T, B, H, F32, seed=T + 1)
+    dout[T - 3, 0, 0], dh[0, 1] = float("inf"), -float("inf")
+    x, s = gi.to(dev).requires_grad_(True), h0.to(dev).requires_grad_(True)
+    out, last = G.gated_linear_scan(x, s)
+    dgi, dh0 = torch.autograd.grad((out, last), (x, s), (dout.to(dev), dh.to(dev)))
+    _, _, (dg, _), (d0, _), _, _ = scan._oracle(gi, h0, None, "tanh", dout, dh)
+    _same_kind(dgi, dg, "dgi")
+    _same_kind(dh0, d0, "dh0")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_a_step_with_infinities(dev, dtype):
+    inf = float("inf")
+    gi = torch.tensor([[0.5, 0.5, 20.0, 0.5, 0.5, inf, -inf, inf, -inf, 0.25]]).to(dtype)
+    state = torch.tensor([[1.0, 2.0, 3.0, inf, inf]])
+    want, _ = scan._oracle(gi[None], state, None, "identity")
+    cache = state.to(dev)
+    out = G.gated_linear_step(gi.to(dev), cache, activation="identity")
+    _same_kind(out, want[0][0], "out")
+    _same_kind(cache, want[0][0], "state")
