@@ -55,10 +55,18 @@ int dtype_of(const char* who, const char* name, const Tensor& t) {
   return GS_DTYPE_BF16;
 }
 
+// A tangent of forward-mode differentiation would be lost without a word: the kernels read values
+// alone, and a dual tensor need not require a gradient.
+void check_no_tangent(const char* who, const char* name, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), who, ": forward-mode derivatives are not implemented; ", name,
+                              " has a tangent");
+}
+
 void check_on(const char* who, const char* name, const Tensor& t, const Tensor& ref) {
   TORCH_CHECK_VALUE(t.is_cuda(), who, ": ", name, " must be a CUDA (HIP) tensor; got ", t.device());
   TORCH_CHECK_VALUE(t.device() == ref.device(), who, ": all tensors must be on ", ref.device(), "; ", name, " is on ",
                     t.device());
+  check_no_tangent(who, name, t);
 }
 
 // Unit stride along the last dimension.
@@ -134,6 +142,8 @@ struct GlrFunction : torch::autograd::Function<GlrFunction> {
     const Tensor &gi = saved[0], &h0 = saved[1], &reset = saved[2], &out = saved[3];
     Tensor dout = grads[0], dh = grads[1];
     if (!dout.defined() && !dh.defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    if (dout.defined()) check_no_tangent("gated_linear_scan", "the gradient of out", dout);
+    if (dh.defined()) check_no_tangent("gated_linear_scan", "the gradient of h_T", dh);
     const int64_t T = out.size(0), B = out.size(1), H = out.size(2);
     dout = dout.defined() ? unit(dout) : torch::zeros({H}, out.options()).expand({T, B, H});
     if (dh.defined()) dh = dh.contiguous();
@@ -301,6 +311,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = has_bias && ctx->needs_input_grad(2);
     const Tensor dres = (given & kHasResidual) && ctx->needs_input_grad(2 + has_bias) ? grads[0] : Tensor();
     if (!nx && !nw && !nb) return {Tensor(), Tensor(), Tensor(), dres, Tensor()};
+    check_no_tangent("linear_act", "the output's gradient", grads[0]);
     const Tensor dy = unit(grads[0]);
     gs_linear_bwd_args a{};
     a.M = x.size(0);
@@ -392,6 +403,7 @@ void check_list(const char* name, const Tensors& ts, const std::vector<int64_t>&
     TORCH_CHECK_VALUE(t.numel() == counts[i], who, ": ", name, "[", i, "] must have ", counts[i], " elements; got shape ",
                       t.sizes());
     TORCH_CHECK_VALUE(t.is_contiguous(), who, ": ", name, "[", i, "] must be contiguous; got strides ", t.strides());
+    check_no_tangent(who, name, t);
   }
 }
 
@@ -430,10 +442,12 @@ void adamw_step(const Tensors& params, Tensors grads, const Tensors& exp_avgs, c
                       ref.scalar_type());
     check_list("masters", *masters, counts, torch::kFloat, ref);
   }
-  if (grad_scale.has_value())
+  if (grad_scale.has_value()) {
     TORCH_CHECK_VALUE(grad_scale->device() == ref.device() && grad_scale->scalar_type() == torch::kFloat && grad_scale->numel() == 1,
                       who, ": grad_scale must be one float32 number on the parameters' device; got ",
                       grad_scale->scalar_type(), " ", grad_scale->sizes(), " on ", grad_scale->device());
+    check_no_tangent(who, "grad_scale", *grad_scale);
+  }
   std::vector<gs_adamw_tensor> table(params.size());
   for (size_t i = 0; i < params.size(); ++i) {
     gs_adamw_tensor& t = table[i];
@@ -478,6 +492,7 @@ Tensor adamw_dequantize_state(const Tensor& codes, const Tensor& scales) {
                         scales.numel() == (n + kStateBlock - 1) / kStateBlock,
                     who, ": scales must be ", (n + kStateBlock - 1) / kStateBlock, " contiguous float32 numbers on ",
                     codes.device(), "; got ", scales.scalar_type(), " ", scales.sizes(), " on ", scales.device());
+  check_no_tangent(who, "scales", scales);
   Tensor out = torch::empty(codes.sizes(), codes.options().dtype(torch::kFloat));
   const On on(codes);
   raise_for(gs_adamw_dequantize(codes.data_ptr(), ptr<float>(scales), out.data_ptr<float>(), n, second, on.stream));
