@@ -75,6 +75,11 @@ Tensor unit(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t :
 // A tensor written through its pointer counts as modified in place: autograd refuses graphs
 // that saved it before, and what the package keeps per version of a weight is found anew.
 void modified(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+// Asked before the launch: a tensor made in inference mode has no version to count outside it.
+void check_may_modify(const char* who, const char* name, const Tensor& t) {
+  TORCH_CHECK(!t.is_inference() || c10::InferenceMode::is_enabled(), who, ": ", name,
+              " was made in inference mode and cannot be updated in place outside it");
+}
 
 // A backward's results. Where a graph of them is asked for (create_graph), it goes on to
 // `from`, which they were computed from, through an error for whoever asks for a second
@@ -235,6 +240,7 @@ Tensor gated_linear_step(const Tensor& gi_, const Tensor& state, const OptTensor
                     ": state must be float32 [S, H] with H=", H, "; got ", state.scalar_type(), " ", state.sizes());
   TORCH_CHECK_VALUE(state.stride(1) == 1 || H == 1, who,
                     ": state is updated in place and must have unit stride along H; got strides ", state.strides());
+  check_may_modify(who, "state", state);
   Tensor slots;
   if (slots_.has_value()) {
     check_on(who, "slots", *slots_, gi_);
@@ -389,8 +395,9 @@ typedef std::vector<Tensor> Tensors;
 const Tensors* get(const std::optional<Tensors>& t) { return t.has_value() ? &*t : nullptr; }
 
 // One contiguous tensor of counts[i] elements for each parameter, of type `kind`, on ref's device.
+// `updated`: the step writes them.
 void check_list(const char* name, const Tensors& ts, const std::vector<int64_t>& counts, torch::ScalarType kind,
-                const Tensor& ref) {
+                const Tensor& ref, bool updated = true) {
   const char* who = "adamw_step";
   TORCH_CHECK_VALUE(ts.size() == counts.size(), who, ": ", ts.size(), " tensors in ", name, " for ", counts.size(),
                     " parameters");
@@ -404,6 +411,7 @@ void check_list(const char* name, const Tensors& ts, const std::vector<int64_t>&
                       t.sizes());
     TORCH_CHECK_VALUE(t.is_contiguous(), who, ": ", name, "[", i, "] must be contiguous; got strides ", t.strides());
     check_no_tangent(who, name, t);
+    if (updated) check_may_modify(who, name, t);
   }
 }
 
@@ -430,7 +438,7 @@ void adamw_step(const Tensors& params, Tensors grads, const Tensors& exp_avgs, c
   for (Tensor& g : grads)
     if (!g.is_contiguous()) g = g.contiguous();
   check_list("params", params, counts, ref.scalar_type(), ref);
-  check_list("grads", grads, counts, grads[0].scalar_type(), ref);
+  check_list("grads", grads, counts, grads[0].scalar_type(), ref, false);
   check_list("exp_avgs", exp_avgs, counts, bytes ? torch::kChar : torch::kFloat, ref);
   check_list("exp_avg_sqs", exp_avg_sqs, counts, bytes ? torch::kByte : torch::kFloat, ref);
   if (bytes) {

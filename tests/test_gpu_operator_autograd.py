@@ -67,3 +67,42 @@ def test_a_tangent_of_the_gradient_is_refused(dev, call):
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, x, dy, retain_graph=True)
     torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+def test_a_state_of_inference_mode_is_not_advanced_outside_it(dev):
+    gi = torch.randn(2, 6, device=dev)
+    with torch.inference_mode():
+        state = torch.randn(2, 3, device=dev)
+        before = state.clone()
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="state was made in inference mode"):
+            G.gated_linear_step(gi, state)
+        assert torch.equal(state, before)
+    with torch.inference_mode():
+        G.gated_linear_step(gi, state)
+        assert not torch.equal(state, before)
+
+
+@pytest.mark.parametrize("name", ["params", "exp_avgs", "exp_avg_sqs", "masters", "exp_avg_scales", "exp_avg_sq_scales"])
+def test_tensors_of_inference_mode_are_not_stepped_outside_it(dev, name):
+    def make(dtype, n=300):
+        return torch.ones(n, dtype=dtype, device=dev)
+
+    bf = torch.bfloat16
+    lists = dict(params=make(bf), grads=make(bf), exp_avgs=make(torch.int8), exp_avg_sqs=make(torch.uint8),
+                 masters=make(torch.float32), exp_avg_scales=make(torch.float32, 2), exp_avg_sq_scales=make(torch.float32, 2))
+    with torch.inference_mode():
+        lists[name] = lists[name].clone()
+        lists["grads"] = lists["grads"].clone()  # only read: one of inference mode is taken
+
+    def step():
+        G.adamw_step(*([lists[k]] for k in ("params", "grads", "exp_avgs", "exp_avg_sqs")), step=1, lr=0.1,
+                     **{k: [lists[k]] for k in ("masters", "exp_avg_scales", "exp_avg_sq_scales")})
+
+    before = {k: t.clone() for k, t in lists.items()}
+    with pytest.raises(RuntimeError, match=f"{name} was made in inference mode"):
+        step()
+    assert all(torch.equal(t, before[k]) for k, t in lists.items())
+    with torch.inference_mode():
+        step()
+    assert not torch.equal(lists["params"], before["params"])
