@@ -50,10 +50,12 @@ struct GlrParams {
   uint64_t* maps;      // chained layout only: see Chain
   uint32_t* states;
   uint32_t* tickets;
+  uint32_t* fault;     // host-visible word, or NULL: see chain()
   int64_t sg_t, sg_b, sh0_b, sr_t, sr_b, so_t, so_b, sd_t, sd_b, sdg_t, sdg_b;
   int T, B, H;
   int blocks;          // channel blocks per batch row
   int tiles;           // chained layout: tiles of the time axis
+  int polls;           // chained layout: bound of a workgroup's polls
 };
 
 // The map h -> a h + b. A reset is a = -0 (a is never negative otherwise; a NaN
@@ -185,10 +187,11 @@ struct Place {
       if (threadIdx.x == 0)
         *shared = (int)__hip_atomic_fetch_add(p.tickets + 32 * xcd, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __syncthreads();
-      const int ticket = __builtin_amdgcn_readfirstlane(*shared + 1);  // the counters start at -1
+      const int ticket = __builtin_amdgcn_readfirstlane(*shared + 1);  // the counters start at -1 (or past the first tile)
       const int per = gridDim.x / p.tiles >> 3;
       tile = ticket / per;
       at_group(p, xcd * per + ticket - tile * per);
+      if (tile >= p.tiles) ok = any = false;  // glr_fill_kernel's second start
     } else {
       at_group(p, xcd * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3));
     }
@@ -202,11 +205,13 @@ struct Place {
 // before the state is there, so that results do not depend on timing, and the chain of
 // waits along the axis has one link in kLink tiles. Words are published with one 64-bit
 // (map) or 32-bit (state) store and are all ones before that; NaNs are stored in one form,
-// which is not all ones.
+// which is not all ones. A workgroup whose polls run out takes NaN for what is not there and says
+// so in the host's fault word, so that a launch ends whatever happens and the host can tell why its
+// results are NaN.
 constexpr int kLink = 16;
 constexpr uint32_t kNaN = 0x7fc00000u, kNone32 = 0xffffffffu;
 constexpr uint64_t kNone64 = ~uint64_t(0);
-constexpr int kMostPolls = 1 << 22;  // seconds; then NaN, so that a launch ends whatever happens
+constexpr int kMostPolls = 1 << 22;  // seconds
 
 __device__ __forceinline__ uint32_t word_of(float x) { return x != x ? kNaN : __float_as_uint(x); }
 
@@ -247,7 +252,7 @@ __device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>
             w[k][v] = __hip_atomic_load(src + (k0 + k) * plane + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           ready = ready && w[k][v] != kNone64;
         }
-      if (__builtin_amdgcn_ballot_w64(!ready) == 0 || polls >= kMostPolls) break;
+      if (__builtin_amdgcn_ballot_w64(!ready) == 0 || polls >= p.polls) break;
       __builtin_amdgcn_s_sleep(1);
     }
 #pragma unroll
@@ -278,7 +283,7 @@ __device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>
         h[v] = __hip_atomic_load(state + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         ready = ready && h[v] != kNone32;
       }
-      if (__builtin_amdgcn_ballot_w64(!ready) == 0 || polls >= kMostPolls) break;
+      if (__builtin_amdgcn_ballot_w64(!ready) == 0 || polls >= p.polls) break;
     }
   } else {
 #pragma unroll
@@ -296,6 +301,8 @@ __device__ __forceinline__ void chain(const GlrParams& p, const Place<V, LC, NW>
                          __HIP_MEMORY_SCOPE_AGENT);
     carry[v] = apply<RESET>(all[v], c);
   }
+  if (polls >= p.polls && p.fault != nullptr && (threadIdx.x & 63) == 0)
+    __hip_atomic_store(p.fault, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
 // The maps before a lane's own steps: given each lane's map of its U steps,
@@ -603,10 +610,14 @@ __global__ __launch_bounds__(64 * NW) void glr_bwd_kernel(GlrParams p) {
   }
 }
 
-// All ones over the chain's words and counters.
-__global__ __launch_bounds__(256) void glr_fill_kernel(u4v* p, int64_t n) {
+// All ones over the chain's words and counters. `start`: the counters'
+// first value, before the first tile (-1) or the second, which then waits in vain.
+__global__ __launch_bounds__(256) void glr_fill_kernel(u4v* p, int64_t n, uint32_t start) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e < n) p[e] = u4v{kNone32, kNone32, kNone32, kNone32};
+  if (e >= n) return;
+  u4v w{kNone32, kNone32, kNone32, kNone32};
+  if (e < 8 * 8 && e % 8 == 0) w[0] = start;  // the counters' lines
+  p[e] = w;
 }
 
 // One step for each row of a batch of requests, whose states are rows of a cache: one lane a
@@ -808,13 +819,15 @@ int64_t scratch_most(int dtype, bool back, int64_t T, int64_t B, int64_t H) {
 }
 
 int launch(const char* who, int dtype, const Plan& plan, GlrParams& p, bool back, bool tanh, void* scratch,
-           int64_t scratch_bytes, hipStream_t stream) {
+           int64_t scratch_bytes, uint32_t* fault_mirror, int32_t poll_limit, hipStream_t stream) {
   const ChainBytes c = chain_bytes(plan, p.B);
   if (c.total > 0 && (scratch == nullptr || scratch_bytes < c.total || !unit_aligned(scratch, 256)))
     return set_error(GS_ERR_INVALID, "%s: scratch of %lld bytes, 256-byte aligned, required; got %lld at %p", who,
                      (long long)c.total, (long long)scratch_bytes, scratch);
   p.blocks = plan.blocks;
   p.tiles = plan.tiles;
+  p.fault = fault_mirror;
+  p.polls = poll_limit ? (int)std::min<int64_t>(std::abs((int64_t)poll_limit), INT32_MAX) : kMostPolls;
   const int threads = 64 * kLayouts[plan.layout].waves;
   int64_t groups = ((int64_t)p.B * plan.blocks + 7) / 8 * 8;
   if (c.total > 0) {
@@ -823,8 +836,9 @@ int launch(const char* who, int dtype, const Plan& plan, GlrParams& p, bool back
     p.maps = reinterpret_cast<uint64_t*>(static_cast<char*>(scratch) + c.maps);
     p.states = reinterpret_cast<uint32_t*>(static_cast<char*>(scratch) + c.states);
     const int64_t n = c.total / 16;
+    const uint32_t start = kNone32 + (poll_limit < 0 ? (uint32_t)(groups / plan.tiles / 8) : 0u);
     hipLaunchKernelGGL(glr_fill_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream,
-                       static_cast<u4v*>(scratch), n);
+                       static_cast<u4v*>(scratch), n, start);
     GS_CHECK_HIP(hipGetLastError());
   }
   if (groups * threads > UINT32_MAX)
@@ -903,7 +917,8 @@ extern "C" int gs_glr_fwd(const gs_glr_args* a, hipStream_t stream) {
   p.T = (int)a->T;
   p.B = (int)a->B;
   p.H = (int)a->H;
-  return launch(who, a->dtype, plan_fwd(a), p, false, a->activation == GS_ACT_TANH, a->scratch, a->scratch_bytes, stream);
+  return launch(who, a->dtype, plan_fwd(a), p, false, a->activation == GS_ACT_TANH, a->scratch, a->scratch_bytes,
+                a->fault_mirror, a->poll_limit, stream);
 }
 
 extern "C" int64_t gs_glr_bwd_scratch_bytes(const gs_glr_bwd_args* a) {
@@ -942,7 +957,8 @@ extern "C" int gs_glr_bwd(const gs_glr_bwd_args* a, hipStream_t stream) {
   p.T = (int)a->T;
   p.B = (int)a->B;
   p.H = (int)a->H;
-  return launch(who, a->dtype, plan_bwd(a), p, true, a->activation == GS_ACT_TANH, a->scratch, a->scratch_bytes, stream);
+  return launch(who, a->dtype, plan_bwd(a), p, true, a->activation == GS_ACT_TANH, a->scratch, a->scratch_bytes,
+                a->fault_mirror, a->poll_limit, stream);
 }
 
 extern "C" int gs_glr_step(const gs_glr_step_args* a, hipStream_t stream) {

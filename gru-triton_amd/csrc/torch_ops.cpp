@@ -6,11 +6,13 @@
 //
 // Errors are ValueError (device, dtype, shape, arguments) and RuntimeError (HIP), as in
 // the rest of the package.
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <string>
 #include <vector>
 
@@ -101,6 +103,31 @@ Tensor scratch(int64_t bytes, const Tensor& like) {
 
 // ---- gated linear recurrence ---------------------------------------------------------
 
+// The device's fault mirror, which a chained scan writes when a wait runs out (_lib.py holds
+// them all). The first scan that needs it makes it, unless it is being captured, where no host
+// memory may be allocated: that scan then reports by its NaNs alone.
+constexpr int kMostDevices = 64;
+std::atomic<uint32_t*> fault_words[kMostDevices];
+
+uint32_t* fault_word(int64_t device) {
+  if (device >= kMostDevices) return nullptr;
+  uint32_t* word = fault_words[device].load(std::memory_order_acquire);
+  if (word == nullptr && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) {
+    py::gil_scoped_acquire gil;
+    word = reinterpret_cast<uint32_t*>(
+        py::module_::import("gru_qat_amd._lib").attr("scan_fault_word")(device).cast<uintptr_t>());
+    fault_words[device].store(word, std::memory_order_release);
+  }
+  return word;
+}
+
+void raise_scan_fault(const char* who, int64_t device) {
+  const uint32_t* word = device < kMostDevices ? fault_words[device].load(std::memory_order_acquire) : nullptr;
+  if (word == nullptr || *static_cast<const volatile uint32_t*>(word) == 0) return;
+  py::gil_scoped_acquire gil;
+  py::module_::import("gru_qat_amd._lib").attr("raise_scan_fault")(device, who);
+}
+
 // out as [T, B, H], batch rows outermost in memory where gi's are (batch_first).
 std::tuple<Tensor, Tensor> glr_forward(const Tensor& gi, const Tensor& h0, const Tensor& reset, int64_t act,
                                        bool batch_first) {
@@ -129,6 +156,7 @@ std::tuple<Tensor, Tensor> glr_forward(const Tensor& gi, const Tensor& h0, const
   const Tensor buf = scratch(gs_glr_scratch_bytes(&a), gi);
   a.scratch = ptr<void>(buf);
   a.scratch_bytes = buf.defined() ? buf.numel() : 0;
+  if (buf.defined()) a.fault_mirror = fault_word(gi.get_device());
   raise_for(gs_glr_fwd(&a, on.stream));
   return {out, h_last};  // the caching allocator keeps buf until the stream's work is done
 }
@@ -185,6 +213,7 @@ struct GlrFunction : torch::autograd::Function<GlrFunction> {
     const Tensor buf = scratch(gs_glr_bwd_scratch_bytes(&a), gi);
     a.scratch = ptr<void>(buf);
     a.scratch_bytes = buf.defined() ? buf.numel() : 0;
+    if (buf.defined()) a.fault_mirror = fault_word(gi.get_device());
     raise_for(gs_glr_bwd(&a, on.stream));
     return once("gated_linear_scan", {dgi, dh0, Tensor(), Tensor(), Tensor()}, {gi, h0, grads[0], grads[1]});
   }
@@ -216,6 +245,7 @@ std::tuple<Tensor, Tensor> gated_linear_scan(Tensor gi, OptTensor h0, OptTensor 
                       reset->sizes());
   }
   gi = unit(gi);
+  raise_scan_fault(who, gi.get_device());
   Tensor out, h_last;
   if (grad && torch::GradMode::is_enabled()) {
     auto r = GlrFunction::apply(gi, h0, reset, act, batch_first);

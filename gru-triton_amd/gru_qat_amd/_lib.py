@@ -83,7 +83,7 @@ EXPORTS = (
     "gs_abi_version",
 )
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 QuantTuple = Optional[Tuple[float, int, int]]
 
@@ -376,6 +376,7 @@ class GsGlrArgs(ctypes.Structure):
         + [(k, ctypes.c_int64) for k in ("scratch_bytes", "T", "B", "H", "sg_t", "sg_b", "sh0_b", "sr_t", "sr_b",
                                          "so_t", "so_b")]
         + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
+        + [("fault_mirror", ctypes.c_void_p), ("poll_limit", ctypes.c_int32)]
     )
 
 
@@ -385,6 +386,7 @@ class GsGlrBwdArgs(ctypes.Structure):
         + [(k, ctypes.c_int64) for k in ("scratch_bytes", "T", "B", "H", "sg_t", "sg_b", "sh0_b", "sr_t", "sr_b",
                                          "so_t", "so_b", "sd_t", "sd_b", "sdg_t", "sdg_b")]
         + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
+        + [("fault_mirror", ctypes.c_void_p), ("poll_limit", ctypes.c_int32)]
     )
 
 
@@ -587,10 +589,12 @@ _mirrors: dict = {}
 class PersistentScanFault(RuntimeError):
     """A persistent scan launched earlier on this stream gave up a bounded
     wait: its workgroups were not all resident at once (another kernel held
-    the device's CUs), and its output is NaN from the failed step on."""
+    the device's CUs), and its output is NaN from the failed step on. Or a
+    gated linear scan did so, anywhere on this device, while one workgroup
+    waited for another's state (``scan_fault_word``)."""
 
 
-def _mirror(dev: torch.device, stream_handle: int):
+def _mirror(dev: torch.device, stream_handle: Any):
     key = (dev.index, stream_handle)
     m = _mirrors.get(key)
     if m is None:
@@ -604,9 +608,26 @@ def _raise_if_faulted(m, what: str) -> None:
         value = int(m[1][0])
         m[1][0] = 0
         raise PersistentScanFault(
-            f"{what}: a persistent scan launched earlier on this stream ran out of its bounded wait "
-            f"(fault value {value}); its output is invalid (NaN from the failed step on). Another kernel "
-            "holding the device's compute units while the scan ran is the usual cause.")
+            f"{what}: a persistent scan launched earlier on this stream (or a gated linear scan on this device) "
+            f"ran out of its bounded wait (fault value {value}); its output is invalid (NaN from the failed step "
+            "on). Another kernel holding the device's compute units while the scan ran is the usual cause.")
+
+
+# The gated linear scans of a device share one mirror: csrc/torch_ops.cpp asks for it once a
+# device, hands it to the kernels and looks at it before each scan.
+_GATED_SCAN = "gated linear scan"
+
+
+def scan_fault_word(index: int) -> int:
+    """The address of device ``index``'s fault mirror for the gated linear scan."""
+    return int(_mirror(torch.device("cuda", index), _GATED_SCAN)[0].data_ptr())
+
+
+def raise_scan_fault(index: int, what: str) -> None:
+    """Raises PersistentScanFault if a gated linear scan on device ``index`` gave up a wait."""
+    m = _mirrors.get((index, _GATED_SCAN))
+    if m is not None:
+        _raise_if_faulted(m, what)
 
 
 def check_faults(device: Optional[torch.device] = None) -> None:
@@ -684,7 +705,8 @@ def workspace(device: torch.device, stream_handle: int, nbytes: int, steps: int 
 
 def workspace_faults(device: Optional[torch.device] = None) -> int:
     """Read and clear the fault word of every cached workspace and its host
-    mirror (synchronises each stream); returns how many were set.
+    mirror, and the mirror of the gated linear scans (synchronises each stream,
+    and each device that ran such scans); returns how many were set.
 
     Nonzero means a persistent kernel ran out of its bounded wait and the output
     of that launch is invalid.
@@ -704,6 +726,12 @@ def workspace_faults(device: Optional[torch.device] = None) -> int:
         m = _mirrors.get((dev, stream_handle))
         if m is not None:
             m[1][0] = 0
+    for (dev, kind), m in list(_mirrors.items()):
+        if kind != _GATED_SCAN or (device is not None and device.index != dev):
+            continue
+        torch.cuda.synchronize(dev)
+        total += int(m[1][0] != 0)
+        m[1][0] = 0
     return total
 
 

@@ -38,7 +38,11 @@ def gated_linear_scan(
     ``batch_first``): ``out`` [T, B, H] in gi's type (float32 or bfloat16), ``h_T`` [B, H]
     in float32, with which a following call continues. ``h0`` [B, H] float32 (zeros when
     None). ``reset`` [T, B] bool starts a new sequence at a step: the state before it is
-    taken as zero, whatever it is. Differentiable in gi and h0 (once)."""
+    taken as zero, whatever it is. Differentiable in gi and h0 (once).
+
+    On few channels and a long axis workgroups wait for each other, for seconds at most; a wait
+    that runs out leaves NaN from there on, and the next scan on the device, or ``check_faults``,
+    raises ``PersistentScanFault``."""
     act = _activation("gated_linear_scan", activation)
     try:
         return (_lib._ops or _lib.ops()).gated_linear_scan(gi, h0, reset, act, batch_first)

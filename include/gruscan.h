@@ -62,7 +62,7 @@
 extern "C" {
 #endif
 
-#define GS_ABI_VERSION 6
+#define GS_ABI_VERSION 7
 
 #define GS_OK 0
 #define GS_ERR_INVALID (-1)  /* bad pointer, shape, stride or quant parameter (Python: ValueError) */
@@ -597,7 +597,14 @@ int gs_observe_scan(const gs_observe_args* args, hipStream_t stream);
  * so the sequence is a scan of B H independent channels. reset[t][b] != 0 takes
  * h_{t-1} as 0 at step t (a new sequence starts in the row), whatever it held.
  * gi, out, dout and dgi are of one type; states, their gradients and every sum
- * are fp32. No counterpart in the reference. */
+ * are fp32. No counterpart in the reference.
+ *
+ * With few channels and a long axis, workgroups hand states on along the axis. They wait
+ * only for workgroups that started before them, for a bounded number of polls (2^22,
+ * seconds). Where one runs out (the device held up), the launch still ends: its results are
+ * NaN from there along the axis (up to a reset), and a nonzero value is in *fault_mirror, which the
+ * caller clears. poll_limit is another bound; below 0 the bound is its magnitude and the launch leaves
+ * the axis' first workgroups out, for which the others then wait in vain: a rehearsal of this. */
 #define GS_DTYPE_F32 0
 #define GS_DTYPE_BF16 1
 #define GS_ACT_NONE 0
@@ -618,6 +625,8 @@ typedef struct gs_glr_args {
   int64_t T, B, H;
   int64_t sg_t, sg_b, sh0_b, sr_t, sr_b, so_t, so_b;
   int32_t dtype, activation;
+  uint32_t* fault_mirror; /* optional host-visible word (hipHostMalloc memory) or NULL    */
+  int32_t poll_limit;     /* 0 in production                                             */
 } gs_glr_args;
 
 int64_t gs_glr_scratch_bytes(const gs_glr_args* args);
@@ -639,6 +648,8 @@ typedef struct gs_glr_bwd_args {
   int64_t T, B, H;
   int64_t sg_t, sg_b, sh0_b, sr_t, sr_b, so_t, so_b, sd_t, sd_b, sdg_t, sdg_b;
   int32_t dtype, activation;
+  uint32_t* fault_mirror; /* as gs_glr_args                                              */
+  int32_t poll_limit;
 } gs_glr_bwd_args;
 
 int64_t gs_glr_bwd_scratch_bytes(const gs_glr_bwd_args* args);
