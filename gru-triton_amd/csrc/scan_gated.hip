@@ -667,6 +667,12 @@ struct Plan {
   int v, layout, blocks, tiles;
 };
 
+int64_t groups_of(const Plan& p, int64_t B) {
+  return (B * p.blocks + 7) / 8 * 8 * (kLayouts[p.layout].chain ? p.tiles : 1);
+}
+// A launch counts its threads in 32 bits.
+bool fits_launch(const Plan& p, int64_t B) { return groups_of(p, B) * 64 * kLayouts[p.layout].waves <= UINT32_MAX; }
+
 // Few channels leave the CUs with few waves, and a row's steps then go to more of them at
 // once; many channels have their waves without that, and each layer of it (LDS, barriers,
 // runs of 16 lanes in memory) costs. Measured in us, forward / backward, tanh, one layout
@@ -697,13 +703,18 @@ Plan make_plan(int64_t T, int64_t B, int64_t H, int v, bool near, bool lines) {
   const double want = 131072.0 / (double)(B * ((H + v - 1) / v));
   int l = want <= 1.5 ? 0 : want <= 10 ? 1 : want <= 28 ? 2 : 3;
   while (l > 0 && tile_of(l) >= 4 * T) --l;
-  if (want > 12 && T > (want > 48 ? 2 : 4) * tile_of(kChain)) l = lines && want <= 256 ? kWideChain : kChain;
-  if (!near) l = l > 1 ? 1 : l;
-  Plan r{v, l, 0, 0};
-  const int lanes = kLayouts[l].lanes;
-  r.blocks = (int)((H + lanes * v - 1) / (lanes * v));
-  r.tiles = (int)((T + tile_of(l) - 1) / tile_of(l));
-  return r;
+  auto plan = [&](int layout) {
+    Plan r{v, layout, 0, 0};
+    const int lanes = kLayouts[layout].lanes;
+    r.blocks = (int)((H + lanes * v - 1) / (lanes * v));
+    r.tiles = (int)((T + tile_of(layout) - 1) / tile_of(layout));
+    return r;
+  };
+  if (near && want > 12 && T > (want > 48 ? 2 : 4) * tile_of(kChain)) {
+    const Plan r = plan(lines && want <= 256 ? kWideChain : kChain);
+    if (fits_launch(r, B)) return r;  // from T = 2^28 on, tiles make more workgroups than a launch holds
+  }
+  return plan(near || l < 1 ? l : 1);
 }
 
 bool unit_aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
@@ -820,6 +831,8 @@ int64_t scratch_most(int dtype, bool back, int64_t T, int64_t B, int64_t H) {
 
 int launch(const char* who, int dtype, const Plan& plan, GlrParams& p, bool back, bool tanh, void* scratch,
            int64_t scratch_bytes, uint32_t* fault_mirror, int32_t poll_limit, hipStream_t stream) {
+  if (!fits_launch(plan, p.B))
+    return set_error(GS_ERR_INVALID, "%s: more workgroups than a launch holds (T=%d, B=%d, H=%d)", who, p.T, p.B, p.H);
   const ChainBytes c = chain_bytes(plan, p.B);
   if (c.total > 0 && (scratch == nullptr || scratch_bytes < c.total || !unit_aligned(scratch, 256)))
     return set_error(GS_ERR_INVALID, "%s: scratch of %lld bytes, 256-byte aligned, required; got %lld at %p", who,
@@ -829,9 +842,8 @@ int launch(const char* who, int dtype, const Plan& plan, GlrParams& p, bool back
   p.fault = fault_mirror;
   p.polls = poll_limit ? (int)std::min<int64_t>(std::abs((int64_t)poll_limit), INT32_MAX) : kMostPolls;
   const int threads = 64 * kLayouts[plan.layout].waves;
-  int64_t groups = ((int64_t)p.B * plan.blocks + 7) / 8 * 8;
+  const int64_t groups = groups_of(plan, p.B);
   if (c.total > 0) {
-    groups *= plan.tiles;
     p.tickets = static_cast<uint32_t*>(scratch);
     p.maps = reinterpret_cast<uint64_t*>(static_cast<char*>(scratch) + c.maps);
     p.states = reinterpret_cast<uint32_t*>(static_cast<char*>(scratch) + c.states);
@@ -841,8 +853,6 @@ int launch(const char* who, int dtype, const Plan& plan, GlrParams& p, bool back
                        static_cast<u4v*>(scratch), n, start);
     GS_CHECK_HIP(hipGetLastError());
   }
-  if (groups * threads > UINT32_MAX)
-    return set_error(GS_ERR_INVALID, "%s: too many channels (B=%d, H=%d)", who, p.B, p.H);
   hipLaunchKernelGGL(kernel_of(dtype, plan, back, tanh, p.reset != nullptr), dim3((unsigned)groups), dim3(threads), 0,
                      stream, p);
   GS_CHECK_HIP(hipGetLastError());

@@ -75,3 +75,18 @@ def test_a_step_with_infinities(dev, dtype):
     out = G.gated_linear_step(gi.to(dev), cache, activation="identity")
     _same_kind(out, want[0][0], "out")
     _same_kind(cache, want[0][0], "state")
+
+
+def test_an_axis_past_a_launch(dev):
+    """2^28 steps and more are walked, not chained: the end, after a reset, is that of the end alone."""
+    T, tail = (1 << 28) + 5, 700
+    gi, h0, _, _, _ = scan._inputs(tail, 1, 1, F32, seed=3)
+    long = torch.zeros(T, 1, 2, device=dev)
+    long[-tail:] = gi.to(dev)
+    reset = torch.zeros(T, 1, dtype=torch.bool, device=dev)
+    reset[-tail] = True
+    out, last = G.gated_linear_scan(long, torch.ones(1, 1, device=dev), reset=reset)
+    (o, e), (hl, el) = scan._oracle(gi, torch.zeros(1, 1), None, "tanh")
+    scan._near(out[-tail:], o, e, "out")
+    scan._near(last, hl, el, "h_T")
+    assert (out[:30, 0, 0].cpu() == 2.0 ** -torch.arange(1.0, 31)).all() and not out[200:-tail].any()
