@@ -9,6 +9,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
@@ -429,6 +430,8 @@ const Tensors* get(const std::optional<Tensors>& t) { return t.has_value() ? &*t
 void check_list(const char* name, const Tensors& ts, const std::vector<int64_t>& counts, torch::ScalarType kind,
                 const Tensor& ref, bool updated = true) {
   const char* who = "adamw_step";
+  // without a level of forward-mode differentiation no tensor has a tangent: asking each costs 30 ns where it is a view
+  const bool dual = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
   TORCH_CHECK_VALUE(ts.size() == counts.size(), who, ": ", ts.size(), " tensors in ", name, " for ", counts.size(),
                     " parameters");
   for (size_t i = 0; i < ts.size(); ++i) {
@@ -440,7 +443,7 @@ void check_list(const char* name, const Tensors& ts, const std::vector<int64_t>&
     TORCH_CHECK_VALUE(t.numel() == counts[i], who, ": ", name, "[", i, "] must have ", counts[i], " elements; got shape ",
                       t.sizes());
     TORCH_CHECK_VALUE(t.is_contiguous(), who, ": ", name, "[", i, "] must be contiguous; got strides ", t.strides());
-    check_no_tangent(who, name, t);
+    if (dual) check_no_tangent(who, name, t);
     if (updated) check_may_modify(who, name, t);
   }
 }
