@@ -132,7 +132,8 @@ __device__ __forceinline__ void values(uint32_t w, float scale, float (&x)[4]) {
 }
 
 // Codes of a wave's 256 elements, four to a lane, and their block's scale. The largest
-// magnitude is taken over bit patterns, in which NaN is above every number.
+// magnitude is taken over bit patterns, in which infinity and NaN are above every number;
+// with either the scale is NaN, and so is every value of the block.
 template <bool QUARTIC>
 __device__ __forceinline__ uint32_t codes(const float (&x)[4], float* scale) {
 #pragma clang fp contract(off)
@@ -141,7 +142,7 @@ __device__ __forceinline__ uint32_t codes(const float (&x)[4], float* scale) {
   for (int i = 0; i < 4; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
   for (int d = 32; d >= 1; d /= 2) most = max(most, (uint32_t)__shfl_xor((int)most, d));
-  const float A = __uint_as_float(most);
+  const float A = most >= 0x7f800000u ? __builtin_nanf("") : __uint_as_float(most);
   const bool none = A < kTiny;
   const float inv = none ? 0.0f : 1.0f / A;
   *scale = none ? 0.0f : A;
