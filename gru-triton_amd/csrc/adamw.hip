@@ -11,12 +11,24 @@
 // divides). A second moment under 1.5e-11 A is held as 0: the gradient of the step, which
 // enters in fp32, and eps then bound that element's update. A block of largest magnitude
 // under 2^-120 is held as zeros; one with a NaN or an infinity becomes NaN as a whole.
+//
+// Rounded to the nearest code, a moment loses every change of less than half a code while A
+// holds: at b2 = 0.999 a step takes 0.001 of v, a code is 4 / c of it, so v falls with A alone,
+// and rises only where g^2 passes about 9 v (c = 255) to 40 v (c = 50); at b1 = 0.9 m stays
+// where it is from |c| = 9 down. An element whose gradients grow from 0.1 to 0.4 of the block's
+// largest then moves 3.6 times as far as it should, one whose gradients end keeps moving, for
+// good. Unbiased rounding instead takes the upper of the two codes around a value
+// with the probability of where the value is between theirs, so that the moments are right on average over
+// steps. Its random words are a hash of the step, the tensor's place in the list and the
+// element, so results repeat. A second moment that is not 0 is then never rounded to 0 (a
+// first moment of one code over a second of none would be a step of any size): elements whose
+// gradients are under 1.5e-5 of the block's largest move less than they should.
 // Everything is computed in fp32 and rounds operation by operation in the order written
 // (no fused products, IEEE quotients and roots), so that codes depend on the inputs alone.
 //
 // Bound by memory: each word is read once and written once. 50 M bf16 parameters with fp32
-// masters and moments in 8 bits (18 bytes each, 0.91 GB) take 180 us, 5.0 TB/s where a copy
-// reaches 5.2; 4.7 M in fp32 (28 bytes, 132 MB, held by the last cache) 21 us. A table of
+// masters and moments in 8 bits (18 bytes each, 0.91 GB) take 188 us, 4.8 TB/s where a copy
+// reaches 5.2, and 225 with unbiased rounding, whose hashes and comparisons memory does not hide; 4.7 M in fp32 (28 bytes, 132 MB, held by the last cache) 21 us. A table of
 // tensors in the kernel's arguments makes one launch of up to 48 tensors, so that small
 // ones fill the device together and nothing is uploaded for the call.
 #include "gs_host.h"
@@ -32,8 +44,28 @@ constexpr int kTensors = 48;                 // tensors of one launch: their tab
 struct Table {
   gs_adamw_tensor t[kTensors];
   uint32_t first[kTensors];  // first workgroup of each tensor
+  uint32_t key[kTensors];    // of its random words in this step
   int count;
 };
+
+enum { kWords = 0, kNearest = 1, kUnbiased = 2 };  // moments in fp32, or codes and their rounding
+
+// A permutation of 32-bit words in which each bit of x changes each bit of the result half the
+// time (over 20000 words to within 0.003): shifts and products with the fractions of the roots of 2 and 3.
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x = (x ^ x >> 16) * 0x6a09e667u;
+  x = (x ^ x >> 15) * 0xbb67ae85u;
+  return x ^ x >> 16;
+}
+constexpr uint32_t kGolden = 0x9e3779b9u;  // 2^32 over the golden ratio: spreads consecutive numbers
+uint32_t key_of(int64_t step, int64_t tensor) {
+  return mix(mix((uint32_t)step) + (uint32_t)tensor * kGolden + (uint32_t)(step >> 32));
+}
+// Element e's word for the first moment; that of the second is it times kGolden.
+__device__ __forceinline__ uint32_t random_word(uint32_t key, int64_t e) {
+  return mix(key + (uint32_t)e * kGolden + (uint32_t)(e >> 32));
+}
+__device__ __forceinline__ float uniform(uint32_t w) { return (float)(w >> 8) * 0x1p-24f; }  // [0, 1)
 
 struct Scalars {
   float b1, c1m, b2, c2m, decay, root, eps, rate;  // b, 1 - b, 1 - lr wd, 1 / sqrt(c2), lr / c1
@@ -133,9 +165,10 @@ __device__ __forceinline__ void values(uint32_t w, float scale, float (&x)[4]) {
 
 // Codes of a wave's 256 elements, four to a lane, and their block's scale. The largest
 // magnitude is taken over bit patterns, in which infinity and NaN are above every number;
-// with either the scale is NaN, and so is every value of the block.
-template <bool QUARTIC>
-__device__ __forceinline__ uint32_t codes(const float (&x)[4], float* scale) {
+// with either the scale is NaN, and so is every value of the block. UNBIASED: `key` and e, the
+// first of the lane's elements, give the random words.
+template <bool QUARTIC, bool UNBIASED>
+__device__ __forceinline__ uint32_t codes(const float (&x)[4], float* scale, uint32_t key, int64_t e) {
 #pragma clang fp contract(off)
   uint32_t most = 0;
 #pragma unroll
@@ -149,10 +182,25 @@ __device__ __forceinline__ uint32_t codes(const float (&x)[4], float* scale) {
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float r = __builtin_sqrtf(__builtin_fabsf(x[i]) * inv);
+    const float part = __builtin_fabsf(x[i]) * inv;
+    float r = __builtin_sqrtf(part);
     if constexpr (QUARTIC) r = __builtin_sqrtf(r);
     constexpr float levels = QUARTIC ? 255.0f : 127.0f;
-    int c = (int)__builtin_fminf(__builtin_rintf(r * levels), levels);
+    int c;
+    if constexpr (UNBIASED) {
+      // between the values of codes lo and lo + 1, in units of code 1's
+      const float lo = __builtin_fminf(__builtin_floorf(r * levels), levels - 1.0f), up = lo + 1.0f;
+      const float l2 = lo * lo, u2 = up * up;
+      const float below = QUARTIC ? l2 * l2 : l2, above = QUARTIC ? u2 * u2 : u2;
+      const float at = part * (QUARTIC ? levels * levels * levels * levels : levels * levels);
+      const uint32_t w = random_word(key, e + i);
+      c = (int)lo + (uniform(QUARTIC ? w * kGolden : w) * (above - below) < at - below ? 1 : 0);
+      if ((__float_as_uint(x[i]) & 0x7fffffffu) == most) c = (int)levels;
+      if (QUARTIC && x[i] > 0.0f) c = max(c, 1);
+      if (none) c = 0;
+    } else {
+      c = (int)__builtin_fminf(__builtin_rintf(r * levels), levels);
+    }
     if (!QUARTIC && x[i] < 0.0f) c = -c;
     w |= ((uint32_t)c & 255u) << (8 * i);
   }
@@ -161,9 +209,10 @@ __device__ __forceinline__ uint32_t codes(const float (&x)[4], float* scale) {
 
 // P: the parameter's type, G: the gradient's. MASTER: the parameter is the rounded copy
 // of an fp32 master. Four elements a lane, so that a wave holds one block of 256.
-template <typename P, typename G, bool MASTER, bool BYTES>
+template <typename P, typename G, bool MASTER, int CODES>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(Table tab, Scalars s) {
 #pragma clang fp contract(off)
+  constexpr bool BYTES = CODES != kWords;
   int lo = 0, hi = tab.count - 1;  // the tensor whose workgroups hold this one
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -214,7 +263,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(Table tab, Scalars s) {
       for (int i = 0; i < 4; ++i)
         if (e + i >= n) m[i] = v[i] = 0.0f;
       float sm, sv;
-      const uint32_t cm = codes<false>(m, &sm), cv = codes<true>(v, &sv);
+      const uint32_t cm = codes<false, CODES == kUnbiased>(m, &sm, tab.key[lo], e);
+      const uint32_t cv = codes<true, CODES == kUnbiased>(v, &sv, tab.key[lo], e);
       store4(static_cast<uint8_t*>(t.exp_avg), e, n, cm);
       store4(static_cast<uint8_t*>(t.exp_avg_sq), e, n, cv);
       if ((threadIdx.x & 63) == 0) {
@@ -240,8 +290,8 @@ __global__ __launch_bounds__(kThreads) void adamw_values_kernel(const uint8_t* c
 
 typedef void (*AdamwFn)(Table, Scalars);
 
-AdamwFn kernel_of(int pd, int gd, bool master, bool bytes) {
-#define GS_ADAMW(P, G, M) (bytes ? adamw_kernel<P, G, M, true> : adamw_kernel<P, G, M, false>)
+AdamwFn kernel_of(int pd, int gd, bool master, int codes) {
+#define GS_ADAMW(P, G, M) (codes == kUnbiased ? adamw_kernel<P, G, M, kUnbiased> : codes == kNearest ? adamw_kernel<P, G, M, kNearest> : adamw_kernel<P, G, M, kWords>)
   const bool gf = gd == GS_DTYPE_F32;
   if (pd == GS_DTYPE_F32) return gf ? GS_ADAMW(float, float, false) : GS_ADAMW(float, __bf16, false);
   if (master) return gf ? GS_ADAMW(__bf16, float, true) : GS_ADAMW(__bf16, __bf16, true);
@@ -274,6 +324,8 @@ extern "C" int gs_adamw_step(const gs_adamw_args* a, hipStream_t stream) {
       !(a->weight_decay >= 0.0 && std::isfinite(a->weight_decay)))
     return set_error(GS_ERR_INVALID, "%s: lr, eps and weight_decay must be finite and >= 0; got %g, %g, %g", who, a->lr,
                      a->eps, a->weight_decay);
+  if (a->rounding != GS_ROUND_NEAREST && a->rounding != GS_ROUND_UNBIASED)
+    return set_error(GS_ERR_INVALID, "%s: unknown rounding %d", who, a->rounding);
   const bool bytes = a->state_bits == 8;
   for (int64_t i = 0; i < a->count; ++i) {
     const gs_adamw_tensor& t = a->tensors[i];
@@ -294,7 +346,8 @@ extern "C" int gs_adamw_step(const gs_adamw_args* a, hipStream_t stream) {
   s.eps = (float)a->eps;
   s.rate = (float)(a->lr / c1);
   s.grad_scale = a->grad_scale;
-  const AdamwFn fn = kernel_of(a->param_dtype, a->grad_dtype, a->has_master != 0, bytes);
+  const AdamwFn fn = kernel_of(a->param_dtype, a->grad_dtype, a->has_master != 0,
+                               !bytes ? kWords : a->rounding == GS_ROUND_UNBIASED ? kUnbiased : kNearest);
   Table tab;
   tab.count = 0;
   int64_t groups = 0;
@@ -315,6 +368,7 @@ extern "C" int gs_adamw_step(const gs_adamw_args* a, hipStream_t stream) {
       if (rc) return rc;
     }
     tab.t[tab.count] = t;
+    tab.key[tab.count] = key_of(a->step, i);
     tab.first[tab.count++] = (uint32_t)groups;
     groups += need;
   }

@@ -451,7 +451,7 @@ void check_list(const char* name, const Tensors& ts, const std::vector<int64_t>&
 void adamw_step(const Tensors& params, Tensors grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs, int64_t step,
                 double lr, double beta1, double beta2, double eps, double weight_decay,
                 const std::optional<Tensors>& masters, const std::optional<Tensors>& exp_avg_scales,
-                const std::optional<Tensors>& exp_avg_sq_scales, const OptTensor& grad_scale) {
+                const std::optional<Tensors>& exp_avg_sq_scales, const OptTensor& grad_scale, int64_t rounding) {
   const char* who = "adamw_step";
   if (params.empty()) return;
   const Tensor& ref = params[0];
@@ -515,6 +515,7 @@ void adamw_step(const Tensors& params, Tensors grads, const Tensors& exp_avgs, c
   a.grad_scale = grad_scale.has_value() ? static_cast<const float*>(grad_scale->data_ptr()) : nullptr;
   a.state_bits = bytes ? 8 : 32;
   a.has_master = masters.has_value();
+  a.rounding = (int32_t)rounding;
   const On on(ref);
   raise_for(gs_adamw_step(&a, on.stream));
   for (const Tensors* ts : {&params, &exp_avgs, &exp_avg_sqs, get(masters), get(exp_avg_scales), get(exp_avg_sq_scales)})

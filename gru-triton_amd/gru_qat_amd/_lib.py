@@ -83,7 +83,7 @@ EXPORTS = (
     "gs_abi_version",
 )
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 QuantTuple = Optional[Tuple[float, int, int]]
 
@@ -368,6 +368,8 @@ ACT_RELU = 2
 ACT_GELU = 3
 ACT_SILU = 4
 ACT_SIGMOID = 5
+ROUND_NEAREST = 0
+ROUND_UNBIASED = 1
 
 
 class GsGlrArgs(ctypes.Structure):
@@ -427,7 +429,7 @@ class GsAdamwArgs(ctypes.Structure):
         [("tensors", ctypes.POINTER(GsAdamwTensor)), ("count", ctypes.c_int64)]
         + [(k, ctypes.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")]
         + [("step", ctypes.c_int64), ("grad_scale", ctypes.c_void_p)]
-        + [(k, ctypes.c_int32) for k in ("param_dtype", "grad_dtype", "state_bits", "has_master")]
+        + [(k, ctypes.c_int32) for k in ("param_dtype", "grad_dtype", "state_bits", "has_master", "rounding")]
     )
 
 

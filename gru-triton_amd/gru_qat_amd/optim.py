@@ -14,6 +14,14 @@ import torch
 from . import _lib
 
 STATE_BLOCK = 256  # elements of a tensor that share a scale where moments are held in 8 bits
+_ROUNDINGS = {"nearest": _lib.ROUND_NEAREST, "unbiased": _lib.ROUND_UNBIASED}
+
+
+def _rounding(who: str, rounding: Any) -> int:
+    try:
+        return _ROUNDINGS[rounding]
+    except (KeyError, TypeError):
+        raise ValueError(f"{who}: rounding must be 'nearest' or 'unbiased'; got {rounding!r}") from None
 
 
 def _blocks(n: int) -> int:
@@ -35,6 +43,7 @@ def adamw_step(
     exp_avg_scales: Optional[Sequence[torch.Tensor]] = None,
     exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
     grad_scale: Optional[torch.Tensor] = None,
+    rounding: str = "nearest",
 ) -> None:
     """One AdamW step in place, the ``step``-th (from 1), on contiguous tensors of one device.
 
@@ -43,10 +52,18 @@ def adamw_step(
     type, and ``grads`` too. The moments are float32, or, with ``exp_avg_scales`` and
     ``exp_avg_sq_scales`` (float32, one number per 256 elements), int8 and uint8 codes (see
     ``adamw_dequantize_state``). ``grad_scale``: a float32 tensor of one element on the
-    device that multiplies the gradients; where it is not finite the step does nothing."""
+    device that multiplies the gradients; where it is not finite the step does nothing.
+
+    ``rounding`` of 8-bit moments: "nearest" stores the nearest code and loses every change of
+    less than half a code. While a block's largest magnitude holds and betas are (0.9, 0.999), a second
+    moment then never falls, rises only where g^2 passes 9 to 40 times it, and a first moment of
+    code 9 or less (0.5 % of the largest) stays for good. "unbiased" stores one of the two codes
+    around a value so that the average over steps is right; which one is a hash of ``step``,
+    the tensor's place in the list and the element, so that results repeat."""
+    how = _rounding("adamw_step", rounding)
     try:
         (_lib._ops or _lib.ops()).adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas[0], betas[1], eps,
-                                             weight_decay, masters, exp_avg_scales, exp_avg_sq_scales, grad_scale)
+                                             weight_decay, masters, exp_avg_scales, exp_avg_sq_scales, grad_scale, how)
     except TypeError as e:
         raise ValueError(f"adamw_step: params, grads and states must be lists of tensors ({e})") from None
 
@@ -65,9 +82,13 @@ class AdamW(torch.optim.Optimizer):
     """AdamW whose step is ``adamw_step``: one launch for up to 48 parameters.
 
     ``state_bits`` 32 keeps float32 moments, 8 keeps codes of 8 bits with a float32 scale
-    per 256 elements (2 bytes an element instead of 8); an element whose gradients are
-    under four millionths of its block's largest keeps a second moment of 0 there, and an
-    ``eps`` of the size of such gradients keeps its updates small. bfloat16 parameters get float32
+    per 256 elements (2 bytes an element instead of 8). ``state_rounding`` is the ``rounding`` of
+    those codes: "unbiased" follows gradients that grow, shrink or end, with a noise of a few per
+    cent of an update where gradients are within a hundredth of their block's largest and as large as the
+    update under a ten thousandth; elements under 1.5e-5 of it move less than they should. "nearest"
+    has no noise, but does not follow such changes (``adamw_step``), and an element
+    under four millionths of the largest keeps a second moment of 0: an ``eps`` of the size of such
+    gradients keeps its updates small. bfloat16 parameters get float32
     masters unless ``master_weights`` is off (taken at a parameter's first step; from then on
     a parameter is its master's rounding, whatever else is written to it). ``step(grad_scale=...)`` multiplies the
     gradients by a device scalar (a clipping factor, an inverse loss scale); where that is
@@ -76,11 +97,12 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params: Iterable[Any], lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.01, *, state_bits: int = 32,
-                 master_weights: bool = True) -> None:
+                 master_weights: bool = True, state_rounding: str = "unbiased") -> None:
         if state_bits not in (8, 32):
             raise ValueError(f"AdamW: state_bits must be 8 or 32; got {state_bits}")
+        _rounding("AdamW", state_rounding)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                                      master_weights=master_weights))
+                                      master_weights=master_weights, state_rounding=state_rounding))
 
     def _init_state(self, p: torch.Tensor, group: dict) -> None:
         s = self.state[p]
@@ -125,7 +147,8 @@ class AdamW(torch.optim.Optimizer):
                 adamw_step([p for p, _, _ in rows], [g for _, g, _ in rows], [s["exp_avg"] for s in states],
                            [s["exp_avg_sq"] for s in states], step=count + 1, lr=group["lr"], betas=group["betas"],
                            eps=group["eps"], weight_decay=group["weight_decay"],
-                           masters=[s["master"] for s in states] if master else None, grad_scale=grad_scale, **scales)
+                           masters=[s["master"] for s in states] if master else None, grad_scale=grad_scale,
+                           rounding=group.get("state_rounding", "unbiased"), **scales)
                 for s in states:
                     s["step"] = count + 1
         return loss

@@ -62,7 +62,7 @@
 extern "C" {
 #endif
 
-#define GS_ABI_VERSION 7
+#define GS_ABI_VERSION 8
 
 #define GS_OK 0
 #define GS_ERR_INVALID (-1)  /* bad pointer, shape, stride or quant parameter (Python: ValueError) */
@@ -729,7 +729,17 @@ int gs_linear_bwd(const gs_linear_bwd_args* args, hipStream_t stream);
  * int8 c for A sign(c) (c / 127)^2, and uint8 c for A (c / 255)^4. A block with a NaN
  * or an infinity becomes NaN as a whole. grad_scale (device, optional) multiplies the
  * gradients; where it is not finite the whole step is skipped. No counterpart in the
- * reference. */
+ * reference.
+ *
+ * GS_ROUND_NEAREST stores the nearest code, and loses every change of a moment of less than half a
+ * code: with a block's A constant and b2 = 0.999 an element's second moment never falls, and
+ * rises only where g^2 passes 9 to 40 times it; with b1 = 0.9 a first moment of code 9 or less stays
+ * for good. GS_ROUND_UNBIASED stores one of the two codes around a value, so that the average
+ * over steps is the value; which one is a hash of step, place in the array and element, so that
+ * results repeat. A second moment that is not 0 is never stored as 0 there. */
+#define GS_ROUND_NEAREST 0
+#define GS_ROUND_UNBIASED 1
+
 typedef struct gs_adamw_tensor {
   void* param;
   const void* grad;
@@ -748,6 +758,7 @@ typedef struct gs_adamw_args {
   int64_t step;             /* 1 at the first step                                */
   const float* grad_scale;  /* device scalar or NULL                              */
   int32_t param_dtype, grad_dtype, state_bits, has_master;
+  int32_t rounding;         /* GS_ROUND_* of codes of 8 bits                      */
 } gs_adamw_args;
 
 int gs_adamw_step(const gs_adamw_args* args, hipStream_t stream);
