@@ -90,3 +90,71 @@ def test_an_axis_past_a_launch(dev):
     scan._near(out[-tail:], o, e, "out")
     scan._near(last, hl, el, "h_T")
     assert (out[:30, 0, 0].cpu() == 2.0 ** -torch.arange(1.0, 31)).all() and not out[200:-tail].any()
+
+
+# Walked layouts over four tiles and more, so that both LDS buffers are written again: four waves (tiles of 32
+# steps), eight by 32 lanes (128) and eight by 16 (256); odd channel counts, and even ones that bfloat16 takes in pairs.
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("p", [0.0, 0.03], ids=["", "resets"])
+@pytest.mark.parametrize("shape", [(140, 20, 701), (140, 20, 1402), (500, 20, 301), (500, 20, 600), (1000, 10, 301),
+                                   (1000, 10, 600)], ids=str)
+def test_many_tiles(dev, shape, p, dtype):
+    scan._check(dev, *scan._inputs(*shape, dtype, seed=sum(shape), p_reset=p), "tanh")
+
+
+def _check_linked(dev, gi, h0, reset, dout, dh, nans):
+    """scan._check with NaN where the formula has it (and nowhere else), whose bounds a reset ends too."""
+    dtype, H = gi.dtype, h0.shape[1]
+    for t, b, j in nans["gi"]:
+        gi[t, b, j] = float("nan")
+    for t, b, j in nans["dout"]:
+        dout[t, b, j] = float("nan")
+    x, s = gi.to(dev).requires_grad_(True), h0.to(dev).requires_grad_(True)
+    out, last = G.gated_linear_scan(x, s, reset=None if reset is None else reset.to(dev))
+    dgi, dh0 = torch.autograd.grad((out, last), (x, s), (dout.to(dev), dh.to(dev)))
+    (o, eo), (hl, el), (dg, edg), (d0, e0), hp, z = scan._oracle(gi, h0, reset, "tanh", dout, dh)
+    if dtype == BF16:
+        u, size, run = scan.U16, torch.empty_like(o), dh.double().abs()
+        for t in range(o.shape[0] - 1, -1, -1):
+            if t + 1 < o.shape[0]:
+                run = run * z[t + 1]
+                if reset is not None:
+                    run = torch.where(reset[t + 1][:, None], 0.0, run)
+            size[t] = run = run + dout[t].double().abs()
+        edg[..., :H] += u * hp.abs() * size * z * (1 - z)
+        eo, edg = eo * (1 + u) + u * o.abs(), edg * (1 + u) + u * dg.abs()
+    for got, want, bound, what in ((out, o, eo, "out"), (last, hl, el, "h_T"), (dgi, dg, edg + 1e-38, "dgi"),
+                                   (dh0, d0, e0 + 1e-38, "dh0")):
+        ok = _same_kind(got, want, what)
+        off = (got.detach().cpu().double() - want).abs()
+        assert (off[ok] <= bound[ok]).all(), what
+
+
+# 50 tiles and a part: chained tiles of 16 lanes are 256 steps, of 32 lanes 128, and every 16th publishes its state.
+# Few channels take 16 lanes, from 512 on (pairs of them in bfloat16, backwards only) 32.
+LINKED = [(50 * 256 + 9, 3, 20, 256), (50 * 256, 3, 21, 256), (50 * 128 + 9, 2, 270, 128), (50 * 128, 4, 270, 128)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("resets", ["none", "at links", "many"])
+@pytest.mark.parametrize("shape", LINKED, ids=str)
+def test_chains_over_links(dev, shape, resets, dtype):
+    """States handed on over three links, and NaN that a reset before or after a link stops, from both ends."""
+    T, B, H, tile = shape
+    link = 16 * tile
+    gi, h0, reset, dout, dh = scan._inputs(T, B, H, dtype, seed=T + H, p_reset=0.002 if resets == "many" else 0.0)
+    nans = dict(gi=[], dout=[])
+    if resets == "at links":
+        reset = torch.zeros(T, B, dtype=torch.bool)
+        # row 0: in the last tile before a link, NaN before it; the group of links after that has none
+        reset[link - 100, 0] = True
+        nans["gi"] += [(link - 110, 0, 3), (link - 110, 0, H + 4)]
+        # row 1: in the first tile after a link, the NaN before the link
+        reset[2 * link + 10, 1] = True
+        nans["gi"] += [(2 * link - 7, 1, 0), (2 * link - 7, 1, H + H - 1)]
+        # the same from the end, where the backward's links are
+        reset[T - 1 - (link - 100), 1] = True
+        nans["dout"] += [(T - 1 - (link - 110), 1, 5)]
+        reset[T - 1 - (2 * link + 10), 0] = True
+        nans["dout"] += [(T - 1 - (2 * link - 7), 0, 2)]
+    _check_linked(dev, gi, h0, reset, dout, dh, nans)
