@@ -32,7 +32,6 @@
 namespace gs {
 namespace {
 
-typedef unsigned int u2v __attribute__((ext_vector_type(2)));
 typedef unsigned int u4v __attribute__((ext_vector_type(4)));
 typedef float f2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
@@ -85,62 +84,35 @@ __device__ __forceinline__ Map then_span(const Map& first, const Map& second) {
   return r;
 }
 
-// V elements of type T in one buffer access.
+// V elements of type T in one buffer access: an fp32, a bf16 or two of those.
 template <typename T, int V>
 struct Pack {
   static constexpr int kBytes = V * (int)sizeof(T);
-  static_assert(kBytes == 2 || kBytes == 4 || kBytes == 8, "2, 4 or 8 bytes a lane");
-  typedef typename std::conditional<kBytes == 8, u2v, unsigned int>::type Raw;
+  static_assert(kBytes == 2 || kBytes == 4, "2 or 4 bytes a lane");
+  typedef unsigned int Raw;
   static __device__ __forceinline__ Raw load(const void* base, uint32_t off) {
     const auto r = bounded_rsrc(base, 0x7fffffffu);
     if constexpr (kBytes == 2)
       return (unsigned int)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, (int)off, 0, 0);
-    else if constexpr (kBytes == 4)
-      return __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0);
     else
-      return __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0);
+      return __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0);
   }
   static __device__ __forceinline__ void store(void* base, uint32_t off, const float (&x)[V]) {
     const auto r = bounded_rsrc(base, 0x7fffffffu);
-    if constexpr (sizeof(T) == 4) {
-      if constexpr (V == 1)
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[0]), r, (int)off, 0, 0);
-      else
-        __builtin_amdgcn_raw_buffer_store_b64(u2v{__float_as_uint(x[0]), __float_as_uint(x[1])}, r, (int)off, 0, 0);
-    } else if constexpr (V == 1) {
+    if constexpr (kBytes == 2)
       __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)x[0]), r, (int)off, 0, 0);
-    } else {
-      unsigned int w[V / 2];
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i)
-        w[i] = __builtin_bit_cast(unsigned int, __builtin_convertvector((f2v{x[2 * i], x[2 * i + 1]}), bf2v));
-      if constexpr (V == 2)
-        __builtin_amdgcn_raw_buffer_store_b32(w[0], r, (int)off, 0, 0);
-      else
-        __builtin_amdgcn_raw_buffer_store_b64(u2v{w[0], w[1]}, r, (int)off, 0, 0);
-    }
+    else if constexpr (V == 1)
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[0]), r, (int)off, 0, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b32(
+          __builtin_bit_cast(unsigned int, __builtin_convertvector((f2v{x[0], x[1]}), bf2v)), r, (int)off, 0, 0);
   }
-  static __device__ __forceinline__ void unpack(const Raw& w, float (&x)[V]) {
-    if constexpr (sizeof(T) == 4) {
-      if constexpr (V == 1)
-        x[0] = __uint_as_float(w);
-      else {
-        x[0] = __uint_as_float(w[0]);
-        x[1] = __uint_as_float(w[1]);
-      }
-    } else if constexpr (V == 1) {
+  static __device__ __forceinline__ void unpack(Raw w, float (&x)[V]) {
+    if constexpr (V == 2) {
       x[0] = __uint_as_float(w << 16);
+      x[1] = __uint_as_float(w & 0xffff0000u);
     } else {
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        unsigned int u;
-        if constexpr (V == 2)
-          u = w;
-        else
-          u = w[i];
-        x[2 * i] = __uint_as_float(u << 16);
-        x[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
-      }
+      x[0] = __uint_as_float(kBytes == 2 ? w << 16 : w);
     }
   }
 };
