@@ -180,12 +180,27 @@ __device__ __forceinline__ void store_row8(void* row, int j, int N, const float 
   }
 }
 
+// A row's eight elements of pre from column j on, as the backward takes them.
+__device__ __forceinline__ void keep_row8(void* row, int j, int N, const float (&x)[8]) {
+  GranuleAt w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = kept_pair(x[2 * i], x[2 * i + 1]);
+  unsigned short* p = static_cast<unsigned short*>(row) + j;
+  if (j + 8 <= N) {
+    *reinterpret_cast<GranuleAt*>(p) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (j + i < N) p[i] = (unsigned short)(w[i >> 1] >> (16 * (i & 1)));
+  }
+}
+
 // What follows the sums of columns j .. j + 7 of row i (< M; columns from N on do not exist).
 __device__ __forceinline__ void finish8(const LinearEpilogue& e, __bf16* y, int64_t ldy, int i, int j, int N,
                                         const float (&bias)[8], float (&x)[8]) {
 #pragma unroll
   for (int v = 0; v < 8; ++v) x[v] += bias[v];
-  if (e.pre != nullptr) store_row8(static_cast<__bf16*>(e.pre) + (int64_t)i * N, j, N, x);
+  if (e.pre != nullptr) keep_row8(static_cast<unsigned short*>(e.pre) + (int64_t)i * N, j, N, x);
   if (e.act != GS_ACT_NONE) act_values(x, e.act);
   if (e.residual != nullptr) {
     float r[8];

@@ -6,12 +6,12 @@
 
 namespace gs {
 
-// pre = sums + bias[j] (stored to `pre` where asked), y = act(pre) + residual[i, j]. All in
-// the operands' type.
+// pre = sums + bias[j] (stored to `pre` where asked), y = act(pre) + residual[i, j]. All but
+// `pre` in the operands' type.
 struct LinearEpilogue {
   const void* bias = nullptr;      // [N]
   const void* residual = nullptr;  // [M, N], row stride ldr
-  void* pre = nullptr;             // [M, N] contiguous
+  void* pre = nullptr;             // [M, N] contiguous, halves where the type is bf16
   int64_t ldr = 0;
   int act = GS_ACT_NONE;
 };

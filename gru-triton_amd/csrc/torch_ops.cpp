@@ -333,7 +333,8 @@ constexpr int64_t kHasBias = 256, kHasResidual = 512;  // beside the activation'
 struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias,
                         const OptTensor& residual, int64_t act) {
-    const Tensor pre = act != GS_ACT_NONE ? torch::empty({x.size(0), w.size(0)}, x.options()) : Tensor();
+    const auto kept = x.scalar_type() == torch::kFloat ? torch::kFloat : torch::kHalf;
+    const Tensor pre = act != GS_ACT_NONE ? torch::empty({x.size(0), w.size(0)}, x.options().dtype(kept)) : Tensor();
     Tensor y = linear_forward(x, w, get(bias), get(residual), act, pre);
     ctx->save_for_backward({x, w, pre});
     ctx->saved_data["act"] = act | (bias.has_value() ? kHasBias : 0) | (residual.has_value() ? kHasResidual : 0);

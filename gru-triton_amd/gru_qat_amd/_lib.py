@@ -83,7 +83,7 @@ EXPORTS = (
     "gs_abi_version",
 )
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 QuantTuple = Optional[Tuple[float, int, int]]
 

@@ -29,8 +29,10 @@ def linear_act(
     """``act(x @ weight.T + bias) + residual`` for ``x`` [..., K], ``weight`` [N, K], ``bias``
     [N] and ``residual`` [..., N], all float32 or all bfloat16 on one GPU; returns [..., N] in
     that type, every sum in float32. ``activation``: "none", "relu", "gelu" (of erf), "silu",
-    "tanh" or "sigmoid". Differentiable in all four tensors (once); with an activation, a training
-    forward keeps its argument [..., N] in x's type."""
+    "tanh" or "sigmoid". Differentiable in all four tensors (once). With an activation, a training
+    forward keeps its argument [..., N], in bfloat16 as halves, and a bfloat16 backward rounds the
+    argument's gradient to bfloat16, as an operand of the products for x and weight, whose error that
+    takes from 0.0017 of their size (their own rounding) to 0.0024."""
     try:
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):

@@ -62,7 +62,7 @@
 extern "C" {
 #endif
 
-#define GS_ABI_VERSION 8
+#define GS_ABI_VERSION 9
 
 #define GS_OK 0
 #define GS_ERR_INVALID (-1)  /* bad pointer, shape, stride or quant parameter (Python: ValueError) */
@@ -676,7 +676,8 @@ int gs_glr_step(const gs_glr_step_args* args, hipStream_t stream);
  *   pre = x w^T + bias,  y = act(pre) + residual
  * x [M, K], w [N, K], all tensors of one type (GS_DTYPE_*), every sum in fp32 (bf16
  * operands on the bf16 MFMA, fp32 ones on the fp32 MFMA). A training forward with an
- * activation also stores pre, rounded to the type, for the backward. No counterpart in
+ * activation also stores pre for the backward: in fp32, or as IEEE halves where the type
+ * is bf16 (clamped to their range, in which act' has its changes). No counterpart in
  * the reference (its projections are gs_input_proj's). */
 typedef struct gs_linear_args {
   const void* x;         /* [M, K], row stride sx                                         */
@@ -684,7 +685,7 @@ typedef struct gs_linear_args {
   const void* bias;      /* [N] or NULL                                                   */
   const void* residual;  /* [M, N], row stride sr, or NULL                                */
   void* y;               /* [M, N], row stride sy                                         */
-  void* pre;             /* [M, N] contiguous, or NULL                                    */
+  void* pre;             /* [M, N] contiguous, floats or (bf16) halves, or NULL           */
   void* scratch;         /* gs_linear_scratch_bytes() bytes, 256-byte aligned             */
   int64_t scratch_bytes;
   int64_t M, N, K;
