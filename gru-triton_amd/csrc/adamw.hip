@@ -28,7 +28,8 @@
 //
 // Bound by memory: each word is read once and written once. 50 M bf16 parameters with fp32
 // masters and moments in 8 bits (18 bytes each, 0.91 GB) take 188 us, 4.8 TB/s where a copy
-// reaches 5.2, and 225 with unbiased rounding, whose hashes and comparisons memory does not hide; 4.7 M in fp32 (28 bytes, 132 MB, held by the last cache) 21 us. A table of
+// reaches 5.2, and 225 with unbiased rounding, whose hashes and comparisons memory does not
+// hide; 4.7 M in fp32 (28 bytes, 132 MB, held by the last cache) 21 us. A table of
 // tensors in the kernel's arguments makes one launch of up to 48 tensors, so that small
 // ones fill the device together and nothing is uploaded for the call.
 #include "gs_host.h"

@@ -12,9 +12,9 @@
 // Time on the GPU of a training step's kernels, in us (the products' own comments say what
 // bounds them; the dpre pass reads dy, and pre where there is an activation, at 3.9 TB/s):
 //   M, N, K                    forward  dpre  dx    dw    sums joined
-//   2048, 1024, 512 bf16 gelu  11.1     6.4   15.0 together
-//   32768, 2048, 1024 bf16     172      35    130   112   18
-//   1650, 1002, 301 fp32 silu  26       7.4   39 together 4.1
+//   2048, 1024, 512 bf16 gelu  11.4     6.4   15.1 together
+//   32768, 2048, 1024 bf16     170      35    132   110   19
+//   1650, 1002, 301 fp32 silu  26       8     39 together 4.1
 #include "gs_gemm_bf16.h"
 
 namespace gs {

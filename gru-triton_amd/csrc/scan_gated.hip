@@ -22,11 +22,13 @@
 // takes one tile instead, and tiles hand their states on through memory (see chain()).
 //
 // Bound by memory where there are enough waves: T 256, B 64, H 2048 in bf16 takes 37 us
-// forward and 86 backward, 5.4 and 4.7 TB/s where a copy reaches 5.2; T 512, B 16, H 512 in
-// fp32 11.4 and 19.5 (4.4, 5.2). The chained layouts reach 3.4 to 5.4: T 4096, B 8, H 1024
-// in bf16 44 and 85 us, T 65536, B 1, H 1024 113 and 191, in fp32 171 and 301. What keeps
-// them below a copy is the start of each workgroup (its ticket, its loads and the wait for
-// its carry, one after the other), which six waves a SIMD only partly hide.
+// forward and 77 backward, 5.4 and 5.2 TB/s where a copy reaches 5.2; T 512, B 16, H 512 in
+// fp32 11 and 19 (4.5, 5.4). The chained layouts reach 3.3 to 5.6: T 4096, B 8, H 1024
+// in bf16 46 and 84 us (in a training step, with its memory cold, 50 to 53 and 88), T 65536,
+// B 1, H 1024 121 and 193, in fp32 172 and 287, and 5 us each before them to clear the chain's
+// words. What keeps them below a copy is the start of each workgroup (its ticket, its loads
+// and the wait for its carry, one after the other), which six waves a SIMD only partly hide;
+// and, forwards in bf16, rows of 64 bytes a workgroup.
 #include "gs_mfma.h"
 
 namespace gs {
