@@ -626,7 +626,7 @@ typedef struct gs_glr_args {
   int64_t sg_t, sg_b, sh0_b, sr_t, sr_b, so_t, so_b;
   int32_t dtype, activation;
   uint32_t* fault_mirror; /* optional host-visible word (hipHostMalloc memory) or NULL    */
-  int32_t poll_limit;     /* 0 in production                                             */
+  int32_t poll_limit;     /* 0 in production (both: ABI version 7)                        */
 } gs_glr_args;
 
 int64_t gs_glr_scratch_bytes(const gs_glr_args* args);
@@ -685,7 +685,7 @@ typedef struct gs_linear_args {
   const void* bias;      /* [N] or NULL                                                   */
   const void* residual;  /* [M, N], row stride sr, or NULL                                */
   void* y;               /* [M, N], row stride sy                                         */
-  void* pre;             /* [M, N] contiguous, floats or (bf16) halves, or NULL           */
+  void* pre;             /* [M, N] contiguous, floats or (bf16: since 9) halves, or NULL  */
   void* scratch;         /* gs_linear_scratch_bytes() bytes, 256-byte aligned             */
   int64_t scratch_bytes;
   int64_t M, N, K;
@@ -759,7 +759,7 @@ typedef struct gs_adamw_args {
   int64_t step;             /* 1 at the first step                                */
   const float* grad_scale;  /* device scalar or NULL                              */
   int32_t param_dtype, grad_dtype, state_bits, has_master;
-  int32_t rounding;         /* GS_ROUND_* of codes of 8 bits                      */
+  int32_t rounding;         /* GS_ROUND_* of codes of 8 bits (ABI version 8)      */
 } gs_adamw_args;
 
 int gs_adamw_step(const gs_adamw_args* args, hipStream_t stream);
