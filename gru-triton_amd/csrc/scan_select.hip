@@ -1,0 +1,906 @@
+// Selective state space scan (gfx950): a recurrence whose decay depends on its input,
+//   dt = softplus(delta + delta_bias),  a[n] = exp(dt A[c][n]),
+//   h_t[n] = a[n] h_{t-1}[n] + dt u B_t[n],  y = sum_n C_t[n] h_t[n] + D u,  out = y silu(z),
+// for every channel c of a batch row with N states each; B and C are shared by the channels.
+// reset[t][b] != 0 starts a new sequence at step t: h_{t-1} is taken as 0, whatever it holds.
+//
+// Backward, with G_t[n] the gradient of h_t[n] and dy that of y:
+//   G_t = C_t dy + a_{t+1} G_{t+1},  dC_t[n] = sum_c h_t[n] dy,  dB_t[n] = sum_c G_t[n] dt u,
+//   S = sum_n G_t[n] B_t[n],  q[n] = G_t[n] a_t[n] h_{t-1}[n],
+//   du = dt S + D dy,  ddt = u S + sum_n q[n] A[n],  dA[n] = sum_t q[n] dt,  dD = sum_t u dy.
+//
+// Layout: a workgroup owns 64 channels (a lane each) of one batch row and walks a chunk of
+// the time axis in tiles of 16 steps. Its waves share the N states, P a wave, and the steps of a tile:
+// a wave loads its steps' rows, computes what is shared by the states (softplus, the gate) and leaves
+// it in LDS; every wave then runs its states over the whole tile, one exponential a state and step,
+// and leaves its part of y; and each wave sums the parts of its steps. With few channels the
+// time axis is cut into chunks for more workgroups: a first pass finds what each chunk makes of a
+// zero state, a second joins those along the axis, and the third is the scan from the right states.
+// A training forward keeps the state before every tile, from which the backward runs the
+// tile's steps again, forwards and then back. Sums over channels (dB, dC) are those of the workgroup's
+// 64 in registers, then of the workgroups in order through memory: results are reproducible.
+#include "gs_seq.h"
+
+namespace gs {
+namespace {
+
+constexpr int kTile = 16;  // steps of a tile, and between kept states
+
+struct SsmParams {
+  const void *u, *delta, *z, *bm, *cm;
+  const float *A, *D, *bias, *h0;
+  const uint8_t* reset;
+  void* y;             // forward
+  float* h_last;
+  float* saved;        // [ceil(T / kTile)][B][N][H]: forward written (or NULL), backward read
+  float* ends;         // [chunks][B][N][H]: see ssm_join_kernel
+  float* span;         // [chunks][B][H]: sum of dt over a chunk
+  float* dropped;      // [chunks][B]: 1 where a chunk holds a reset
+  const void* dy;      // backward only from here
+  const float* dh_last;
+  void *du, *ddelta, *dz;
+  float* dh0;
+  float* part_bc;      // [blocks][T][B][2N]
+  float* part_a;       // [chunks][B][N + 2][H]
+  int64_t su_t, su_b, sdl_t, sdl_b, sz_t, sz_b, sb_t, sb_b, sc_t, sc_b, sr_t, sr_b, sy_t, sy_b, sdy_t, sdy_b;
+  int64_t sdu_t, sdu_b, sdd_t, sdd_b, sdz_t, sdz_b;
+  int T, B, H, N;
+  int blocks;          // channel blocks of 64
+  int chunks, length;  // of the time axis, in steps
+};
+
+// Where a workgroup is.
+struct At {
+  int block, b, chunk, lane, wave, ch, t0, t1;
+  bool ok;  // the lane's channel exists
+  __device__ __forceinline__ explicit At(const SsmParams& p) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int g = blockIdx.x;
+    block = g % p.blocks;
+    g /= p.blocks;
+    b = g % p.B;
+    chunk = g / p.B;
+    ch = block * 64 + lane;
+    ok = ch < p.H;
+    t0 = chunk * p.length;
+    t1 = min(p.T, t0 + p.length);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t lane_off(const At& at) {
+  return at.ok ? (uint32_t)(at.ch * (int)sizeof(T)) : kOffNone;
+}
+template <typename T>
+__device__ __forceinline__ const T* row_of(const void* base, int64_t st, int64_t sb, int t, int b) {
+  return static_cast<const T*>(base) + t * st + b * sb;
+}
+
+// The flags of a tile's steps as a bit mask.
+__device__ __forceinline__ uint32_t flags_of(const SsmParams& p, const At& at, int t0) {
+  if (p.reset == nullptr) return 0;
+  bool f = false;
+  if (at.lane < kTile && t0 + at.lane < at.t1) f = p.reset[(t0 + at.lane) * p.sr_t + at.b * p.sr_b] != 0;
+  return (uint32_t)__builtin_amdgcn_ballot_w64(f);
+}
+
+// B and C of a tile as floats, a wave's P states side by side; zero where there is no step or state.
+template <typename T, int P, int NW>
+__device__ __forceinline__ void stage_bc(const SsmParams& p, const At& at, int t0, float (*bc)[NW][2 * P]) {
+  constexpr int NP = NW * P, kAll = kTile * 2 * NP;
+#pragma unroll
+  for (int k = 0; k < kAll; k += 64 * NW) {
+    const int e = k + threadIdx.x;
+    if (kAll % (64 * NW) == 0 || e < kAll) {
+      const int s = e / (2 * NP), r = e % (2 * NP), c = r / NP, n = r % NP, t = t0 + s;
+      float x = 0.0f;
+      if (n < p.N && t < at.t1)
+        x = (float)(c ? row_of<T>(p.cm, p.sc_t, p.sc_b, t, at.b) : row_of<T>(p.bm, p.sb_t, p.sb_b, t, at.b))[n];
+      bc[s][n / P][c * P + n % P] = x;
+    }
+  }
+}
+
+// f(std::true_type) where a tile holds a reset, else f(std::false_type): uniform.
+template <typename F>
+__device__ __forceinline__ void with_flags(uint32_t flags, F&& f) {
+  if (flags) f(std::true_type{});
+  else f(std::false_type{});
+}
+
+// OUT: the scan itself. Otherwise what a chunk makes of a zero state, and its sum of dt.
+// PAD: N is not P NW; states that do not exist are left out.
+template <typename T, int P, int NW, bool PAD, bool OUT>
+__global__ __launch_bounds__(64 * NW) void ssm_fwd_kernel(SsmParams p) {
+  typedef Elem<T> E;
+  constexpr int kOwn = kTile / NW;  // steps of a tile that a wave prepares
+  __shared__ float2 xs[kTile][64];  // dt, dt u
+  __shared__ float bc[kTile][NW][2 * P];
+  __shared__ float part[OUT ? NW : 1][kTile][64];
+  const At at(p);
+  const int n0 = at.wave * P, live = PAD ? min(max(p.N - n0, 0), P) : P;
+  float A2[P], h[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int n = n0 + i;
+    const bool some = at.ok && n < p.N;
+    A2[i] = some ? p.A[(int64_t)at.ch * p.N + n] * kLog2e : 0.0f;
+    h[i] = 0.0f;
+    if (OUT && some) {
+      if (at.chunk) h[i] = p.ends[(((int64_t)(at.chunk - 1) * p.B + at.b) * p.N + n) * p.H + at.ch];
+      else if (p.h0 != nullptr) h[i] = p.h0[((int64_t)at.b * p.H + at.ch) * p.N + n];
+    }
+  }
+  const float bias = p.bias != nullptr && at.ok ? p.bias[at.ch] : 0.0f;
+  const float D = OUT && p.D != nullptr && at.ok ? p.D[at.ch] : 0.0f;
+  const uint32_t off = lane_off<T>(at);
+  float span = 0.0f;
+  bool drop = false;
+  unsigned int rd[kOwn], ru[kOwn], rz[kOwn];
+  auto fetch = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int t = t0 + at.wave + NW * i;
+      const uint32_t o = t < at.t1 ? off : kOffNone;
+      const int r = min(t, at.t1 - 1);
+      rd[i] = E::load(row_of<T>(p.delta, p.sdl_t, p.sdl_b, r, at.b), o);
+      ru[i] = E::load(row_of<T>(p.u, p.su_t, p.su_b, r, at.b), o);
+      if (OUT && p.z != nullptr) rz[i] = E::load(row_of<T>(p.z, p.sz_t, p.sz_b, r, at.b), o);
+    }
+  };
+  fetch(at.t0);
+  for (int t0 = at.t0; t0 < at.t1; t0 += kTile) {
+    float u[kOwn], z[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int s = at.wave + NW * i;
+      u[i] = E::value(ru[i]);
+      if (OUT) z[i] = E::value(rz[i]);
+      const float dt = t0 + s < at.t1 ? softplus(E::value(rd[i]) + bias) : 0.0f;
+      xs[s][at.lane] = float2{dt, dt * u[i]};
+    }
+    stage_bc<T, P, NW>(p, at, t0, bc);
+    const uint32_t flags = flags_of(p, at, t0);
+    lds_barrier();
+    if (t0 + kTile < at.t1) fetch(t0 + kTile);
+    if (OUT && p.saved != nullptr && at.ok) {
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if (n0 + i < p.N) p.saved[(((int64_t)(t0 / kTile) * p.B + at.b) * p.N + n0 + i) * p.H + at.ch] = h[i];
+    }
+    with_flags(flags, [&](auto F) __attribute__((always_inline)) {
+      constexpr bool RESET = decltype(F)::value;
+#pragma unroll
+      for (int s = 0; s < kTile; ++s) {
+        const float2 x = xs[s][at.lane];
+        const bool start = RESET && (flags >> s & 1);
+        float y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          if (PAD && i >= live) continue;
+          if (start) h[i] = 0.0f;
+          h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(x.x * A2[i]), h[i], x.y * bc[s][at.wave][i]);
+          if (OUT) y = __builtin_fmaf(bc[s][at.wave][P + i], h[i], y);
+        }
+        if constexpr (OUT) {
+          part[at.wave][s][at.lane] = y;
+        } else {
+          span += x.x;
+        }
+      }
+    });
+    if (!OUT && flags) drop = true;
+    lds_barrier();
+    if constexpr (OUT) {
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const int s = at.wave + NW * i;
+        float y = part[0][s][at.lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w)
+          if (!PAD || w * P < p.N) y += part[w][s][at.lane];
+        y = __builtin_fmaf(D, u[i], y);
+        if (p.z != nullptr) y *= z[i] * sigmoid(z[i]);
+        const int t = min(t0 + s, at.t1 - 1);
+        E::store(const_cast<T*>(row_of<T>(p.y, p.sy_t, p.sy_b, t, at.b)), t0 + s < at.t1 ? off : kOffNone, y);
+      }
+    }
+  }
+  if (!at.ok) return;
+  if constexpr (OUT) {
+    if (p.h_last != nullptr && at.chunk == p.chunks - 1) {
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if (n0 + i < p.N) p.h_last[((int64_t)at.b * p.H + at.ch) * p.N + n0 + i] = h[i];
+    }
+  } else {
+    const int64_t row = (int64_t)at.chunk * p.B + at.b;
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (n0 + i < p.N) p.ends[(row * p.N + n0 + i) * p.H + at.ch] = h[i];
+    if (at.wave == 0) p.span[row * p.H + at.ch] = span;
+    if (threadIdx.x == 0 && at.block == 0) p.dropped[row] = drop ? 1.0f : 0.0f;
+  }
+}
+
+// The states at the chunks' ends, from what each chunk makes of zero: slot c of `ends` holds
+// the latter on entry and the state after chunk c on return. BACK: the same from the last
+// chunk to the second, for the gradients that chunks send to the one before; slot c then
+// holds, on return, what chunk c sends to c - 1.
+template <bool BACK>
+__global__ __launch_bounds__(256) void ssm_join_kernel(SsmParams p) {
+  const int64_t plane = (int64_t)p.B * p.N * p.H, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= plane) return;
+  const int ch = (int)(e % p.H), n = (int)(e / p.H % p.N), b = (int)(e / p.H / p.N);
+  const float A2 = p.A[(int64_t)ch * p.N + n] * kLog2e;
+  float s = 0.0f;
+  if (!BACK && p.h0 != nullptr) s = p.h0[((int64_t)b * p.H + ch) * p.N + n];
+  if (BACK && p.dh_last != nullptr) s = p.dh_last[((int64_t)b * p.H + ch) * p.N + n];
+  const int count = p.chunks - 1;
+  constexpr int kAhead = 8;
+  for (int k0 = 0; k0 < count; k0 += kAhead) {
+    float end[kAhead], span[kAhead], drop[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int c = BACK ? p.chunks - 1 - min(k0 + k, count - 1) : min(k0 + k, count - 1);
+      end[k] = p.ends[c * plane + e];
+      span[k] = p.span[((int64_t)c * p.B + b) * p.H + ch];
+      drop[k] = p.dropped[(int64_t)c * p.B + b];
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (k0 + k >= count) break;
+      s = drop[k] != 0.0f ? end[k] : __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * span[k]), s, end[k]);
+      p.ends[(BACK ? p.chunks - 1 - (k0 + k) : k0 + k) * plane + e] = s;
+    }
+  }
+}
+
+// What a step's row holds for the backward: dt, the gradient of y before the gate.
+struct Row {
+  float dt, u, dy;
+};
+
+// The gradient that chunk c > 0 sends to the state before it, from a zero gradient after it.
+template <typename T, int P, int NW, bool PAD>
+__global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams p) {
+  typedef Elem<T> E;
+  constexpr int kOwn = kTile / NW;
+  __shared__ float2 xs[kTile][64];  // dt, dy
+  __shared__ float bc[kTile][NW][2 * P];
+  At at(p);
+  at.chunk += 1;
+  at.t0 += p.length;
+  at.t1 = min(p.T, at.t0 + p.length);
+  const int n0 = at.wave * P, live = PAD ? min(max(p.N - n0, 0), P) : P;
+  float A2[P], e[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    A2[i] = at.ok && n0 + i < p.N ? p.A[(int64_t)at.ch * p.N + n0 + i] * kLog2e : 0.0f;
+    e[i] = 0.0f;
+  }
+  const float bias = p.bias != nullptr && at.ok ? p.bias[at.ch] : 0.0f;
+  const uint32_t off = lane_off<T>(at);
+  float span = 0.0f;
+  bool drop = false;
+  unsigned int rd[kOwn], rz[kOwn], rg[kOwn];
+  auto fetch = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int t = t0 + at.wave + NW * i, r = min(t, at.t1 - 1);
+      const uint32_t o = t < at.t1 ? off : kOffNone;
+      rd[i] = E::load(row_of<T>(p.delta, p.sdl_t, p.sdl_b, r, at.b), o);
+      rg[i] = E::load(row_of<T>(p.dy, p.sdy_t, p.sdy_b, r, at.b), o);
+      if (p.z != nullptr) rz[i] = E::load(row_of<T>(p.z, p.sz_t, p.sz_b, r, at.b), o);
+    }
+  };
+  const int last = at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile;
+  fetch(last);
+  for (int t0 = last; t0 >= at.t0; t0 -= kTile) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int s = at.wave + NW * i;
+      const float dt = t0 + s < at.t1 ? softplus(E::value(rd[i]) + bias) : 0.0f;
+      float dy = E::value(rg[i]);
+      if (p.z != nullptr) {
+        const float z = E::value(rz[i]);
+        dy *= z * sigmoid(z);
+      }
+      xs[s][at.lane] = float2{dt, dy};
+    }
+    stage_bc<T, P, NW>(p, at, t0, bc);
+    const uint32_t flags = flags_of(p, at, t0);
+    lds_barrier();
+    if (t0 > at.t0) fetch(t0 - kTile);
+    with_flags(flags, [&](auto F) __attribute__((always_inline)) {
+      constexpr bool RESET = decltype(F)::value;
+#pragma unroll
+      for (int s = kTile - 1; s >= 0; --s) {
+        const float2 x = xs[s][at.lane];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          if (PAD && i >= live) continue;
+          e[i] = __builtin_amdgcn_exp2f(x.x * A2[i]) * __builtin_fmaf(bc[s][at.wave][P + i], x.y, e[i]);
+          if (RESET && (flags >> s & 1)) e[i] = 0.0f;
+        }
+        span += x.x;
+      }
+    });
+    if (flags) drop = true;
+    lds_barrier();
+  }
+  if (!at.ok) return;
+  const int64_t row = (int64_t)at.chunk * p.B + at.b;
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    if (n0 + i < p.N) p.ends[(row * p.N + n0 + i) * p.H + at.ch] = e[i];
+  if (at.wave == 0) p.span[row * p.H + at.ch] = span;
+  if (threadIdx.x == 0 && at.block == 0) p.dropped[row] = drop ? 1.0f : 0.0f;
+}
+
+template <typename T, int P, int NW, bool PAD>
+__global__ __launch_bounds__(64 * NW) void ssm_bwd_kernel(SsmParams p) {
+  typedef Elem<T> E;
+  constexpr int kOwn = kTile / NW;
+  __shared__ float2 xs[kTile][64];  // dt, dt u
+  __shared__ float ds[kTile][64];   // dy
+  __shared__ float bc[kTile][NW][2 * P];
+  // the waves' parts of y, then of S and of sum_n q A
+  __shared__ float2 part[NW][kTile][64];
+  float(*const ypart)[kTile][64] = reinterpret_cast<float(*)[kTile][64]>(&part[0][0][0]);
+  const At at(p);
+  const int n0 = at.wave * P, live = PAD ? min(max(p.N - n0, 0), P) : P;
+  const bool gated = p.z != nullptr;
+  float A[P], e[P], dA[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int n = n0 + i;
+    const bool some = at.ok && n < p.N;
+    A[i] = some ? p.A[(int64_t)at.ch * p.N + n] : 0.0f;
+    dA[i] = 0.0f;
+    e[i] = 0.0f;
+    if (some) {
+      if (at.chunk < p.chunks - 1) e[i] = p.ends[(((int64_t)(at.chunk + 1) * p.B + at.b) * p.N + n) * p.H + at.ch];
+      else if (p.dh_last != nullptr) e[i] = p.dh_last[((int64_t)at.b * p.H + at.ch) * p.N + n];
+    }
+  }
+  const float bias = p.bias != nullptr && at.ok ? p.bias[at.ch] : 0.0f;
+  const float D = p.D != nullptr && at.ok ? p.D[at.ch] : 0.0f;
+  const uint32_t off = lane_off<T>(at);
+  const bool tail = at.block == p.blocks - 1 && p.H % 64 != 0;
+  float dD = 0.0f, dbias = 0.0f;
+  unsigned int rd[kOwn], ru[kOwn], rz[kOwn], rg[kOwn];
+  auto fetch = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int t = t0 + at.wave + NW * i, r = min(t, at.t1 - 1);
+      const uint32_t o = t < at.t1 ? off : kOffNone;
+      rd[i] = E::load(row_of<T>(p.delta, p.sdl_t, p.sdl_b, r, at.b), o);
+      ru[i] = E::load(row_of<T>(p.u, p.su_t, p.su_b, r, at.b), o);
+      rg[i] = E::load(row_of<T>(p.dy, p.sdy_t, p.sdy_b, r, at.b), o);
+      if (gated) rz[i] = E::load(row_of<T>(p.z, p.sz_t, p.sz_b, r, at.b), o);
+    }
+  };
+  const int last = at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile;
+  fetch(last);
+  for (int t0 = last; t0 >= at.t0; t0 -= kTile) {
+    float u[kOwn], x[kOwn], dt[kOwn], dy[kOwn], dzy[kOwn];  // dzy: dz / y
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int s = at.wave + NW * i;
+      u[i] = E::value(ru[i]);
+      x[i] = E::value(rd[i]) + bias;
+      dt[i] = t0 + s < at.t1 ? softplus(x[i]) : 0.0f;
+      dy[i] = E::value(rg[i]);
+      dzy[i] = 0.0f;
+      if (gated) {
+        const float z = E::value(rz[i]), g = sigmoid(z);
+        dzy[i] = dy[i] * g * __builtin_fmaf(z, 1.0f - g, 1.0f);
+        dy[i] *= z * g;
+      }
+      xs[s][at.lane] = float2{dt[i], dt[i] * u[i]};
+      ds[s][at.lane] = dy[i];
+    }
+    stage_bc<T, P, NW>(p, at, t0, bc);
+    const uint32_t flags = flags_of(p, at, t0);
+    float start[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      start[i] = at.ok && n0 + i < p.N ? p.saved[(((int64_t)(t0 / kTile) * p.B + at.b) * p.N + n0 + i) * p.H + at.ch] : 0.0f;
+    lds_barrier();
+    if (t0 > at.t0) fetch(t0 - kTile);
+    with_flags(flags, [&](auto F) __attribute__((always_inline)) {
+      constexpr bool RESET = decltype(F)::value;
+      float a[kTile][P], h[kTile][P];  // h: after the step
+#pragma unroll
+      for (int s = 0; s < kTile; ++s) {
+        const float2 v = xs[s][at.lane];
+        float y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          a[s][i] = h[s][i] = 0.0f;
+          if (PAD && i >= live) continue;
+          a[s][i] = __builtin_amdgcn_exp2f(v.x * (A[i] * kLog2e));
+          float before = s ? h[s > 0 ? s - 1 : 0][i] : start[i];
+          if (RESET && (flags >> s & 1)) before = 0.0f;
+          h[s][i] = __builtin_fmaf(a[s][i], before, v.y * bc[s][at.wave][i]);
+          y = __builtin_fmaf(bc[s][at.wave][P + i], h[s][i], y);
+        }
+        if (gated) ypart[at.wave][s][at.lane] = y;
+      }
+      if (gated) {
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+          const int s = at.wave + NW * i;
+          float y = ypart[0][s][at.lane];
+#pragma unroll
+          for (int w = 1; w < NW; ++w)
+            if (!PAD || w * P < p.N) y += ypart[w][s][at.lane];
+          y = __builtin_fmaf(D, u[i], y);
+          const int t = min(t0 + s, at.t1 - 1);
+          E::store(const_cast<T*>(row_of<T>(p.dz, p.sdz_t, p.sdz_b, t, at.b)), t0 + s < at.t1 ? off : kOffNone, dzy[i] * y);
+        }
+        lds_barrier();
+      }
+      // back over the tile; sums over the lanes of dB and dC of a pair of states in one register a step
+      float sums[P > 1 ? P / 2 : 1][kTile];
+#pragma unroll
+      for (int s = kTile - 1; s >= 0; --s) {
+        const float2 v = xs[s][at.lane];
+        const float g = ds[s][at.lane];
+        float S = 0.0f, Q = 0.0f, db[P], dc[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          db[i] = dc[i] = 0.0f;
+          if (PAD && i >= live) continue;
+          const float G = __builtin_fmaf(bc[s][at.wave][P + i], g, e[i]);
+          float before = s ? h[s > 0 ? s - 1 : 0][i] : start[i];
+          e[i] = a[s][i] * G;
+          if (RESET && (flags >> s & 1)) e[i] = before = 0.0f;
+          const float q = e[i] * before;
+          S = __builtin_fmaf(G, bc[s][at.wave][i], S);
+          Q = __builtin_fmaf(q, A[i], Q);
+          dA[i] = __builtin_fmaf(q, v.x, dA[i]);
+          db[i] = G * v.y;
+          dc[i] = h[s][i] * g;
+          if (tail && !at.ok) db[i] = dc[i] = 0.0f;
+        }
+        part[at.wave][s][at.lane] = float2{S, Q};
+#pragma unroll
+        for (int i = 0; i < P; i += 2)
+          sums[i / 2][s] = join<16>(join<32>(db[i], db[i + 1]), join<32>(dc[i], dc[i + 1]));
+      }
+#pragma unroll
+      for (int k = 0; k < P / 2; ++k) {
+        float w8[8], w4[4], w2[2];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) w8[s] = join<1>(sums[k][2 * s], sums[k][2 * s + 1]);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) w4[s] = join<2>(w8[2 * s], w8[2 * s + 1]);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) w2[s] = join<4>(w4[2 * s], w4[2 * s + 1]);
+        const float sum = join<8>(w2[0], w2[1]);
+        const int t = t0 + (at.lane & 15), n = n0 + 2 * k + (at.lane >> 5);
+        if (t < at.t1 && n < p.N)
+          p.part_bc[(((int64_t)at.block * p.T + t) * p.B + at.b) * 2 * p.N + (at.lane & 16 ? p.N : 0) + n] = sum;
+      }
+    });
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      const int s = at.wave + NW * i;
+      float2 v = part[0][s][at.lane];
+#pragma unroll
+      for (int w = 1; w < NW; ++w)
+        if (!PAD || w * P < p.N) {
+          const float2 o = part[w][s][at.lane];
+          v.x += o.x;
+          v.y += o.y;
+        }
+      const float dd = __builtin_fmaf(u[i], v.x, v.y) * sigmoid(x[i]);
+      const int t = min(t0 + s, at.t1 - 1);
+      const uint32_t o = t0 + s < at.t1 ? off : kOffNone;
+      E::store(const_cast<T*>(row_of<T>(p.du, p.sdu_t, p.sdu_b, t, at.b)), o, __builtin_fmaf(dt[i], v.x, D * dy[i]));
+      E::store(const_cast<T*>(row_of<T>(p.ddelta, p.sdd_t, p.sdd_b, t, at.b)), o, dd);
+      if (t0 + s < at.t1) {
+        dD = __builtin_fmaf(u[i], dy[i], dD);
+        dbias += dd;
+      }
+    }
+  }
+  // sums over the chunk: dA of the wave's states, dD and dbias over the waves
+  const int64_t row = ((int64_t)at.chunk * p.B + at.b) * (p.N + 2);
+  if (at.ok) {
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (n0 + i < p.N) {
+        p.part_a[(row + n0 + i) * p.H + at.ch] = dA[i];
+        if (at.chunk == 0 && p.dh0 != nullptr) p.dh0[((int64_t)at.b * p.H + at.ch) * p.N + n0 + i] = e[i];
+      }
+  }
+  lds_barrier();
+  part[at.wave][0][at.lane] = float2{dD, dbias};
+  lds_barrier();
+  if (at.wave == 0 && at.ok) {
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+      dD += part[w][0][at.lane].x;
+      dbias += part[w][0][at.lane].y;
+    }
+    p.part_a[(row + p.N) * p.H + at.ch] = dD;
+    p.part_a[(row + p.N + 1) * p.H + at.ch] = dbias;
+  }
+}
+
+// dB and dC [T, B, N]: the channel blocks' sums in order.
+template <typename T>
+__global__ __launch_bounds__(256) void ssm_sum_bc_kernel(const float* part, void* dbm, void* dcm, int64_t rows, int N,
+                                                          int blocks) {
+  const int64_t plane = rows * 2 * N;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < plane; e += (int64_t)gridDim.x * 256) {
+    float s = 0.0f;
+    for (int k0 = 0; k0 < blocks; k0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = k0 + k < blocks ? part[(k0 + k) * plane + e] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k < blocks) s += x[k];
+    }
+    const int64_t row = e / (2 * N);
+    const int n = (int)(e - row * 2 * N);
+    void* dst = n < N ? dbm : dcm;
+    if (dst != nullptr) static_cast<T*>(dst)[row * N + (n < N ? n : n - N)] = (T)s;
+  }
+}
+
+// dA [H, N], dD and dbias [H]: sums over chunks and batch rows. Lanes are channels; a workgroup's four
+// waves take every fourth part, joined in order.
+__global__ __launch_bounds__(256) void ssm_sum_a_kernel(const float* part, float* dA, float* dD, float* dbias, int H, int N,
+                                                         int parts) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ch = blockIdx.x * 64 + lane, n = blockIdx.y;
+  const int64_t plane = (int64_t)(N + 2) * H;
+  const float* src = part + (int64_t)n * H + ch;
+  float s = 0.0f;
+  if (ch < H) {
+    for (int k0 = wave; k0 < parts; k0 += 4 * 8) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = k0 + 4 * k < parts ? src[(k0 + 4 * k) * plane] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k0 + 4 * k < parts) s += x[k];
+    }
+  }
+  red[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || ch >= H) return;
+  s = ((s + red[1][lane]) + red[2][lane]) + red[3][lane];
+  float* dst = n < N ? dA : n == N ? dD : dbias;
+  if (dst != nullptr) dst[n < N ? (int64_t)ch * N + n : ch] = s;
+}
+
+// One token for each row of a batch of requests, whose states are rows of a cache [S, H, N]:
+// four lanes a channel, which hold every fourth state. One launch.
+struct SsmStepParams {
+  const void *u, *delta, *z, *bm, *cm;
+  const float *A, *D, *bias;
+  float* state;
+  const int32_t* slots;
+  void* y;
+  int64_t su, sdl, sz, sb, sc, ss, sy;
+  int B, H, N, S;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepParams p) {
+  const int q = threadIdx.x & 3, ch = blockIdx.x * 64 + (threadIdx.x >> 2), b = blockIdx.y;
+  if (ch >= p.H) return;
+  const int slot = p.slots ? p.slots[b] : b;
+  T* out = static_cast<T*>(p.y) + b * p.sy + ch;
+  if (slot < 0 || slot >= p.S) {
+    if (q == 0) *out = (T)(slot < 0 ? 0.0f : __builtin_nanf(""));
+    return;
+  }
+  const float u = (float)(static_cast<const T*>(p.u) + b * p.su)[ch];
+  const float dt = softplus((float)(static_cast<const T*>(p.delta) + b * p.sdl)[ch] + (p.bias ? p.bias[ch] : 0.0f));
+  const T *bm = static_cast<const T*>(p.bm) + b * p.sb, *cm = static_cast<const T*>(p.cm) + b * p.sc;
+  const float* A = p.A + (int64_t)ch * p.N;
+  float* h = p.state + slot * p.ss + (int64_t)ch * p.N;
+  float y = 0.0f;
+  for (int n = q; n < p.N; n += 4) {
+    const float x = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * (A[n] * kLog2e)), h[n], dt * u * (float)bm[n]);
+    h[n] = x;
+    y = __builtin_fmaf((float)cm[n], x, y);
+  }
+  y += lane_xor_c<1>(y);
+  y += lane_xor_c<2>(y);
+  if (p.D) y = __builtin_fmaf(p.D[ch], u, y);
+  if (p.z) {
+    const float z = (float)(static_cast<const T*>(p.z) + b * p.sz)[ch];
+    y *= z * sigmoid(z);
+  }
+  if (q == 0) *out = (T)y;
+}
+
+// ---- host ---------------------------------------------------------------------------
+
+constexpr int kMostStates = 32;
+
+// Chunks of the time axis: workgroups for every CU, chunks of 64 steps at least.
+struct Plan {
+  int blocks, chunks, length;
+};
+Plan make_plan(int64_t T, int64_t B, int64_t H) {
+  Plan r;
+  r.blocks = (int)((H + 63) / 64);
+  const int64_t groups = r.blocks * B, want = 512;
+  int64_t chunks = std::max<int64_t>(1, std::min(want / groups, T / 64));
+  const int64_t length = (T + chunks - 1) / chunks;
+  r.length = (int)((length + kTile - 1) / kTile * kTile);
+  r.chunks = (int)((T + r.length - 1) / r.length);
+  return r;
+}
+
+typedef void (*SsmFn)(SsmParams);
+enum { kFwd, kFwdEnds, kBwd, kBwdEnds };
+template <typename T, int P, int NW, bool PAD>
+SsmFn kernel_at(int which) {
+  switch (which) {
+    case kFwd: return ssm_fwd_kernel<T, P, NW, PAD, true>;
+    case kFwdEnds: return ssm_fwd_kernel<T, P, NW, PAD, false>;
+    case kBwd: return ssm_bwd_kernel<T, P, NW, PAD>;
+    default: return ssm_bwd_ends_kernel<T, P, NW, PAD>;
+  }
+}
+template <typename T, int P, int NW>
+SsmFn kernel_in(int which, int N, int& threads) {
+  threads = 64 * NW;
+  return N == P * NW ? kernel_at<T, P, NW, false>(which) : kernel_at<T, P, NW, true>(which);
+}
+template <typename T>
+SsmFn kernel_for(int which, int N, int& threads) {
+  if (N <= 4) return kernel_in<T, 2, 2>(which, N, threads);
+  if (N <= 8) return kernel_in<T, 2, 4>(which, N, threads);
+  if (N <= 16) return kernel_in<T, 2, 8>(which, N, threads);
+  return kernel_in<T, 4, 8>(which, N, threads);
+}
+
+int launch(int which, int dtype, const SsmParams& p, int64_t groups, hipStream_t stream) {
+  int threads = 0;
+  const SsmFn fn = dtype == GS_DTYPE_F32 ? kernel_for<float>(which, p.N, threads) : kernel_for<__bf16>(which, p.N, threads);
+  hipLaunchKernelGGL(fn, dim3((unsigned)groups), dim3(threads), 0, stream, p);
+  GS_CHECK_HIP(hipGetLastError());
+  return GS_OK;
+}
+
+int check_sizes(const char* who, int64_t T, int64_t B, int64_t H, int64_t N, int dtype) {
+  if (T < 1) return set_error(GS_ERR_INVALID, "%s: seq length T must be > 0; got T=%lld", who, (long long)T);
+  if (B < 1) return set_error(GS_ERR_INVALID, "%s: batch size B must be > 0; got B=%lld", who, (long long)B);
+  if (H < 1) return set_error(GS_ERR_INVALID, "%s: channels H must be > 0; got H=%lld", who, (long long)H);
+  if (N < 1 || N > kMostStates)
+    return set_error(GS_ERR_INVALID, "%s: states N must be 1 to %d; got N=%lld", who, kMostStates, (long long)N);
+  if (T > (1ll << 30) || B > (1ll << 20) || H > (1ll << 20))
+    return set_error(GS_ERR_INVALID, "%s: T/B/H out of supported range (T=%lld, B=%lld, H=%lld)", who, (long long)T,
+                     (long long)B, (long long)H);
+  // workgroups of 512 threads, counted in 32 bits by a launch; chunks only add some where these are few
+  if ((H + 63) / 64 * B > (1ll << 22))
+    return set_error(GS_ERR_INVALID, "%s: more workgroups than a launch holds (B=%lld, H=%lld)", who, (long long)B, (long long)H);
+  return check_dtype(who, dtype);
+}
+
+struct Bytes {
+  int64_t ends = 0, span = 0, dropped = 0, bc = 0, a = 0, total = 0;  // offsets
+};
+Bytes bytes_of(const Plan& plan, int64_t T, int64_t B, int64_t H, int64_t N, bool back) {
+  Bytes r;
+  if (plan.chunks > 1) {
+    r.span = r.ends + align256(plan.chunks * B * N * H * 4);
+    r.dropped = r.span + align256(plan.chunks * B * H * 4);
+    r.total = r.dropped + align256(plan.chunks * B * 4);
+  }
+  if (back) {
+    r.bc = r.total;
+    r.a = r.bc + align256(plan.blocks * T * B * 2 * N * 4);
+    r.total = r.a + align256(plan.chunks * B * (N + 2) * H * 4);
+  }
+  return r;
+}
+
+int check_fwd(const gs_ssm_args* a, const char* who) {
+  if (a == nullptr) return set_error(GS_ERR_INVALID, "%s: args is NULL", who);
+  int rc = check_sizes(who, a->T, a->B, a->H, a->N, a->dtype);
+  if (rc) return rc;
+  if ((rc = check_step_rows(who, "u", a->T, a->B, a->H, a->su_t, a->su_b, false))) return rc;
+  if ((rc = check_step_rows(who, "delta", a->T, a->B, a->H, a->sdl_t, a->sdl_b, false))) return rc;
+  if ((rc = check_step_rows(who, "z", a->T, a->B, a->H, a->sz_t, a->sz_b, false))) return rc;
+  if ((rc = check_step_rows(who, "B", a->T, a->B, a->N, a->sb_t, a->sb_b, false))) return rc;
+  if ((rc = check_step_rows(who, "C", a->T, a->B, a->N, a->sc_t, a->sc_b, false))) return rc;
+  if ((rc = check_step_rows(who, "reset", a->T, a->B, 1, a->sr_t, a->sr_b, false))) return rc;
+  return check_step_rows(who, "y", a->T, a->B, a->H, a->sy_t, a->sy_b, true);
+}
+
+int check_bwd(const gs_ssm_bwd_args* a, const char* who) {
+  if (a == nullptr) return set_error(GS_ERR_INVALID, "%s: args is NULL", who);
+  int rc = check_sizes(who, a->T, a->B, a->H, a->N, a->dtype);
+  if (rc) return rc;
+  if ((rc = check_step_rows(who, "u", a->T, a->B, a->H, a->su_t, a->su_b, false))) return rc;
+  if ((rc = check_step_rows(who, "delta", a->T, a->B, a->H, a->sdl_t, a->sdl_b, false))) return rc;
+  if ((rc = check_step_rows(who, "z", a->T, a->B, a->H, a->sz_t, a->sz_b, false))) return rc;
+  if ((rc = check_step_rows(who, "B", a->T, a->B, a->N, a->sb_t, a->sb_b, false))) return rc;
+  if ((rc = check_step_rows(who, "C", a->T, a->B, a->N, a->sc_t, a->sc_b, false))) return rc;
+  if ((rc = check_step_rows(who, "reset", a->T, a->B, 1, a->sr_t, a->sr_b, false))) return rc;
+  if ((rc = check_step_rows(who, "dy", a->T, a->B, a->H, a->sdy_t, a->sdy_b, false))) return rc;
+  if ((rc = check_step_rows(who, "du", a->T, a->B, a->H, a->sdu_t, a->sdu_b, true))) return rc;
+  if ((rc = check_step_rows(who, "ddelta", a->T, a->B, a->H, a->sdd_t, a->sdd_b, true))) return rc;
+  return a->z ? check_step_rows(who, "dz", a->T, a->B, a->H, a->sdz_t, a->sdz_b, true) : GS_OK;
+}
+
+template <typename Args>
+SsmParams params_of(const Args* a, const Plan& plan, const Bytes& bytes) {
+  SsmParams p{};
+  p.u = a->u;
+  p.delta = a->delta;
+  p.z = a->z;
+  p.bm = a->bm;
+  p.cm = a->cm;
+  p.A = a->A;
+  p.D = a->D;
+  p.bias = a->delta_bias;
+  p.h0 = a->h0;
+  p.reset = a->reset;
+  p.su_t = a->su_t;
+  p.su_b = a->su_b;
+  p.sdl_t = a->sdl_t;
+  p.sdl_b = a->sdl_b;
+  p.sz_t = a->sz_t;
+  p.sz_b = a->sz_b;
+  p.sb_t = a->sb_t;
+  p.sb_b = a->sb_b;
+  p.sc_t = a->sc_t;
+  p.sc_b = a->sc_b;
+  p.sr_t = a->sr_t;
+  p.sr_b = a->sr_b;
+  p.T = (int)a->T;
+  p.B = (int)a->B;
+  p.H = (int)a->H;
+  p.N = (int)a->N;
+  p.blocks = plan.blocks;
+  p.chunks = plan.chunks;
+  p.length = plan.length;
+  char* s = static_cast<char*>(a->scratch);
+  p.ends = reinterpret_cast<float*>(s + bytes.ends);
+  p.span = reinterpret_cast<float*>(s + bytes.span);
+  p.dropped = reinterpret_cast<float*>(s + bytes.dropped);
+  p.part_bc = reinterpret_cast<float*>(s + bytes.bc);
+  p.part_a = reinterpret_cast<float*>(s + bytes.a);
+  return p;
+}
+
+int join_ends(const SsmParams& p, bool back, hipStream_t stream) {
+  const int64_t n = (int64_t)p.B * p.N * p.H;
+  hipLaunchKernelGGL(back ? ssm_join_kernel<true> : ssm_join_kernel<false>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0,
+                     stream, p);
+  GS_CHECK_HIP(hipGetLastError());
+  return GS_OK;
+}
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" int64_t gs_ssm_scratch_bytes(const gs_ssm_args* a) {
+  clear_error();
+  const int rc = check_fwd(a, "gs_ssm_scratch_bytes");
+  return rc ? rc : bytes_of(make_plan(a->T, a->B, a->H), a->T, a->B, a->H, a->N, false).total;
+}
+
+extern "C" int64_t gs_ssm_saved_bytes(const gs_ssm_args* a) {
+  clear_error();
+  const int rc = check_fwd(a, "gs_ssm_saved_bytes");
+  return rc ? rc : (a->T + kTile - 1) / kTile * a->B * a->N * a->H * 4;
+}
+
+extern "C" int gs_ssm_fwd(const gs_ssm_args* a, hipStream_t stream) {
+  const char* who = "gs_ssm_fwd";
+  clear_error();
+  int rc = check_fwd(a, who);
+  if (rc) return rc;
+  if (!a->u || !a->delta || !a->bm || !a->cm || !a->A || !a->y)
+    return set_error(GS_ERR_INVALID, "%s: u, delta, A, bm, cm and y must be non-NULL device pointers", who);
+  const Plan plan = make_plan(a->T, a->B, a->H);
+  const Bytes bytes = bytes_of(plan, a->T, a->B, a->H, a->N, false);
+  if ((rc = check_plain_scratch(who, a->scratch, a->scratch_bytes, bytes.total))) return rc;
+  SsmParams p = params_of(a, plan, bytes);
+  p.y = a->y;
+  p.h_last = a->h_last;
+  p.saved = a->saved;
+  p.sy_t = a->sy_t;
+  p.sy_b = a->sy_b;
+  const int64_t each = (int64_t)plan.blocks * a->B;
+  if (plan.chunks > 1) {
+    if ((rc = launch(kFwdEnds, a->dtype, p, each * (plan.chunks - 1), stream))) return rc;
+    if ((rc = join_ends(p, false, stream))) return rc;
+  }
+  return launch(kFwd, a->dtype, p, each * plan.chunks, stream);
+}
+
+extern "C" int64_t gs_ssm_bwd_scratch_bytes(const gs_ssm_bwd_args* a) {
+  clear_error();
+  const int rc = check_bwd(a, "gs_ssm_bwd_scratch_bytes");
+  return rc ? rc : bytes_of(make_plan(a->T, a->B, a->H), a->T, a->B, a->H, a->N, true).total;
+}
+
+extern "C" int gs_ssm_bwd(const gs_ssm_bwd_args* a, hipStream_t stream) {
+  const char* who = "gs_ssm_bwd";
+  clear_error();
+  int rc = check_bwd(a, who);
+  if (rc) return rc;
+  if (!a->u || !a->delta || !a->bm || !a->cm || !a->A || !a->saved || !a->dy || !a->du || !a->ddelta || (a->z && !a->dz))
+    return set_error(GS_ERR_INVALID, "%s: u, delta, A, bm, cm, saved, dy, du and ddelta (and dz where z is given) must be "
+                     "non-NULL device pointers", who);
+  const Plan plan = make_plan(a->T, a->B, a->H);
+  const Bytes bytes = bytes_of(plan, a->T, a->B, a->H, a->N, true);
+  if ((rc = check_plain_scratch(who, a->scratch, a->scratch_bytes, bytes.total))) return rc;
+  SsmParams p = params_of(a, plan, bytes);
+  p.saved = const_cast<float*>(a->saved);
+  p.dy = a->dy;
+  p.dh_last = a->dh_last;
+  p.du = a->du;
+  p.ddelta = a->ddelta;
+  p.dz = a->dz;
+  p.dh0 = a->dh0;
+  p.sdy_t = a->sdy_t;
+  p.sdy_b = a->sdy_b;
+  p.sdu_t = a->sdu_t;
+  p.sdu_b = a->sdu_b;
+  p.sdd_t = a->sdd_t;
+  p.sdd_b = a->sdd_b;
+  p.sdz_t = a->sdz_t;
+  p.sdz_b = a->sdz_b;
+  const int64_t each = (int64_t)plan.blocks * a->B, rows = a->T * a->B;
+  if (plan.chunks > 1) {
+    if ((rc = launch(kBwdEnds, a->dtype, p, each * (plan.chunks - 1), stream))) return rc;
+    if ((rc = join_ends(p, true, stream))) return rc;
+  }
+  if ((rc = launch(kBwd, a->dtype, p, each * plan.chunks, stream))) return rc;
+  if (a->dbm != nullptr || a->dcm != nullptr) {
+    const dim3 grid((unsigned)std::min<int64_t>((rows * 2 * a->N + 255) / 256, 1 << 20));
+    hipLaunchKernelGGL(a->dtype == GS_DTYPE_F32 ? ssm_sum_bc_kernel<float> : ssm_sum_bc_kernel<__bf16>, grid, dim3(256), 0,
+                       stream, p.part_bc, a->dbm, a->dcm, rows, (int)a->N, plan.blocks);
+    GS_CHECK_HIP(hipGetLastError());
+  }
+  if (a->dA != nullptr || a->dD != nullptr || a->ddelta_bias != nullptr) {
+    hipLaunchKernelGGL(ssm_sum_a_kernel, dim3((unsigned)plan.blocks, (unsigned)(a->N + 2)), dim3(256), 0, stream, p.part_a,
+                       a->dA, a->dD, a->ddelta_bias, (int)a->H, (int)a->N, (int)(plan.chunks * a->B));
+    GS_CHECK_HIP(hipGetLastError());
+  }
+  return GS_OK;
+}
+
+extern "C" int gs_ssm_step(const gs_ssm_step_args* a, hipStream_t stream) {
+  const char* who = "gs_ssm_step";
+  clear_error();
+  if (a == nullptr) return set_error(GS_ERR_INVALID, "%s: args is NULL", who);
+  const int rc = check_sizes(who, 1, a->B, a->H, a->N, a->dtype);
+  if (rc) return rc;
+  if (!a->u || !a->delta || !a->bm || !a->cm || !a->A || !a->state || !a->y)
+    return set_error(GS_ERR_INVALID, "%s: u, delta, A, bm, cm, state and y must be non-NULL device pointers", who);
+  if (a->S < 1 || a->S > (1ll << 30) || (a->slots == nullptr && a->S < a->B))
+    return set_error(GS_ERR_INVALID, "%s: a cache of S=%lld states does not hold B=%lld rows", who, (long long)a->S,
+                     (long long)a->B);
+  if (a->su < 0 || a->sdl < 0 || a->sz < 0 || a->sb < 0 || a->sc < 0 || (a->S > 1 && a->ss < a->H * a->N) ||
+      (a->B > 1 && a->sy < a->H))
+    return set_error(GS_ERR_INVALID, "%s: strides do not describe rows of H=%lld and states of [H, N]", who, (long long)a->H);
+  if (a->B > 65535) return set_error(GS_ERR_INVALID, "%s: B=%lld exceeds 65535", who, (long long)a->B);
+  SsmStepParams p{a->u, a->delta, a->z, a->bm, a->cm, a->A, a->D, a->delta_bias, a->state, a->slots, a->y,
+                  a->su, a->sdl, a->sz, a->sb, a->sc, a->ss, a->sy, (int)a->B, (int)a->H, (int)a->N, (int)a->S};
+  hipLaunchKernelGGL(a->dtype == GS_DTYPE_F32 ? ssm_step_kernel<float> : ssm_step_kernel<__bf16>,
+                     dim3((unsigned)((a->H + 63) / 64), (unsigned)a->B), dim3(256), 0, stream, p);
+  GS_CHECK_HIP(hipGetLastError());
+  return GS_OK;
+}

@@ -34,6 +34,10 @@ from .calibration import calibrate, freeze_all
 from .gated_linear import gated_linear_scan, gated_linear_step
 from .gated_layer import GatedLinearLayer
 from .linear import linear_act
+from .conv import causal_conv, causal_conv_step
+from .selective import selective_scan, selective_step
+from .selective_layer import SelectiveLayer
+from .tokens import embedding, token_logprobs
 from .optim import AdamW, adamw_dequantize_state, adamw_step
 from .export import dequantize_int_weights, export_int_weights, quantize_rows
 
@@ -43,12 +47,16 @@ __all__ = [
     "adamw_step",
     "FakeQuantizePerTensor",
     "GatedLinearLayer",
+    "SelectiveLayer",
     "GRUScanFunction",
     "GRUScanPersistentFunction",
     "QuantizerConfig",
     "ScanLayer",
     "calibrate",
+    "causal_conv",
+    "causal_conv_step",
     "dequantize_int_weights",
+    "embedding",
     "export_int_weights",
     "extract_butterfly_twiddles",
     "extract_diagonal_factors",
@@ -78,6 +86,9 @@ __all__ = [
     "quantize_input_weights",
     "quantize_rows",
     "resolve_use_triton",
+    "selective_scan",
+    "selective_step",
+    "token_logprobs",
     "workspace_faults",
     "structured_input_projection",
     "gru_scan_circulant",

@@ -75,6 +75,22 @@ EXPORTS = (
     "gs_linear_bwd",
     "gs_adamw_step",
     "gs_adamw_dequantize",
+    "gs_conv_fwd",
+    "gs_conv_bwd_scratch_bytes",
+    "gs_conv_bwd",
+    "gs_conv_step",
+    "gs_ssm_scratch_bytes",
+    "gs_ssm_saved_bytes",
+    "gs_ssm_fwd",
+    "gs_ssm_bwd_scratch_bytes",
+    "gs_ssm_bwd",
+    "gs_ssm_step",
+    "gs_embedding_fwd",
+    "gs_embedding_bwd_scratch_bytes",
+    "gs_embedding_bwd",
+    "gs_logprobs_scratch_bytes",
+    "gs_logprobs_fwd",
+    "gs_logprobs_bwd",
     "gs_workspace_bytes",
     "gs_bwd_workspace_bytes",
     "gs_bwd_scratch_bytes",
@@ -83,7 +99,7 @@ EXPORTS = (
     "gs_abi_version",
 )
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 QuantTuple = Optional[Tuple[float, int, int]]
 
@@ -416,6 +432,98 @@ class GsLinearBwdArgs(ctypes.Structure):
     )
 
 
+class GsConvArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("x", "w", "bias", "state", "reset", "y", "last")]
+        + [(k, ctypes.c_int64) for k in ("T", "B", "C", "W", "sx_t", "sx_b", "sr_t", "sr_b", "sy_t", "sy_b")]
+        + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
+    )
+
+
+class GsConvBwdArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("x", "w", "bias", "state", "reset", "dy", "dlast", "dx", "dstate", "dw",
+                                        "dbias", "scratch")]
+        + [(k, ctypes.c_int64) for k in ("scratch_bytes", "T", "B", "C", "W", "sx_t", "sx_b", "sr_t", "sr_b",
+                                         "sdy_t", "sdy_b", "sdx_t", "sdx_b")]
+        + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
+    )
+
+
+class GsConvStepArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("x", "w", "bias", "state", "slots", "y")]
+        + [(k, ctypes.c_int64) for k in ("B", "C", "W", "S", "sx", "ss", "sy")]
+        + [(k, ctypes.c_int32) for k in ("dtype", "activation")]
+    )
+
+
+class GsSsmArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("u", "delta", "z", "bm", "cm", "A", "D", "delta_bias", "h0", "reset", "y",
+                                        "h_last", "saved", "scratch")]
+        + [(k, ctypes.c_int64) for k in ("scratch_bytes", "T", "B", "H", "N", "su_t", "su_b", "sdl_t", "sdl_b",
+                                         "sz_t", "sz_b", "sb_t", "sb_b", "sc_t", "sc_b", "sr_t", "sr_b", "sy_t",
+                                         "sy_b")]
+        + [(k, ctypes.c_int32) for k in ("dtype",)]
+    )
+
+
+class GsSsmBwdArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("u", "delta", "z", "bm", "cm", "A", "D", "delta_bias", "h0", "reset",
+                                        "saved", "dy", "dh_last", "du", "ddelta", "dz", "dbm", "dcm", "dA", "dD",
+                                        "ddelta_bias", "dh0", "scratch")]
+        + [(k, ctypes.c_int64) for k in ("scratch_bytes", "T", "B", "H", "N", "su_t", "su_b", "sdl_t", "sdl_b",
+                                         "sz_t", "sz_b", "sb_t", "sb_b", "sc_t", "sc_b", "sr_t", "sr_b", "sdy_t",
+                                         "sdy_b", "sdu_t", "sdu_b", "sdd_t", "sdd_b", "sdz_t", "sdz_b")]
+        + [(k, ctypes.c_int32) for k in ("dtype",)]
+    )
+
+
+class GsSsmStepArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("u", "delta", "z", "bm", "cm", "A", "D", "delta_bias", "state", "slots", "y")]
+        + [(k, ctypes.c_int64) for k in ("B", "H", "N", "S", "su", "sdl", "sz", "sb", "sc", "ss", "sy")]
+        + [(k, ctypes.c_int32) for k in ("dtype",)]
+    )
+
+
+class GsEmbeddingArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("tokens", "w", "out")]
+        + [(k, ctypes.c_int64) for k in ("M", "V", "K", "so")]
+        + [(k, ctypes.c_float) for k in ("scale",)]
+        + [(k, ctypes.c_int32) for k in ("token_bits", "dtype")]
+    )
+
+
+class GsEmbeddingBwdArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("tokens", "dout", "dw", "scratch")]
+        + [(k, ctypes.c_int64) for k in ("scratch_bytes", "M", "V", "K", "sdo")]
+        + [(k, ctypes.c_float) for k in ("scale",)]
+        + [(k, ctypes.c_int32) for k in ("token_bits", "dtype")]
+    )
+
+
+class GsLogprobsArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("x", "tokens", "logprob", "entropy", "stats", "top_logprob", "top_token",
+                                        "scratch")]
+        + [(k, ctypes.c_int64) for k in ("scratch_bytes", "M", "V", "top", "sx")]
+        + [(k, ctypes.c_int32) for k in ("token_bits", "dtype")]
+    )
+
+
+class GsLogprobsBwdArgs(ctypes.Structure):
+    _fields_ = (
+        [(k, ctypes.c_void_p) for k in ("x", "tokens", "entropy", "stats", "dlogprob", "dentropy", "dx")]
+        + [(k, ctypes.c_int64) for k in ("M", "V", "sx", "sdx")]
+        + [(k, ctypes.c_int32) for k in ("token_bits", "dtype")]
+    )
+
+
 class GsAdamwTensor(ctypes.Structure):
     _fields_ = (
         [(k, ctypes.c_void_p) for k in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale",
@@ -487,6 +595,20 @@ def load() -> ctypes.CDLL:
             run.argtypes = [ctypes.POINTER(argt), ctypes.c_void_p]
             run.restype = ctypes.c_int
             size = getattr(lib, name + "_scratch_bytes")
+            size.argtypes = [ctypes.POINTER(argt)]
+            size.restype = ctypes.c_int64
+        for name, argt in (("gs_conv_fwd", GsConvArgs), ("gs_conv_bwd", GsConvBwdArgs), ("gs_conv_step", GsConvStepArgs),
+                           ("gs_ssm_fwd", GsSsmArgs), ("gs_ssm_bwd", GsSsmBwdArgs), ("gs_ssm_step", GsSsmStepArgs),
+                           ("gs_embedding_fwd", GsEmbeddingArgs), ("gs_embedding_bwd", GsEmbeddingBwdArgs),
+                           ("gs_logprobs_fwd", GsLogprobsArgs), ("gs_logprobs_bwd", GsLogprobsBwdArgs)):
+            run = getattr(lib, name)
+            run.argtypes = [ctypes.POINTER(argt), ctypes.c_void_p]
+            run.restype = ctypes.c_int
+        for name, argt in (("gs_conv_bwd_scratch_bytes", GsConvBwdArgs), ("gs_ssm_scratch_bytes", GsSsmArgs),
+                           ("gs_ssm_saved_bytes", GsSsmArgs), ("gs_ssm_bwd_scratch_bytes", GsSsmBwdArgs),
+                           ("gs_embedding_bwd_scratch_bytes", GsEmbeddingBwdArgs),
+                           ("gs_logprobs_scratch_bytes", GsLogprobsArgs)):
+            size = getattr(lib, name)
             size.argtypes = [ctypes.POINTER(argt)]
             size.restype = ctypes.c_int64
         lib.gs_adamw_step.argtypes = [ctypes.POINTER(GsAdamwArgs), ctypes.c_void_p]

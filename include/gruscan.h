@@ -62,7 +62,7 @@
 extern "C" {
 #endif
 
-#define GS_ABI_VERSION 9
+#define GS_ABI_VERSION 10
 
 #define GS_OK 0
 #define GS_ERR_INVALID (-1)  /* bad pointer, shape, stride or quant parameter (Python: ValueError) */
@@ -768,6 +768,201 @@ int gs_adamw_step(const gs_adamw_args* args, hipStream_t stream);
  * uint8 codes of exp_avg_sq, otherwise the int8 ones of exp_avg. */
 int gs_adamw_dequantize(const void* codes, const float* scale, float* out, int64_t n, int32_t second,
                         hipStream_t stream);
+
+/* ---- short causal convolution (ABI version 10) --------------------------------------
+ *   pre_t = bias + sum_k w[c][k] x_{t-W+1+k},  y = act(pre)   (GS_ACT_NONE or GS_ACT_SILU)
+ * of each channel over time, W = 2 to 4 taps. Inputs before the first step are those of
+ * `state` (zero where NULL); reset[t][b] != 0 starts a new sequence at step t, for which
+ * everything before counts as zero, whatever it holds. `last` receives the inputs of the last
+ * W - 1 steps (of `state` where there are fewer), zero before the last start, with which a
+ * following call continues. All tensors are of one type (GS_DTYPE_*), sums are fp32. No
+ * counterpart in the reference. */
+typedef struct gs_conv_args {
+  const void* x;         /* [T, B, C], strides sx_t, sx_b, 1                              */
+  const void* w;         /* [C, W] contiguous                                             */
+  const void* bias;      /* [C] or NULL                                                   */
+  const void* state;     /* [B, W - 1, C] contiguous, oldest first, or NULL               */
+  const uint8_t* reset;  /* [T, B], strides sr_t, sr_b (bytes), or NULL                   */
+  void* y;               /* [T, B, C], strides sy_t, sy_b, 1; rows must not overlap       */
+  void* last;            /* [B, W - 1, C] contiguous, or NULL                             */
+  int64_t T, B, C, W;
+  int64_t sx_t, sx_b, sr_t, sr_b, sy_t, sy_b;
+  int32_t dtype, activation;
+} gs_conv_args;
+
+int gs_conv_fwd(const gs_conv_args* args, hipStream_t stream);
+
+/* Gradients of gs_conv_fwd; pre is computed again from x. dstate, dw and dbias may be NULL. */
+typedef struct gs_conv_bwd_args {
+  const void *x, *w, *bias, *state; /* the forward's                                      */
+  const uint8_t* reset;
+  const void* dy;        /* [T, B, C], strides sdy_t, sdy_b, 1                            */
+  const void* dlast;     /* [B, W - 1, C] contiguous: gradient of `last`, or NULL         */
+  void* dx;              /* [T, B, C], strides sdx_t, sdx_b, 1; rows must not overlap     */
+  void* dstate;          /* [B, W - 1, C] contiguous                                      */
+  void* dw;              /* [C, W]                                                        */
+  void* dbias;           /* [C]                                                           */
+  void* scratch;         /* gs_conv_bwd_scratch_bytes() bytes, 256-byte aligned           */
+  int64_t scratch_bytes;
+  int64_t T, B, C, W;
+  int64_t sx_t, sx_b, sr_t, sr_b, sdy_t, sdy_b, sdx_t, sdx_b;
+  int32_t dtype, activation;
+} gs_conv_bwd_args;
+
+int64_t gs_conv_bwd_scratch_bytes(const gs_conv_bwd_args* args);
+int gs_conv_bwd(const gs_conv_bwd_args* args, hipStream_t stream);
+
+/* One step for serving: row b of x [B, C] is convolved with the inputs in row slots[b] of a
+ * cache [S, W - 1, C], which moves on by one in place. Slots are gs_glr_step's: NULL, negative
+ * and out of range ones mean the same. */
+typedef struct gs_conv_step_args {
+  const void* x;         /* [B, C], row stride sx                                         */
+  const void* w;
+  const void* bias;
+  void* state;           /* [S, W - 1, C], slot stride ss, rows contiguous                */
+  const int32_t* slots;
+  void* y;               /* [B, C], row stride sy                                         */
+  int64_t B, C, W, S;
+  int64_t sx, ss, sy;
+  int32_t dtype, activation;
+} gs_conv_step_args;
+
+int gs_conv_step(const gs_conv_step_args* args, hipStream_t stream);
+
+/* ---- selective state space scan (ABI version 10) ------------------------------------
+ *   dt = softplus(delta + delta_bias),  a[n] = exp(dt A[c][n]),
+ *   h_t[n] = a[n] h_{t-1}[n] + dt u bm_t[n],
+ *   y = (sum_n cm_t[n] h_t[n] + D u) silu(z)
+ * of every channel c with N states (1 to 32) each. bm and cm are shared by a row's channels.
+ * reset[t][b] != 0 takes h_{t-1} as 0 at step t, whatever it held. u, delta, z, bm, cm, y
+ * and their gradients are of one type; A, D, delta_bias, states and every sum are fp32. A
+ * training forward stores the states before every 16th step in `saved`. No counterpart in the
+ * reference. */
+typedef struct gs_ssm_args {
+  const void *u, *delta, *z; /* [T, B, H], strides s*_t, s*_b, 1; z may be NULL (no gate)  */
+  const void *bm, *cm;       /* [T, B, N], strides s*_t, s*_b, 1                          */
+  const float* A;            /* [H, N] contiguous                                         */
+  const float* D;            /* [H] or NULL                                               */
+  const float* delta_bias;   /* [H] or NULL                                               */
+  const float* h0;           /* [B, H, N] contiguous, or NULL for zeros                   */
+  const uint8_t* reset;      /* [T, B], strides sr_t, sr_b (bytes), or NULL               */
+  void* y;                   /* [T, B, H], strides sy_t, sy_b, 1; rows must not overlap   */
+  float* h_last;             /* [B, H, N] contiguous, or NULL                             */
+  float* saved;              /* gs_ssm_saved_bytes() bytes, or NULL                       */
+  void* scratch;             /* gs_ssm_scratch_bytes() bytes, 256-byte aligned            */
+  int64_t scratch_bytes;
+  int64_t T, B, H, N;
+  int64_t su_t, su_b, sdl_t, sdl_b, sz_t, sz_b, sb_t, sb_b, sc_t, sc_b, sr_t, sr_b, sy_t, sy_b;
+  int32_t dtype;
+} gs_ssm_args;
+
+int64_t gs_ssm_scratch_bytes(const gs_ssm_args* args);
+int64_t gs_ssm_saved_bytes(const gs_ssm_args* args);
+int gs_ssm_fwd(const gs_ssm_args* args, hipStream_t stream);
+
+/* Gradients of gs_ssm_fwd. dbm, dcm, dA, dD, ddelta_bias and dh0 may be NULL. */
+typedef struct gs_ssm_bwd_args {
+  const void *u, *delta, *z, *bm, *cm; /* the forward's                                   */
+  const float *A, *D, *delta_bias, *h0;
+  const uint8_t* reset;
+  const float* saved;        /* the forward's                                             */
+  const void* dy;            /* [T, B, H], strides sdy_t, sdy_b, 1                        */
+  const float* dh_last;      /* [B, H, N] contiguous: gradient of h_last, or NULL         */
+  void *du, *ddelta, *dz;    /* [T, B, H], strides s*_t, s*_b, 1; rows must not overlap   */
+  void *dbm, *dcm;           /* [T, B, N] contiguous                                      */
+  float *dA, *dD, *ddelta_bias, *dh0; /* [H, N], [H], [H], [B, H, N]                      */
+  void* scratch;             /* gs_ssm_bwd_scratch_bytes() bytes, 256-byte aligned        */
+  int64_t scratch_bytes;
+  int64_t T, B, H, N;
+  int64_t su_t, su_b, sdl_t, sdl_b, sz_t, sz_b, sb_t, sb_b, sc_t, sc_b, sr_t, sr_b, sdy_t, sdy_b;
+  int64_t sdu_t, sdu_b, sdd_t, sdd_b, sdz_t, sdz_b;
+  int32_t dtype;
+} gs_ssm_bwd_args;
+
+int64_t gs_ssm_bwd_scratch_bytes(const gs_ssm_bwd_args* args);
+int gs_ssm_bwd(const gs_ssm_bwd_args* args, hipStream_t stream);
+
+/* One step for serving: row b advances the state slots[b] of a cache [S, H, N] in place.
+ * Slots are gs_glr_step's. */
+typedef struct gs_ssm_step_args {
+  const void *u, *delta, *z; /* [B, H], row strides su, sdl, sz; z may be NULL            */
+  const void *bm, *cm;       /* [B, N], row strides sb, sc                                */
+  const float *A, *D, *delta_bias;
+  float* state;              /* [S, H, N], slot stride ss, [H, N] contiguous              */
+  const int32_t* slots;      /* [B] or NULL                                               */
+  void* y;                   /* [B, H], row stride sy                                     */
+  int64_t B, H, N, S;
+  int64_t su, sdl, sz, sb, sc, ss, sy;
+  int32_t dtype;
+} gs_ssm_step_args;
+
+int gs_ssm_step(const gs_ssm_step_args* args, hipStream_t stream);
+
+/* ---- embedding (ABI version 10) -----------------------------------------------------
+ * out[m] = scale w[tokens[m]], and dw[v] = scale (sum of dout[m] over the m of token v), with
+ * sums in fp32 and zeros where a token does not occur. A negative token marks padding (a row
+ * of zeros, no gradient), one of V or more gives NaN and no gradient. */
+typedef struct gs_embedding_args {
+  const void* tokens;    /* [M], int32 or int64 (token_bits 32 or 64)                     */
+  const void* w;         /* [V, K] contiguous                                             */
+  void* out;             /* [M, K], row stride so                                         */
+  int64_t M, V, K, so;
+  float scale;
+  int32_t token_bits, dtype;
+} gs_embedding_args;
+
+int gs_embedding_fwd(const gs_embedding_args* args, hipStream_t stream);
+
+typedef struct gs_embedding_bwd_args {
+  const void* tokens;
+  const void* dout;      /* [M, K], row stride sdo                                        */
+  void* dw;              /* [V, K] contiguous, all of it written                          */
+  void* scratch;         /* gs_embedding_bwd_scratch_bytes() bytes, 256-byte aligned      */
+  int64_t scratch_bytes;
+  int64_t M, V, K, sdo;
+  float scale;
+  int32_t token_bits, dtype;
+} gs_embedding_bwd_args;
+
+int64_t gs_embedding_bwd_scratch_bytes(const gs_embedding_bwd_args* args);
+int gs_embedding_bwd(const gs_embedding_bwd_args* args, hipStream_t stream);
+
+/* ---- log probabilities of given tokens (ABI version 10) -------------------------------
+ * Of logits x [M, V]: logprob[m] = log softmax(x[m])[tokens[m]], entropy[m] = -sum p log p, and
+ * the `top` (0 to 32) likeliest tokens in falling order, of equal ones the lowest index first,
+ * with their log probabilities. Results are fp32. A logit of -infinity is a token that cannot
+ * come; a row of those alone has log probabilities -infinity, entropy 0 and no gradient. A NaN
+ * or +infinity makes a row's results NaN. A negative token has log probability 0 and sends no
+ * gradient, one of V or more NaN. */
+typedef struct gs_logprobs_args {
+  const void* x;         /* [M, V], row stride sx                                         */
+  const void* tokens;    /* [M], int32 or int64                                           */
+  float* logprob;        /* [M]                                                           */
+  float* entropy;        /* [M]                                                           */
+  float* stats;          /* [M, 2]: kept for the backward, or NULL                        */
+  float* top_logprob;    /* [M, top]                                                      */
+  int64_t* top_token;    /* [M, top]                                                      */
+  void* scratch;         /* gs_logprobs_scratch_bytes() bytes, 256-byte aligned           */
+  int64_t scratch_bytes;
+  int64_t M, V, top, sx;
+  int32_t token_bits, dtype;
+} gs_logprobs_args;
+
+int64_t gs_logprobs_scratch_bytes(const gs_logprobs_args* args);
+int gs_logprobs_fwd(const gs_logprobs_args* args, hipStream_t stream);
+
+/* dx[m][v] = dlogprob[m] ([v = token] - p_v) - dentropy[m] p_v (log p_v + entropy). */
+typedef struct gs_logprobs_bwd_args {
+  const void* x;
+  const void* tokens;
+  const float *entropy, *stats;       /* the forward's                                    */
+  const float *dlogprob, *dentropy;   /* [M] each, or NULL                                */
+  void* dx;              /* [M, V], row stride sdx                                        */
+  int64_t M, V, sx, sdx;
+  int32_t token_bits, dtype;
+} gs_logprobs_bwd_args;
+
+int gs_logprobs_bwd(const gs_logprobs_bwd_args* args, hipStream_t stream);
 
 /* Message for the last failing call on this thread ("" if none). */
 const char* gs_last_error(void);
