@@ -28,6 +28,14 @@ struct Elem {
   static __device__ __forceinline__ float value(unsigned int w) { return __uint_as_float(sizeof(T) == 2 ? w << 16 : w); }
 };
 
+// A workgroup barrier that orders LDS alone (global loads stay in flight), for the compiler too:
+// values read from LDS before it are read again after it.
+__device__ __forceinline__ void share_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // In lanes whose bit M is clear a[l] + a[l ^ M], in the others b[l] + b[l ^ M]: six of these,
 // each over half as many registers as the one before, leave 64 sums over a wave in one register.
 template <int M>

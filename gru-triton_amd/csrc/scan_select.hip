@@ -25,6 +25,7 @@ namespace gs {
 namespace {
 
 constexpr int kTile = 16;  // steps of a tile, and between kept states
+constexpr float kLn2 = 0.6931471805599453f;
 
 struct SsmParams {
   const void *u, *delta, *z, *bm, *cm;
@@ -47,24 +48,35 @@ struct SsmParams {
   int T, B, H, N;
   int blocks;          // channel blocks of 64
   int chunks, length;  // of the time axis, in steps
+  int each;            // backward: parts of a chunk whose ends are found one by one
 };
+
+// The kernel's arguments, read anew from memory wherever this is called: kept in scalar
+// registers throughout, forty strides and pointers would be spilled to lanes of vector ones.
+typedef const __attribute__((address_space(4))) SsmParams* Args;
+__device__ __forceinline__ Args args() {
+  Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
 // Where a workgroup is.
 struct At {
   int block, b, chunk, lane, wave, ch, t0, t1;
   bool ok;  // the lane's channel exists
-  __device__ __forceinline__ explicit At(const SsmParams& p) {
+  // `first`: the chunk of the launch's first workgroups; `length`: of a chunk
+  __device__ __forceinline__ At(const SsmParams& p, int first, int length) {
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int g = blockIdx.x;
     block = g % p.blocks;
     g /= p.blocks;
     b = g % p.B;
-    chunk = g / p.B;
+    chunk = first + g / p.B;
     ch = block * 64 + lane;
     ok = ch < p.H;
-    t0 = chunk * p.length;
-    t1 = min(p.T, t0 + p.length);
+    t0 = chunk * length;
+    t1 = min(p.T, t0 + length);
   }
 };
 
@@ -72,34 +84,63 @@ template <typename T>
 __device__ __forceinline__ uint32_t lane_off(const At& at) {
   return at.ok ? (uint32_t)(at.ch * (int)sizeof(T)) : kOffNone;
 }
+// Row t of batch row b. One past the axis is only named, with an offset that reads and writes nothing.
 template <typename T>
-__device__ __forceinline__ const T* row_of(const void* base, int64_t st, int64_t sb, int t, int b) {
-  return static_cast<const T*>(base) + t * st + b * sb;
+__device__ __forceinline__ T* row_of(const void* base, int64_t st, int64_t sb, int t, int b) {
+  return const_cast<T*>(static_cast<const T*>(base)) + t * st + b * sb;
 }
 
 // The flags of a tile's steps as a bit mask.
-__device__ __forceinline__ uint32_t flags_of(const SsmParams& p, const At& at, int t0) {
-  if (p.reset == nullptr) return 0;
+__device__ __forceinline__ uint32_t flags_of(Args p, const At& at, int t0) {
+  if (p->reset == nullptr) return 0;
   bool f = false;
-  if (at.lane < kTile && t0 + at.lane < at.t1) f = p.reset[(t0 + at.lane) * p.sr_t + at.b * p.sr_b] != 0;
+  if (at.lane < kTile && t0 + at.lane < at.t1) f = p->reset[(t0 + at.lane) * p->sr_t + at.b * p->sr_b] != 0;
   return (uint32_t)__builtin_amdgcn_ballot_w64(f);
 }
 
 // B and C of a tile as floats, a wave's P states side by side; zero where there is no step or state.
-template <typename T, int P, int NW>
-__device__ __forceinline__ void stage_bc(const SsmParams& p, const At& at, int t0, float (*bc)[NW][2 * P]) {
-  constexpr int NP = NW * P, kAll = kTile * 2 * NP;
+typedef float f4v __attribute__((ext_vector_type(4)));
+// B, then C of a wave's P states. Read in accesses of 16 bytes, whose offsets are part of the
+// instruction: shorter ones in pairs need a register for the address of every fourth step.
+template <int P>
+struct alignas(16) Pair {
+  float x[2 * P];
+  __device__ __forceinline__ void read(float (&b)[P], float (&c)[P]) const {
+    float v[2 * P];
 #pragma unroll
-  for (int k = 0; k < kAll; k += 64 * NW) {
-    const int e = k + threadIdx.x;
-    if (kAll % (64 * NW) == 0 || e < kAll) {
-      const int s = e / (2 * NP), r = e % (2 * NP), c = r / NP, n = r % NP, t = t0 + s;
-      float x = 0.0f;
-      if (n < p.N && t < at.t1)
-        x = (float)(c ? row_of<T>(p.cm, p.sc_t, p.sc_b, t, at.b) : row_of<T>(p.bm, p.sb_t, p.sb_b, t, at.b))[n];
-      bc[s][n / P][c * P + n % P] = x;
+    for (int i = 0; i < 2 * P; i += 4) {
+      const f4v q = *reinterpret_cast<const f4v*>(x + i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[i + k] = q[k];
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      b[i] = v[i];
+      c[i] = v[P + i];
     }
   }
+};
+template <typename T, int P, int NW>
+__device__ __forceinline__ void stage_bc(Args p, const At& at, int t0, Pair<P> (*bc)[NW]) {
+  constexpr int NP = NW * P, kEach = kTile * NP;
+  static_assert(kEach % 64 == 0, "a wave's elements are all of B or all of C");
+#pragma unroll
+  for (int k = 0; k < 2 * kEach; k += 64 * NW) {
+    const int first = k + at.wave * 64;  // uniform
+    const bool c = first >= kEach;
+    const int e = (c ? first - kEach : first) + at.lane, s = e / NP, n = e % NP;
+    const T* row = c ? row_of<T>(p->cm, p->sc_t, p->sc_b, t0, at.b) : row_of<T>(p->bm, p->sb_t, p->sb_b, t0, at.b);
+    const int64_t st = c ? p->sc_t : p->sb_t;
+    float x = 0.0f;
+    if (n < p->N && t0 + s < at.t1) x = (float)row[s * st + n];
+    bc[s][n / P].x[(c ? P : 0) + n % P] = x;
+  }
+}
+
+// Backward: parts of the axis whose ends are found one by one; p.each of them make a chunk.
+__device__ __forceinline__ int parts_of(const SsmParams& p) {
+  const int length = p.length / p.each;
+  return (p.T + length - 1) / length;
 }
 
 // f(std::true_type) where a tile holds a reset, else f(std::false_type): uniform.
@@ -109,44 +150,57 @@ __device__ __forceinline__ void with_flags(uint32_t flags, F&& f) {
   else f(std::false_type{});
 }
 
+// ---- forward ------------------------------------------------------------------------
+//
+// Of a cut axis the first of two launches (FIRST) scans the first chunk and finds the ends of those between
+// it and the last; the second one, or the only one, scans the others.
+
+template <int P, int NW>
+struct FwdShared {
+  float2 xs[kTile][64];  // dt, dt u
+  Pair<P> bc[kTile][NW];
+  float part[NW][kTile][64];
+};
+
 // OUT: the scan itself. Otherwise what a chunk makes of a zero state, and its sum of dt.
 // PAD: N is not P NW; states that do not exist are left out.
 template <typename T, int P, int NW, bool PAD, bool OUT>
-__global__ __launch_bounds__(64 * NW) void ssm_fwd_kernel(SsmParams p) {
+__device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
   typedef Elem<T> E;
   constexpr int kOwn = kTile / NW;  // steps of a tile that a wave prepares
-  __shared__ float2 xs[kTile][64];  // dt, dt u
-  __shared__ float bc[kTile][NW][2 * P];
-  __shared__ float part[OUT ? NW : 1][kTile][64];
-  const At at(p);
-  const int n0 = at.wave * P, live = PAD ? min(max(p.N - n0, 0), P) : P;
+  Args p = args();
+  const int n0 = at.wave * P, live = PAD ? min(max(p->N - n0, 0), P) : P;
   float A2[P], h[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int n = n0 + i;
-    const bool some = at.ok && n < p.N;
-    A2[i] = some ? p.A[(int64_t)at.ch * p.N + n] * kLog2e : 0.0f;
+    const bool some = at.ok && n < p->N;
+    A2[i] = some ? p->A[(int64_t)at.ch * p->N + n] * kLog2e : 0.0f;
     h[i] = 0.0f;
     if (OUT && some) {
-      if (at.chunk) h[i] = p.ends[(((int64_t)(at.chunk - 1) * p.B + at.b) * p.N + n) * p.H + at.ch];
-      else if (p.h0 != nullptr) h[i] = p.h0[((int64_t)at.b * p.H + at.ch) * p.N + n];
+      if (at.chunk) h[i] = p->ends[(((int64_t)(at.chunk - 1) * p->B + at.b) * p->N + n) * p->H + at.ch];
+      else if (p->h0 != nullptr) h[i] = p->h0[((int64_t)at.b * p->H + at.ch) * p->N + n];
     }
   }
-  const float bias = p.bias != nullptr && at.ok ? p.bias[at.ch] : 0.0f;
-  const float D = OUT && p.D != nullptr && at.ok ? p.D[at.ch] : 0.0f;
+  const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
+  const float D = OUT && p->D != nullptr && at.ok ? p->D[at.ch] : 0.0f;
   const uint32_t off = lane_off<T>(at);
   float span = 0.0f;
   bool drop = false;
   unsigned int rd[kOwn], ru[kOwn], rz[kOwn];
   auto fetch = [&](int t0) __attribute__((always_inline)) {
+    Args p = args();
+    const int t = t0 + at.wave;
+    const T* d = row_of<T>(p->delta, p->sdl_t, p->sdl_b, t, at.b);
+    const T* u = row_of<T>(p->u, p->su_t, p->su_b, t, at.b);
+    const T* z = row_of<T>(p->z, p->sz_t, p->sz_b, t, at.b);
+    const bool gated = OUT && p->z != nullptr;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const int t = t0 + at.wave + NW * i;
-      const uint32_t o = t < at.t1 ? off : kOffNone;
-      const int r = min(t, at.t1 - 1);
-      rd[i] = E::load(row_of<T>(p.delta, p.sdl_t, p.sdl_b, r, at.b), o);
-      ru[i] = E::load(row_of<T>(p.u, p.su_t, p.su_b, r, at.b), o);
-      if (OUT && p.z != nullptr) rz[i] = E::load(row_of<T>(p.z, p.sz_t, p.sz_b, r, at.b), o);
+      const uint32_t o = t + NW * i < at.t1 ? off : kOffNone;
+      rd[i] = E::load(d + i * NW * p->sdl_t, o);
+      ru[i] = E::load(u + i * NW * p->su_t, o);
+      if (OUT) rz[i] = E::load(z + i * NW * p->sz_t, gated ? o : kOffNone);
     }
   };
   fetch(at.t0);
@@ -158,76 +212,249 @@ __global__ __launch_bounds__(64 * NW) void ssm_fwd_kernel(SsmParams p) {
       u[i] = E::value(ru[i]);
       if (OUT) z[i] = E::value(rz[i]);
       const float dt = t0 + s < at.t1 ? softplus(E::value(rd[i]) + bias) : 0.0f;
-      xs[s][at.lane] = float2{dt, dt * u[i]};
+      lds.xs[s][at.lane] = float2{dt, dt * u[i]};
     }
-    stage_bc<T, P, NW>(p, at, t0, bc);
+    p = args();
+    stage_bc<T, P, NW>(p, at, t0, lds.bc);
     const uint32_t flags = flags_of(p, at, t0);
-    lds_barrier();
+    share_barrier();
     if (t0 + kTile < at.t1) fetch(t0 + kTile);
-    if (OUT && p.saved != nullptr && at.ok) {
+    if (OUT) {
+      p = args();
+      if (p->saved != nullptr && at.ok) {
+        float* to = p->saved + (((int64_t)(t0 / kTile) * p->B + at.b) * p->N + n0) * p->H + at.ch;
 #pragma unroll
-      for (int i = 0; i < P; ++i)
-        if (n0 + i < p.N) p.saved[(((int64_t)(t0 / kTile) * p.B + at.b) * p.N + n0 + i) * p.H + at.ch] = h[i];
+        for (int i = 0; i < P; ++i)
+          if (!PAD || i < live) to[(int64_t)i * p->H] = h[i];
+      }
     }
     with_flags(flags, [&](auto F) __attribute__((always_inline)) {
       constexpr bool RESET = decltype(F)::value;
 #pragma unroll
       for (int s = 0; s < kTile; ++s) {
-        const float2 x = xs[s][at.lane];
+        const float2 x = lds.xs[s][at.lane];
+        float bm[P], cm[P];
+        lds.bc[s][at.wave].read(bm, cm);
         const bool start = RESET && (flags >> s & 1);
         float y = 0.0f;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           if (PAD && i >= live) continue;
           if (start) h[i] = 0.0f;
-          h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(x.x * A2[i]), h[i], x.y * bc[s][at.wave][i]);
-          if (OUT) y = __builtin_fmaf(bc[s][at.wave][P + i], h[i], y);
+          h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(x.x * A2[i]), h[i], x.y * bm[i]);
+          if (OUT) y = __builtin_fmaf(cm[i], h[i], y);
         }
-        if constexpr (OUT) {
-          part[at.wave][s][at.lane] = y;
-        } else {
-          span += x.x;
-        }
+        if constexpr (OUT) lds.part[at.wave][s][at.lane] = y;
+        else span += x.x;
       }
     });
     if (!OUT && flags) drop = true;
-    lds_barrier();
+    share_barrier();
     if constexpr (OUT) {
+      p = args();
+      T* to = row_of<T>(p->y, p->sy_t, p->sy_b, t0 + at.wave, at.b);
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
         const int s = at.wave + NW * i;
-        float y = part[0][s][at.lane];
+        float y = lds.part[0][s][at.lane];
 #pragma unroll
         for (int w = 1; w < NW; ++w)
-          if (!PAD || w * P < p.N) y += part[w][s][at.lane];
+          if (!PAD || w * P < p->N) y += lds.part[w][s][at.lane];
         y = __builtin_fmaf(D, u[i], y);
-        if (p.z != nullptr) y *= z[i] * sigmoid(z[i]);
-        const int t = min(t0 + s, at.t1 - 1);
-        E::store(const_cast<T*>(row_of<T>(p.y, p.sy_t, p.sy_b, t, at.b)), t0 + s < at.t1 ? off : kOffNone, y);
+        const float gate = z[i] * sigmoid(z[i]);
+        y = p->z != nullptr ? y * gate : y;
+        E::store(to + i * NW * p->sy_t, t0 + s < at.t1 ? off : kOffNone, y);
       }
     }
   }
   if (!at.ok) return;
-  if constexpr (OUT) {
-    if (p.h_last != nullptr && at.chunk == p.chunks - 1) {
+  p = args();
+  const int64_t row = (int64_t)at.chunk * p->B + at.b;
 #pragma unroll
-      for (int i = 0; i < P; ++i)
-        if (n0 + i < p.N) p.h_last[((int64_t)at.b * p.H + at.ch) * p.N + n0 + i] = h[i];
-    }
-  } else {
-    const int64_t row = (int64_t)at.chunk * p.B + at.b;
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-      if (n0 + i < p.N) p.ends[(row * p.N + n0 + i) * p.H + at.ch] = h[i];
-    if (at.wave == 0) p.span[row * p.H + at.ch] = span;
-    if (threadIdx.x == 0 && at.block == 0) p.dropped[row] = drop ? 1.0f : 0.0f;
+  for (int i = 0; i < P; ++i) {
+    const int n = n0 + i;
+    if (n >= p->N) continue;
+    // what follows a chunk needs its end: the last one's is h_T, the first one's the state itself
+    if (OUT && p->h_last != nullptr && at.chunk == p->chunks - 1) p->h_last[((int64_t)at.b * p->H + at.ch) * p->N + n] = h[i];
+    if (!OUT || (at.chunk == 0 && p->chunks > 1)) p->ends[(row * p->N + n) * p->H + at.ch] = h[i];
+  }
+  if (!OUT) {
+    if (at.wave == 0) p->span[row * p->H + at.ch] = span;
+    if (threadIdx.x == 0 && at.block == 0) p->dropped[row] = drop ? 1.0f : 0.0f;
   }
 }
 
-// The states at the chunks' ends, from what each chunk makes of zero: slot c of `ends` holds
-// the latter on entry and the state after chunk c on return. BACK: the same from the last
-// chunk to the second, for the gradients that chunks send to the one before; slot c then
-// holds, on return, what chunk c sends to c - 1.
+template <typename T, int P, int NW, bool PAD, bool FIRST>
+__global__ __launch_bounds__(64 * NW) void ssm_fwd_kernel(SsmParams p) {
+  __shared__ FwdShared<P, NW> lds;
+  const At at(p, !FIRST && p.chunks > 1 ? 1 : 0, p.length);
+  if (FIRST && at.chunk > 0) fwd_chunk<T, P, NW, PAD, false>(at, lds);
+  else fwd_chunk<T, P, NW, PAD, true>(at, lds);
+}
+
+// Where waves are many without that, one has 64 channels with all their states to itself, which nothing has to
+// be shared for: B and C come from LDS, the same for all lanes.
+constexpr int kGroup = 4;  // steps whose loads are in flight together
+
+// A group's B and C on their way to LDS as floats, [step][B, C][NP] with kEach of them a lane side by side.
+template <typename T, int NP>
+struct Rows {
+  static constexpr int kEach = kGroup * 2 * NP >= 64 ? kGroup * 2 * NP / 64 : 1, kLanes = 2 * NP / kEach;  // kLanes a step
+  static_assert(NP % kEach == 0, "a lane's elements are of one row");
+  const T* at_row;  // of the group that is loaded next
+  int64_t by;       // to the group after it
+  int step, some;   // the lane's step of a group, and how many of its states exist
+  unsigned int x[kEach];
+  // groups from t0 on, or back
+  __device__ __forceinline__ void init(Args p, const At& at, int t0, bool back) {
+    step = at.lane / kLanes;
+    const int e = at.lane % kLanes * kEach, n = e % NP;
+    const bool c = e >= NP;
+    const int64_t st = c ? p->sc_t : p->sb_t;
+    at_row = static_cast<const T*>(c ? p->cm : p->bm) + (t0 + step) * st + at.b * (c ? p->sc_b : p->sb_b) + n;
+    by = (back ? -kGroup : kGroup) * st;
+    some = step < kGroup ? p->N - n : 0;
+  }
+  __device__ __forceinline__ void load(const At& at, int t0) {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      x[k] = 0;
+      if (t0 + step < at.t1 && k < some) x[k] = sizeof(T) == 2 ? *reinterpret_cast<const unsigned short*>(at_row + k)
+                                                               : *reinterpret_cast<const unsigned int*>(at_row + k);
+    }
+    at_row += by;
+  }
+  __device__ __forceinline__ void put(float (*lds)[2 * NP], const At& at) const {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+      if (kGroup * kLanes == 64 || at.lane < kGroup * kLanes) (&lds[0][0])[at.lane * kEach + k] = Elem<T>::value(x[k]);
+  }
+};
+// The same NP floats of LDS in every lane.
+template <int NP>
+__device__ __forceinline__ void read_row(const float* lds, float (&x)[NP]) {
+#pragma unroll
+  for (int n = 0; n < NP; n += 4) {
+    const f4v q = *reinterpret_cast<const f4v*>(lds + n);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[n + k] = q[k];
+  }
+}
+
+// A wave scans 64 channels, a lane each with all its states, over a chunk. OUT: the scan itself. Otherwise what
+// the chunk makes of a zero state, and its sum of dt. PAD: N is less than NP; states that do
+// not exist are left out.
+template <typename T, int NP, bool PAD, bool OUT>
+__device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]) {
+  typedef Elem<T> E;
+  Args p = args();
+  const int N = PAD ? p->N : NP;
+  float A2[NP], h[NP];
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    const bool some = at.ok && n < N;
+    A2[n] = some ? p->A[(int64_t)at.ch * N + n] * kLog2e : 0.0f;
+    h[n] = 0.0f;
+    if (OUT && some) {
+      if (at.chunk) h[n] = p->ends[(((int64_t)(at.chunk - 1) * p->B + at.b) * N + n) * p->H + at.ch];
+      else if (p->h0 != nullptr) h[n] = p->h0[((int64_t)at.b * p->H + at.ch) * N + n];
+    }
+  }
+  const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
+  const float D = OUT && p->D != nullptr && at.ok ? p->D[at.ch] : 0.0f;
+  const uint32_t off = lane_off<T>(at);
+  const bool gated = OUT && p->z != nullptr;
+  float span = 0.0f;
+  bool drop = false;
+  unsigned int rd[kGroup], ru[kGroup], rz[kGroup];
+  Rows<T, NP> rows;
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    rows.load(at, t);
+    const T* d = row_of<T>(p->delta, p->sdl_t, p->sdl_b, t, at.b);
+    const T* u = row_of<T>(p->u, p->su_t, p->su_b, t, at.b);
+    const T* z = row_of<T>(p->z, p->sz_t, p->sz_b, t, at.b);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      const uint32_t o = t + i < at.t1 ? off : kOffNone;
+      rd[i] = E::load(d + i * p->sdl_t, o);
+      ru[i] = E::load(u + i * p->su_t, o);
+      if (OUT) rz[i] = E::load(z + i * p->sz_t, gated ? o : kOffNone);
+    }
+  };
+  rows.init(p, at, at.t0, false);
+  fetch(at.t0);
+  for (int t0 = at.t0; t0 < at.t1; t0 += kGroup) {
+    const uint32_t flags = flags_of(p, at, t0);
+    if (OUT && p->saved != nullptr && t0 % kTile == 0 && at.ok) {
+      float* to = p->saved + ((int64_t)(t0 / kTile) * p->B + at.b) * N * p->H + at.ch;
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+        if (n < N) to[(int64_t)n * p->H] = h[n];
+    }
+    rows.put(bc, at);
+    float dt[kGroup], u[kGroup], z[kGroup];
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      dt[i] = t0 + i < at.t1 ? softplus(E::value(rd[i]) + bias) : 0.0f;
+      u[i] = E::value(ru[i]);
+      if (OUT) z[i] = E::value(rz[i]);
+    }
+    if (t0 + kGroup < at.t1) fetch(t0 + kGroup);
+    T* to = OUT ? row_of<T>(p->y, p->sy_t, p->sy_b, t0, at.b) : nullptr;
+    if (!OUT && (flags & ((1u << kGroup) - 1))) drop = true;
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      float bm[NP], cm[NP];
+      read_row<NP>(bc[i], bm);
+      if (OUT) read_row<NP>(bc[i] + NP, cm);
+      const float du = dt[i] * u[i];
+      if (flags >> i & 1) {  // uniform
+#pragma unroll
+        for (int n = 0; n < NP; ++n) h[n] = 0.0f;
+      }
+      float y = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        if (PAD && n >= N) continue;
+        h[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt[i] * A2[n]), h[n], du * bm[n]);
+        if (OUT) y = __builtin_fmaf(cm[n], h[n], y);
+      }
+      if constexpr (OUT) {
+        y = __builtin_fmaf(D, u[i], y);
+        const float gate = z[i] * sigmoid(z[i]);
+        E::store(to + i * p->sy_t, t0 + i < at.t1 ? off : kOffNone, gated ? y * gate : y);
+      } else {
+        span += dt[i];
+      }
+      if (i % 2) __builtin_amdgcn_sched_barrier(0);  // rows of few steps ahead: registers are short
+    }
+  }
+  if (!at.ok) return;
+  const int64_t row = (int64_t)at.chunk * p->B + at.b;
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    if (n >= N) continue;
+    // what follows a chunk needs its end: the last one's is h_T, the first one's the state itself
+    if (OUT && p->h_last != nullptr && at.chunk == p->chunks - 1) p->h_last[((int64_t)at.b * p->H + at.ch) * N + n] = h[n];
+    if (!OUT || (at.chunk == 0 && p->chunks > 1)) p->ends[(row * N + n) * p->H + at.ch] = h[n];
+  }
+  if (!OUT) {
+    p->span[row * p->H + at.ch] = span;
+    if (at.lane == 0 && at.block == 0) p->dropped[row] = drop ? 1.0f : 0.0f;
+  }
+}
+
+template <typename T, int NP, bool PAD, bool FIRST>
+__global__ __launch_bounds__(64) void ssm_fwd_wide_kernel(SsmParams p) {
+  __shared__ alignas(16) float bc[kGroup][2 * NP];
+  const At at(p, !FIRST && p.chunks > 1 ? 1 : 0, p.length);
+  if (FIRST && at.chunk > 0) wide_fwd_chunk<T, NP, PAD, false>(at, bc);
+  else wide_fwd_chunk<T, NP, PAD, true>(at, bc);
+}
+
+// Forward: the states at the chunks' ends. Slot 0 of `ends` holds that of the first chunk, slot c what
+// chunk c makes of zero, and on return the state after it. BACK: slot c holds what part c of the axis
+// sends back of a zero gradient, and on return of the whole: from the last part to the second chunk's first.
 template <bool BACK>
 __global__ __launch_bounds__(256) void ssm_join_kernel(SsmParams p) {
   const int64_t plane = (int64_t)p.B * p.N * p.H, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -235,15 +462,16 @@ __global__ __launch_bounds__(256) void ssm_join_kernel(SsmParams p) {
   const int ch = (int)(e % p.H), n = (int)(e / p.H % p.N), b = (int)(e / p.H / p.N);
   const float A2 = p.A[(int64_t)ch * p.N + n] * kLog2e;
   float s = 0.0f;
-  if (!BACK && p.h0 != nullptr) s = p.h0[((int64_t)b * p.H + ch) * p.N + n];
+  if (!BACK) s = p.ends[e];
   if (BACK && p.dh_last != nullptr) s = p.dh_last[((int64_t)b * p.H + ch) * p.N + n];
-  const int count = p.chunks - 1;
+  const int all = parts_of(p);
+  const int count = BACK ? all - p.each : p.chunks - 2;
   constexpr int kAhead = 8;
   for (int k0 = 0; k0 < count; k0 += kAhead) {
     float end[kAhead], span[kAhead], drop[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int c = BACK ? p.chunks - 1 - min(k0 + k, count - 1) : min(k0 + k, count - 1);
+      const int j = min(k0 + k, count - 1), c = BACK ? all - 1 - j : 1 + j;
       end[k] = p.ends[c * plane + e];
       span[k] = p.span[((int64_t)c * p.B + b) * p.H + ch];
       drop[k] = p.dropped[(int64_t)c * p.B + b];
@@ -252,226 +480,320 @@ __global__ __launch_bounds__(256) void ssm_join_kernel(SsmParams p) {
     for (int k = 0; k < kAhead; ++k) {
       if (k0 + k >= count) break;
       s = drop[k] != 0.0f ? end[k] : __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * span[k]), s, end[k]);
-      p.ends[(BACK ? p.chunks - 1 - (k0 + k) : k0 + k) * plane + e] = s;
+      p.ends[(BACK ? all - 1 - (k0 + k) : 1 + k0 + k) * plane + e] = s;
     }
   }
 }
 
-// What a step's row holds for the backward: dt, the gradient of y before the gate.
-struct Row {
-  float dt, u, dy;
+template <int P, int NW>
+struct BwdShared {
+  float2 xs[kTile][64];  // dt, dt u
+  float ds[kTile][64];   // dy
+  // [1] stays zero: what lanes without a channel read, so that sums over lanes do not see them
+  Pair<P> bc[2][kTile][NW];
+  union {  // the waves' parts of y, then of S and of sum_n q A / ln 2
+    float y[NW][kTile][64];
+    float2 sq[NW][kTile][64];
+  } part;
 };
 
-// The gradient that chunk c > 0 sends to the state before it, from a zero gradient after it.
+// The gradient that a chunk sends to the state before it, from a zero gradient after it.
 template <typename T, int P, int NW, bool PAD>
-__global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams p) {
+__global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams kernel_args) {
+  __shared__ float2 xs[kTile][64];  // dt, dy
+  __shared__ Pair<P> bc[kTile][NW];
   typedef Elem<T> E;
   constexpr int kOwn = kTile / NW;
-  __shared__ float2 xs[kTile][64];  // dt, dy
-  __shared__ float bc[kTile][NW][2 * P];
-  At at(p);
-  at.chunk += 1;
-  at.t0 += p.length;
-  at.t1 = min(p.T, at.t0 + p.length);
-  const int n0 = at.wave * P, live = PAD ? min(max(p.N - n0, 0), P) : P;
+  const At at(kernel_args, 1, kernel_args.length);
+  Args p = args();
+  const int n0 = at.wave * P, live = PAD ? min(max(p->N - n0, 0), P) : P;
   float A2[P], e[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    A2[i] = at.ok && n0 + i < p.N ? p.A[(int64_t)at.ch * p.N + n0 + i] * kLog2e : 0.0f;
+    A2[i] = at.ok && n0 + i < p->N ? p->A[(int64_t)at.ch * p->N + n0 + i] * kLog2e : 0.0f;
     e[i] = 0.0f;
   }
-  const float bias = p.bias != nullptr && at.ok ? p.bias[at.ch] : 0.0f;
+  const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
   const uint32_t off = lane_off<T>(at);
   float span = 0.0f;
   bool drop = false;
   unsigned int rd[kOwn], rz[kOwn], rg[kOwn];
   auto fetch = [&](int t0) __attribute__((always_inline)) {
+    Args p = args();
+    const int t = t0 + at.wave;
+    const T* d = row_of<T>(p->delta, p->sdl_t, p->sdl_b, t, at.b);
+    const T* g = row_of<T>(p->dy, p->sdy_t, p->sdy_b, t, at.b);
+    const T* z = row_of<T>(p->z, p->sz_t, p->sz_b, t, at.b);
+    const bool gated = p->z != nullptr;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const int t = t0 + at.wave + NW * i, r = min(t, at.t1 - 1);
-      const uint32_t o = t < at.t1 ? off : kOffNone;
-      rd[i] = E::load(row_of<T>(p.delta, p.sdl_t, p.sdl_b, r, at.b), o);
-      rg[i] = E::load(row_of<T>(p.dy, p.sdy_t, p.sdy_b, r, at.b), o);
-      if (p.z != nullptr) rz[i] = E::load(row_of<T>(p.z, p.sz_t, p.sz_b, r, at.b), o);
+      const uint32_t o = t + NW * i < at.t1 ? off : kOffNone;
+      rd[i] = E::load(d + i * NW * p->sdl_t, o);
+      rg[i] = E::load(g + i * NW * p->sdy_t, o);
+      rz[i] = E::load(z + i * NW * p->sz_t, gated ? o : kOffNone);
     }
   };
   const int last = at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile;
   fetch(last);
   for (int t0 = last; t0 >= at.t0; t0 -= kTile) {
+    p = args();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int s = at.wave + NW * i;
       const float dt = t0 + s < at.t1 ? softplus(E::value(rd[i]) + bias) : 0.0f;
-      float dy = E::value(rg[i]);
-      if (p.z != nullptr) {
-        const float z = E::value(rz[i]);
-        dy *= z * sigmoid(z);
-      }
-      xs[s][at.lane] = float2{dt, dy};
+      const float z = E::value(rz[i]), g = E::value(rg[i]);
+      xs[s][at.lane] = float2{dt, p->z != nullptr ? g * (z * sigmoid(z)) : g};
     }
     stage_bc<T, P, NW>(p, at, t0, bc);
     const uint32_t flags = flags_of(p, at, t0);
-    lds_barrier();
+    share_barrier();
     if (t0 > at.t0) fetch(t0 - kTile);
     with_flags(flags, [&](auto F) __attribute__((always_inline)) {
       constexpr bool RESET = decltype(F)::value;
 #pragma unroll
       for (int s = kTile - 1; s >= 0; --s) {
         const float2 x = xs[s][at.lane];
+        float bm[P], cm[P];
+        bc[s][at.wave].read(bm, cm);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           if (PAD && i >= live) continue;
-          e[i] = __builtin_amdgcn_exp2f(x.x * A2[i]) * __builtin_fmaf(bc[s][at.wave][P + i], x.y, e[i]);
+          e[i] = __builtin_amdgcn_exp2f(x.x * A2[i]) * __builtin_fmaf(cm[i], x.y, e[i]);
           if (RESET && (flags >> s & 1)) e[i] = 0.0f;
         }
         span += x.x;
       }
     });
     if (flags) drop = true;
-    lds_barrier();
+    share_barrier();
   }
   if (!at.ok) return;
-  const int64_t row = (int64_t)at.chunk * p.B + at.b;
+  p = args();
+  const int64_t row = (int64_t)at.chunk * p->B + at.b;
 #pragma unroll
   for (int i = 0; i < P; ++i)
-    if (n0 + i < p.N) p.ends[(row * p.N + n0 + i) * p.H + at.ch] = e[i];
-  if (at.wave == 0) p.span[row * p.H + at.ch] = span;
-  if (threadIdx.x == 0 && at.block == 0) p.dropped[row] = drop ? 1.0f : 0.0f;
+    if (n0 + i < p->N) p->ends[(row * p->N + n0 + i) * p->H + at.ch] = e[i];
+  if (at.wave == 0) p->span[row * p->H + at.ch] = span;
+  if (threadIdx.x == 0 && at.block == 0) p->dropped[row] = drop ? 1.0f : 0.0f;
+}
+
+// The gradient that a part of the axis sends to the state before it, from a zero gradient after
+// it, and its sum of dt. A wave takes 64 channels, as forwards.
+template <typename T, int NP, bool PAD>
+__global__ __launch_bounds__(64) void ssm_bwd_ends_wide_kernel(SsmParams) {
+  typedef Elem<T> E;
+  __shared__ alignas(16) float bc[kGroup][2 * NP];
+  Args p = args();
+  SsmParams q;
+  q.blocks = p->blocks;
+  q.B = p->B;
+  q.H = p->H;
+  q.T = p->T;
+  const At at(q, p->each, p->length / p->each);
+  const int N = PAD ? p->N : NP;
+  float A2[NP], e[NP];
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    A2[n] = at.ok && n < N ? p->A[(int64_t)at.ch * N + n] * kLog2e : 0.0f;
+    e[n] = 0.0f;
+  }
+  const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
+  const uint32_t off = lane_off<T>(at);
+  const bool gated = p->z != nullptr;
+  float span = 0.0f;
+  bool drop = false;
+  unsigned int rd[kGroup], rz[kGroup], rg[kGroup];
+  Rows<T, NP> rows;
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    rows.load(at, t);
+    const T* d = row_of<T>(p->delta, p->sdl_t, p->sdl_b, t, at.b);
+    const T* g = row_of<T>(p->dy, p->sdy_t, p->sdy_b, t, at.b);
+    const T* z = row_of<T>(p->z, p->sz_t, p->sz_b, t, at.b);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      const uint32_t o = t + i < at.t1 ? off : kOffNone;
+      rd[i] = E::load(d + i * p->sdl_t, o);
+      rg[i] = E::load(g + i * p->sdy_t, o);
+      rz[i] = E::load(z + i * p->sz_t, gated ? o : kOffNone);
+    }
+  };
+  const int last = at.t0 + (at.t1 - at.t0 - 1) / kGroup * kGroup;
+  rows.init(p, at, last, true);
+  fetch(last);
+  for (int t0 = last; t0 >= at.t0; t0 -= kGroup) {
+    const uint32_t flags = flags_of(p, at, t0);
+    rows.put(bc, at);
+    float dt[kGroup], dy[kGroup];
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      dt[i] = t0 + i < at.t1 ? softplus(E::value(rd[i]) + bias) : 0.0f;
+      const float z = E::value(rz[i]), g = E::value(rg[i]);
+      dy[i] = gated ? g * (z * sigmoid(z)) : g;
+    }
+    if (t0 > at.t0) fetch(t0 - kGroup);
+    if (flags & ((1u << kGroup) - 1)) drop = true;
+#pragma unroll
+    for (int i = kGroup - 1; i >= 0; --i) {
+      float cm[NP];
+      read_row<NP>(bc[i] + NP, cm);
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        if (PAD && n >= N) continue;
+        e[n] = __builtin_amdgcn_exp2f(dt[i] * A2[n]) * __builtin_fmaf(cm[n], dy[i], e[n]);
+      }
+      if (flags >> i & 1) {  // uniform
+#pragma unroll
+        for (int n = 0; n < NP; ++n) e[n] = 0.0f;
+      }
+      span += dt[i];
+    }
+  }
+  if (!at.ok) return;
+  const int64_t row = (int64_t)at.chunk * p->B + at.b;
+#pragma unroll
+  for (int n = 0; n < NP; ++n)
+    if (n < N) p->ends[(row * N + n) * p->H + at.ch] = e[n];
+  p->span[row * p->H + at.ch] = span;
+  if (at.lane == 0 && at.block == 0) p->dropped[row] = drop ? 1.0f : 0.0f;
 }
 
 template <typename T, int P, int NW, bool PAD>
-__global__ __launch_bounds__(64 * NW) void ssm_bwd_kernel(SsmParams p) {
+__device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
   typedef Elem<T> E;
   constexpr int kOwn = kTile / NW;
-  __shared__ float2 xs[kTile][64];  // dt, dt u
-  __shared__ float ds[kTile][64];   // dy
-  __shared__ float bc[kTile][NW][2 * P];
-  // the waves' parts of y, then of S and of sum_n q A
-  __shared__ float2 part[NW][kTile][64];
-  float(*const ypart)[kTile][64] = reinterpret_cast<float(*)[kTile][64]>(&part[0][0][0]);
-  const At at(p);
-  const int n0 = at.wave * P, live = PAD ? min(max(p.N - n0, 0), P) : P;
-  const bool gated = p.z != nullptr;
-  float A[P], e[P], dA[P];
+  Args p = args();
+  const int n0 = at.wave * P, live = PAD ? min(max(p->N - n0, 0), P) : P;
+  float A2[P], e[P], dA[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int n = n0 + i;
-    const bool some = at.ok && n < p.N;
-    A[i] = some ? p.A[(int64_t)at.ch * p.N + n] : 0.0f;
+    const bool some = at.ok && n < p->N;
+    A2[i] = some ? p->A[(int64_t)at.ch * p->N + n] * kLog2e : 0.0f;
     dA[i] = 0.0f;
     e[i] = 0.0f;
     if (some) {
-      if (at.chunk < p.chunks - 1) e[i] = p.ends[(((int64_t)(at.chunk + 1) * p.B + at.b) * p.N + n) * p.H + at.ch];
-      else if (p.dh_last != nullptr) e[i] = p.dh_last[((int64_t)at.b * p.H + at.ch) * p.N + n];
+      if (at.chunk < p->chunks - 1) e[i] = p->ends[(((int64_t)(at.chunk + 1) * p->each * p->B + at.b) * p->N + n) * p->H + at.ch];
+      else if (p->dh_last != nullptr) e[i] = p->dh_last[((int64_t)at.b * p->H + at.ch) * p->N + n];
     }
   }
-  const float bias = p.bias != nullptr && at.ok ? p.bias[at.ch] : 0.0f;
-  const float D = p.D != nullptr && at.ok ? p.D[at.ch] : 0.0f;
+  const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
+  const float D = p->D != nullptr && at.ok ? p->D[at.ch] : 0.0f;
   const uint32_t off = lane_off<T>(at);
-  const bool tail = at.block == p.blocks - 1 && p.H % 64 != 0;
   float dD = 0.0f, dbias = 0.0f;
+  for (int i = threadIdx.x; i < kTile * NW * 2 * P; i += 64 * NW) (&lds.bc[1][0][0].x[0])[i] = 0.0f;
   unsigned int rd[kOwn], ru[kOwn], rz[kOwn], rg[kOwn];
   auto fetch = [&](int t0) __attribute__((always_inline)) {
+    Args p = args();
+    const int t = t0 + at.wave;
+    const T* d = row_of<T>(p->delta, p->sdl_t, p->sdl_b, t, at.b);
+    const T* u = row_of<T>(p->u, p->su_t, p->su_b, t, at.b);
+    const T* g = row_of<T>(p->dy, p->sdy_t, p->sdy_b, t, at.b);
+    const T* z = row_of<T>(p->z, p->sz_t, p->sz_b, t, at.b);
+    const bool gated = p->z != nullptr;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const int t = t0 + at.wave + NW * i, r = min(t, at.t1 - 1);
-      const uint32_t o = t < at.t1 ? off : kOffNone;
-      rd[i] = E::load(row_of<T>(p.delta, p.sdl_t, p.sdl_b, r, at.b), o);
-      ru[i] = E::load(row_of<T>(p.u, p.su_t, p.su_b, r, at.b), o);
-      rg[i] = E::load(row_of<T>(p.dy, p.sdy_t, p.sdy_b, r, at.b), o);
-      if (gated) rz[i] = E::load(row_of<T>(p.z, p.sz_t, p.sz_b, r, at.b), o);
+      const uint32_t o = t + NW * i < at.t1 ? off : kOffNone;
+      rd[i] = E::load(d + i * NW * p->sdl_t, o);
+      ru[i] = E::load(u + i * NW * p->su_t, o);
+      rg[i] = E::load(g + i * NW * p->sdy_t, o);
+      rz[i] = E::load(z + i * NW * p->sz_t, gated ? o : kOffNone);
     }
   };
   const int last = at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile;
   fetch(last);
   for (int t0 = last; t0 >= at.t0; t0 -= kTile) {
-    float u[kOwn], x[kOwn], dt[kOwn], dy[kOwn], dzy[kOwn];  // dzy: dz / y
+    p = args();
+    asm volatile("" : "+v"(at.lane), "+s"(at.wave));  // addresses made from these are made anew, not kept
+    const Pair<P>(*const bc)[NW] = lds.bc[at.ok ? 0 : 1];
+    const bool gated = p->z != nullptr;
+    float u[kOwn], x[kOwn], dzy[kOwn];  // dzy: dz / y
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int s = at.wave + NW * i;
       u[i] = E::value(ru[i]);
       x[i] = E::value(rd[i]) + bias;
-      dt[i] = t0 + s < at.t1 ? softplus(x[i]) : 0.0f;
-      dy[i] = E::value(rg[i]);
-      dzy[i] = 0.0f;
-      if (gated) {
-        const float z = E::value(rz[i]), g = sigmoid(z);
-        dzy[i] = dy[i] * g * __builtin_fmaf(z, 1.0f - g, 1.0f);
-        dy[i] *= z * g;
-      }
-      xs[s][at.lane] = float2{dt[i], dt[i] * u[i]};
-      ds[s][at.lane] = dy[i];
+      const float dt = t0 + s < at.t1 ? softplus(x[i]) : 0.0f;
+      const float z = E::value(rz[i]), g = sigmoid(z), d = E::value(rg[i]);
+      dzy[i] = d * g * __builtin_fmaf(z, 1.0f - g, 1.0f);
+      lds.xs[s][at.lane] = float2{dt, dt * u[i]};
+      lds.ds[s][at.lane] = gated ? d * (z * g) : d;
     }
-    stage_bc<T, P, NW>(p, at, t0, bc);
+    stage_bc<T, P, NW>(p, at, t0, lds.bc[0]);
     const uint32_t flags = flags_of(p, at, t0);
     float start[P];
+    {
+      const float* from = p->saved + (((int64_t)(t0 / kTile) * p->B + at.b) * p->N + n0) * p->H + at.ch;
 #pragma unroll
-    for (int i = 0; i < P; ++i)
-      start[i] = at.ok && n0 + i < p.N ? p.saved[(((int64_t)(t0 / kTile) * p.B + at.b) * p.N + n0 + i) * p.H + at.ch] : 0.0f;
-    lds_barrier();
-    if (t0 > at.t0) fetch(t0 - kTile);
+      for (int i = 0; i < P; ++i) start[i] = at.ok && (!PAD || i < live) ? from[(int64_t)i * p->H] : 0.0f;
+    }
+    share_barrier();
     with_flags(flags, [&](auto F) __attribute__((always_inline)) {
       constexpr bool RESET = decltype(F)::value;
-      float a[kTile][P], h[kTile][P];  // h: after the step
+      // After each step. The decays are computed again on the way back: sixteen registers of them would leave half as many waves.
+      float h[kTile][P];
 #pragma unroll
       for (int s = 0; s < kTile; ++s) {
-        const float2 v = xs[s][at.lane];
-        float y = 0.0f;
+        const float2 v = lds.xs[s][at.lane];
+        float bm[P], cm[P], y = 0.0f;
+        bc[s][at.wave].read(bm, cm);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          a[s][i] = h[s][i] = 0.0f;
+          h[s][i] = 0.0f;
           if (PAD && i >= live) continue;
-          a[s][i] = __builtin_amdgcn_exp2f(v.x * (A[i] * kLog2e));
           float before = s ? h[s > 0 ? s - 1 : 0][i] : start[i];
           if (RESET && (flags >> s & 1)) before = 0.0f;
-          h[s][i] = __builtin_fmaf(a[s][i], before, v.y * bc[s][at.wave][i]);
-          y = __builtin_fmaf(bc[s][at.wave][P + i], h[s][i], y);
+          h[s][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(v.x * A2[i]), before, v.y * bm[i]);
+          y = __builtin_fmaf(cm[i], h[s][i], y);
         }
-        if (gated) ypart[at.wave][s][at.lane] = y;
+        lds.part.y[at.wave][s][at.lane] = y;
+        if (s % 2) __builtin_amdgcn_sched_barrier(0);  // loads of few steps ahead: registers are short
       }
+      share_barrier();
       if (gated) {
-        lds_barrier();
+        Args p = args();
+        T* to = row_of<T>(p->dz, p->sdz_t, p->sdz_b, t0 + at.wave, at.b);
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
           const int s = at.wave + NW * i;
-          float y = ypart[0][s][at.lane];
+          float y = lds.part.y[0][s][at.lane];
 #pragma unroll
           for (int w = 1; w < NW; ++w)
-            if (!PAD || w * P < p.N) y += ypart[w][s][at.lane];
-          y = __builtin_fmaf(D, u[i], y);
-          const int t = min(t0 + s, at.t1 - 1);
-          E::store(const_cast<T*>(row_of<T>(p.dz, p.sdz_t, p.sdz_b, t, at.b)), t0 + s < at.t1 ? off : kOffNone, dzy[i] * y);
+            if (!PAD || w * P < p->N) y += lds.part.y[w][s][at.lane];
+          E::store(to + i * NW * p->sdz_t, t0 + s < at.t1 ? off : kOffNone, dzy[i] * __builtin_fmaf(D, u[i], y));
         }
-        lds_barrier();
       }
+      share_barrier();
       // back over the tile; sums over the lanes of dB and dC of a pair of states in one register a step
-      float sums[P > 1 ? P / 2 : 1][kTile];
+      float sums[P / 2][kTile];
 #pragma unroll
       for (int s = kTile - 1; s >= 0; --s) {
-        const float2 v = xs[s][at.lane];
-        const float g = ds[s][at.lane];
-        float S = 0.0f, Q = 0.0f, db[P], dc[P];
+        const float2 v = lds.xs[s][at.lane];
+        const float g = lds.ds[s][at.lane];
+        float bm[P], cm[P], S = 0.0f, Q = 0.0f, db[P], dc[P];
+        bc[s][at.wave].read(bm, cm);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           db[i] = dc[i] = 0.0f;
           if (PAD && i >= live) continue;
-          const float G = __builtin_fmaf(bc[s][at.wave][P + i], g, e[i]);
+          const float G = __builtin_fmaf(cm[i], g, e[i]);
           float before = s ? h[s > 0 ? s - 1 : 0][i] : start[i];
-          e[i] = a[s][i] * G;
+          e[i] = __builtin_amdgcn_exp2f(v.x * A2[i]) * G;
           if (RESET && (flags >> s & 1)) e[i] = before = 0.0f;
           const float q = e[i] * before;
-          S = __builtin_fmaf(G, bc[s][at.wave][i], S);
-          Q = __builtin_fmaf(q, A[i], Q);
+          S = __builtin_fmaf(G, bm[i], S);
+          Q = __builtin_fmaf(q, A2[i], Q);
           dA[i] = __builtin_fmaf(q, v.x, dA[i]);
           db[i] = G * v.y;
           dc[i] = h[s][i] * g;
-          if (tail && !at.ok) db[i] = dc[i] = 0.0f;
         }
-        part[at.wave][s][at.lane] = float2{S, Q};
+        lds.part.sq[at.wave][s][at.lane] = float2{S, Q};
 #pragma unroll
         for (int i = 0; i < P; i += 2)
           sums[i / 2][s] = join<16>(join<32>(db[i], db[i + 1]), join<32>(dc[i], dc[i + 1]));
+        if (s == kTile / 2 && t0 > at.t0) fetch(t0 - kTile);  // half of h is done with
+        if (s % 2 == 0) __builtin_amdgcn_sched_barrier(0);
       }
+      Args p = args();
 #pragma unroll
       for (int k = 0; k < P / 2; ++k) {
         float w8[8], w4[4], w2[2];
@@ -483,55 +805,66 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_kernel(SsmParams p) {
         for (int s = 0; s < 2; ++s) w2[s] = join<4>(w4[2 * s], w4[2 * s + 1]);
         const float sum = join<8>(w2[0], w2[1]);
         const int t = t0 + (at.lane & 15), n = n0 + 2 * k + (at.lane >> 5);
-        if (t < at.t1 && n < p.N)
-          p.part_bc[(((int64_t)at.block * p.T + t) * p.B + at.b) * 2 * p.N + (at.lane & 16 ? p.N : 0) + n] = sum;
+        if (t < at.t1 && n < p->N)
+          p->part_bc[(((int64_t)at.block * p->T + t) * p->B + at.b) * 2 * p->N + (at.lane & 16 ? p->N : 0) + n] = sum;
       }
     });
-    lds_barrier();
+    share_barrier();
+    p = args();
+    T* to_u = row_of<T>(p->du, p->sdu_t, p->sdu_b, t0 + at.wave, at.b);
+    T* to_d = row_of<T>(p->ddelta, p->sdd_t, p->sdd_b, t0 + at.wave, at.b);
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int s = at.wave + NW * i;
-      float2 v = part[0][s][at.lane];
+      float2 v = lds.part.sq[0][s][at.lane];
 #pragma unroll
       for (int w = 1; w < NW; ++w)
-        if (!PAD || w * P < p.N) {
-          const float2 o = part[w][s][at.lane];
+        if (!PAD || w * P < p->N) {
+          const float2 o = lds.part.sq[w][s][at.lane];
           v.x += o.x;
           v.y += o.y;
         }
-      const float dd = __builtin_fmaf(u[i], v.x, v.y) * sigmoid(x[i]);
-      const int t = min(t0 + s, at.t1 - 1);
+      const float dt = lds.xs[s][at.lane].x, dy = lds.ds[s][at.lane];
+      const float dd = __builtin_fmaf(u[i], v.x, v.y * kLn2) * sigmoid(x[i]);
       const uint32_t o = t0 + s < at.t1 ? off : kOffNone;
-      E::store(const_cast<T*>(row_of<T>(p.du, p.sdu_t, p.sdu_b, t, at.b)), o, __builtin_fmaf(dt[i], v.x, D * dy[i]));
-      E::store(const_cast<T*>(row_of<T>(p.ddelta, p.sdd_t, p.sdd_b, t, at.b)), o, dd);
+      E::store(to_u + i * NW * p->sdu_t, o, __builtin_fmaf(dt, v.x, D * dy));
+      E::store(to_d + i * NW * p->sdd_t, o, dd);
       if (t0 + s < at.t1) {
-        dD = __builtin_fmaf(u[i], dy[i], dD);
+        dD = __builtin_fmaf(u[i], dy, dD);
         dbias += dd;
       }
     }
   }
   // sums over the chunk: dA of the wave's states, dD and dbias over the waves
-  const int64_t row = ((int64_t)at.chunk * p.B + at.b) * (p.N + 2);
+  p = args();
+  const int64_t row = (int64_t)at.chunk * p->B + at.b, parts = row * (p->N + 2);
   if (at.ok) {
 #pragma unroll
-    for (int i = 0; i < P; ++i)
-      if (n0 + i < p.N) {
-        p.part_a[(row + n0 + i) * p.H + at.ch] = dA[i];
-        if (at.chunk == 0 && p.dh0 != nullptr) p.dh0[((int64_t)at.b * p.H + at.ch) * p.N + n0 + i] = e[i];
-      }
+    for (int i = 0; i < P; ++i) {
+      const int n = n0 + i;
+      if (n >= p->N) continue;
+      p->part_a[(parts + n) * p->H + at.ch] = dA[i];
+      if (at.chunk == 0 && p->dh0 != nullptr) p->dh0[((int64_t)at.b * p->H + at.ch) * p->N + n] = e[i];
+    }
   }
-  lds_barrier();
-  part[at.wave][0][at.lane] = float2{dD, dbias};
-  lds_barrier();
+  share_barrier();
+  lds.part.sq[at.wave][0][at.lane] = float2{dD, dbias};
+  share_barrier();
   if (at.wave == 0 && at.ok) {
 #pragma unroll
     for (int w = 1; w < NW; ++w) {
-      dD += part[w][0][at.lane].x;
-      dbias += part[w][0][at.lane].y;
+      dD += lds.part.sq[w][0][at.lane].x;
+      dbias += lds.part.sq[w][0][at.lane].y;
     }
-    p.part_a[(row + p.N) * p.H + at.ch] = dD;
-    p.part_a[(row + p.N + 1) * p.H + at.ch] = dbias;
+    p->part_a[(parts + p->N) * p->H + at.ch] = dD;
+    p->part_a[(parts + p->N + 1) * p->H + at.ch] = dbias;
   }
+}
+
+template <typename T, int P, int NW, bool PAD>
+__global__ __launch_bounds__(64 * NW, P == 2 && NW == 8 ? 4 : 2) void ssm_bwd_kernel(SsmParams p) {
+  __shared__ BwdShared<P, NW> lds;
+  bwd_chunk<T, P, NW, PAD>(At(p, 0, p.length), lds);
 }
 
 // dB and dC [T, B, N]: the channel blocks' sums in order.
@@ -630,48 +963,75 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepParams p) {
 
 constexpr int kMostStates = 32;
 
-// Chunks of the time axis: workgroups for every CU, chunks of 64 steps at least.
+// Chunks of the time axis, multiples of a tile: workgroups (or, for kernels that share nothing, waves) for every
+// CU in each launch. Forwards there are two launches, which have one chunk fewer each; backwards one over
+// all chunks, after the waves that find the ends of their parts.
 struct Plan {
-  int blocks, chunks, length;
+  int blocks, chunks, length, each;
+  bool wide;  // the kernels that share nothing, for the forward or the backward's ends
 };
-Plan make_plan(int64_t T, int64_t B, int64_t H) {
+constexpr int64_t kGroups = 512;    // workgroups asked for: two a CU
+constexpr int64_t kWaves = 4096;    // waves asked for, where they share nothing
+constexpr int64_t kFewWaves = 2048; // up to these, states are spread over the waves of a workgroup
+constexpr int kLeastChunk = 64, kLeastPart = 32;  // steps
+Plan make_plan(int64_t T, int64_t B, int64_t H, bool back) {
   Plan r;
   r.blocks = (int)((H + 63) / 64);
-  const int64_t groups = r.blocks * B, want = 512;
-  int64_t chunks = std::max<int64_t>(1, std::min(want / groups, T / 64));
-  const int64_t length = (T + chunks - 1) / chunks;
-  r.length = (int)((length + kTile - 1) / kTile * kTile);
-  r.chunks = (int)((T + r.length - 1) / r.length);
+  const int64_t groups = r.blocks * B, fine = std::max<int64_t>(1, T / kLeastPart), most = std::max<int64_t>(1, T / kLeastChunk);
+  auto cut = [](int64_t n, int64_t parts) { return ((n + parts - 1) / parts + kTile - 1) / kTile * kTile; };
+  int64_t length;
+  r.each = 1;
+  r.wide = groups * fine > kFewWaves;
+  if (back) {
+    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(kGroups / groups, most));
+    length = cut(T, chunks);
+    if (chunks > 1 && r.wide) {
+      r.each = (int)std::max<int64_t>(1, std::min<int64_t>(kWaves / (groups * chunks), length / kLeastPart));
+      length = cut(length, r.each) * r.each;
+    }
+  } else {
+    int64_t chunks = r.wide ? std::min<int64_t>(1 + kWaves / groups, fine) : std::min<int64_t>(1 + kGroups / groups, most);
+    if (chunks < 3) chunks = 1;  // two launches of one chunk each
+    length = cut(T, chunks);
+  }
+  r.length = (int)length;
+  r.chunks = (int)((T + length - 1) / length);
   return r;
 }
 
+// States that the kernels are made for.
+int padded(int64_t N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : 32; }
+
 typedef void (*SsmFn)(SsmParams);
-enum { kFwd, kFwdEnds, kBwd, kBwdEnds };
-template <typename T, int P, int NW, bool PAD>
-SsmFn kernel_at(int which) {
+enum { kFwd, kFwdFirst, kBwdEnds, kBwd };
+template <typename T, int NP, int P, bool PAD>
+SsmFn kernel_at(int which, bool wide) {
   switch (which) {
-    case kFwd: return ssm_fwd_kernel<T, P, NW, PAD, true>;
-    case kFwdEnds: return ssm_fwd_kernel<T, P, NW, PAD, false>;
-    case kBwd: return ssm_bwd_kernel<T, P, NW, PAD>;
-    default: return ssm_bwd_ends_kernel<T, P, NW, PAD>;
+    case kFwd: return wide ? ssm_fwd_wide_kernel<T, NP, PAD, false> : ssm_fwd_kernel<T, P, NP / P, PAD, false>;
+    case kFwdFirst: return wide ? ssm_fwd_wide_kernel<T, NP, PAD, true> : ssm_fwd_kernel<T, P, NP / P, PAD, true>;
+    case kBwdEnds: return wide ? ssm_bwd_ends_wide_kernel<T, NP, PAD> : ssm_bwd_ends_kernel<T, P, NP / P, PAD>;
+    default: return ssm_bwd_kernel<T, P, NP / P, PAD>;
   }
 }
-template <typename T, int P, int NW>
-SsmFn kernel_in(int which, int N, int& threads) {
-  threads = 64 * NW;
-  return N == P * NW ? kernel_at<T, P, NW, false>(which) : kernel_at<T, P, NW, true>(which);
+template <typename T, int NP, int P>
+SsmFn kernel_in(int which, bool wide, int N, int& threads) {
+  threads = wide && which != kBwd ? 64 : 64 * NP / P;
+  return N == NP ? kernel_at<T, NP, P, false>(which, wide) : kernel_at<T, NP, P, true>(which, wide);
 }
 template <typename T>
-SsmFn kernel_for(int which, int N, int& threads) {
-  if (N <= 4) return kernel_in<T, 2, 2>(which, N, threads);
-  if (N <= 8) return kernel_in<T, 2, 4>(which, N, threads);
-  if (N <= 16) return kernel_in<T, 2, 8>(which, N, threads);
-  return kernel_in<T, 4, 8>(which, N, threads);
+SsmFn kernel_for(int which, bool wide, int N, int& threads) {
+  switch (padded(N)) {
+    case 4: return kernel_in<T, 4, 2>(which, wide, N, threads);
+    case 8: return kernel_in<T, 8, 2>(which, wide, N, threads);
+    case 16: return kernel_in<T, 16, 2>(which, wide, N, threads);
+    default: return kernel_in<T, 32, 4>(which, wide, N, threads);
+  }
 }
 
-int launch(int which, int dtype, const SsmParams& p, int64_t groups, hipStream_t stream) {
+int launch(int which, bool wide, int dtype, const SsmParams& p, int64_t groups, hipStream_t stream) {
   int threads = 0;
-  const SsmFn fn = dtype == GS_DTYPE_F32 ? kernel_for<float>(which, p.N, threads) : kernel_for<__bf16>(which, p.N, threads);
+  const SsmFn fn = dtype == GS_DTYPE_F32 ? kernel_for<float>(which, wide, p.N, threads)
+                                         : kernel_for<__bf16>(which, wide, p.N, threads);
   hipLaunchKernelGGL(fn, dim3((unsigned)groups), dim3(threads), 0, stream, p);
   GS_CHECK_HIP(hipGetLastError());
   return GS_OK;
@@ -698,9 +1058,10 @@ struct Bytes {
 Bytes bytes_of(const Plan& plan, int64_t T, int64_t B, int64_t H, int64_t N, bool back) {
   Bytes r;
   if (plan.chunks > 1) {
-    r.span = r.ends + align256(plan.chunks * B * N * H * 4);
-    r.dropped = r.span + align256(plan.chunks * B * H * 4);
-    r.total = r.dropped + align256(plan.chunks * B * 4);
+    const int64_t parts = (int64_t)plan.chunks * plan.each;
+    r.span = align256(parts * B * N * H * 4);
+    r.dropped = r.span + align256(parts * B * H * 4);
+    r.total = r.dropped + align256(parts * B * 4);
   }
   if (back) {
     r.bc = r.total;
@@ -771,6 +1132,7 @@ SsmParams params_of(const Args* a, const Plan& plan, const Bytes& bytes) {
   p.blocks = plan.blocks;
   p.chunks = plan.chunks;
   p.length = plan.length;
+  p.each = plan.each;
   char* s = static_cast<char*>(a->scratch);
   p.ends = reinterpret_cast<float*>(s + bytes.ends);
   p.span = reinterpret_cast<float*>(s + bytes.span);
@@ -796,7 +1158,7 @@ using namespace gs;
 extern "C" int64_t gs_ssm_scratch_bytes(const gs_ssm_args* a) {
   clear_error();
   const int rc = check_fwd(a, "gs_ssm_scratch_bytes");
-  return rc ? rc : bytes_of(make_plan(a->T, a->B, a->H), a->T, a->B, a->H, a->N, false).total;
+  return rc ? rc : bytes_of(make_plan(a->T, a->B, a->H, false), a->T, a->B, a->H, a->N, false).total;
 }
 
 extern "C" int64_t gs_ssm_saved_bytes(const gs_ssm_args* a) {
@@ -812,7 +1174,7 @@ extern "C" int gs_ssm_fwd(const gs_ssm_args* a, hipStream_t stream) {
   if (rc) return rc;
   if (!a->u || !a->delta || !a->bm || !a->cm || !a->A || !a->y)
     return set_error(GS_ERR_INVALID, "%s: u, delta, A, bm, cm and y must be non-NULL device pointers", who);
-  const Plan plan = make_plan(a->T, a->B, a->H);
+  const Plan plan = make_plan(a->T, a->B, a->H, false);
   const Bytes bytes = bytes_of(plan, a->T, a->B, a->H, a->N, false);
   if ((rc = check_plain_scratch(who, a->scratch, a->scratch_bytes, bytes.total))) return rc;
   SsmParams p = params_of(a, plan, bytes);
@@ -821,18 +1183,18 @@ extern "C" int gs_ssm_fwd(const gs_ssm_args* a, hipStream_t stream) {
   p.saved = a->saved;
   p.sy_t = a->sy_t;
   p.sy_b = a->sy_b;
-  const int64_t each = (int64_t)plan.blocks * a->B;
+  const int64_t groups = (int64_t)plan.blocks * a->B * std::max(1, plan.chunks - 1);
   if (plan.chunks > 1) {
-    if ((rc = launch(kFwdEnds, a->dtype, p, each * (plan.chunks - 1), stream))) return rc;
-    if ((rc = join_ends(p, false, stream))) return rc;
+    if ((rc = launch(kFwdFirst, plan.wide, a->dtype, p, groups, stream))) return rc;
+    if (plan.chunks > 2 && (rc = join_ends(p, false, stream))) return rc;
   }
-  return launch(kFwd, a->dtype, p, each * plan.chunks, stream);
+  return launch(kFwd, plan.wide, a->dtype, p, groups, stream);
 }
 
 extern "C" int64_t gs_ssm_bwd_scratch_bytes(const gs_ssm_bwd_args* a) {
   clear_error();
   const int rc = check_bwd(a, "gs_ssm_bwd_scratch_bytes");
-  return rc ? rc : bytes_of(make_plan(a->T, a->B, a->H), a->T, a->B, a->H, a->N, true).total;
+  return rc ? rc : bytes_of(make_plan(a->T, a->B, a->H, true), a->T, a->B, a->H, a->N, true).total;
 }
 
 extern "C" int gs_ssm_bwd(const gs_ssm_bwd_args* a, hipStream_t stream) {
@@ -843,7 +1205,7 @@ extern "C" int gs_ssm_bwd(const gs_ssm_bwd_args* a, hipStream_t stream) {
   if (!a->u || !a->delta || !a->bm || !a->cm || !a->A || !a->saved || !a->dy || !a->du || !a->ddelta || (a->z && !a->dz))
     return set_error(GS_ERR_INVALID, "%s: u, delta, A, bm, cm, saved, dy, du and ddelta (and dz where z is given) must be "
                      "non-NULL device pointers", who);
-  const Plan plan = make_plan(a->T, a->B, a->H);
+  const Plan plan = make_plan(a->T, a->B, a->H, true);
   const Bytes bytes = bytes_of(plan, a->T, a->B, a->H, a->N, true);
   if ((rc = check_plain_scratch(who, a->scratch, a->scratch_bytes, bytes.total))) return rc;
   SsmParams p = params_of(a, plan, bytes);
@@ -862,12 +1224,13 @@ extern "C" int gs_ssm_bwd(const gs_ssm_bwd_args* a, hipStream_t stream) {
   p.sdd_b = a->sdd_b;
   p.sdz_t = a->sdz_t;
   p.sdz_b = a->sdz_b;
-  const int64_t each = (int64_t)plan.blocks * a->B, rows = a->T * a->B;
+  const int64_t groups = (int64_t)plan.blocks * a->B, rows = a->T * a->B;
   if (plan.chunks > 1) {
-    if ((rc = launch(kBwdEnds, a->dtype, p, each * (plan.chunks - 1), stream))) return rc;
+    const int64_t part = plan.length / plan.each, parts = (a->T + part - 1) / part;
+    if ((rc = launch(kBwdEnds, plan.wide, a->dtype, p, groups * (parts - plan.each), stream))) return rc;
     if ((rc = join_ends(p, true, stream))) return rc;
   }
-  if ((rc = launch(kBwd, a->dtype, p, each * plan.chunks, stream))) return rc;
+  if ((rc = launch(kBwd, plan.wide, a->dtype, p, groups * plan.chunks, stream))) return rc;
   if (a->dbm != nullptr || a->dcm != nullptr) {
     const dim3 grid((unsigned)std::min<int64_t>((rows * 2 * a->N + 255) / 256, 1 << 20));
     hipLaunchKernelGGL(a->dtype == GS_DTYPE_F32 ? ssm_sum_bc_kernel<float> : ssm_sum_bc_kernel<__bf16>, grid, dim3(256), 0,

@@ -73,6 +73,29 @@ def test_forward_and_backward(dev, T, H, N, dtype):
     _check(t, dy, dh, _roundings(T, B, H, N))
 
 
+# rows, channels and steps enough for waves that share nothing: several chunks, the last one short
+@pytest.mark.parametrize("T,B,H,N", [(610, 60, 130, 3), (1100, 40, 65, 16), (2100, 12, 130, 5), (1060, 40, 70, 20)])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_many_channels(dev, T, B, H, N, dtype):
+    t, dy, dh = _make(T, B, H, N, dtype, dev, seed=20, reset=0.003)
+    _check(t, dy, dh, _roundings(T, B, H, N))
+
+
+def test_nan_before_a_reset_among_many_channels(dev):
+    T, B, H, N = 1100, 40, 65, 4
+    t, dy, dh = _make(T, B, H, N, F32, dev, seed=21)
+    t["reset"] = torch.zeros(T, B, dtype=torch.bool, device=dev)
+    t["reset"][700, 3] = True
+    clean = _run(t, dy, dh)
+    t["h0"] = t["h0"].clone()
+    t["h0"][3, 7] = float("nan")
+    y, h, grads = _run(t, dy, dh)
+    assert y[:700, 3, 7].isnan().all() and torch.equal(y[700:], clean[0][700:]) and torch.equal(h, clean[1])
+    for k in ("u", "delta", "z", "B", "C"):
+        assert torch.equal(grads[k][700:], clean[2][k][700:]), k
+        assert torch.equal(grads[k][:, 4:], clean[2][k][:, 4:]), k
+
+
 @pytest.mark.parametrize("missing", [(), ("D",), ("z",), ("h0",), ("delta_bias",), ("D", "z", "h0", "delta_bias")], ids=str)
 @pytest.mark.parametrize("reset", [0.0, 0.2, 1.0])
 def test_optional_inputs_and_resets(dev, missing, reset):
