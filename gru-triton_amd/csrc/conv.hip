@@ -405,13 +405,13 @@ struct Plan {
 
 int64_t groups_of(const Plan& p, int64_t B) { return (int64_t)p.blocks * ((p.runs + 3) / 4) * B; }
 
-// Runs of 64 steps at most, whose ends cost little, and shorter ones where there are few waves.
+// Runs of 128 steps at most, whose ends cost little, and shorter ones where there are few waves.
 Plan make_plan(int64_t T, int64_t B, int64_t C, int v) {
   Plan r;
   r.v = v;
   r.blocks = (int)((C + 64 * v - 1) / (64 * v));
   const int64_t steps = r.blocks * B * T;
-  int64_t length = 64;
+  int64_t length = 128;
   while (length > 8 && steps / length < 4096) length /= 2;
   r.length = (int)length;
   r.runs = (int)((T + length - 1) / length);

@@ -6,10 +6,10 @@
 // Bound by memory: rows of w, out and dout, once each, and dw. For the gradient the positions m are
 // brought into lists by token: counted (a position's place in its list is what the counter held),
 // given room, and put down; the order within a list depends on timing until the sum sorts it, so that
-// results do not. A wave sorts a list of 64 or fewer by counting smaller ones, lane by lane, and
-// sums its rows in that order. Longer lists are cut into chunks, a workgroup each, which
-// finds its share of the sorted list from a bit for every position; the chunks' sums
-// are joined in order.
+// results do not. A wave sorts a list of 16 or fewer by counting smaller ones, lane by lane, and
+// sums its rows in that order. Longer lists are cut into chunks, a workgroup each, whose waves take a
+// quarter of its rows; a list's order there comes from counting smaller ones too or, where it is long, from a bit
+// for every position. The chunks' sums are joined in order.
 #include "gs_seq.h"
 
 namespace gs {
@@ -38,28 +38,41 @@ __device__ __forceinline__ int64_t token_at(const EmbedParams& p, int64_t m) {
   return p.wide ? static_cast<const int64_t*>(p.tokens)[m] : static_cast<const int32_t*>(p.tokens)[m];
 }
 
-// VW words of 4 bytes a lane, or one element where rows are not aligned to that (VW 0).
-template <typename T, int VW>
+// 16 bytes a lane, or one element where rows are not aligned to that.
+template <typename T, bool VEC>
 struct Row {
-  static constexpr int kElems = VW ? VW * 4 / (int)sizeof(T) : 1;
-  static __device__ __forceinline__ void load(const T* src, float (&x)[kElems]) {
-    if constexpr (VW == 0) {
-      x[0] = (float)src[0];
-    } else {
+  static constexpr int kElems = VEC ? 16 / (int)sizeof(T) : 1;
+  struct Raw {
+    unsigned int w[VEC ? 4 : 1];
+  };
+  static __device__ __forceinline__ Raw load(const T* src) {
+    Raw r;
+    if constexpr (VEC) {
       const u4v q = *reinterpret_cast<const u4v*>(src);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.w[i] = q[i];
+    } else {
+      r.w[0] = sizeof(T) == 2 ? *reinterpret_cast<const unsigned short*>(src) : *reinterpret_cast<const unsigned int*>(src);
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&x)[kElems]) {
+    if constexpr (!VEC) {
+      x[0] = Elem<T>::value(r.w[0]);
+    } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (sizeof(T) == 2) {
-          x[2 * i] = __uint_as_float(q[i] << 16);
-          x[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+          x[2 * i] = __uint_as_float(r.w[i] << 16);
+          x[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
         } else {
-          x[i] = __uint_as_float(q[i]);
+          x[i] = __uint_as_float(r.w[i]);
         }
       }
     }
   }
   static __device__ __forceinline__ void store(T* dst, const float (&x)[kElems]) {
-    if constexpr (VW == 0) {
+    if constexpr (!VEC) {
       dst[0] = (T)x[0];
     } else {
       u4v q;
@@ -79,9 +92,9 @@ struct Row {
 };
 
 // A wave a row.
-template <typename T, int VW>
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedParams p) {
-  typedef Row<T, VW> R;
+  typedef Row<T, VEC> R;
   const int lane = threadIdx.x & 63;
   const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (m >= p.M) return;
@@ -91,7 +104,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedParams p) {
   for (int k = lane * R::kElems; k < p.K; k += 64 * R::kElems) {
     float x[R::kElems];
     if (v >= 0 && v < p.V) {
-      R::load(w + k, x);
+      R::unpack(R::load(w + k), x);
 #pragma unroll
       for (int i = 0; i < R::kElems; ++i) x[i] *= p.scale;
     } else {
@@ -107,31 +120,62 @@ __global__ __launch_bounds__(256) void embed_clear_kernel(uint32_t* p, int64_t n
   if (e < n) p[e] = 0;
 }
 
+// Equal tokens of a wave are counted together, in one access: those of a frequent token would
+// wait for each other (16384 tokens, one in 15 the same: 15 -> 5 us).
 __global__ __launch_bounds__(256) void embed_count_kernel(EmbedParams p) {
   const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (m >= p.M) return;
-  const int64_t v = token_at(p, m);
-  if (v >= 0 && v < p.V) p.place[m] = atomicAdd(p.count + v, 1u);
-}
-
-// Room for each token's list, in no particular order, and the chunks of the long ones.
-__global__ __launch_bounds__(256) void embed_room_kernel(EmbedParams p) {
-  const int v = blockIdx.x * 256 + threadIdx.x, lane = threadIdx.x & 63;
-  const uint32_t n = v < p.V ? p.count[v] : 0;
-  uint32_t upto = n;  // room of the wave's lanes up to this one
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t o = __shfl_up(upto, d);
-    if (lane >= d) upto += o;
+  const int64_t token = m < p.M ? token_at(p, m) : -1;
+  const bool some = token >= 0 && token < p.V;
+  const int v = (int)token, lane = threadIdx.x & 63;
+  uint64_t left = __builtin_amdgcn_ballot_w64(some);
+  int leader = lane, before = 0, count = 0;
+  while (left) {  // uniform: once for each token of the wave
+    const int l = __builtin_ctzll(left);
+    const uint64_t same = __builtin_amdgcn_ballot_w64(some && v == __builtin_amdgcn_readlane(v, l));
+    if (same >> lane & 1) {
+      leader = l;
+      before = __popcll(same & ((uint64_t(1) << lane) - 1));
+      count = __popcll(same);
+    }
+    left &= ~same;
   }
   uint32_t base = 0;
-  if (lane == 63 && upto) base = atomicAdd(p.cursor, upto);
-  base = __shfl(base, 63);
-  if (n) p.start[v] = base + upto - n;
-  if (n > 64) {
-    const uint32_t parts = (n + p.chunk - 1) / p.chunk, first = atomicAdd(p.cursor + 1, parts);
-    for (uint32_t c = 0; c < parts && first + c < (uint32_t)p.most_chunks; ++c) p.chunks[first + c] = uint4{(uint32_t)v, first, c, parts};
+  if (some && leader == lane) base = atomicAdd(p.count + v, (uint32_t)count);
+  base = __shfl(base, leader);
+  if (some) p.place[m] = base + before;
+}
+
+constexpr uint32_t kShort = 16;  // positions of a list that a wave sums
+
+// Room for each token's list, in no particular order, and the chunks of the long ones.
+__global__ __launch_bounds__(1024) void embed_room_kernel(EmbedParams p) {
+  __shared__ uint32_t waves[2][16], base[2];
+  const int v = blockIdx.x * 1024 + threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t n = v < p.V ? p.count[v] : 0, parts = n > kShort ? (n + p.chunk - 1) / p.chunk : 0;
+  uint32_t upto[2] = {n, parts};  // of the wave's lanes up to this one
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t o = __shfl_up(upto[k], d);
+      if (lane >= d) upto[k] += o;
+    }
+    if (lane == 63) waves[k][wave] = upto[k];
   }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    uint32_t all = 0;
+    for (int w = 0; w < 16; ++w) {
+      const uint32_t x = waves[threadIdx.x][w];
+      waves[threadIdx.x][w] = all;
+      all += x;
+    }
+    base[threadIdx.x] = all ? atomicAdd(p.cursor + threadIdx.x, all) : 0;
+  }
+  __syncthreads();
+  if (n) p.start[v] = base[0] + waves[0][wave] + upto[0] - n;
+  const uint32_t first = base[1] + waves[1][wave] + upto[1] - parts;
+  for (uint32_t c = 0; c < parts && first + c < (uint32_t)p.most_chunks; ++c) p.chunks[first + c] = uint4{(uint32_t)v, first, c, parts};
 }
 
 __global__ __launch_bounds__(256) void embed_place_kernel(EmbedParams p) {
@@ -141,110 +185,256 @@ __global__ __launch_bounds__(256) void embed_place_kernel(EmbedParams p) {
   if (v >= 0 && v < p.V) p.list[p.start[v] + p.place[m]] = (uint32_t)m;
 }
 
-// The rows rows[0 .. n) of dout, in that order, from column k on. Loads of four are in flight.
-template <typename T, int VW>
-__device__ __forceinline__ void sum_rows(const EmbedParams& p, const uint32_t* rows, int n, int k, float (&s)[Row<T, VW>::kElems]) {
-  typedef Row<T, VW> R;
-  const T* dout = static_cast<const T*>(p.dout) + k;
+// All of the lists by one workgroup, whose counters are in LDS, where tokens are few: one launch instead of
+// four (1237 tokens of 1003: 14 -> 4.6 us on the GPU; 16384 of 32000 would take 61, four launches 19).
+constexpr int kOneTokens = 4096, kOneVocabulary = 4096;
+__global__ __launch_bounds__(1024) void embed_lists_kernel(EmbedParams p) {
+  constexpr int kEach = kOneTokens / 1024;
+  __shared__ uint32_t count[kOneVocabulary];
+  __shared__ uint32_t waves[2][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int v = threadIdx.x; v < p.V; v += 1024) count[v] = 0;
+  int token[kEach];
 #pragma unroll
-  for (int i = 0; i < R::kElems; ++i) s[i] = 0.0f;
-  for (int j0 = 0; j0 < n; j0 += 4) {
-    float x[4][R::kElems];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j0 + j < n) R::load(dout + (int64_t)rows[j0 + j] * p.so, x[j]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j0 + j < n)
-#pragma unroll
-        for (int i = 0; i < R::kElems; ++i) s[i] += x[j][i];
-  }
-}
-
-// A wave a token whose list is short: sorts it and sums its rows.
-template <typename T, int VW>
-__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedParams p) {
-  typedef Row<T, VW> R;
-  __shared__ uint32_t sorted[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v = blockIdx.x * 4 + wave;
-  const int n = v < p.V ? __builtin_amdgcn_readfirstlane((int)p.count[v]) : 0;
-  if (n > 0 && n <= 64) {
-    const uint32_t mine = lane < n ? p.list[p.start[v] + lane] : 0xffffffffu;
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, j) < mine ? 1 : 0;
-    if (lane < n) sorted[wave][rank] = mine;
+  for (int i = 0; i < kEach; ++i) {
+    const int64_t m = i * 1024 + (int64_t)threadIdx.x, t = m < p.M ? token_at(p, m) : -1;
+    token[i] = t >= 0 && t < p.V ? (int)t : -1;
   }
   __syncthreads();
-  if (v >= p.V || n > 64) return;
-  T* dw = static_cast<T*>(p.dw) + (int64_t)v * p.K;
-  for (int k = lane * R::kElems; k < p.K; k += 64 * R::kElems) {
-    float s[R::kElems];
-    sum_rows<T, VW>(p, sorted[wave], n, k, s);
+  uint32_t place[kEach];
 #pragma unroll
-    for (int i = 0; i < R::kElems; ++i) s[i] *= p.scale;
-    R::store(dw + k, s);
+  for (int i = 0; i < kEach; ++i) place[i] = token[i] >= 0 ? atomicAdd(count + token[i], 1u) : 0;
+  __syncthreads();
+  // room: a thread takes `per` tokens; then the room of the threads before it
+  const int per = (p.V + 1023) / 1024, v0 = threadIdx.x * per;
+  uint32_t mine[2] = {0, 0};
+  for (int v = v0; v < min(v0 + per, p.V); ++v) {
+    mine[0] += count[v];
+    mine[1] += count[v] > kShort ? (count[v] + p.chunk - 1) / p.chunk : 0;
   }
+  uint32_t upto[2] = {mine[0], mine[1]};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t o = __shfl_up(upto[k], d);
+      if (lane >= d) upto[k] += o;
+    }
+    if (lane == 63) waves[k][wave] = upto[k];
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    uint32_t all = 0;
+    for (int w = 0; w < 16; ++w) {
+      const uint32_t x = waves[threadIdx.x][w];
+      waves[threadIdx.x][w] = all;
+      all += x;
+    }
+    p.cursor[threadIdx.x] = all;
+  }
+  __syncthreads();
+  uint32_t at = waves[0][wave] + upto[0] - mine[0], chunk = waves[1][wave] + upto[1] - mine[1];
+  for (int v = v0; v < min(v0 + per, p.V); ++v) {
+    const uint32_t n = count[v];
+    p.count[v] = n;
+    p.start[v] = at;
+    count[v] = at;
+    at += n;
+    const uint32_t parts = n > kShort ? (n + p.chunk - 1) / p.chunk : 0;
+    for (uint32_t c = 0; c < parts && chunk + c < (uint32_t)p.most_chunks; ++c) p.chunks[chunk + c] = uint4{(uint32_t)v, chunk, c, parts};
+    chunk += parts;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (token[i] >= 0) p.list[count[token[i]] + place[i]] = (uint32_t)(i * 1024 + threadIdx.x);
 }
 
-// A workgroup a chunk of a long list: the positions of ranks chunk c to chunk (c + 1).
-// Bits of kWindow positions at a time say which are in the list; the bits before one are its rank.
-constexpr int kWindow = 1 << 17, kMostChunk = 2048;
-template <typename T, int VW>
-__global__ __launch_bounds__(256) void embed_chunk_kernel(EmbedParams p) {
-  typedef Row<T, VW> R;
-  __shared__ uint32_t bits[kWindow / 32];
-  __shared__ uint32_t rows[kMostChunk];
-  __shared__ uint32_t upto[256];
-  if (blockIdx.x >= min(p.cursor[1], (uint32_t)p.most_chunks)) return;  // uniform
-  const uint4 c = p.chunks[blockIdx.x];
+// What a wave sums at once: kCols elements of a lane, of columns from k on, in rows whose loads are in flight together.
+template <typename T, bool VEC>
+struct Sum {
+  typedef Row<T, VEC> R;
+  static constexpr int kCols = VEC ? 2 : 8, kRows = 4, kSpan = 64 * R::kElems * kCols;
+  float s[kCols][R::kElems];
+  // rows row(0) .. row(n - 1) of dout, in that order (row: uniform)
+  template <typename F>
+  __device__ __forceinline__ void rows(const EmbedParams& p, int n, int k, F&& row) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int i = 0; i < R::kElems; ++i) s[c][i] = 0.0f;
+    const T* dout = static_cast<const T*>(p.dout);
+    for (int j0 = 0; j0 < n; j0 += kRows) {
+      typename R::Raw raw[kRows][kCols];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        if (j0 + j >= n) break;  // uniform
+        const T* src = dout + (int64_t)row(j0 + j) * p.so;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          if (k + c * 64 * R::kElems < p.K) raw[j][c] = R::load(src + k + c * 64 * R::kElems);
+      }
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        if (j0 + j >= n) break;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          if (k + c * 64 * R::kElems >= p.K) continue;
+          float x[R::kElems];
+          R::unpack(raw[j][c], x);
+#pragma unroll
+          for (int i = 0; i < R::kElems; ++i) s[c][i] += x[i];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(const EmbedParams& p, int64_t v, int k) {
+    T* dw = static_cast<T*>(p.dw) + v * p.K;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      if (k + c * 64 * R::kElems >= p.K) continue;
+      float x[R::kElems];
+#pragma unroll
+      for (int i = 0; i < R::kElems; ++i) x[i] = s[c][i] * p.scale;
+      R::store(dw + k + c * 64 * R::kElems, x);
+    }
+  }
+};
+
+// A workgroup a chunk of a long list: the positions of ranks chunk c to chunk (c + 1). With kAll
+// positions or fewer, a rank is counted; otherwise bits of kWindow positions at a time say which are in
+// the list, and the bits before one are its rank.
+constexpr int kWindow = 1 << 17, kMostChunk = 2048, kAll = 256, kMostSpan = 1024;
+union ChunkShared {
+  struct {
+    uint32_t bits[kWindow / 32], upto[256];
+  } sort;
+  uint32_t all[kAll];
+  float sums[3][kMostSpan];
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void sum_chunk(const EmbedParams& p, const uint4 c, int id, ChunkShared& lds, uint32_t* rows) {
+  typedef Sum<T, VEC> S;
+  static_assert(S::kSpan <= kMostSpan, "columns of a pass");
   const uint32_t n = p.count[c.x], from = c.z * p.chunk, to = min(n, from + p.chunk);
   const uint32_t* list = p.list + p.start[c.x];
-  uint32_t before = 0;  // positions of the list in the windows before
-  for (int64_t base = 0; base < p.M && before < to; base += kWindow) {
-    const int words = (int)min((int64_t)kWindow, p.M - base + 31) / 32;
-    for (int i = threadIdx.x; i < words; i += 256) bits[i] = 0;
+  if (n <= kAll) {
+    const uint32_t mine = threadIdx.x < n ? list[threadIdx.x] : 0xffffffffu;
+    lds.all[threadIdx.x] = mine;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += 256) {
-      const int64_t at = (int64_t)list[i] - base;
-      if (at >= 0 && at < kWindow) atomicOr(bits + at / 32, 1u << (at & 31));
-    }
-    __syncthreads();
-    // each thread counts the bits of a run of words; then the runs before it
-    const int per = (words + 255) / 256, w0 = threadIdx.x * per;
-    uint32_t mine = 0;
-    for (int i = w0; i < min(w0 + per, words); ++i) mine += __popc(bits[i]);
-    upto[threadIdx.x] = mine;
-    __syncthreads();
-    for (int d = 1; d < 256; d *= 2) {
-      const uint32_t o = (int)threadIdx.x >= d ? upto[threadIdx.x - d] : 0;
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < n; ++j) rank += lds.all[j] < mine ? 1 : 0;
+    if (threadIdx.x < n && rank >= from && rank < to) rows[rank - from] = mine;
+  } else {
+    uint32_t before = 0;  // positions of the list in the windows before
+    for (int64_t base = 0; base < p.M && before < to; base += kWindow) {
+      const int words = (int)min((int64_t)kWindow, p.M - base + 31) / 32;
+      for (int i = threadIdx.x; i < words; i += 256) lds.sort.bits[i] = 0;
       __syncthreads();
-      upto[threadIdx.x] += o;
+      for (uint32_t i = threadIdx.x; i < n; i += 256) {
+        const int64_t at = (int64_t)list[i] - base;
+        if (at >= 0 && at < kWindow) atomicOr(lds.sort.bits + at / 32, 1u << (at & 31));
+      }
+      __syncthreads();
+      // each thread counts the bits of a run of words; then the runs before it
+      const int per = (words + 255) / 256, w0 = threadIdx.x * per;
+      uint32_t mine = 0;
+      for (int i = w0; i < min(w0 + per, words); ++i) mine += __popc(lds.sort.bits[i]);
+      lds.sort.upto[threadIdx.x] = mine;
+      __syncthreads();
+      for (int d = 1; d < 256; d *= 2) {
+        const uint32_t o = (int)threadIdx.x >= d ? lds.sort.upto[threadIdx.x - d] : 0;
+        __syncthreads();
+        lds.sort.upto[threadIdx.x] += o;
+        __syncthreads();
+      }
+      uint32_t rank = before + lds.sort.upto[threadIdx.x] - mine;
+      if (rank < to && rank + mine > from) {
+        for (int i = w0; i < min(w0 + per, words); ++i)
+          for (uint32_t w = lds.sort.bits[i]; w; w &= w - 1, ++rank)
+            if (rank >= from && rank < to) rows[rank - from] = (uint32_t)(base + 32 * i + __ffs(w) - 1);
+      }
+      before += lds.sort.upto[255];
       __syncthreads();
     }
-    uint32_t rank = before + upto[threadIdx.x] - mine;
-    if (rank < to && rank + mine > from) {
-      for (int i = w0; i < min(w0 + per, words); ++i)
-        for (uint32_t w = bits[i]; w; w &= w - 1, ++rank)
-          if (rank >= from && rank < to) rows[rank - from] = (uint32_t)(base + 32 * i + __ffs(w) - 1);
-    }
-    before += upto[255];
-    __syncthreads();
   }
-  const int count = (int)(to - from);
-  for (int k = threadIdx.x * R::kElems; k < p.K; k += 256 * R::kElems) {
-    float s[R::kElems];
-    sum_rows<T, VW>(p, rows, count, k, s);
+  // a quarter of the rows a wave, joined in order
+  const int count = (int)(to - from), quarter = (count + 3) / 4, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), first = min(count, wave * quarter);
+  const int mine = min(count, first + quarter) - first;
+  for (int k0 = 0; k0 < p.K; k0 += S::kSpan) {
+    const int k = k0 + lane * S::R::kElems;
+    __syncthreads();
+    S sum;
+    sum.rows(p, mine, k, [&](int j) { return __builtin_amdgcn_readfirstlane(rows[first + j]); });
+    if (wave > 0) {
 #pragma unroll
-    for (int i = 0; i < R::kElems; ++i) p.sums[(int64_t)blockIdx.x * p.K + k + i] = s[i];
+      for (int e = 0; e < S::kCols; ++e)
+#pragma unroll
+        for (int i = 0; i < S::R::kElems; ++i) lds.sums[wave - 1][(e * S::R::kElems + i) * 64 + lane] = sum.s[e][i];
+    }
+    __syncthreads();
+    if (wave != 0) continue;
+#pragma unroll
+    for (int e = 0; e < S::kCols; ++e)
+#pragma unroll
+      for (int i = 0; i < S::R::kElems; ++i) {
+        float& x = sum.s[e][i];
+#pragma unroll
+        for (int w = 0; w < 3; ++w) x += lds.sums[w][(e * S::R::kElems + i) * 64 + lane];
+        const int at = k + e * 64 * S::R::kElems + i;
+        if (c.w > 1 && at < p.K) p.sums[(int64_t)id * p.K + at] = x;
+      }
+    if (c.w == 1) sum.store(p, c.x, k);
   }
 }
 
-// The chunks of a long list in order: a workgroup a chunk, of which the first of each list works.
+// The first workgroups take a chunk of a long list each; a wave of the others four tokens
+// whose lists are short or empty.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedParams p) {
+  typedef Sum<T, VEC> S;
+  __shared__ ChunkShared lds;
+  __shared__ uint32_t rows[kMostChunk];
+  if ((int)blockIdx.x < p.most_chunks) {  // uniform
+    if (blockIdx.x < p.cursor[1]) sum_chunk<T, VEC>(p, p.chunks[blockIdx.x], (int)blockIdx.x, lds, rows);
+    return;
+  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int v0 = ((int)(blockIdx.x - p.most_chunks) * 4 + wave) * 4;
+  const bool some = lane < 4 && v0 + lane < p.V;
+  const int counts = some ? (int)p.count[v0 + lane] : -1;
+  const int starts = counts > 0 ? (int)p.start[v0 + lane] : 0;
+  int list[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int n = __builtin_amdgcn_readlane(counts, t);
+    list[t] = lane < n && n <= (int)kShort ? (int)p.list[(uint32_t)__builtin_amdgcn_readlane(starts, t) + lane] : 0x7fffffff;
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int n = __builtin_amdgcn_readlane(counts, t);
+    if (n < 0 || n > (int)kShort) continue;
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += __builtin_amdgcn_readlane(list[t], j) < list[t] ? 1 : 0;
+    // lane r gets the position of rank r (lanes without one send theirs past the list)
+    const int sorted = __builtin_amdgcn_ds_permute(4 * (lane < n ? rank : lane), list[t]);
+    for (int k0 = 0; k0 < p.K; k0 += S::kSpan) {
+      const int k = k0 + lane * S::R::kElems;
+      S sum;
+      sum.rows(p, n, k, [&](int j) { return __builtin_amdgcn_readlane(sorted, j); });
+      sum.store(p, v0 + t, k);
+    }
+  }
+}
+
+// The chunks of a list of several in order: a workgroup a chunk, of which the first of each list works.
 template <typename T>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedParams p) {
   if (blockIdx.x >= min(p.cursor[1], (uint32_t)p.most_chunks)) return;
   const uint4 c = p.chunks[blockIdx.x];
-  if (c.z != 0) return;
+  if (c.z != 0 || c.w == 1) return;
   for (int k = blockIdx.y * 256 + threadIdx.x; k < p.K; k += gridDim.y * 256) {
     const float* src = p.sums + (int64_t)c.y * p.K + k;
     float s = 0.0f;
@@ -270,8 +460,8 @@ struct Plan {
 Plan make_plan(int64_t M, int64_t V, int64_t K) {
   Plan r;
   r.chunk = (int)std::min<int64_t>(kMostChunk, std::max<int64_t>(64, (M / 512 + 63) / 64 * 64));
-  // a list of n > 64 has n / chunk rounded up
-  r.most_chunks = (int)(M / r.chunk + std::min<int64_t>(V, M / 65) + 1);
+  // a list of n > kShort has n / chunk rounded up
+  r.most_chunks = M > kShort ? (int)(M / r.chunk + std::min<int64_t>(V, M / (kShort + 1))) : 0;
   r.clear = 64 + V;  // cursors on a line of their own, counts
   r.start = align256(r.clear * 4);
   r.place = r.start + align256(V * 4);
@@ -297,6 +487,19 @@ int check(const Args* a, const char* who, int64_t stride) {
   if (a->M > 1 && stride < a->K)
     return set_error(GS_ERR_INVALID, "%s: a row stride of %lld does not hold K=%lld", who, (long long)stride, (long long)a->K);
   return check_dtype(who, a->dtype);
+}
+
+int make_lists(const EmbedParams& p, const Plan& plan, hipStream_t stream) {
+  const dim3 rows((unsigned)((p.M + 255) / 256));
+  hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)((plan.clear + 255) / 256)), dim3(256), 0, stream, p.cursor, plan.clear);
+  GS_CHECK_HIP(hipGetLastError());
+  hipLaunchKernelGGL(embed_count_kernel, rows, dim3(256), 0, stream, p);
+  GS_CHECK_HIP(hipGetLastError());
+  hipLaunchKernelGGL(embed_room_kernel, dim3((unsigned)((p.V + 1023) / 1024)), dim3(1024), 0, stream, p);
+  GS_CHECK_HIP(hipGetLastError());
+  hipLaunchKernelGGL(embed_place_kernel, rows, dim3(256), 0, stream, p);
+  GS_CHECK_HIP(hipGetLastError());
+  return GS_OK;
 }
 
 bool aligned16(const void* p, int64_t stride, int size) {
@@ -327,8 +530,8 @@ extern "C" int gs_embedding_fwd(const gs_embedding_args* a, hipStream_t stream) 
   p.K = (int)a->K;
   p.wide = a->token_bits == 64;
   const bool vec = aligned16(a->w, a->K, size) && aligned16(a->out, a->so, size);
-  auto fn = size == 4 ? (vec ? embed_fwd_kernel<float, 4> : embed_fwd_kernel<float, 0>)
-                      : (vec ? embed_fwd_kernel<__bf16, 4> : embed_fwd_kernel<__bf16, 0>);
+  auto fn = size == 4 ? (vec ? embed_fwd_kernel<float, true> : embed_fwd_kernel<float, false>)
+                      : (vec ? embed_fwd_kernel<__bf16, true> : embed_fwd_kernel<__bf16, false>);
   hipLaunchKernelGGL(fn, dim3((unsigned)((a->M + 3) / 4)), dim3(256), 0, stream, p);
   GS_CHECK_HIP(hipGetLastError());
   return GS_OK;
@@ -371,25 +574,18 @@ extern "C" int gs_embedding_bwd(const gs_embedding_bwd_args* a, hipStream_t stre
   p.sums = reinterpret_cast<float*>(s + plan.sums);
   p.chunk = plan.chunk;
   p.most_chunks = plan.most_chunks;
-  const dim3 rows((unsigned)((a->M + 255) / 256)), words((unsigned)((a->V + 255) / 256));
-  hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)((plan.clear + 255) / 256)), dim3(256), 0, stream, p.cursor, plan.clear);
-  GS_CHECK_HIP(hipGetLastError());
-  hipLaunchKernelGGL(embed_count_kernel, rows, dim3(256), 0, stream, p);
-  GS_CHECK_HIP(hipGetLastError());
-  hipLaunchKernelGGL(embed_room_kernel, words, dim3(256), 0, stream, p);
-  GS_CHECK_HIP(hipGetLastError());
-  hipLaunchKernelGGL(embed_place_kernel, rows, dim3(256), 0, stream, p);
-  GS_CHECK_HIP(hipGetLastError());
-  const bool vec = aligned16(a->dw, a->K, size) && aligned16(a->dout, a->sdo, size);
-  auto sum = size == 4 ? (vec ? embed_sum_kernel<float, 4> : embed_sum_kernel<float, 0>)
-                       : (vec ? embed_sum_kernel<__bf16, 4> : embed_sum_kernel<__bf16, 0>);
-  hipLaunchKernelGGL(sum, dim3((unsigned)((a->V + 3) / 4)), dim3(256), 0, stream, p);
-  GS_CHECK_HIP(hipGetLastError());
-  if (a->M > 64) {
-    auto chunk = size == 4 ? (vec ? embed_chunk_kernel<float, 4> : embed_chunk_kernel<float, 0>)
-                           : (vec ? embed_chunk_kernel<__bf16, 4> : embed_chunk_kernel<__bf16, 0>);
-    hipLaunchKernelGGL(chunk, dim3((unsigned)plan.most_chunks), dim3(256), 0, stream, p);
+  if (a->M <= kOneTokens && a->V <= kOneVocabulary) {
+    hipLaunchKernelGGL(embed_lists_kernel, dim3(1), dim3(1024), 0, stream, p);
     GS_CHECK_HIP(hipGetLastError());
+  } else {
+    if ((rc = make_lists(p, plan, stream))) return rc;
+  }
+  const bool vec = aligned16(a->dw, a->K, size) && aligned16(a->dout, a->sdo, size);
+  auto sum = size == 4 ? (vec ? embed_sum_kernel<float, true> : embed_sum_kernel<float, false>)
+                       : (vec ? embed_sum_kernel<__bf16, true> : embed_sum_kernel<__bf16, false>);
+  hipLaunchKernelGGL(sum, dim3((unsigned)(plan.most_chunks + (a->V + 15) / 16)), dim3(256), 0, stream, p);
+  GS_CHECK_HIP(hipGetLastError());
+  if (a->M > plan.chunk) {  // there may be a list of several chunks
     hipLaunchKernelGGL(size == 4 ? embed_join_kernel<float> : embed_join_kernel<__bf16>, dim3((unsigned)plan.most_chunks, 4),
                        dim3(256), 0, stream, p);
     GS_CHECK_HIP(hipGetLastError());

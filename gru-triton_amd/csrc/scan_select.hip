@@ -90,13 +90,12 @@ __device__ __forceinline__ T* row_of(const void* base, int64_t st, int64_t sb, i
   return const_cast<T*>(static_cast<const T*>(base)) + t * st + b * sb;
 }
 
-// The flags of a tile's steps as a bit mask.
-__device__ __forceinline__ uint32_t flags_of(Args p, const At& at, int t0) {
-  if (p->reset == nullptr) return 0;
-  bool f = false;
-  if (at.lane < kTile && t0 + at.lane < at.t1) f = p->reset[(t0 + at.lane) * p->sr_t + at.b * p->sr_b] != 0;
-  return (uint32_t)__builtin_amdgcn_ballot_w64(f);
+// The flags of kTile steps from t0 on, a lane each, and as a bit mask.
+__device__ __forceinline__ bool load_flag(Args p, const At& at, int t0) {
+  if (p->reset == nullptr) return false;
+  return at.lane < kTile && t0 + at.lane < at.t1 && p->reset[(t0 + at.lane) * p->sr_t + at.b * p->sr_b] != 0;
 }
+__device__ __forceinline__ uint32_t mask_of(bool flag) { return (uint32_t)__builtin_amdgcn_ballot_w64(flag); }
 
 // B and C of a tile as floats, a wave's P states side by side; zero where there is no step or state.
 typedef float f4v __attribute__((ext_vector_type(4)));
@@ -121,21 +120,33 @@ struct alignas(16) Pair {
   }
 };
 template <typename T, int P, int NW>
-__device__ __forceinline__ void stage_bc(Args p, const At& at, int t0, Pair<P> (*bc)[NW]) {
-  constexpr int NP = NW * P, kEach = kTile * NP;
+struct Tile {
+  static constexpr int NP = NW * P, kEach = kTile * NP, kPer = 2 * kEach / (64 * NW);
   static_assert(kEach % 64 == 0, "a wave's elements are all of B or all of C");
+  unsigned int x[kPer];  // on their way
+  __device__ __forceinline__ void load(Args p, const At& at, int t0) {
 #pragma unroll
-  for (int k = 0; k < 2 * kEach; k += 64 * NW) {
-    const int first = k + at.wave * 64;  // uniform
-    const bool c = first >= kEach;
-    const int e = (c ? first - kEach : first) + at.lane, s = e / NP, n = e % NP;
-    const T* row = c ? row_of<T>(p->cm, p->sc_t, p->sc_b, t0, at.b) : row_of<T>(p->bm, p->sb_t, p->sb_b, t0, at.b);
-    const int64_t st = c ? p->sc_t : p->sb_t;
-    float x = 0.0f;
-    if (n < p->N && t0 + s < at.t1) x = (float)row[s * st + n];
-    bc[s][n / P].x[(c ? P : 0) + n % P] = x;
+    for (int k = 0; k < kPer; ++k) {
+      const int first = (k * NW + at.wave) * 64;  // uniform
+      const bool c = first >= kEach;
+      const int e = (c ? first - kEach : first) + at.lane, s = e / NP, n = e % NP;
+      const T* row = c ? row_of<T>(p->cm, p->sc_t, p->sc_b, t0, at.b) : row_of<T>(p->bm, p->sb_t, p->sb_b, t0, at.b);
+      const int64_t st = c ? p->sc_t : p->sb_t;
+      x[k] = 0;
+      if (n < p->N && t0 + s < at.t1) x[k] = sizeof(T) == 2 ? *reinterpret_cast<const unsigned short*>(row + s * st + n)
+                                                            : *reinterpret_cast<const unsigned int*>(row + s * st + n);
+    }
   }
-}
+  __device__ __forceinline__ void put(const At& at, Pair<P> (*bc)[NW]) const {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int first = (k * NW + at.wave) * 64;
+      const bool c = first >= kEach;
+      const int e = (c ? first - kEach : first) + at.lane, s = e / NP, n = e % NP;
+      bc[s][n / P].x[(c ? P : 0) + n % P] = Elem<T>::value(x[k]);
+    }
+  }
+};
 
 // Backward: parts of the axis whose ends are found one by one; p.each of them make a chunk.
 __device__ __forceinline__ int parts_of(const SsmParams& p) {
@@ -188,8 +199,11 @@ __device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
   float span = 0.0f;
   bool drop = false;
   unsigned int rd[kOwn], ru[kOwn], rz[kOwn];
+  Tile<T, P, NW> tile;
+  bool flag;
   auto fetch = [&](int t0) __attribute__((always_inline)) {
-    Args p = args();
+    tile.load(p, at, t0);
+    flag = load_flag(p, at, t0);
     const int t = t0 + at.wave;
     const T* d = row_of<T>(p->delta, p->sdl_t, p->sdl_b, t, at.b);
     const T* u = row_of<T>(p->u, p->su_t, p->su_b, t, at.b);
@@ -214,13 +228,11 @@ __device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
       const float dt = t0 + s < at.t1 ? softplus(E::value(rd[i]) + bias) : 0.0f;
       lds.xs[s][at.lane] = float2{dt, dt * u[i]};
     }
-    p = args();
-    stage_bc<T, P, NW>(p, at, t0, lds.bc);
-    const uint32_t flags = flags_of(p, at, t0);
+    tile.put(at, lds.bc);
+    const uint32_t flags = mask_of(flag);
     share_barrier();
     if (t0 + kTile < at.t1) fetch(t0 + kTile);
     if (OUT) {
-      p = args();
       if (p->saved != nullptr && at.ok) {
         float* to = p->saved + (((int64_t)(t0 / kTile) * p->B + at.b) * p->N + n0) * p->H + at.ch;
 #pragma unroll
@@ -251,7 +263,6 @@ __device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
     if (!OUT && flags) drop = true;
     share_barrier();
     if constexpr (OUT) {
-      p = args();
       T* to = row_of<T>(p->y, p->sy_t, p->sy_b, t0 + at.wave, at.b);
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
@@ -268,7 +279,6 @@ __device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
     }
   }
   if (!at.ok) return;
-  p = args();
   const int64_t row = (int64_t)at.chunk * p->B + at.b;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
@@ -368,8 +378,10 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
   bool drop = false;
   unsigned int rd[kGroup], ru[kGroup], rz[kGroup];
   Rows<T, NP> rows;
+  bool flag;
   auto fetch = [&](int t) __attribute__((always_inline)) {
     rows.load(at, t);
+    flag = load_flag(p, at, t);
     const T* d = row_of<T>(p->delta, p->sdl_t, p->sdl_b, t, at.b);
     const T* u = row_of<T>(p->u, p->su_t, p->su_b, t, at.b);
     const T* z = row_of<T>(p->z, p->sz_t, p->sz_b, t, at.b);
@@ -384,7 +396,7 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
   rows.init(p, at, at.t0, false);
   fetch(at.t0);
   for (int t0 = at.t0; t0 < at.t1; t0 += kGroup) {
-    const uint32_t flags = flags_of(p, at, t0);
+    const uint32_t flags = mask_of(flag);
     if (OUT && p->saved != nullptr && t0 % kTile == 0 && at.ok) {
       float* to = p->saved + ((int64_t)(t0 / kTile) * p->B + at.b) * N * p->H + at.ch;
 #pragma unroll
@@ -518,8 +530,11 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams kernel_
   float span = 0.0f;
   bool drop = false;
   unsigned int rd[kOwn], rz[kOwn], rg[kOwn];
+  Tile<T, P, NW> tile;
+  bool flag;
   auto fetch = [&](int t0) __attribute__((always_inline)) {
-    Args p = args();
+    tile.load(p, at, t0);
+    flag = load_flag(p, at, t0);
     const int t = t0 + at.wave;
     const T* d = row_of<T>(p->delta, p->sdl_t, p->sdl_b, t, at.b);
     const T* g = row_of<T>(p->dy, p->sdy_t, p->sdy_b, t, at.b);
@@ -536,7 +551,6 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams kernel_
   const int last = at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile;
   fetch(last);
   for (int t0 = last; t0 >= at.t0; t0 -= kTile) {
-    p = args();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int s = at.wave + NW * i;
@@ -544,8 +558,8 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams kernel_
       const float z = E::value(rz[i]), g = E::value(rg[i]);
       xs[s][at.lane] = float2{dt, p->z != nullptr ? g * (z * sigmoid(z)) : g};
     }
-    stage_bc<T, P, NW>(p, at, t0, bc);
-    const uint32_t flags = flags_of(p, at, t0);
+    tile.put(at, bc);
+    const uint32_t flags = mask_of(flag);
     share_barrier();
     if (t0 > at.t0) fetch(t0 - kTile);
     with_flags(flags, [&](auto F) __attribute__((always_inline)) {
@@ -568,7 +582,6 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams kernel_
     share_barrier();
   }
   if (!at.ok) return;
-  p = args();
   const int64_t row = (int64_t)at.chunk * p->B + at.b;
 #pragma unroll
   for (int i = 0; i < P; ++i)
@@ -604,8 +617,10 @@ __global__ __launch_bounds__(64) void ssm_bwd_ends_wide_kernel(SsmParams) {
   bool drop = false;
   unsigned int rd[kGroup], rz[kGroup], rg[kGroup];
   Rows<T, NP> rows;
+  bool flag;
   auto fetch = [&](int t) __attribute__((always_inline)) {
     rows.load(at, t);
+    flag = load_flag(p, at, t);
     const T* d = row_of<T>(p->delta, p->sdl_t, p->sdl_b, t, at.b);
     const T* g = row_of<T>(p->dy, p->sdy_t, p->sdy_b, t, at.b);
     const T* z = row_of<T>(p->z, p->sz_t, p->sz_b, t, at.b);
@@ -621,7 +636,7 @@ __global__ __launch_bounds__(64) void ssm_bwd_ends_wide_kernel(SsmParams) {
   rows.init(p, at, last, true);
   fetch(last);
   for (int t0 = last; t0 >= at.t0; t0 -= kGroup) {
-    const uint32_t flags = flags_of(p, at, t0);
+    const uint32_t flags = mask_of(flag);
     rows.put(bc, at);
     float dt[kGroup], dy[kGroup];
 #pragma unroll
@@ -706,6 +721,14 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
     asm volatile("" : "+v"(at.lane), "+s"(at.wave));  // addresses made from these are made anew, not kept
     const Pair<P>(*const bc)[NW] = lds.bc[at.ok ? 0 : 1];
     const bool gated = p->z != nullptr;
+    // loaded a tile ahead, these would take registers that are not there
+    Tile<T, P, NW> tile;
+    tile.load(p, at, t0);
+    const bool flag = load_flag(p, at, t0);
+    float start[P];
+    const float* from = p->saved + (((int64_t)(t0 / kTile) * p->B + at.b) * p->N + n0) * p->H + at.ch;
+#pragma unroll
+    for (int i = 0; i < P; ++i) start[i] = at.ok && (!PAD || i < live) ? from[(int64_t)i * p->H] : 0.0f;
     float u[kOwn], x[kOwn], dzy[kOwn];  // dzy: dz / y
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
@@ -718,14 +741,8 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
       lds.xs[s][at.lane] = float2{dt, dt * u[i]};
       lds.ds[s][at.lane] = gated ? d * (z * g) : d;
     }
-    stage_bc<T, P, NW>(p, at, t0, lds.bc[0]);
-    const uint32_t flags = flags_of(p, at, t0);
-    float start[P];
-    {
-      const float* from = p->saved + (((int64_t)(t0 / kTile) * p->B + at.b) * p->N + n0) * p->H + at.ch;
-#pragma unroll
-      for (int i = 0; i < P; ++i) start[i] = at.ok && (!PAD || i < live) ? from[(int64_t)i * p->H] : 0.0f;
-    }
+    tile.put(at, lds.bc[0]);
+    const uint32_t flags = mask_of(flag);
     share_barrier();
     with_flags(flags, [&](auto F) __attribute__((always_inline)) {
       constexpr bool RESET = decltype(F)::value;
@@ -917,7 +934,8 @@ __global__ __launch_bounds__(256) void ssm_sum_a_kernel(const float* part, float
 }
 
 // One token for each row of a batch of requests, whose states are rows of a cache [S, H, N]:
-// four lanes a channel, which hold every fourth state. One launch.
+// four lanes a channel, which hold four states side by side in turn (or, where states are not a multiple of
+// four, every fourth one). One launch. B 301, H 1002 in fp32: 15.2 -> 10.8 us with whole accesses, 4 TB/s.
 struct SsmStepParams {
   const void *u, *delta, *z, *bm, *cm;
   const float *A, *D, *bias;
@@ -928,7 +946,7 @@ struct SsmStepParams {
   int B, H, N, S;
 };
 
-template <typename T>
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepParams p) {
   const int q = threadIdx.x & 3, ch = blockIdx.x * 64 + (threadIdx.x >> 2), b = blockIdx.y;
   if (ch >= p.H) return;
@@ -944,10 +962,21 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepParams p) {
   const float* A = p.A + (int64_t)ch * p.N;
   float* h = p.state + slot * p.ss + (int64_t)ch * p.N;
   float y = 0.0f;
-  for (int n = q; n < p.N; n += 4) {
-    const float x = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * (A[n] * kLog2e)), h[n], dt * u * (float)bm[n]);
-    h[n] = x;
+  auto state = [&](int n, float a, float before) __attribute__((always_inline)) {
+    const float x = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * (a * kLog2e)), before, dt * u * (float)bm[n]);
     y = __builtin_fmaf((float)cm[n], x, y);
+    return x;
+  };
+  if constexpr (VEC) {
+    for (int n = 4 * q; n < p.N; n += 16) {
+      const f4v a = *reinterpret_cast<const f4v*>(A + n);
+      f4v x = *reinterpret_cast<const f4v*>(h + n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = state(n + i, a[i], x[i]);
+      *reinterpret_cast<f4v*>(h + n) = x;
+    }
+  } else {
+    for (int n = q; n < p.N; n += 4) h[n] = state(n, A[n], h[n]);
   }
   y += lane_xor_c<1>(y);
   y += lane_xor_c<2>(y);
@@ -1262,8 +1291,11 @@ extern "C" int gs_ssm_step(const gs_ssm_step_args* a, hipStream_t stream) {
   if (a->B > 65535) return set_error(GS_ERR_INVALID, "%s: B=%lld exceeds 65535", who, (long long)a->B);
   SsmStepParams p{a->u, a->delta, a->z, a->bm, a->cm, a->A, a->D, a->delta_bias, a->state, a->slots, a->y,
                   a->su, a->sdl, a->sz, a->sb, a->sc, a->ss, a->sy, (int)a->B, (int)a->H, (int)a->N, (int)a->S};
-  hipLaunchKernelGGL(a->dtype == GS_DTYPE_F32 ? ssm_step_kernel<float> : ssm_step_kernel<__bf16>,
-                     dim3((unsigned)((a->H + 63) / 64), (unsigned)a->B), dim3(256), 0, stream, p);
+  const bool vec = a->N % 4 == 0 && a->ss % 4 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(a->A) | reinterpret_cast<uintptr_t>(a->state)) & 15u) == 0;
+  void (*fn)(SsmStepParams) = a->dtype == GS_DTYPE_F32 ? (vec ? ssm_step_kernel<float, true> : ssm_step_kernel<float, false>)
+                                                       : (vec ? ssm_step_kernel<__bf16, true> : ssm_step_kernel<__bf16, false>);
+  hipLaunchKernelGGL(fn, dim3((unsigned)((a->H + 63) / 64), (unsigned)a->B), dim3(256), 0, stream, p);
   GS_CHECK_HIP(hipGetLastError());
   return GS_OK;
 }
