@@ -37,6 +37,7 @@ from .linear import linear_act
 from .conv import causal_conv, causal_conv_step
 from .selective import selective_scan, selective_step
 from .selective_layer import SelectiveLayer
+from .token_model import TokenModel
 from .tokens import embedding, token_logprobs
 from .optim import AdamW, adamw_dequantize_state, adamw_step
 from .export import dequantize_int_weights, export_int_weights, quantize_rows
@@ -48,6 +49,7 @@ __all__ = [
     "FakeQuantizePerTensor",
     "GatedLinearLayer",
     "SelectiveLayer",
+    "TokenModel",
     "GRUScanFunction",
     "GRUScanPersistentFunction",
     "QuantizerConfig",

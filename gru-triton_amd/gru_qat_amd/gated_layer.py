@@ -47,6 +47,10 @@ class GatedLinearLayer(torch.nn.Module):
         out, h = gated_linear_scan(gi, h0, activation=self.activation, reset=reset, batch_first=self.batch_first)
         return linear_act(out, self.weight_o, self.bias_o, residual=x), h
 
+    def new_state(self, rows: int) -> torch.Tensor:
+        """A cache of ``rows`` requests that have seen nothing yet."""
+        return torch.zeros(rows, self.hidden, device=self.weight_g.device)
+
     @torch.no_grad()
     def step(self, x: torch.Tensor, state: torch.Tensor, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
         """y [B, size] for one token x [B, size] of each request; ``state`` [S, hidden] float32
