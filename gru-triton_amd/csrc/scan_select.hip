@@ -35,8 +35,7 @@ struct SsmParams {
   float* h_last;
   float* saved;        // [ceil(T / kTile)][B][N][H]: forward written (or NULL), backward read
   float* ends;         // [chunks][B][N][H]: see ssm_join_kernel
-  float* span;         // [chunks][B][H]: sum of dt over a chunk
-  float* dropped;      // [chunks][B]: 1 where a chunk holds a reset
+  float* span;         // [chunks][B][H]: sum of dt over a chunk, -1 where it holds a reset
   const void* dy;      // backward only from here
   const float* dh_last;
   void *du, *ddelta, *dz;
@@ -154,6 +153,10 @@ __device__ __forceinline__ int parts_of(const SsmParams& p) {
   return (p.T + length - 1) / length;
 }
 
+// A as the exponent of 2. One of -infinity, a state that lasts a step, is held finite: the steps behind the
+// axis' end have step size 0, which must not make a NaN with it.
+__device__ __forceinline__ float rate(float A) { return A == -__builtin_inff() ? -3.0e38f : A * kLog2e; }
+
 // f(std::true_type) where a tile holds a reset, else f(std::false_type): uniform.
 template <typename F>
 __device__ __forceinline__ void with_flags(uint32_t flags, F&& f) {
@@ -186,7 +189,7 @@ __device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
   for (int i = 0; i < P; ++i) {
     const int n = n0 + i;
     const bool some = at.ok && n < p->N;
-    A2[i] = some ? p->A[(int64_t)at.ch * p->N + n] * kLog2e : 0.0f;
+    A2[i] = some ? rate(p->A[(int64_t)at.ch * p->N + n]) : 0.0f;
     h[i] = 0.0f;
     if (OUT && some) {
       if (at.chunk) h[i] = p->ends[(((int64_t)(at.chunk - 1) * p->B + at.b) * p->N + n) * p->H + at.ch];
@@ -289,8 +292,7 @@ __device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
     if (!OUT || (at.chunk == 0 && p->chunks > 1)) p->ends[(row * p->N + n) * p->H + at.ch] = h[i];
   }
   if (!OUT) {
-    if (at.wave == 0) p->span[row * p->H + at.ch] = span;
-    if (threadIdx.x == 0 && at.block == 0) p->dropped[row] = drop ? 1.0f : 0.0f;
+    if (at.wave == 0) p->span[row * p->H + at.ch] = drop ? -1.0f : span;
   }
 }
 
@@ -363,7 +365,7 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
 #pragma unroll
   for (int n = 0; n < NP; ++n) {
     const bool some = at.ok && n < N;
-    A2[n] = some ? p->A[(int64_t)at.ch * N + n] * kLog2e : 0.0f;
+    A2[n] = some ? rate(p->A[(int64_t)at.ch * N + n]) : 0.0f;
     h[n] = 0.0f;
     if (OUT && some) {
       if (at.chunk) h[n] = p->ends[(((int64_t)(at.chunk - 1) * p->B + at.b) * N + n) * p->H + at.ch];
@@ -451,8 +453,7 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
     if (!OUT || (at.chunk == 0 && p->chunks > 1)) p->ends[(row * N + n) * p->H + at.ch] = h[n];
   }
   if (!OUT) {
-    p->span[row * p->H + at.ch] = span;
-    if (at.lane == 0 && at.block == 0) p->dropped[row] = drop ? 1.0f : 0.0f;
+    p->span[row * p->H + at.ch] = drop ? -1.0f : span;
   }
 }
 
@@ -468,32 +469,36 @@ __global__ __launch_bounds__(64) void ssm_fwd_wide_kernel(SsmParams p) {
 // chunk c makes of zero, and on return the state after it. BACK: slot c holds what part c of the axis
 // sends back of a zero gradient, and on return of the whole: from the last part to the second chunk's first.
 template <bool BACK>
-__global__ __launch_bounds__(256) void ssm_join_kernel(SsmParams p) {
-  const int64_t plane = (int64_t)p.B * p.N * p.H, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(64) void ssm_join_kernel(SsmParams p) {
+  constexpr int kAhead = 16;  // slots whose loads are in flight together
+  const int64_t plane = (int64_t)p.B * p.N * p.H, e = (int64_t)blockIdx.x * 64 + threadIdx.x;
   if (e >= plane) return;
   const int ch = (int)(e % p.H), n = (int)(e / p.H % p.N), b = (int)(e / p.H / p.N);
-  const float A2 = p.A[(int64_t)ch * p.N + n] * kLog2e;
+  const float A2 = rate(p.A[(int64_t)ch * p.N + n]);
   float s = 0.0f;
   if (!BACK) s = p.ends[e];
   if (BACK && p.dh_last != nullptr) s = p.dh_last[((int64_t)b * p.H + ch) * p.N + n];
-  const int all = parts_of(p);
-  const int count = BACK ? all - p.each : p.chunks - 2;
-  constexpr int kAhead = 8;
+  const int all = parts_of(p), count = BACK ? all - p.each : p.chunks - 2, first = BACK ? all - 1 : 1;
+  const int64_t step = BACK ? -plane : plane, span_step = (BACK ? -1 : 1) * (int64_t)p.B * p.H;
+  float* slot = p.ends + first * plane + e;
+  const float* span = p.span + ((int64_t)first * p.B + b) * p.H + ch;
   for (int k0 = 0; k0 < count; k0 += kAhead) {
-    float end[kAhead], span[kAhead], drop[kAhead];
+    float end[kAhead], over[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int j = min(k0 + k, count - 1), c = BACK ? all - 1 - j : 1 + j;
-      end[k] = p.ends[c * plane + e];
-      span[k] = p.span[((int64_t)c * p.B + b) * p.H + ch];
-      drop[k] = p.dropped[(int64_t)c * p.B + b];
+      end[k] = over[k] = 0.0f;
+      if (k0 + k >= count) continue;  // uniform
+      end[k] = slot[k * step];
+      over[k] = span[k * span_step];
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      if (k0 + k >= count) break;
-      s = drop[k] != 0.0f ? end[k] : __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * span[k]), s, end[k]);
-      p.ends[(BACK ? all - 1 - (k0 + k) : 1 + k0 + k) * plane + e] = s;
+      if (k0 + k >= count) continue;
+      s = over[k] < 0.0f ? end[k] : __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * over[k]), s, end[k]);
+      slot[k * step] = s;
     }
+    slot += kAhead * step;
+    span += kAhead * span_step;
   }
 }
 
@@ -522,7 +527,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams kernel_
   float A2[P], e[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    A2[i] = at.ok && n0 + i < p->N ? p->A[(int64_t)at.ch * p->N + n0 + i] * kLog2e : 0.0f;
+    A2[i] = at.ok && n0 + i < p->N ? rate(p->A[(int64_t)at.ch * p->N + n0 + i]) : 0.0f;
     e[i] = 0.0f;
   }
   const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
@@ -586,8 +591,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams kernel_
 #pragma unroll
   for (int i = 0; i < P; ++i)
     if (n0 + i < p->N) p->ends[(row * p->N + n0 + i) * p->H + at.ch] = e[i];
-  if (at.wave == 0) p->span[row * p->H + at.ch] = span;
-  if (threadIdx.x == 0 && at.block == 0) p->dropped[row] = drop ? 1.0f : 0.0f;
+  if (at.wave == 0) p->span[row * p->H + at.ch] = drop ? -1.0f : span;
 }
 
 // The gradient that a part of the axis sends to the state before it, from a zero gradient after
@@ -607,7 +611,7 @@ __global__ __launch_bounds__(64) void ssm_bwd_ends_wide_kernel(SsmParams) {
   float A2[NP], e[NP];
 #pragma unroll
   for (int n = 0; n < NP; ++n) {
-    A2[n] = at.ok && n < N ? p->A[(int64_t)at.ch * N + n] * kLog2e : 0.0f;
+    A2[n] = at.ok && n < N ? rate(p->A[(int64_t)at.ch * N + n]) : 0.0f;
     e[n] = 0.0f;
   }
   const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
@@ -668,8 +672,7 @@ __global__ __launch_bounds__(64) void ssm_bwd_ends_wide_kernel(SsmParams) {
 #pragma unroll
   for (int n = 0; n < NP; ++n)
     if (n < N) p->ends[(row * N + n) * p->H + at.ch] = e[n];
-  p->span[row * p->H + at.ch] = span;
-  if (at.lane == 0 && at.block == 0) p->dropped[row] = drop ? 1.0f : 0.0f;
+  p->span[row * p->H + at.ch] = drop ? -1.0f : span;
 }
 
 template <typename T, int P, int NW, bool PAD>
@@ -683,7 +686,7 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
   for (int i = 0; i < P; ++i) {
     const int n = n0 + i;
     const bool some = at.ok && n < p->N;
-    A2[i] = some ? p->A[(int64_t)at.ch * p->N + n] * kLog2e : 0.0f;
+    A2[i] = some ? rate(p->A[(int64_t)at.ch * p->N + n]) : 0.0f;
     dA[i] = 0.0f;
     e[i] = 0.0f;
     if (some) {
@@ -884,53 +887,65 @@ __global__ __launch_bounds__(64 * NW, P == 2 && NW == 8 ? 4 : 2) void ssm_bwd_ke
   bwd_chunk<T, P, NW, PAD>(At(p, 0, p.length), lds);
 }
 
-// dB and dC [T, B, N]: the channel blocks' sums in order.
+// What the workgroups' sums make together, in order: dB and dC [T, B, N] over the channel blocks, by the first
+// bc_groups workgroups; dA [H, N], dD and dbias [H] over chunks and batch rows by the others, whose lanes are channels
+// and whose four waves take every fourth part.
+struct SumParams {
+  const float *part_bc, *part_a;
+  void *dbm, *dcm;
+  float *dA, *dD, *dbias;
+  int64_t rows;  // T B
+  int H, N, blocks, parts, bc_groups;
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void ssm_sum_bc_kernel(const float* part, void* dbm, void* dcm, int64_t rows, int N,
-                                                          int blocks) {
-  const int64_t plane = rows * 2 * N;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < plane; e += (int64_t)gridDim.x * 256) {
+__device__ __forceinline__ void sum_bc(const SumParams& p) {
+  const int64_t plane = p.rows * 2 * p.N;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < plane; e += (int64_t)p.bc_groups * 256) {
     float s = 0.0f;
-    for (int k0 = 0; k0 < blocks; k0 += 8) {
+    for (int k0 = 0; k0 < p.blocks; k0 += 8) {
       float x[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = k0 + k < blocks ? part[(k0 + k) * plane + e] : 0.0f;
+      for (int k = 0; k < 8; ++k) x[k] = k0 + k < p.blocks ? p.part_bc[(k0 + k) * plane + e] : 0.0f;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (k0 + k < blocks) s += x[k];
+        if (k0 + k < p.blocks) s += x[k];
     }
-    const int64_t row = e / (2 * N);
-    const int n = (int)(e - row * 2 * N);
-    void* dst = n < N ? dbm : dcm;
-    if (dst != nullptr) static_cast<T*>(dst)[row * N + (n < N ? n : n - N)] = (T)s;
+    const int64_t row = e / (2 * p.N);
+    const int n = (int)(e - row * 2 * p.N);
+    void* dst = n < p.N ? p.dbm : p.dcm;
+    if (dst != nullptr) static_cast<T*>(dst)[row * p.N + (n < p.N ? n : n - p.N)] = (T)s;
   }
 }
 
-// dA [H, N], dD and dbias [H]: sums over chunks and batch rows. Lanes are channels; a workgroup's four
-// waves take every fourth part, joined in order.
-__global__ __launch_bounds__(256) void ssm_sum_a_kernel(const float* part, float* dA, float* dD, float* dbias, int H, int N,
-                                                         int parts) {
-  __shared__ float red[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ch = blockIdx.x * 64 + lane, n = blockIdx.y;
-  const int64_t plane = (int64_t)(N + 2) * H;
-  const float* src = part + (int64_t)n * H + ch;
+__device__ __forceinline__ void sum_a(const SumParams& p, int group, float (*red)[64]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = group / p.blocks, ch = (group - n * p.blocks) * 64 + lane;
+  const int64_t plane = (int64_t)(p.N + 2) * p.H;
+  const float* src = p.part_a + (int64_t)n * p.H + ch;
   float s = 0.0f;
-  if (ch < H) {
-    for (int k0 = wave; k0 < parts; k0 += 4 * 8) {
+  if (ch < p.H) {
+    for (int k0 = wave; k0 < p.parts; k0 += 4 * 8) {
       float x[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = k0 + 4 * k < parts ? src[(k0 + 4 * k) * plane] : 0.0f;
+      for (int k = 0; k < 8; ++k) x[k] = k0 + 4 * k < p.parts ? src[(k0 + 4 * k) * plane] : 0.0f;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (k0 + 4 * k < parts) s += x[k];
+        if (k0 + 4 * k < p.parts) s += x[k];
     }
   }
   red[wave][lane] = s;
   __syncthreads();
-  if (wave != 0 || ch >= H) return;
+  if (wave != 0 || ch >= p.H) return;
   s = ((s + red[1][lane]) + red[2][lane]) + red[3][lane];
-  float* dst = n < N ? dA : n == N ? dD : dbias;
-  if (dst != nullptr) dst[n < N ? (int64_t)ch * N + n : ch] = s;
+  float* dst = n < p.N ? p.dA : n == p.N ? p.dD : p.dbias;
+  if (dst != nullptr) dst[n < p.N ? (int64_t)ch * p.N + n : ch] = s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void ssm_sum_kernel(SumParams p) {
+  __shared__ float red[4][64];
+  if ((int)blockIdx.x < p.bc_groups) sum_bc<T>(p);
+  else sum_a(p, (int)blockIdx.x - p.bc_groups, red);
 }
 
 // One token for each row of a batch of requests, whose states are rows of a cache [S, H, N]:
@@ -1082,15 +1097,14 @@ int check_sizes(const char* who, int64_t T, int64_t B, int64_t H, int64_t N, int
 }
 
 struct Bytes {
-  int64_t ends = 0, span = 0, dropped = 0, bc = 0, a = 0, total = 0;  // offsets
+  int64_t ends = 0, span = 0, bc = 0, a = 0, total = 0;  // offsets
 };
 Bytes bytes_of(const Plan& plan, int64_t T, int64_t B, int64_t H, int64_t N, bool back) {
   Bytes r;
   if (plan.chunks > 1) {
     const int64_t parts = (int64_t)plan.chunks * plan.each;
     r.span = align256(parts * B * N * H * 4);
-    r.dropped = r.span + align256(parts * B * H * 4);
-    r.total = r.dropped + align256(parts * B * 4);
+    r.total = r.span + align256(parts * B * H * 4);
   }
   if (back) {
     r.bc = r.total;
@@ -1165,7 +1179,6 @@ SsmParams params_of(const Args* a, const Plan& plan, const Bytes& bytes) {
   char* s = static_cast<char*>(a->scratch);
   p.ends = reinterpret_cast<float*>(s + bytes.ends);
   p.span = reinterpret_cast<float*>(s + bytes.span);
-  p.dropped = reinterpret_cast<float*>(s + bytes.dropped);
   p.part_bc = reinterpret_cast<float*>(s + bytes.bc);
   p.part_a = reinterpret_cast<float*>(s + bytes.a);
   return p;
@@ -1173,7 +1186,7 @@ SsmParams params_of(const Args* a, const Plan& plan, const Bytes& bytes) {
 
 int join_ends(const SsmParams& p, bool back, hipStream_t stream) {
   const int64_t n = (int64_t)p.B * p.N * p.H;
-  hipLaunchKernelGGL(back ? ssm_join_kernel<true> : ssm_join_kernel<false>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0,
+  hipLaunchKernelGGL(back ? ssm_join_kernel<true> : ssm_join_kernel<false>, dim3((unsigned)((n + 63) / 64)), dim3(64), 0,
                      stream, p);
   GS_CHECK_HIP(hipGetLastError());
   return GS_OK;
@@ -1260,17 +1273,12 @@ extern "C" int gs_ssm_bwd(const gs_ssm_bwd_args* a, hipStream_t stream) {
     if ((rc = join_ends(p, true, stream))) return rc;
   }
   if ((rc = launch(kBwd, plan.wide, a->dtype, p, groups * plan.chunks, stream))) return rc;
-  if (a->dbm != nullptr || a->dcm != nullptr) {
-    const dim3 grid((unsigned)std::min<int64_t>((rows * 2 * a->N + 255) / 256, 1 << 20));
-    hipLaunchKernelGGL(a->dtype == GS_DTYPE_F32 ? ssm_sum_bc_kernel<float> : ssm_sum_bc_kernel<__bf16>, grid, dim3(256), 0,
-                       stream, p.part_bc, a->dbm, a->dcm, rows, (int)a->N, plan.blocks);
-    GS_CHECK_HIP(hipGetLastError());
-  }
-  if (a->dA != nullptr || a->dD != nullptr || a->ddelta_bias != nullptr) {
-    hipLaunchKernelGGL(ssm_sum_a_kernel, dim3((unsigned)plan.blocks, (unsigned)(a->N + 2)), dim3(256), 0, stream, p.part_a,
-                       a->dA, a->dD, a->ddelta_bias, (int)a->H, (int)a->N, (int)(plan.chunks * a->B));
-    GS_CHECK_HIP(hipGetLastError());
-  }
+  const int bc_groups = (int)std::min<int64_t>((rows * 2 * a->N + 255) / 256, 1 << 20);
+  const SumParams sums{p.part_bc, p.part_a, a->dbm, a->dcm, a->dA, a->dD, a->ddelta_bias, rows, (int)a->H, (int)a->N, plan.blocks,
+                       (int)(plan.chunks * a->B), bc_groups};
+  hipLaunchKernelGGL(a->dtype == GS_DTYPE_F32 ? ssm_sum_kernel<float> : ssm_sum_kernel<__bf16>,
+                     dim3((unsigned)(bc_groups + plan.blocks * (a->N + 2))), dim3(256), 0, stream, sums);
+  GS_CHECK_HIP(hipGetLastError());
   return GS_OK;
 }
 

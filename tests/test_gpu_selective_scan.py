@@ -138,6 +138,18 @@ def test_large_decays_and_step_sizes(dev):
     _check(t, dy, dh, _roundings(T, B, H, N))
 
 
+@pytest.mark.parametrize("T,B,H", [(21, 2, 24), (150, 2, 24), (1061, 40, 70)])
+def test_a_rate_of_minus_infinity(dev, T, B, H):
+    """A state that forgets at once: exp(-infinity) is 0 at every step, also before the axis ends in a tile."""
+    t, _, _ = _make(T, B, H, 4, F32, dev, seed=22)
+    t["A"][:, 1] = -float("inf")
+    y, h, _ = _run(t)
+    args = [t[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "h0")]
+    want, size = P.selective_scan(*args, delta_bias=t["delta_bias"]), P.selective_scan(*args, delta_bias=t["delta_bias"], size=True)
+    P.assert_within(y, want[0], size[0], _roundings(T, B, H, 4), "y")
+    P.assert_within(h, want[1], size[1], _roundings(T, B, H, 4), "h_T")
+
+
 def test_split_in_two_calls(dev):
     """h_T continues the sequence, and its gradient goes back through the first call."""
     T, B, H, N = 90, 2, 30, 16
