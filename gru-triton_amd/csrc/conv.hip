@@ -335,29 +335,30 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvParams p) {
   }
 }
 
-// dw [C][W] and dbias [C]: sums over the parts. Lanes are channels; a workgroup's four waves
-// take every fourth part, joined in order.
+// dw [C][W] and dbias [C]: sums over the parts. Lanes are channels; a workgroup's sixteen waves
+// take every sixteenth part, joined in order.
 template <typename T>
-__global__ __launch_bounds__(256) void conv_sum_kernel(const float* part, void* dw, void* dbias, int C, int W, int parts) {
-  __shared__ float red[4][64];
+__global__ __launch_bounds__(1024) void conv_sum_kernel(const float* part, void* dw, void* dbias, int C, int W, int parts) {
+  __shared__ float red[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ch = blockIdx.x * 64 + lane, k = blockIdx.y;
   const int64_t plane = (int64_t)(W + 1) * C;
   const float* src = part + (int64_t)k * C + ch;
   float s = 0.0f;
   if (ch < C) {
-    for (int k0 = wave; k0 < parts; k0 += 4 * 8) {
+    for (int k0 = wave; k0 < parts; k0 += 16 * 8) {
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = k0 + 4 * i < parts ? src[(k0 + 4 * i) * plane] : 0.0f;
+      for (int i = 0; i < 8; ++i) x[i] = k0 + 16 * i < parts ? src[(k0 + 16 * i) * plane] : 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (k0 + 4 * i < parts) s += x[i];
+        if (k0 + 16 * i < parts) s += x[i];
     }
   }
   red[wave][lane] = s;
   __syncthreads();
   if (wave != 0 || ch >= C) return;
-  s = ((s + red[1][lane]) + red[2][lane]) + red[3][lane];
+#pragma unroll
+  for (int w = 1; w < 16; ++w) s += red[w][lane];
   if (k < W && dw != nullptr) static_cast<T*>(dw)[(int64_t)ch * W + k] = (T)s;
   if (k == W && dbias != nullptr) static_cast<T*>(dbias)[ch] = (T)s;
 }
@@ -405,14 +406,15 @@ struct Plan {
 
 int64_t groups_of(const Plan& p, int64_t B) { return (int64_t)p.blocks * ((p.runs + 3) / 4) * B; }
 
-// Runs of 128 steps at most, whose ends cost little, and shorter ones where there are few waves.
+// Runs of 128 steps at most, whose ends cost little, and shorter ones, of 8 at least, where there are fewer than a
+// thousand waves (T 2000, B 16, C 96: 38 us with four thousand asked for, 35 with one).
 Plan make_plan(int64_t T, int64_t B, int64_t C, int v) {
   Plan r;
   r.v = v;
   r.blocks = (int)((C + 64 * v - 1) / (64 * v));
   const int64_t steps = r.blocks * B * T;
   int64_t length = 128;
-  while (length > 8 && steps / length < 4096) length /= 2;
+  while (length > 8 && steps / length < 1024) length /= 2;
   r.length = (int)length;
   r.runs = (int)((T + length - 1) / length);
   return r;
@@ -422,10 +424,11 @@ struct Strided {
   const void* p;
   int64_t st, sb;
 };
-// Four channels a lane where every row allows the access and there are lanes enough for them.
+// Four channels a lane where every row allows the access and there are lanes enough for them (a training step of
+// T 8192, B 8, C 2048 bf16 takes 322 us so and 521 with one; T 2000, B 16, C 96: 50 and 55).
 Plan plan_of(int dtype, int64_t T, int64_t B, int64_t C, const Strided* t, int count) {
   const int bytes = dtype == GS_DTYPE_F32 ? 16 : 8;
-  bool four = C % 4 == 0 && C > 128;
+  bool four = C % 4 == 0 && C >= 64;
   for (int i = 0; i < count; ++i)
     four = four && (reinterpret_cast<uintptr_t>(t[i].p) & (uintptr_t)(bytes - 1)) == 0 && t[i].st % 4 == 0 && t[i].sb % 4 == 0;
   return make_plan(T, B, C, four ? 4 : 1);
@@ -574,7 +577,7 @@ extern "C" int gs_conv_bwd(const gs_conv_bwd_args* a, hipStream_t stream) {
   GS_CHECK_HIP(hipGetLastError());
   if (a->dw != nullptr || a->dbias != nullptr) {
     hipLaunchKernelGGL(a->dtype == GS_DTYPE_F32 ? conv_sum_kernel<float> : conv_sum_kernel<__bf16>,
-                       dim3((unsigned)((a->C + 63) / 64), (unsigned)(a->W + 1)), dim3(256), 0, stream, p.part, a->dw, a->dbias,
+                       dim3((unsigned)((a->C + 63) / 64), (unsigned)(a->W + 1)), dim3(1024), 0, stream, p.part, a->dw, a->dbias,
                        (int)a->C, (int)a->W, (int)((plan.runs + 3) / 4 * a->B));
     GS_CHECK_HIP(hipGetLastError());
   }

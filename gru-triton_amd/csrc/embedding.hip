@@ -145,7 +145,9 @@ __global__ __launch_bounds__(256) void embed_count_kernel(EmbedParams p) {
   if (some) p.place[m] = base + before;
 }
 
-constexpr uint32_t kShort = 16;  // positions of a list that a wave sums
+// Positions of a list that a wave sums. A step of 16384 tokens of 32000 x 1024 bf16, of 1237 of 1003 x 333 fp32 and
+// of 30000 of 3000 x 512 bf16 takes 54, 25 and 55 us with 4, 53, 24 and 55 with 16, 61, 30 and 74 with 64.
+constexpr uint32_t kShort = 16;
 
 // Room for each token's list, in no particular order, and the chunks of the long ones.
 __global__ __launch_bounds__(1024) void embed_room_kernel(EmbedParams p) {

@@ -334,7 +334,8 @@ struct Plan {
   bool few;              // parts of 256 kFewHeld logits
   int64_t lists, total;  // offset of the lists
 };
-// A row a workgroup; parts of 2048 logits at least where there are fewer rows than fill the device.
+// A row a workgroup; parts of 2048 logits at least where there are fewer rows than fill the device (8 rows of 32000,
+// forward and backward: 20.5 us in whole rows, 16.5 in parts; 64 rows 21.4 and 17.3).
 // Where the likeliest are asked for, parts of what a workgroup's registers hold.
 Plan make_plan(int64_t M, int64_t V, int64_t top) {
   Plan r;

@@ -924,12 +924,12 @@ __device__ __forceinline__ void sum_a(const SumParams& p, int group, float (*red
   const float* src = p.part_a + (int64_t)n * p.H + ch;
   float s = 0.0f;
   if (ch < p.H) {
-    for (int k0 = wave; k0 < p.parts; k0 += 4 * 8) {
-      float x[8];
+    for (int k0 = wave; k0 < p.parts; k0 += 4 * 16) {
+      float x[16];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = k0 + 4 * k < p.parts ? src[(k0 + 4 * k) * plane] : 0.0f;
+      for (int k = 0; k < 16; ++k) x[k] = k0 + 4 * k < p.parts ? src[(k0 + 4 * k) * plane] : 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < 16; ++k)
         if (k0 + 4 * k < p.parts) s += x[k];
     }
   }
@@ -1014,6 +1014,10 @@ struct Plan {
   int blocks, chunks, length, each;
   bool wide;  // the kernels that share nothing, for the forward or the backward's ends
 };
+// In us, states over a workgroup's waves / waves that share nothing, the same tensors (N 16):
+//   T 4096, B 8, H 1024 bf16 training   1133 / 1046     T 512, B 16, H 512 fp32 training   164 / 178
+//   T 65536, B 1, H 1024 bf16 forward    736 / 548      T 1001, B 3, H 333 fp32 training   110 / 150
+// With 256 and 1024 workgroups asked for in place of 512 the first takes 1459 and 1157 (backward alone).
 constexpr int64_t kGroups = 512;    // workgroups asked for: two a CU
 constexpr int64_t kWaves = 4096;    // waves asked for, where they share nothing
 constexpr int64_t kFewWaves = 2048; // up to these, states are spread over the waves of a workgroup
