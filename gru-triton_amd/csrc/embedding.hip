@@ -9,7 +9,8 @@
 // results do not. A wave sorts a list of 16 or fewer by counting smaller ones, lane by lane, and
 // sums its rows in that order. Longer lists are cut into chunks, a workgroup each, whose waves take a
 // quarter of its rows; a list's order there comes from counting smaller ones too or, where it is long, from a bit
-// for every position. The chunks' sums are joined in order.
+// for every position. The chunks' sums are joined in order. 16384 tokens of 32000 x 1024 bf16:
+// forward 10 us; backward 10 to count, 8 to give room, put down and clear, 18 for the sums (5.5 TB/s), 4 to join.
 #include "gs_seq.h"
 
 namespace gs {
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(256) void embed_clear_kernel(uint32_t* p, int64_t n
 }
 
 // Equal tokens of a wave are counted together, in one access: those of a frequent token would
-// wait for each other (16384 tokens, one in 15 the same: 15 -> 5 us).
+// wait for each other (16384 tokens, one in 15 the same: 15 -> 10 us).
 __global__ __launch_bounds__(256) void embed_count_kernel(EmbedParams p) {
   const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t token = m < p.M ? token_at(p, m) : -1;

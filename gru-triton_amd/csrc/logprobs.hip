@@ -10,7 +10,9 @@
 // Bound by memory: one pass over the logits forward with the running maximum, s and t, and one backward.
 // A workgroup takes a row, or a part of one where there are few rows; the parts of a row are
 // then joined in order. For `top` a part's logits stay in registers as sortable words; each wave takes
-// the largest out of its 2048 one after the other, and lists are merged, of waves and then of parts.
+// the largest out of its 512 or 2048 one after the other, and lists are merged, of waves and then of parts.
+// 8192 rows of 32000 bf16: forward 126 to 145 us (3.6 to 4.2 TB/s of reads; a read alone reached 4.0), backward 189 (5.5 TB/s);
+// 8 rows with the 8 likeliest 9 + 6, where launches and the chains of comparisons count.
 #include "gs_seq.h"
 
 namespace gs {

@@ -9,16 +9,23 @@
 //   S = sum_n G_t[n] B_t[n],  q[n] = G_t[n] a_t[n] h_{t-1}[n],
 //   du = dt S + D dy,  ddt = u S + sum_n q[n] A[n],  dA[n] = sum_t q[n] dt,  dD = sum_t u dy.
 //
-// Layout: a workgroup owns 64 channels (a lane each) of one batch row and walks a chunk of
-// the time axis in tiles of 16 steps. Its waves share the N states, P a wave, and the steps of a tile:
-// a wave loads its steps' rows, computes what is shared by the states (softplus, the gate) and leaves
-// it in LDS; every wave then runs its states over the whole tile, one exponential a state and step,
-// and leaves its part of y; and each wave sums the parts of its steps. With few channels the
-// time axis is cut into chunks for more workgroups: a first pass finds what each chunk makes of a
-// zero state, a second joins those along the axis, and the third is the scan from the right states.
-// A training forward keeps the state before every tile, from which the backward runs the
-// tile's steps again, forwards and then back. Sums over channels (dB, dC) are those of the workgroup's
-// 64 in registers, then of the workgroups in order through memory: results are reproducible.
+// Layout: a lane is a channel, 64 channels of one batch row a wave, and steps come in tiles of 16. Two forms of
+// the forward and of the launch that finds ends (make_plan says when each):
+//   * States over the waves of a workgroup, two each (four of 32): a wave loads the rows of its steps of a
+//     tile, computes what the states share (softplus, the gate) and leaves it in LDS; every wave runs its states
+//     over the tile, one exponential a state and step, and leaves its part of y; each sums its steps' parts.
+//   * Waves that share nothing: one has all states of its channels, and reads B and C from LDS.
+// With few channels the time axis is cut into chunks. The first launch scans the first chunk and finds what each
+// one between it and the last makes of a zero state; the second joins those along the axis; the
+// third scans the others from their states. A training forward keeps the state before every tile. The backward
+// finds what chunks send back, joins that, and runs each tile's steps again, forwards and then back.
+// Sums over channels (dB, dC) are those of the workgroup's 64 in registers, then of the workgroups in order
+// through memory: results are reproducible.
+//
+// Bound by the vector ALU and its exponentials: forwards 16 states at a step take some 6 instructions and an exponential each,
+// every step a softplus. Measured, T 4096, B 8, H 1024, N 16 bf16: forward 132 us and 152 with the gate and
+// the kept states, ends 108, backward 684 (its VALU busy for three quarters; 747 MB take 145 at a copy's rate); T 65536, B 1, H 1024
+// forward 267 + 24 + 302 (540 MB: 105); T 512, B 16, H 512 fp32 training 25 + 22 forward, 22 + 78 backward and 15 of joins and sums.
 #include "gs_seq.h"
 
 namespace gs {

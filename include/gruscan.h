@@ -933,7 +933,7 @@ int gs_embedding_bwd(const gs_embedding_bwd_args* args, hipStream_t stream);
  * with their log probabilities. Results are fp32. A logit of -infinity is a token that cannot
  * come; a row of those alone has log probabilities -infinity, entropy 0 and no gradient. A NaN
  * or +infinity makes a row's results NaN. A negative token has log probability 0 and sends no
- * gradient, one of V or more NaN. */
+ * gradient, one of V or more NaN. M is at most 2^23, V 2^24 (2^19 with `top`). */
 typedef struct gs_logprobs_args {
   const void* x;         /* [M, V], row stride sx                                         */
   const void* tokens;    /* [M], int32 or int64                                           */
