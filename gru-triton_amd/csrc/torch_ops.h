@@ -6,6 +6,7 @@
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/forward_grad.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
@@ -77,10 +78,25 @@ void check_may_modify(const char* who, const char* name, const Tensor& t) {
               " was made in inference mode and cannot be updated in place outside it");
 }
 
+// A captured backward hands a leaf's gradient to the leaf's accumulator on the stream that this was made on.
+// An eager graph of the leaf that is still alive keeps it on the default stream, which no capture can wait
+// for: torch's engine would end the process there.
+void check_capture(const char* who) {
+  const auto node = torch::autograd::get_current_node();
+  if (!node || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const auto& e : node->next_edges()) {
+    const auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get());
+    TORCH_CHECK(leaf == nullptr || !leaf->variable.is_cuda() || leaf->num_inputs() == 0 || leaf->input_metadata(0).stream().id() != 0,
+                who, ": an eager graph of the same leaves, made on the default stream, is alive (through an output or a loss); "
+                "drop it before a backward is captured");
+  }
+}
+
 // A backward's results. Where a graph of them is asked for (create_graph), it goes on to
 // `from`, which they were computed from, through an error for whoever asks for a second
 // derivative: without it that derivative would lack their terms and nobody would know.
 variable_list once(const char* who, variable_list grads, const variable_list& from) {
+  check_capture(who);
   if (!torch::GradMode::is_enabled()) return grads;
   const size_t n = grads.size();
   grads.insert(grads.end(), from.begin(), from.end());
