@@ -41,6 +41,7 @@ struct SsmParams {
   void* y;             // forward
   float* h_last;
   float* saved;        // [ceil(T / kTile)][B][N][H]: forward written (or NULL), backward read
+  float* ungated;      // [T][B][H]: y before its gate, kept with them where there is one, else NULL
   float* ends;         // [chunks][B][N][H]: see ssm_join_kernel
   float* span;         // [chunks][B][H]: sum of dt over a chunk, -1 where it holds a reset
   const void* dy;      // backward only from here
@@ -282,6 +283,9 @@ __device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
         for (int w = 1; w < NW; ++w)
           if (!PAD || w * P < p->N) y += lds.part[w][s][at.lane];
         y = __builtin_fmaf(D, u[i], y);
+        if (p->ungated != nullptr)
+          Elem<float>::store(row_of<float>(p->ungated, (int64_t)p->B * p->H, p->H, t0 + s, at.b),
+                             t0 + s < at.t1 ? lane_off<float>(at) : kOffNone, y);
         const float gate = z[i] * sigmoid(z[i]);
         y = p->z != nullptr ? y * gate : y;
         E::store(to + i * NW * p->sy_t, t0 + s < at.t1 ? off : kOffNone, y);
@@ -382,7 +386,7 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
   const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
   const float D = OUT && p->D != nullptr && at.ok ? p->D[at.ch] : 0.0f;
   const uint32_t off = lane_off<T>(at);
-  const bool gated = OUT && p->z != nullptr;
+  const bool gated = OUT && p->z != nullptr, keep = OUT && p->ungated != nullptr;
   float span = 0.0f;
   bool drop = false;
   unsigned int rd[kGroup], ru[kGroup], rz[kGroup];
@@ -422,6 +426,7 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
     }
     if (t0 + kGroup < at.t1) fetch(t0 + kGroup);
     T* to = OUT ? row_of<T>(p->y, p->sy_t, p->sy_b, t0, at.b) : nullptr;
+    float* to_u = keep ? row_of<float>(p->ungated, (int64_t)p->B * p->H, p->H, t0, at.b) : nullptr;
     if (!OUT && (flags & ((1u << kGroup) - 1))) drop = true;
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) {
@@ -442,6 +447,7 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
       }
       if constexpr (OUT) {
         y = __builtin_fmaf(D, u[i], y);
+        if (keep) Elem<float>::store(to_u + (int64_t)i * p->B * p->H, t0 + i < at.t1 ? lane_off<float>(at) : kOffNone, y);
         const float gate = z[i] * sigmoid(z[i]);
         E::store(to + i * p->sy_t, t0 + i < at.t1 ? off : kOffNone, gated ? y * gate : y);
       } else {
@@ -515,10 +521,11 @@ struct BwdShared {
   float ds[kTile][64];   // dy
   // [1] stays zero: what lanes without a channel read, so that sums over lanes do not see them
   Pair<P> bc[2][kTile][NW];
-  union {  // the waves' parts of y, then of S and of sum_n q A / ln 2
-    float y[NW][kTile][64];
-    float2 sq[NW][kTile][64];
-  } part;
+  // A step's decays of the wave's states, left for the way back, and then, in the first two of their
+  // places, the wave's parts of S and of sum_n q A / ln 2.
+  struct alignas(4 * P) Step {
+    float x[P];
+  } part[NW][kTile][64];
 };
 
 // The gradient that a chunk sends to the state before it, from a zero gradient after it.
@@ -706,7 +713,7 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
   const uint32_t off = lane_off<T>(at);
   float dD = 0.0f, dbias = 0.0f;
   for (int i = threadIdx.x; i < kTile * NW * 2 * P; i += 64 * NW) (&lds.bc[1][0][0].x[0])[i] = 0.0f;
-  unsigned int rd[kOwn], ru[kOwn], rz[kOwn], rg[kOwn];
+  unsigned int rd[kOwn], ru[kOwn], rz[kOwn], rg[kOwn], ry[kOwn];
   auto fetch = [&](int t0) __attribute__((always_inline)) {
     Args p = args();
     const int t = t0 + at.wave;
@@ -714,14 +721,17 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
     const T* u = row_of<T>(p->u, p->su_t, p->su_b, t, at.b);
     const T* g = row_of<T>(p->dy, p->sdy_t, p->sdy_b, t, at.b);
     const T* z = row_of<T>(p->z, p->sz_t, p->sz_b, t, at.b);
+    const float* y = row_of<float>(p->ungated, (int64_t)p->B * p->H, p->H, t, at.b);
     const bool gated = p->z != nullptr;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const uint32_t o = t + NW * i < at.t1 ? off : kOffNone;
+      const bool some = t + NW * i < at.t1;
+      const uint32_t o = some ? off : kOffNone;
       rd[i] = E::load(d + i * NW * p->sdl_t, o);
       ru[i] = E::load(u + i * NW * p->su_t, o);
       rg[i] = E::load(g + i * NW * p->sdy_t, o);
       rz[i] = E::load(z + i * NW * p->sz_t, gated ? o : kOffNone);
+      ry[i] = Elem<float>::load(y + (int64_t)i * NW * p->B * p->H, gated && some ? lane_off<float>(at) : kOffNone);
     }
   };
   const int last = at.t0 + (at.t1 - at.t0 - 1) / kTile * kTile;
@@ -739,7 +749,8 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
     const float* from = p->saved + (((int64_t)(t0 / kTile) * p->B + at.b) * p->N + n0) * p->H + at.ch;
 #pragma unroll
     for (int i = 0; i < P; ++i) start[i] = at.ok && (!PAD || i < live) ? from[(int64_t)i * p->H] : 0.0f;
-    float u[kOwn], x[kOwn], dzy[kOwn];  // dzy: dz / y
+    float u[kOwn], x[kOwn];
+    T* to_z = row_of<T>(p->dz, p->sdz_t, p->sdz_b, t0 + at.wave, at.b);
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int s = at.wave + NW * i;
@@ -747,7 +758,9 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
       x[i] = E::value(rd[i]) + bias;
       const float dt = t0 + s < at.t1 ? softplus(x[i]) : 0.0f;
       const float z = E::value(rz[i]), g = sigmoid(z), d = E::value(rg[i]);
-      dzy[i] = d * g * __builtin_fmaf(z, 1.0f - g, 1.0f);
+      if (gated)
+        E::store(to_z + i * NW * p->sdz_t, t0 + s < at.t1 ? off : kOffNone,
+                 d * g * __builtin_fmaf(z, 1.0f - g, 1.0f) * Elem<float>::value(ry[i]));
       lds.xs[s][at.lane] = float2{dt, dt * u[i]};
       lds.ds[s][at.lane] = gated ? d * (z * g) : d;
     }
@@ -756,40 +769,29 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
     share_barrier();
     with_flags(flags, [&](auto F) __attribute__((always_inline)) {
       constexpr bool RESET = decltype(F)::value;
-      // After each step. The decays are computed again on the way back: sixteen registers of them would leave half as many waves.
+      // after each step
       float h[kTile][P];
 #pragma unroll
       for (int s = 0; s < kTile; ++s) {
         const float2 v = lds.xs[s][at.lane];
-        float bm[P], cm[P], y = 0.0f;
+        float bm[P], cm[P];
         bc[s][at.wave].read(bm, cm);
+        typename BwdShared<P, NW>::Step decay;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          h[s][i] = 0.0f;
+          h[s][i] = decay.x[i] = 0.0f;
           if (PAD && i >= live) continue;
           float before = s ? h[s > 0 ? s - 1 : 0][i] : start[i];
           if (RESET && (flags >> s & 1)) before = 0.0f;
-          h[s][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(v.x * A2[i]), before, v.y * bm[i]);
-          y = __builtin_fmaf(cm[i], h[s][i], y);
+          decay.x[i] = __builtin_amdgcn_exp2f(v.x * A2[i]);
+          h[s][i] = __builtin_fmaf(decay.x[i], before, v.y * bm[i]);
         }
-        lds.part.y[at.wave][s][at.lane] = y;
+        lds.part[at.wave][s][at.lane] = decay;
         if (s % 2) __builtin_amdgcn_sched_barrier(0);  // loads of few steps ahead: registers are short
       }
-      share_barrier();
-      if (gated) {
-        Args p = args();
-        T* to = row_of<T>(p->dz, p->sdz_t, p->sdz_b, t0 + at.wave, at.b);
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-          const int s = at.wave + NW * i;
-          float y = lds.part.y[0][s][at.lane];
-#pragma unroll
-          for (int w = 1; w < NW; ++w)
-            if (!PAD || w * P < p->N) y += lds.part.y[w][s][at.lane];
-          E::store(to + i * NW * p->sdz_t, t0 + s < at.t1 ? off : kOffNone, dzy[i] * __builtin_fmaf(D, u[i], y));
-        }
-      }
-      share_barrier();
+      uint32_t back = flags;
+      asm volatile("" : "+s"(back));  // what a reset drops is found anew, not kept
+      __builtin_amdgcn_sched_barrier(0);
       // back over the tile; sums over the lanes of dB and dC of a pair of states in one register a step
       float sums[P / 2][kTile];
 #pragma unroll
@@ -798,14 +800,15 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
         const float g = lds.ds[s][at.lane];
         float bm[P], cm[P], S = 0.0f, Q = 0.0f, db[P], dc[P];
         bc[s][at.wave].read(bm, cm);
+        const typename BwdShared<P, NW>::Step decay = lds.part[at.wave][s][at.lane];
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           db[i] = dc[i] = 0.0f;
           if (PAD && i >= live) continue;
           const float G = __builtin_fmaf(cm[i], g, e[i]);
           float before = s ? h[s > 0 ? s - 1 : 0][i] : start[i];
-          e[i] = __builtin_amdgcn_exp2f(v.x * A2[i]) * G;
-          if (RESET && (flags >> s & 1)) e[i] = before = 0.0f;
+          e[i] = decay.x[i] * G;
+          if (RESET && (back >> s & 1)) e[i] = before = 0.0f;
           const float q = e[i] * before;
           S = __builtin_fmaf(G, bm[i], S);
           Q = __builtin_fmaf(q, A2[i], Q);
@@ -813,7 +816,8 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
           db[i] = G * v.y;
           dc[i] = h[s][i] * g;
         }
-        lds.part.sq[at.wave][s][at.lane] = float2{S, Q};
+        lds.part[at.wave][s][at.lane].x[0] = S;
+        lds.part[at.wave][s][at.lane].x[1] = Q;
 #pragma unroll
         for (int i = 0; i < P; i += 2)
           sums[i / 2][s] = join<16>(join<32>(db[i], db[i + 1]), join<32>(dc[i], dc[i + 1]));
@@ -843,13 +847,12 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int s = at.wave + NW * i;
-      float2 v = lds.part.sq[0][s][at.lane];
+      float2 v{lds.part[0][s][at.lane].x[0], lds.part[0][s][at.lane].x[1]};
 #pragma unroll
       for (int w = 1; w < NW; ++w)
         if (!PAD || w * P < p->N) {
-          const float2 o = lds.part.sq[w][s][at.lane];
-          v.x += o.x;
-          v.y += o.y;
+          v.x += lds.part[w][s][at.lane].x[0];
+          v.y += lds.part[w][s][at.lane].x[1];
         }
       const float dt = lds.xs[s][at.lane].x, dy = lds.ds[s][at.lane];
       const float dd = __builtin_fmaf(u[i], v.x, v.y * kLn2) * sigmoid(x[i]);
@@ -875,13 +878,14 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
     }
   }
   share_barrier();
-  lds.part.sq[at.wave][0][at.lane] = float2{dD, dbias};
+  lds.part[at.wave][0][at.lane].x[0] = dD;
+  lds.part[at.wave][0][at.lane].x[1] = dbias;
   share_barrier();
   if (at.wave == 0 && at.ok) {
 #pragma unroll
     for (int w = 1; w < NW; ++w) {
-      dD += lds.part.sq[w][0][at.lane].x;
-      dbias += lds.part.sq[w][0][at.lane].y;
+      dD += lds.part[w][0][at.lane].x[0];
+      dbias += lds.part[w][0][at.lane].x[1];
     }
     p->part_a[(parts + p->N) * p->H + at.ch] = dD;
     p->part_a[(parts + p->N + 1) * p->H + at.ch] = dbias;
@@ -1203,6 +1207,12 @@ int join_ends(const SsmParams& p, bool back, hipStream_t stream) {
   return GS_OK;
 }
 
+// What a training forward keeps: states, and behind them the outputs before their gate.
+template <typename Args>
+int64_t saved_states(const Args* a) {
+  return (a->T + kTile - 1) / kTile * a->B * a->N * a->H;
+}
+
 }  // namespace
 }  // namespace gs
 
@@ -1217,7 +1227,7 @@ extern "C" int64_t gs_ssm_scratch_bytes(const gs_ssm_args* a) {
 extern "C" int64_t gs_ssm_saved_bytes(const gs_ssm_args* a) {
   clear_error();
   const int rc = check_fwd(a, "gs_ssm_saved_bytes");
-  return rc ? rc : (a->T + kTile - 1) / kTile * a->B * a->N * a->H * 4;
+  return rc ? rc : (saved_states(a) + (a->z ? a->T * a->B * a->H : 0)) * 4;
 }
 
 extern "C" int gs_ssm_fwd(const gs_ssm_args* a, hipStream_t stream) {
@@ -1234,6 +1244,7 @@ extern "C" int gs_ssm_fwd(const gs_ssm_args* a, hipStream_t stream) {
   p.y = a->y;
   p.h_last = a->h_last;
   p.saved = a->saved;
+  p.ungated = a->saved && a->z ? a->saved + saved_states(a) : nullptr;
   p.sy_t = a->sy_t;
   p.sy_b = a->sy_b;
   const int64_t groups = (int64_t)plan.blocks * a->B * std::max(1, plan.chunks - 1);
@@ -1263,6 +1274,7 @@ extern "C" int gs_ssm_bwd(const gs_ssm_bwd_args* a, hipStream_t stream) {
   if ((rc = check_plain_scratch(who, a->scratch, a->scratch_bytes, bytes.total))) return rc;
   SsmParams p = params_of(a, plan, bytes);
   p.saved = const_cast<float*>(a->saved);
+  p.ungated = a->z ? p.saved + saved_states(a) : nullptr;
   p.dy = a->dy;
   p.dh_last = a->dh_last;
   p.du = a->du;
