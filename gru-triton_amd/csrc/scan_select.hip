@@ -17,15 +17,16 @@
 //   * Waves that share nothing: one has all states of its channels, and reads B and C from LDS.
 // With few channels the time axis is cut into chunks. The first launch scans the first chunk and finds what each
 // one between it and the last makes of a zero state; the second joins those along the axis; the
-// third scans the others from their states. A training forward keeps the state before every tile. The backward
+// third scans the others from their states. A training forward keeps the state before every tile, and the outputs
+// before their gate, which the backward would need sums over the states (and waits) for. The backward
 // finds what chunks send back, joins that, and runs each tile's steps again, forwards and then back.
 // Sums over channels (dB, dC) are those of the workgroup's 64 in registers, then of the workgroups in order
 // through memory: results are reproducible.
 //
 // Bound by the vector ALU and its exponentials: forwards 16 states at a step take some 6 instructions and an exponential each,
-// every step a softplus. Measured, T 4096, B 8, H 1024, N 16 bf16: forward 132 us and 152 with the gate and
-// the kept states, ends 108, backward 684 (its VALU busy for three quarters; 747 MB take 145 at a copy's rate); T 65536, B 1, H 1024
-// forward 267 + 24 + 302 (540 MB: 105); T 512, B 16, H 512 fp32 training 25 + 22 forward, 22 + 78 backward and 15 of joins and sums.
+// every step a softplus. Measured, T 4096, B 8, H 1024, N 16 bf16: forward 134 us for the first
+// launch and 170 with what is kept, ends 111, backward 520 (its VALU busy for some 80 %; 747 MB take 145 at a copy's rate); T 65536, B 1, H 1024
+// forward 267 + 24 + 302 (540 MB: 105); T 512, B 16, H 512 fp32 training 23 + 27 forward, 22 + 68 backward and 14 of joins and sums.
 #include "gs_seq.h"
 
 namespace gs {
@@ -822,7 +823,7 @@ __device__ __forceinline__ void bwd_chunk(At at, BwdShared<P, NW>& lds) {
         for (int i = 0; i < P; i += 2)
           sums[i / 2][s] = join<16>(join<32>(db[i], db[i + 1]), join<32>(dc[i], dc[i + 1]));
         if (s == kTile / 2 && t0 > at.t0) fetch(t0 - kTile);  // half of h is done with
-        if (s % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
       }
       Args p = args();
 #pragma unroll

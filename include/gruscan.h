@@ -836,7 +836,8 @@ int gs_conv_step(const gs_conv_step_args* args, hipStream_t stream);
  * of every channel c with N states (1 to 32) each. bm and cm are shared by a row's channels.
  * reset[t][b] != 0 takes h_{t-1} as 0 at step t, whatever it held. u, delta, z, bm, cm, y
  * and their gradients are of one type; A, D, delta_bias, states and every sum are fp32. A
- * training forward stores the states before every 16th step in `saved`. No counterpart in the
+ * training forward stores the states before every 16th step in `saved`, and behind them, where
+ * z gates, the outputs before their gate. No counterpart in the
  * reference. */
 typedef struct gs_ssm_args {
   const void *u, *delta, *z; /* [T, B, H], strides s*_t, s*_b, 1; z may be NULL (no gate)  */
