@@ -162,9 +162,13 @@ __device__ __forceinline__ int parts_of(const SsmParams& p) {
   return (p.T + length - 1) / length;
 }
 
-// A as the exponent of 2. One of -infinity, a state that lasts a step, is held finite: the steps behind the
-// axis' end have step size 0, which must not make a NaN with it.
-__device__ __forceinline__ float rate(float A) { return A == -__builtin_inff() ? -3.0e38f : A * kLog2e; }
+// A as the exponent of 2, held finite: A of -infinity (a state that lasts a step), or a product past float32's
+// range (the lowest float as a stand-in for it), would make a NaN with a step size of 0, which the steps behind
+// the axis' end have. A NaN passes.
+__device__ __forceinline__ float rate(float A) {
+  const float r = A * kLog2e;
+  return r < -3.0e38f ? -3.0e38f : r > 3.0e38f ? 3.0e38f : r;
+}
 
 // f(std::true_type) where a tile holds a reset, else f(std::false_type): uniform.
 template <typename F>
@@ -990,7 +994,7 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepParams p) {
   float* h = p.state + slot * p.ss + (int64_t)ch * p.N;
   float y = 0.0f;
   auto state = [&](int n, float a, float before) __attribute__((always_inline)) {
-    const float x = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * (a * kLog2e)), before, dt * u * (float)bm[n]);
+    const float x = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * rate(a)), before, dt * u * (float)bm[n]);
     y = __builtin_fmaf((float)cm[n], x, y);
     return x;
   };

@@ -1,0 +1,74 @@
+"""The selective scan and its step at the ends of float32's range, against the definition in 64 bits
+(sequence_plain). Roundings are counted for each result by itself."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import gru_qat_amd as G
+import sequence_plain as P
+from test_gpu_selective_scan import LEAVES, _make, _run
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+INF = float("inf")
+LOWEST = torch.finfo(F32).min
+# an axis within tiles, one in chunks, and one with channels enough for waves that share nothing; none ends with a tile
+SIZES = [(21, 2, 24, 4), (150, 2, 24, 16), (1061, 40, 70, 4)]
+
+
+def roundings(T, B, H, N):
+    """On the way of each result: the chain of T states (y, h_T, dz), of T gradients (du, dh0) or of both (d delta), a sum
+    over N states, over H channels (dB, dC) or over T B steps and rows (dA, dD and d delta_bias), and 64 for
+    softplus, exp and the gate (each within 8 units, at arguments whose error is 8 units)."""
+    own = dict.fromkeys(("y", "h_T", "z", "u", "h0"), T + N + 64)
+    own["delta"] = 2 * T + N + 64
+    own.update(dict.fromkeys(("B", "C"), 2 * T + H + 64))
+    own.update(dict.fromkeys(("A", "D", "delta_bias"), 2 * T + N + T * B + 64))
+    return own
+
+
+def check(t, dy, dh):
+    T, B, H = t["u"].shape
+    most = roundings(T, B, H, t["A"].shape[1])
+    y, h, got = _run(t, dy, dh)
+    args = [t[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "h0")]
+    kw = dict(delta_bias=t["delta_bias"], reset=t["reset"], dy=dy, dh=dh)
+    want, size = P.selective_scan(*args, **kw), P.selective_scan(*args, size=True, **kw)
+    P.assert_within(y, want[0], size[0], most["y"], "y")
+    P.assert_within(h, want[1], size[1], most["h_T"], "h_T")
+    for k in got:
+        P.assert_within(got[k], want[2][k], size[2][k], most[k], "d" + k)
+    return y, h, got
+
+
+@pytest.mark.parametrize("T,B,H,N", SIZES)
+@pytest.mark.parametrize("reset", [0.0, 0.02])
+def test_the_lowest_rate(dev, T, B, H, N, reset):
+    """A finite rate whose product with log2 e is not: a state that lasts a step, with its gradients; -infinity is the same."""
+    t, dy, dh = _make(T, B, H, N, F32, dev, seed=40, reset=reset)
+    t["A"][:, 1] = LOWEST
+    t["A"][::3, 0] = -2.5e38
+    y, h, got = check(t, dy, dh)
+    t["A"] = torch.where(t["A"] < -1e38, -INF, t["A"])
+    y1, h1, got1 = _run(t, dy, dh)
+    assert torch.equal(y, y1) and torch.equal(h, h1)
+    for k in LEAVES:
+        assert torch.equal(got[k], got1[k]), k
+
+
+def test_step_of_rates_and_no_step_size(dev):
+    """A step size of zero (delta of -200) keeps the state, as in the scan, whatever the rate; a usual one drops what decays at once."""
+    B, H, N = 2, 40, 4
+    t, _, _ = _make(1, B, H, N, F32, dev, seed=41)
+    t["A"][:, 1], t["A"][:, 2] = LOWEST, -INF
+    t["delta"][0, 0] = -200.0
+    t["delta_bias"] = None
+    state = t["h0"].clone()
+    y = G.selective_step(t["u"][0], t["delta"][0], t["A"], t["B"][0], t["C"][0], state, D=t["D"], z=t["z"][0])
+    scan, h, _ = _run(t)
+    assert torch.equal(state, h) and torch.equal(state[0], t["h0"][0])
+    assert torch.allclose(y, scan[0], rtol=1e-6, atol=1e-6)  # four products in another order
+    want = (torch.nn.functional.softplus(t["delta"][0, 1].double()) * t["u"][0, 1].double())[:, None] * t["B"][0, 1].double()
+    assert torch.allclose(state[1, :, 1:3].double(), want[:, 1:3], rtol=1e-6)
