@@ -44,7 +44,7 @@ struct SsmParams {
   float* saved;        // [ceil(T / kTile)][B][N][H]: forward written (or NULL), backward read
   float* ungated;      // [T][B][H]: y before its gate, kept with them where there is one, else NULL
   float* ends;         // [chunks][B][N][H]: see ssm_join_kernel
-  float* span;         // [chunks][B][H]: sum of dt over a chunk, -1 where it holds a reset
+  float* span;         // [2][chunks][B][H]: sum of dt over a chunk, -1 where it holds a reset; the largest dt
   const void* dy;      // backward only from here
   const float* dh_last;
   void *du, *ddelta, *dz;
@@ -162,6 +162,12 @@ __device__ __forceinline__ int parts_of(const SsmParams& p) {
   return (p.T + length - 1) / length;
 }
 
+// What steps whose sizes are `sum` together (-1: with a reset) and `most` at the largest are to the join.
+__device__ __forceinline__ void put_span(Args p, int64_t at, float sum, float most) {
+  p->span[at] = sum;
+  p->span[at + (int64_t)p->chunks * p->each * p->B * p->H] = most;
+}
+
 // A as the exponent of 2, held finite: A of -infinity (a state that lasts a step), or a product past float32's
 // range (the lowest float as a stand-in for it), would make a NaN with a step size of 0, which the steps behind
 // the axis' end have. A NaN passes.
@@ -212,7 +218,7 @@ __device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
   const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
   const float D = OUT && p->D != nullptr && at.ok ? p->D[at.ch] : 0.0f;
   const uint32_t off = lane_off<T>(at);
-  float span = 0.0f;
+  float span = 0.0f, most = 0.0f;
   bool drop = false;
   unsigned int rd[kOwn], ru[kOwn], rz[kOwn];
   Tile<T, P, NW> tile;
@@ -272,8 +278,12 @@ __device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
           h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(x.x * A2[i]), h[i], x.y * bm[i]);
           if (OUT) y = __builtin_fmaf(cm[i], h[i], y);
         }
-        if constexpr (OUT) lds.part[at.wave][s][at.lane] = y;
-        else span += x.x;
+        if constexpr (OUT) {
+          lds.part[at.wave][s][at.lane] = y;
+        } else {
+          span += x.x;
+          most = __builtin_fmaxf(most, x.x);
+        }
       }
     });
     if (!OUT && flags) drop = true;
@@ -308,7 +318,7 @@ __device__ __forceinline__ void fwd_chunk(const At& at, FwdShared<P, NW>& lds) {
     if (!OUT || (at.chunk == 0 && p->chunks > 1)) p->ends[(row * p->N + n) * p->H + at.ch] = h[i];
   }
   if (!OUT) {
-    if (at.wave == 0) p->span[row * p->H + at.ch] = drop ? -1.0f : span;
+    if (at.wave == 0) put_span(p, row * p->H + at.ch, drop ? -1.0f : span, most);
   }
 }
 
@@ -392,7 +402,7 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
   const float D = OUT && p->D != nullptr && at.ok ? p->D[at.ch] : 0.0f;
   const uint32_t off = lane_off<T>(at);
   const bool gated = OUT && p->z != nullptr, keep = OUT && p->ungated != nullptr;
-  float span = 0.0f;
+  float span = 0.0f, most = 0.0f;
   bool drop = false;
   unsigned int rd[kGroup], ru[kGroup], rz[kGroup];
   Rows<T, NP> rows;
@@ -457,6 +467,7 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
         E::store(to + i * p->sy_t, t0 + i < at.t1 ? off : kOffNone, gated ? y * gate : y);
       } else {
         span += dt[i];
+        most = __builtin_fmaxf(most, dt[i]);
       }
       if (i % 2) __builtin_amdgcn_sched_barrier(0);  // rows of few steps ahead: registers are short
     }
@@ -471,7 +482,7 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
     if (!OUT || (at.chunk == 0 && p->chunks > 1)) p->ends[(row * N + n) * p->H + at.ch] = h[n];
   }
   if (!OUT) {
-    p->span[row * p->H + at.ch] = drop ? -1.0f : span;
+    put_span(p, row * p->H + at.ch, drop ? -1.0f : span, most);
   }
 }
 
@@ -481,6 +492,20 @@ __global__ __launch_bounds__(64) void ssm_fwd_wide_kernel(SsmParams p) {
   const At at(p, !FIRST && p.chunks > 1 ? 1 : 0, p.length);
   if (FIRST && at.chunk > 0) wide_fwd_chunk<T, NP, PAD, false>(at, bc);
   else wide_fwd_chunk<T, NP, PAD, true>(at, bc);
+}
+
+// What becomes of a state s, or of a gradient on its way back, over steps whose sizes are `over` in sum and `most` at
+// the largest, as a step at a time gives it.
+// The usual case: more than 0 is left of it, so that an infinite one stays infinite (a finite one moves by less
+// than 1.2e-38 of its size).
+__device__ __forceinline__ float decay_over(float A2, float over) { return __builtin_amdgcn_exp2f(__builtin_fmaxf(A2 * over, -126.0f)); }
+// The others: an infinite one, of which a step alone may leave nothing (0 x infinity), and growth past float32's range
+// (a rate above 0) of one that may not get there.
+constexpr float kUnusual = 1.0e38f;  // where a state, or what is left of one, is as large or larger
+__device__ __forceinline__ float passed(float s, float A2, float over, float most) {
+  if (s == 0.0f || __builtin_fabsf(s) == __builtin_inff()) return s * __builtin_amdgcn_exp2f(A2 * most);
+  const float v = __builtin_fminf(__builtin_fmaxf(A2 * over, -126.0f), 1000.0f), e = __builtin_rintf(v);
+  return __builtin_ldexpf(s * __builtin_amdgcn_exp2f(v - e), (int)e);
 }
 
 // Forward: the states at the chunks' ends. Slot 0 of `ends` holds that of the first chunk, slot c what
@@ -500,6 +525,7 @@ __global__ __launch_bounds__(64) void ssm_join_kernel(SsmParams p) {
   const int64_t step = BACK ? -plane : plane, span_step = (BACK ? -1 : 1) * (int64_t)p.B * p.H;
   float* slot = p.ends + first * plane + e;
   const float* span = p.span + ((int64_t)first * p.B + b) * p.H + ch;
+  const int64_t most = (int64_t)p.chunks * p.each * p.B * p.H;  // from a sum to the largest
   for (int k0 = 0; k0 < count; k0 += kAhead) {
     float end[kAhead], over[kAhead];
 #pragma unroll
@@ -509,11 +535,25 @@ __global__ __launch_bounds__(64) void ssm_join_kernel(SsmParams p) {
       end[k] = slot[k * step];
       over[k] = span[k * span_step];
     }
+    const float before = s;
+    float largest = 0.0f;
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (k0 + k >= count) continue;
-      s = over[k] < 0.0f ? end[k] : __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * over[k]), s, end[k]);
+      const float decay = decay_over(A2, over[k]);
+      const bool drop = over[k] < 0.0f;
+      largest = __builtin_fmaxf(__builtin_fmaxf(largest, __builtin_fabsf(s)), decay);
+      s = drop ? end[k] : __builtin_fmaf(decay, s, end[k]);
       slot[k * step] = s;
+    }
+    if (__builtin_amdgcn_ballot_w64(largest >= kUnusual)) {  // uniform, and seldom: these slots again
+      s = before;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (k0 + k >= count) continue;
+        s = over[k] < 0.0f ? end[k] : passed(s, A2, over[k], span[k * span_step + most]) + end[k];
+        slot[k * step] = s;
+      }
     }
     slot += kAhead * step;
     span += kAhead * span_step;
@@ -551,7 +591,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams kernel_
   }
   const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
   const uint32_t off = lane_off<T>(at);
-  float span = 0.0f;
+  float span = 0.0f, most = 0.0f;
   bool drop = false;
   unsigned int rd[kOwn], rz[kOwn], rg[kOwn];
   Tile<T, P, NW> tile;
@@ -600,6 +640,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams kernel_
           if (RESET && (flags >> s & 1)) e[i] = 0.0f;
         }
         span += x.x;
+        most = __builtin_fmaxf(most, x.x);
       }
     });
     if (flags) drop = true;
@@ -610,7 +651,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_ends_kernel(SsmParams kernel_
 #pragma unroll
   for (int i = 0; i < P; ++i)
     if (n0 + i < p->N) p->ends[(row * p->N + n0 + i) * p->H + at.ch] = e[i];
-  if (at.wave == 0) p->span[row * p->H + at.ch] = drop ? -1.0f : span;
+  if (at.wave == 0) put_span(p, row * p->H + at.ch, drop ? -1.0f : span, most);
 }
 
 // The gradient that a part of the axis sends to the state before it, from a zero gradient after
@@ -636,7 +677,7 @@ __global__ __launch_bounds__(64) void ssm_bwd_ends_wide_kernel(SsmParams) {
   const float bias = p->bias != nullptr && at.ok ? p->bias[at.ch] : 0.0f;
   const uint32_t off = lane_off<T>(at);
   const bool gated = p->z != nullptr;
-  float span = 0.0f;
+  float span = 0.0f, most = 0.0f;
   bool drop = false;
   unsigned int rd[kGroup], rz[kGroup], rg[kGroup];
   Rows<T, NP> rows;
@@ -684,6 +725,7 @@ __global__ __launch_bounds__(64) void ssm_bwd_ends_wide_kernel(SsmParams) {
         for (int n = 0; n < NP; ++n) e[n] = 0.0f;
       }
       span += dt[i];
+      most = __builtin_fmaxf(most, dt[i]);
     }
   }
   if (!at.ok) return;
@@ -691,7 +733,7 @@ __global__ __launch_bounds__(64) void ssm_bwd_ends_wide_kernel(SsmParams) {
 #pragma unroll
   for (int n = 0; n < NP; ++n)
     if (n < N) p->ends[(row * N + n) * p->H + at.ch] = e[n];
-  p->span[row * p->H + at.ch] = drop ? -1.0f : span;
+  put_span(p, row * p->H + at.ch, drop ? -1.0f : span, most);
 }
 
 template <typename T, int P, int NW, bool PAD>
@@ -1124,7 +1166,7 @@ Bytes bytes_of(const Plan& plan, int64_t T, int64_t B, int64_t H, int64_t N, boo
   if (plan.chunks > 1) {
     const int64_t parts = (int64_t)plan.chunks * plan.each;
     r.span = align256(parts * B * N * H * 4);
-    r.total = r.span + align256(parts * B * H * 4);
+    r.total = r.span + align256(parts * B * H * 8);
   }
   if (back) {
     r.bc = r.total;

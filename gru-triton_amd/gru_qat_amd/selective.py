@@ -35,7 +35,8 @@ def selective_scan(
     type, ``h_T`` [B, H, N] in float32, with which a following call continues. ``D`` and
     ``delta_bias`` [H] and ``h0`` [B, H, N] are float32 (zeros when None), ``z`` [T, B, H] gates the output
     (no gate when None). ``reset`` [T, B] bool starts a new sequence at a step: the state before it is
-    taken as zero, whatever it is. Differentiable in all of them but reset (once); a training forward
+    taken as zero, whatever it is. An infinite state stays one until then, or until a step whose decay is zero
+    in float32 (exp(dt A) below 1e-38), which makes it NaN. Differentiable in all of them but reset (once); a training forward
     keeps the states before every 16th step and, with z, the outputs before their gate, in float32."""
     try:
         return (_lib._ops or _lib.ops()).selective_scan(u, delta, A, B, C, D, z, h0, delta_bias, reset, batch_first)

@@ -834,7 +834,8 @@ int gs_conv_step(const gs_conv_step_args* args, hipStream_t stream);
  *   h_t[n] = a[n] h_{t-1}[n] + dt u bm_t[n],
  *   y = (sum_n cm_t[n] h_t[n] + D u) silu(z)
  * of every channel c with N states (1 to 32) each. bm and cm are shared by a row's channels.
- * reset[t][b] != 0 takes h_{t-1} as 0 at step t, whatever it held. u, delta, z, bm, cm, y
+ * reset[t][b] != 0 takes h_{t-1} as 0 at step t, whatever it held. An infinite state stays
+ * one until then, or until a step whose a[n] is zero in fp32, which makes it NaN. u, delta, z, bm, cm, y
  * and their gradients are of one type; A, D, delta_bias, states and every sum are fp32. A
  * training forward stores the states before every 16th step in `saved`, and behind them, where
  * z gates, the outputs before their gate. No counterpart in the

@@ -72,3 +72,70 @@ def test_step_of_rates_and_no_step_size(dev):
     assert torch.allclose(y, scan[0], rtol=1e-6, atol=1e-6)  # four products in another order
     want = (torch.nn.functional.softplus(t["delta"][0, 1].double()) * t["u"][0, 1].double())[:, None] * t["B"][0, 1].double()
     assert torch.allclose(state[1, :, 1:3].double(), want[:, 1:3], rtol=1e-6)
+
+
+def _steps_one_by_one(t):
+    state, ys = t["h0"].clone(), []
+    for k in range(t["u"].shape[0]):
+        ys.append(G.selective_step(t["u"][k], t["delta"][k], t["A"], t["B"][k], t["C"][k], state, D=t["D"], z=t["z"][k],
+                                   delta_bias=t["delta_bias"]))
+    return torch.stack(ys), state
+
+
+def _same_oddities(a, b):
+    for odd in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(odd(a), odd(b)), odd.__name__
+    keep = a.isfinite()
+    assert torch.allclose(a[keep], b[keep], rtol=1e-4, atol=1e-4)
+
+
+def _fast(T, B, H, N, dev, seed):
+    """Channels 3 and 4 decay by e^-3.2 a step: to nothing in float32 over a chunk, and not in a step."""
+    t, dy, dh = _make(T, B, H, N, F32, dev, seed=seed)
+    t["A"][3:5] = -16.0
+    t["delta"][..., 3:5] = -1.5  # step sizes of 0.2
+    t["delta_bias"][3:5] = 0.0
+    return t, dy, dh
+
+
+@pytest.mark.parametrize("T,B,H,N", [(300, 2, 24, 4), (1061, 40, 70, 4)])
+def test_an_infinite_state_is_the_steps(dev, T, B, H, N):
+    """However an axis is cut, an infinite state is what one step after the other makes of it: infinite, and
+    NaN behind a step whose own decay is zero."""
+    t, _, _ = _fast(T, B, H, N, dev, 42)
+    t["h0"][0, 3, 1], t["h0"][1, 3, 2], t["h0"][0, 4, 0] = INF, -INF, INF
+    t["delta"][T // 2, 0, 4] = 30.0  # exp(-480)
+    y, h, _ = _run(t)
+    want, last = _steps_one_by_one(t)
+    _same_oddities(y, want)
+    _same_oddities(h, last)
+    assert h[0, 3, 1] == INF and h[1, 3, 2] == -INF and h[0, 4, 0].isnan()
+    assert y[:T // 2, 0, 4].isinf().all() and y[T // 2:, 0, 4].isnan().all()
+
+
+@pytest.mark.parametrize("T,B,H,N", [(300, 2, 24, 4), (1061, 40, 70, 4)])
+def test_an_infinite_gradient_goes_back(dev, T, B, H, N):
+    t, dy, dh = _fast(T, B, H, N, dev, 43)
+    dh[0, 3, 1], dh[1, 4, 2] = INF, -INF
+    _, _, got = check(t, dy, dh)
+    assert got["h0"][0, 3, 1] == INF and got["h0"][1, 4, 2] == -INF
+    assert got["h0"].isfinite().sum() == got["h0"].numel() - 2
+
+
+@pytest.mark.parametrize("T,B,H", [(192, 2, 24), (1100, 40, 70)])
+def test_states_that_grow_past_a_chunk(dev, T, B, H):
+    """Rates above zero: what a chunk makes of a state is outside float32, what becomes of the state is not;
+    a state of zero stays zero."""
+    t, _, _ = _make(T, B, H, 2, F32, dev, seed=44)
+    t["A"][:] = 2.0
+    t["delta"][:], t["delta_bias"] = -200.0, None  # steps that change nothing
+    t["delta"][64:128] = 0.5413  # and 64 that take e^2 each
+    t["u"][:], t["B"][:] = 0.0, 0.0
+    t["h0"][:, :, 0], t["h0"][:, :, 1] = 1e-38, 0.0
+    _, h, _ = _run(t)
+    args = [t[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "h0")]
+    want = P.selective_scan(*args)[1]
+    # a step's exponent of 2 is off by some 10 units (8 of its size), its power and product by 2: 22 x 64;
+    # a span's exponent of 185 by 3 of its own: 400
+    P.assert_within(h, want, want, 2000, "h_T")
+    assert (h[..., 1] == 0).all() and h[..., 0].min() > 1e16
