@@ -5,7 +5,8 @@
 // With d = x - max, s = sum exp d and t = sum d exp d: lse = max + log s, entropy = log s - t / s.
 // A logit of -infinity is a token that cannot come: it adds nothing. A row of those alone has log
 // probabilities -infinity, entropy 0 and no gradient. A NaN or +infinity makes a row NaN. A
-// negative token marks a row whose token does not count: its log probability is 0, and sends no gradient.
+// negative token marks a row whose token does not count: its log probability is 0, and sends no gradient. A row to which
+// no gradient comes has none, also where its logits are NaN.
 //
 // Bound by memory: one pass over the logits forward with the running maximum, s and t, and one backward.
 // A workgroup takes a row, or a part of one where there are few rows; the parts of a row are
@@ -308,10 +309,11 @@ __global__ __launch_bounds__(256) void prob_bwd_kernel(ProbParams p) {
   const T* x = static_cast<const T*>(p.x) + row * p.sx;
   T* dx = static_cast<T*>(p.dx) + row * p.sdx;
   const float m = p.stats[2 * row], logs = p.stats[2 * row + 1];
-  const bool none = m == -__builtin_inff() && logs == -__builtin_inff();
   const int64_t token = token_of(p, row);
   const float g = p.dlogprob != nullptr && token >= 0 && token < p.V ? p.dlogprob[row] : 0.0f;
   const float ge = p.dentropy != nullptr ? p.dentropy[row] : 0.0f;
+  // every logit is -infinity, or no gradient comes (a row of padding), whatever the logits are
+  const bool none = (m == -__builtin_inff() && logs == -__builtin_inff()) || (g == 0.0f && ge == 0.0f);
   // dx = -p (g + ge (log p + entropy)), and g more at the token
   const float base = __builtin_fmaf(ge, p.entropy[row], g);
 #pragma unroll 2

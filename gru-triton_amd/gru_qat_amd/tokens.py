@@ -35,7 +35,8 @@ def token_logprobs(
     A logit of -infinity is a token that cannot come; a row of those alone has log probabilities
     -infinity, entropy 0 and no gradient. A NaN or +infinity makes a row's results NaN. A negative
     token does not count: its log probability is 0 and sends no gradient (its row's entropy does);
-    one of V or more gives NaN. Rows have at most 2^24 logits, 2^19 with ``top``. Differentiable in logits
+    one of V or more gives NaN. The logits of a row to which no gradient comes get zeros, also NaN
+    ones. Rows have at most 2^24 logits, 2^19 with ``top``. Differentiable in logits
     through logprobs and entropy (once): ``-logprobs.mean()`` is the cross entropy."""
     try:
         return (_lib._ops or _lib.ops()).token_logprobs(logits, tokens, top)

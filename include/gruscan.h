@@ -953,7 +953,8 @@ typedef struct gs_logprobs_args {
 int64_t gs_logprobs_scratch_bytes(const gs_logprobs_args* args);
 int gs_logprobs_fwd(const gs_logprobs_args* args, hipStream_t stream);
 
-/* dx[m][v] = dlogprob[m] ([v = token] - p_v) - dentropy[m] p_v (log p_v + entropy). */
+/* dx[m][v] = dlogprob[m] ([v = token] - p_v) - dentropy[m] p_v (log p_v + entropy); zeros where
+ * dlogprob (of a token that counts) and dentropy are zero, whatever the logits are. */
 typedef struct gs_logprobs_bwd_args {
   const void* x;
   const void* tokens;
