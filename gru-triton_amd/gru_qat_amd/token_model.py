@@ -45,7 +45,8 @@ class TokenModel(torch.nn.Module):
     def forward(self, tokens: torch.Tensor, targets: torch.Tensor, *, states: Optional[List[Any]] = None,
                 reset: Optional[torch.Tensor] = None, top: int = 0) -> Tuple[torch.Tensor, ...]:
         """``(logprobs, entropy, top_logprobs, top_tokens)`` of the targets [T, B] that follow the
-        tokens, as ``token_logprobs`` returns them; ``-logprobs.mean()`` is the training loss."""
+        tokens, as ``token_logprobs`` returns them. The training loss is
+        ``-logprobs.sum() / (targets >= 0).sum()``: padded targets add 0, and a mean would count them."""
         y, _ = self.hidden(tokens, states, reset)
         return token_logprobs(linear_act(y, self.weight), targets, top=top)
 

@@ -37,7 +37,8 @@ def token_logprobs(
     token does not count: its log probability is 0 and sends no gradient (its row's entropy does);
     one of V or more gives NaN. The logits of a row to which no gradient comes get zeros, also NaN
     ones. Rows have at most 2^24 logits, 2^19 with ``top``. Differentiable in logits
-    through logprobs and entropy (once): ``-logprobs.mean()`` is the cross entropy."""
+    through logprobs and entropy (once): ``-logprobs.sum() / (tokens >= 0).sum()`` is the
+    cross entropy over the tokens that count."""
     try:
         return (_lib._ops or _lib.ops()).token_logprobs(logits, tokens, top)
     except TypeError as e:

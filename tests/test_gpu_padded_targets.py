@@ -57,3 +57,22 @@ def test_a_row_without_a_gradient(dev):
     dx, = torch.autograd.grad((lp, h), leaf, (dl, de))
     assert (dx[2] == 0).all() and dx[3].isnan().any() and dx[4].isnan().any()
     assert dx[[0, 1, 5, 6, 7, 8, 9, 10, 11]].isfinite().all()
+
+
+@pytest.mark.parametrize("padded", [0, 3, 11])
+def test_the_loss_over_targets_that_count(dev, padded):
+    """What the documents call the loss is the cross entropy that leaves padding out, with its gradient."""
+    x, tokens, _, _ = _rows(301, F32, dev)
+    tokens[:padded] = -1
+    leaf = x.clone().requires_grad_(True)
+    lp = G.token_logprobs(leaf, tokens)[0]
+    loss = -lp.sum() / (tokens >= 0).sum()
+    dx, = torch.autograd.grad(loss, leaf)
+    ref = x.double().cpu().requires_grad_(True)
+    want = torch.nn.functional.cross_entropy(ref, tokens.cpu(), ignore_index=-1)
+    dref, = torch.autograd.grad(want, ref)
+    # a loss of some 8, log probabilities up to 20: 12 sums and V / 64 + 64 roundings of them
+    assert abs(loss.item() - want.item()) < (301 // 64 + 64 + 12) * 2.0 ** -24 * 20
+    hot = torch.nn.functional.one_hot(tokens.clamp(min=0).cpu(), 301) * (tokens >= 0).cpu()[:, None]
+    size = (torch.softmax(x.double().cpu(), -1) * (tokens >= 0).cpu()[:, None] + hot) / (12 - padded)
+    P.assert_within(dx, dref, size, 301 // 64 + 64 + 8 + 20, "dx")
