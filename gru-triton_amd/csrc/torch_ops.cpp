@@ -84,6 +84,7 @@ struct GlrFunction : torch::autograd::Function<GlrFunction> {
     return {out, h_last};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture("gated_linear_scan");
     const auto saved = ctx->get_saved_variables();
     const Tensor &gi = saved[0], &h0 = saved[1], &reset = saved[2], &out = saved[3];
     Tensor dout = grads[0], dh = grads[1];
@@ -253,6 +254,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture("linear_act");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &pre = saved[2];
     const int64_t given = ctx->saved_data["act"].toInt();
@@ -451,6 +453,16 @@ Tensor adamw_dequantize_state(const Tensor& codes, const Tensor& scales) {
   return out;
 }
 
+// The leaves that a backward from t reaches and runs, for tests of check_capture's walk.
+Tensors reached_leaves(const Tensor& t) {
+  Tensors leaves;
+  if (t.grad_fn())
+    each_reached(t.grad_fn().get(), [&](torch::autograd::Node& n) {
+      if (const auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(&n)) leaves.push_back(leaf->variable);
+    });
+  return leaves;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ops, m) {
@@ -460,5 +472,6 @@ PYBIND11_MODULE(_ops, m) {
   m.def("linear_act", &linear_act, py::call_guard<py::gil_scoped_release>());
   m.def("adamw_step", &adamw_step, py::call_guard<py::gil_scoped_release>());
   m.def("adamw_dequantize_state", &adamw_dequantize_state, py::call_guard<py::gil_scoped_release>());
+  m.def("_reached_leaves", &reached_leaves);
   bind_sequence_ops(m);
 }

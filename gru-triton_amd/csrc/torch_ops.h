@@ -8,9 +8,11 @@
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/gruscan.h"
@@ -78,25 +80,52 @@ void check_may_modify(const char* who, const char* name, const Tensor& t) {
               " was made in inference mode and cannot be updated in place outside it");
 }
 
-// A captured backward hands a leaf's gradient to the leaf's accumulator on the stream that this was made on.
-// An eager graph of the leaf that is still alive keeps it on the default stream, which no capture can wait
-// for: torch's engine would end the process there.
+// f(n) for every node that the current backward reaches from `node` and runs: with inputs asked for
+// (torch.autograd.grad) those on the way to them alone, else all.
+template <typename F>
+void each_reached(torch::autograd::Node* node, F&& f) {
+  const auto* asked = torch::autograd::get_current_graph_task_exec_info();
+  if (asked != nullptr && asked->empty()) asked = nullptr;
+  std::vector<torch::autograd::Node*> left{node};
+  std::unordered_set<torch::autograd::Node*> seen{node};
+  while (!left.empty()) {
+    const auto* at = left.back();
+    left.pop_back();
+    for (const auto& e : at->next_edges()) {
+      torch::autograd::Node* next = e.function.get();
+      if (next == nullptr || !seen.insert(next).second) continue;
+      if (asked != nullptr) {
+        const auto it = asked->find(next);
+        if (it == asked->end() || !it->second.should_execute()) continue;
+      }
+      f(*next);
+      left.push_back(next);
+    }
+  }
+}
+
+// What a captured backward goes on to runs on the stream that it was made on, which for the default one no capture can
+// wait for: torch's engine would end the process there. That is so for a leaf's accumulator where an eager graph of
+// the leaf is still alive, however many views, casts or products are between, and for a graph made before.
+// Asked before a backward launches anything.
 void check_capture(const char* who) {
   const auto node = torch::autograd::get_current_node();
   if (!node || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-  for (const auto& e : node->next_edges()) {
-    const auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get());
-    TORCH_CHECK(leaf == nullptr || !leaf->variable.is_cuda() || leaf->num_inputs() == 0 || leaf->input_metadata(0).stream().id() != 0,
+  each_reached(node.get(), [&](torch::autograd::Node& n) {
+    const auto stream = n.stream();
+    if (!stream.has_value() || stream->id() != 0) return;
+    TORCH_CHECK(dynamic_cast<torch::autograd::AccumulateGrad*>(&n) == nullptr,
                 who, ": an eager graph of the same leaves, made on the default stream, is alive (through an output or a loss); "
                 "drop it before a backward is captured");
-  }
+    TORCH_CHECK(false, who, ": a captured backward goes on into a graph that was made on the default stream (", n.name(),
+                "); make all of it under the capture");
+  });
 }
 
 // A backward's results. Where a graph of them is asked for (create_graph), it goes on to
 // `from`, which they were computed from, through an error for whoever asks for a second
 // derivative: without it that derivative would lack their terms and nobody would know.
 variable_list once(const char* who, variable_list grads, const variable_list& from) {
-  check_capture(who);
   if (!torch::GradMode::is_enabled()) return grads;
   const size_t n = grads.size();
   grads.insert(grads.end(), from.begin(), from.end());

@@ -107,6 +107,7 @@ struct ConvFunction : torch::autograd::Function<ConvFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const char* who = "causal_conv";
+    check_capture(who);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &bias = saved[2], &state = saved[3], &reset = saved[4];
     Tensor dy = grads[0], dlast = grads[1];
@@ -286,6 +287,7 @@ struct SsmFunction : torch::autograd::Function<SsmFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const char* who = "selective_scan";
+    check_capture(who);
     const auto s = ctx->get_saved_variables();
     const SsmInputs in{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9]};
     Tensor dy = grads[0], dh = grads[1];
@@ -465,6 +467,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const char* who = "embedding";
+    check_capture(who);
     const Tensor tokens = ctx->get_saved_variables()[0];
     check_no_tangent(who, "the output's gradient", grads[0]);
     const Tensor dout = unit(grads[0]);
@@ -548,6 +551,7 @@ struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const char* who = "token_logprobs";
+    check_capture(who);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &tokens = saved[1];
     Tensor dl = grads[0], de = grads[1];
