@@ -9,8 +9,10 @@
 // results do not. A wave sorts a list of 16 or fewer by counting smaller ones, lane by lane, and
 // sums its rows in that order. Longer lists are cut into chunks, a workgroup each, whose waves take a
 // quarter of its rows; a list's order there comes from counting smaller ones too or, where it is long, from a bit
-// for every position. The chunks' sums are joined in order. 16384 tokens of 32000 x 1024 bf16:
-// forward 10 us; backward 10 to count, 8 to give room, put down and clear, 18 for the sums (5.5 TB/s), 4 to join.
+// for every position of a window. Windows of positions are counted one after the other, so that a list holds
+// them in order and a chunk reads its own windows alone: an entry is read by the chunks of its window, 512 at most and
+// 64 from 2^20 positions on, however long its list is. The chunks' sums are joined in order. 16384 tokens of
+// 32000 x 1024 bf16: forward 10 us; backward 10 to count, 8 to give room, put down and clear, 18 for the sums (5.5 TB/s), 4 to join.
 #include "gs_seq.h"
 
 namespace gs {
@@ -121,10 +123,12 @@ __global__ __launch_bounds__(256) void embed_clear_kernel(uint32_t* p, int64_t n
   if (e < n) p[e] = 0;
 }
 
-// Equal tokens of a wave are counted together, in one access: those of a frequent token would
-// wait for each other (16384 tokens, one in 15 the same: 15 -> 10 us).
-__global__ __launch_bounds__(256) void embed_count_kernel(EmbedParams p) {
-  const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
+constexpr int kWindow = 1 << 17;  // positions that are counted, and ordered, at a time
+
+// The window of positions from `from` on. Equal tokens of a wave are counted together, in one access: those of a
+// frequent token would wait for each other (16384 tokens, one in 15 the same: 15 -> 10 us).
+__global__ __launch_bounds__(256) void embed_count_kernel(EmbedParams p, int64_t from) {
+  const int64_t m = from + (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t token = m < p.M ? token_at(p, m) : -1;
   const bool some = token >= 0 && token < p.V;
   const int v = (int)token, lane = threadIdx.x & 63;
@@ -305,9 +309,9 @@ struct Sum {
 };
 
 // A workgroup a chunk of a long list: the positions of ranks chunk c to chunk (c + 1). With kAll
-// positions or fewer, a rank is counted; otherwise bits of kWindow positions at a time say which are in
-// the list, and the bits before one are its rank.
-constexpr int kWindow = 1 << 17, kMostChunk = 2048, kAll = 256, kMostSpan = 1024;
+// positions or fewer, a rank is counted; otherwise bits of a window's positions say which are in
+// the list, and those before one, with the windows before, are its rank.
+constexpr int kMostChunk = 2048, kAll = 256, kMostSpan = 1024;
 union ChunkShared {
   struct {
     uint32_t bits[kWindow / 32], upto[256];
@@ -330,14 +334,27 @@ __device__ __forceinline__ void sum_chunk(const EmbedParams& p, const uint4 c, i
     for (uint32_t j = 0; j < n; ++j) rank += lds.all[j] < mine ? 1 : 0;
     if (threadIdx.x < n && rank >= from && rank < to) rows[rank - from] = mine;
   } else {
-    uint32_t before = 0;  // positions of the list in the windows before
-    for (int64_t base = 0; base < p.M && before < to; base += kWindow) {
+    // the end of the window that entry i is in, of entries i to i + kWindow (no more than that are in one), or its start
+    auto edge = [&](uint32_t i, bool end) {
+      if (p.M <= kWindow) return end ? n : 0u;
+      const uint32_t w = list[i] / kWindow;
+      uint32_t lo = end ? i : i - min(i, (uint32_t)kWindow), hi = end ? (uint32_t)min((int64_t)n, (int64_t)i + kWindow) : i;
+      while (lo < hi) {  // the first entry in [lo, hi) of a window behind w, or of w, or hi
+        const uint32_t mid = lo + (hi - lo) / 2, v = list[mid] / kWindow;
+        if (end ? v > w : v >= w) hi = mid;
+        else lo = mid + 1;
+      }
+      return lo;
+    };
+    for (uint32_t first = edge(from, false), last; first < to; first = last) {
+      last = edge(first, true);
+      const int64_t base = (int64_t)(list[first] / kWindow) * kWindow;
       const int words = (int)min((int64_t)kWindow, p.M - base + 31) / 32;
       for (int i = threadIdx.x; i < words; i += 256) lds.sort.bits[i] = 0;
       __syncthreads();
-      for (uint32_t i = threadIdx.x; i < n; i += 256) {
-        const int64_t at = (int64_t)list[i] - base;
-        if (at >= 0 && at < kWindow) atomicOr(lds.sort.bits + at / 32, 1u << (at & 31));
+      for (uint32_t i = first + threadIdx.x; i < last; i += 256) {
+        const uint32_t at = list[i] - (uint32_t)base;
+        if (at < (uint32_t)kWindow) atomicOr(lds.sort.bits + at / 32, 1u << (at & 31));
       }
       __syncthreads();
       // each thread counts the bits of a run of words; then the runs before it
@@ -352,13 +369,12 @@ __device__ __forceinline__ void sum_chunk(const EmbedParams& p, const uint4 c, i
         lds.sort.upto[threadIdx.x] += o;
         __syncthreads();
       }
-      uint32_t rank = before + lds.sort.upto[threadIdx.x] - mine;
+      uint32_t rank = first + lds.sort.upto[threadIdx.x] - mine;
       if (rank < to && rank + mine > from) {
         for (int i = w0; i < min(w0 + per, words); ++i)
           for (uint32_t w = lds.sort.bits[i]; w; w &= w - 1, ++rank)
             if (rank >= from && rank < to) rows[rank - from] = (uint32_t)(base + 32 * i + __ffs(w) - 1);
       }
-      before += lds.sort.upto[255];
       __syncthreads();
     }
   }
@@ -496,8 +512,11 @@ int make_lists(const EmbedParams& p, const Plan& plan, hipStream_t stream) {
   const dim3 rows((unsigned)((p.M + 255) / 256));
   hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)((plan.clear + 255) / 256)), dim3(256), 0, stream, p.cursor, plan.clear);
   GS_CHECK_HIP(hipGetLastError());
-  hipLaunchKernelGGL(embed_count_kernel, rows, dim3(256), 0, stream, p);
-  GS_CHECK_HIP(hipGetLastError());
+  for (int64_t from = 0; from < p.M; from += kWindow) {
+    const int64_t n = std::min<int64_t>(kWindow, p.M - from);
+    hipLaunchKernelGGL(embed_count_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, p, from);
+    GS_CHECK_HIP(hipGetLastError());
+  }
   hipLaunchKernelGGL(embed_room_kernel, dim3((unsigned)((p.V + 1023) / 1024)), dim3(1024), 0, stream, p);
   GS_CHECK_HIP(hipGetLastError());
   hipLaunchKernelGGL(embed_place_kernel, rows, dim3(256), 0, stream, p);
