@@ -31,9 +31,9 @@ struct EmbedParams {
   int V, K, wide;     // wide: tokens of 64 bits
   // backward: scratch
   uint32_t *count, *start, *place, *list;  // [V], [V], [M], [M]
-  uint32_t* cursor;                        // room taken, long lists, chunks
-  uint4* chunks;                           // token, first of its chunks, chunk, chunks of the token
-  float* sums;                             // [chunks][K]
+  uint32_t* cursor;                        // room taken, chunks, rows of sums
+  uint4* chunks;                           // token, first row of its sums, chunk, chunks of the token
+  float* sums;                             // [rows][K]: of the chunks of lists that have several
   int chunk, most_chunks;
 };
 
@@ -154,23 +154,43 @@ __global__ __launch_bounds__(256) void embed_count_kernel(EmbedParams p, int64_t
 // of 30000 of 3000 x 512 bf16 takes 54, 25 and 55 us with 4, 53, 24 and 55 with 16, 61, 30 and 74 with 64.
 constexpr uint32_t kShort = 16;
 
-// Room for each token's list, in no particular order, and the chunks of the long ones.
-__global__ __launch_bounds__(1024) void embed_room_kernel(EmbedParams p) {
-  __shared__ uint32_t waves[2][16], base[2];
-  const int v = blockIdx.x * 1024 + threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t n = v < p.V ? p.count[v] : 0, parts = n > kShort ? (n + p.chunk - 1) / p.chunk : 0;
-  uint32_t upto[2] = {n, parts};  // of the wave's lanes up to this one
+// What a list of n positions takes up: room, chunks where it is long, and a row for the sums of each of several chunks.
+struct Needs {
+  uint32_t x[3];
+  __device__ __forceinline__ Needs(const EmbedParams& p, uint32_t n) {
+    x[0] = n;
+    x[1] = n > kShort ? (n + p.chunk - 1) / p.chunk : 0;
+    x[2] = x[1] > 1 ? x[1] : 0;
+  }
+};
+// The needs of the wave's lanes up to this one.
+__device__ __forceinline__ void sum_up(Needs& a) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < 3; ++k) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-      const uint32_t o = __shfl_up(upto[k], d);
-      if (lane >= d) upto[k] += o;
+      const uint32_t o = __shfl_up(a.x[k], d);
+      if (lane >= d) a.x[k] += o;
     }
-    if (lane == 63) waves[k][wave] = upto[k];
   }
+}
+__device__ __forceinline__ void put_chunks(const EmbedParams& p, uint32_t v, uint32_t parts, uint32_t first, uint32_t row) {
+  for (uint32_t c = 0; c < parts && first + c < (uint32_t)p.most_chunks; ++c) p.chunks[first + c] = uint4{v, row, c, parts};
+}
+
+// Room for each token's list, in no particular order, and the chunks of the long ones.
+__global__ __launch_bounds__(1024) void embed_room_kernel(EmbedParams p) {
+  __shared__ uint32_t waves[3][16], base[3];
+  const int v = blockIdx.x * 1024 + threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Needs mine(p, v < p.V ? p.count[v] : 0);
+  Needs upto = mine;
+  sum_up(upto);
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    if (lane == 63) waves[k][wave] = upto.x[k];
   __syncthreads();
-  if (threadIdx.x < 2) {
+  if (threadIdx.x < 3) {
     uint32_t all = 0;
     for (int w = 0; w < 16; ++w) {
       const uint32_t x = waves[threadIdx.x][w];
@@ -180,9 +200,11 @@ __global__ __launch_bounds__(1024) void embed_room_kernel(EmbedParams p) {
     base[threadIdx.x] = all ? atomicAdd(p.cursor + threadIdx.x, all) : 0;
   }
   __syncthreads();
-  if (n) p.start[v] = base[0] + waves[0][wave] + upto[0] - n;
-  const uint32_t first = base[1] + waves[1][wave] + upto[1] - parts;
-  for (uint32_t c = 0; c < parts && first + c < (uint32_t)p.most_chunks; ++c) p.chunks[first + c] = uint4{(uint32_t)v, first, c, parts};
+  uint32_t at[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) at[k] = base[k] + waves[k][wave] + upto.x[k] - mine.x[k];
+  if (mine.x[0]) p.start[v] = at[0];
+  put_chunks(p, (uint32_t)v, mine.x[1], at[1], at[2]);
 }
 
 __global__ __launch_bounds__(256) void embed_place_kernel(EmbedParams p) {
@@ -198,7 +220,7 @@ constexpr int kOneTokens = 4096, kOneVocabulary = 4096;
 __global__ __launch_bounds__(1024) void embed_lists_kernel(EmbedParams p) {
   constexpr int kEach = kOneTokens / 1024;
   __shared__ uint32_t count[kOneVocabulary];
-  __shared__ uint32_t waves[2][16];
+  __shared__ uint32_t waves[3][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int v = threadIdx.x; v < p.V; v += 1024) count[v] = 0;
   int token[kEach];
@@ -214,23 +236,19 @@ __global__ __launch_bounds__(1024) void embed_lists_kernel(EmbedParams p) {
   __syncthreads();
   // room: a thread takes `per` tokens; then the room of the threads before it
   const int per = (p.V + 1023) / 1024, v0 = threadIdx.x * per;
-  uint32_t mine[2] = {0, 0};
+  Needs mine(p, 0);
   for (int v = v0; v < min(v0 + per, p.V); ++v) {
-    mine[0] += count[v];
-    mine[1] += count[v] > kShort ? (count[v] + p.chunk - 1) / p.chunk : 0;
-  }
-  uint32_t upto[2] = {mine[0], mine[1]};
+    const Needs one(p, count[v]);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const uint32_t o = __shfl_up(upto[k], d);
-      if (lane >= d) upto[k] += o;
-    }
-    if (lane == 63) waves[k][wave] = upto[k];
+    for (int k = 0; k < 3; ++k) mine.x[k] += one.x[k];
   }
+  Needs upto = mine;
+  sum_up(upto);
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    if (lane == 63) waves[k][wave] = upto.x[k];
   __syncthreads();
-  if (threadIdx.x < 2) {
+  if (threadIdx.x < 3) {
     uint32_t all = 0;
     for (int w = 0; w < 16; ++w) {
       const uint32_t x = waves[threadIdx.x][w];
@@ -240,16 +258,17 @@ __global__ __launch_bounds__(1024) void embed_lists_kernel(EmbedParams p) {
     p.cursor[threadIdx.x] = all;
   }
   __syncthreads();
-  uint32_t at = waves[0][wave] + upto[0] - mine[0], chunk = waves[1][wave] + upto[1] - mine[1];
+  uint32_t at[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) at[k] = waves[k][wave] + upto.x[k] - mine.x[k];
   for (int v = v0; v < min(v0 + per, p.V); ++v) {
     const uint32_t n = count[v];
+    const Needs one(p, n);
     p.count[v] = n;
-    p.start[v] = at;
-    count[v] = at;
-    at += n;
-    const uint32_t parts = n > kShort ? (n + p.chunk - 1) / p.chunk : 0;
-    for (uint32_t c = 0; c < parts && chunk + c < (uint32_t)p.most_chunks; ++c) p.chunks[chunk + c] = uint4{(uint32_t)v, chunk, c, parts};
-    chunk += parts;
+    p.start[v] = count[v] = at[0];
+    put_chunks(p, (uint32_t)v, one.x[1], at[1], at[2]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) at[k] += one.x[k];
   }
   __syncthreads();
 #pragma unroll
@@ -321,7 +340,7 @@ union ChunkShared {
 };
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void sum_chunk(const EmbedParams& p, const uint4 c, int id, ChunkShared& lds, uint32_t* rows) {
+__device__ __forceinline__ void sum_chunk(const EmbedParams& p, const uint4 c, ChunkShared& lds, uint32_t* rows) {
   typedef Sum<T, VEC> S;
   static_assert(S::kSpan <= kMostSpan, "columns of a pass");
   const uint32_t n = p.count[c.x], from = c.z * p.chunk, to = min(n, from + p.chunk);
@@ -403,7 +422,7 @@ __device__ __forceinline__ void sum_chunk(const EmbedParams& p, const uint4 c, i
 #pragma unroll
         for (int w = 0; w < 3; ++w) x += lds.sums[w][(e * S::R::kElems + i) * 64 + lane];
         const int at = k + e * 64 * S::R::kElems + i;
-        if (c.w > 1 && at < p.K) p.sums[(int64_t)id * p.K + at] = x;
+        if (c.w > 1 && at < p.K) p.sums[((int64_t)c.y + c.z) * p.K + at] = x;
       }
     if (c.w == 1) sum.store(p, c.x, k);
   }
@@ -417,7 +436,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedParams p) {
   __shared__ ChunkShared lds;
   __shared__ uint32_t rows[kMostChunk];
   if ((int)blockIdx.x < p.most_chunks) {  // uniform
-    if (blockIdx.x < p.cursor[1]) sum_chunk<T, VEC>(p, p.chunks[blockIdx.x], (int)blockIdx.x, lds, rows);
+    if (blockIdx.x < p.cursor[1]) sum_chunk<T, VEC>(p, p.chunks[blockIdx.x], lds, rows);
     return;
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -481,13 +500,15 @@ Plan make_plan(int64_t M, int64_t V, int64_t K) {
   r.chunk = (int)std::min<int64_t>(kMostChunk, std::max<int64_t>(64, (M / 512 + 63) / 64 * 64));
   // a list of n > kShort has n / chunk rounded up
   r.most_chunks = M > kShort ? (int)(M / r.chunk + std::min<int64_t>(V, M / (kShort + 1))) : 0;
+  // and, of n > chunk, less than 2 n / chunk, each with a row of sums
+  const int64_t rows = M > r.chunk ? 2 * M / r.chunk : 0;
   r.clear = 64 + V;  // cursors on a line of their own, counts
   r.start = align256(r.clear * 4);
   r.place = r.start + align256(V * 4);
   r.list = r.place + align256(M * 4);
   r.chunks = r.list + align256(M * 4);
   r.sums = r.chunks + align256((int64_t)r.most_chunks * 16);
-  r.total = r.sums + align256((int64_t)r.most_chunks * K * 4);
+  r.total = r.sums + align256(rows * K * 4);
   return r;
 }
 
