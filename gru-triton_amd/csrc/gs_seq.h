@@ -36,6 +36,14 @@ __device__ __forceinline__ void share_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// The same between the lanes of one wave, whose LDS accesses keep their order by themselves: for the compiler
+// alone, no instruction.
+__device__ __forceinline__ void share_in_wave() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // In lanes whose bit M is clear a[l] + a[l ^ M], in the others b[l] + b[l ^ M]: six of these,
 // each over half as many registers as the one before, leave 64 sums over a wave in one register.
 template <int M>

@@ -431,7 +431,9 @@ __device__ __forceinline__ void wide_fwd_chunk(const At& at, float (*bc)[2 * NP]
       for (int n = 0; n < NP; ++n)
         if (n < N) to[(int64_t)n * p->H] = h[n];
     }
+    share_in_wave();
     rows.put(bc, at);
+    share_in_wave();
     float dt[kGroup], u[kGroup], z[kGroup];
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) {
@@ -701,7 +703,9 @@ __global__ __launch_bounds__(64) void ssm_bwd_ends_wide_kernel(SsmParams) {
   fetch(last);
   for (int t0 = last; t0 >= at.t0; t0 -= kGroup) {
     const uint32_t flags = mask_of(flag);
+    share_in_wave();
     rows.put(bc, at);
+    share_in_wave();
     float dt[kGroup], dy[kGroup];
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) {
