@@ -24,9 +24,10 @@
 // through memory: results are reproducible.
 //
 // Bound by the vector ALU and its exponentials: forwards 16 states at a step take some 6 instructions and an exponential each,
-// every step a softplus. Measured, T 4096, B 8, H 1024, N 16 bf16: forward 134 us for the first
-// launch and 170 with what is kept, ends 111, backward 520 (its VALU busy for some 80 %; 747 MB take 145 at a copy's rate); T 65536, B 1, H 1024
-// forward 267 + 24 + 302 (540 MB: 105); T 512, B 16, H 512 fp32 training 23 + 27 forward, 22 + 68 backward and 14 of joins and sums.
+// every step a softplus. Measured, T 4096, B 8, H 1024, N 16 bf16: forward 139 us for the first
+// launch and 174 with what is kept, ends 116, backward 540 (its VALU busy for 77 % by its counters, LDS for 43; 747 MB take
+// 145 at a copy's rate); T 65536, B 1, H 1024 forward 277 + 30 + 324 (540 MB: 105), the VALU busy for 90 and 87 %;
+// T 512, B 16, H 512 fp32 training 24 + 27 forward, 23 + 69 backward and 14 of joins and sums.
 #include "gs_seq.h"
 
 namespace gs {
@@ -1076,11 +1077,15 @@ struct Plan {
   int blocks, chunks, length, each;
   bool wide;  // the kernels that share nothing, for the forward or the backward's ends
 };
-// In us, states over a workgroup's waves / waves that share nothing, the same tensors (N 16):
-//   T 4096, B 8, H 1024 bf16 training   1133 / 1046     T 512, B 16, H 512 fp32 training   164 / 178
-//   T 65536, B 1, H 1024 bf16 forward    736 / 548      T 1001, B 3, H 333 fp32 training   110 / 150
-// With 256 and 1024 workgroups asked for in place of 512 the first takes 1459 and 1157 (backward alone).
-constexpr int64_t kGroups = 512;    // workgroups asked for: two a CU
+// In us, states over a workgroup's waves / waves that share nothing, the same tensors:
+//   T 4096, B 8, H 1024 bf16 training, N 16    912 / 890     T 512, B 16, H 512 fp32 training, N 16   154 / 161
+//   the same, N 4                              969 / 700     the same, N 32                           243 / 280
+//   the same, N 32                            1665 / 1771    T 1001, B 3, H 333 fp32 training, N 16   140 / 148
+//   T 65536, B 1, H 1024 bf16 forward, N 16    627 / 546
+// The first with 256, 512 and 1024 workgroups asked for in the backward: N 16 1099, 890, 916; N 32 1758, 1771, 1829; N 4, whose
+// workgroups are two waves, 1043, 700, 507. With 2048, 4096 and 8192 waves: N 16 1009, 890, 900. The constants are
+// those that are best at N 16; the plan does not ask for N.
+constexpr int64_t kGroups = 512;    // workgroups asked for: two a CU (one at a time of N > 16, which fill its LDS)
 constexpr int64_t kWaves = 4096;    // waves asked for, where they share nothing
 constexpr int64_t kFewWaves = 2048; // up to these, states are spread over the waves of a workgroup
 constexpr int kLeastChunk = 64, kLeastPart = 32;  // steps
