@@ -498,16 +498,13 @@ __global__ __launch_bounds__(64) void ssm_fwd_wide_kernel(SsmParams p) {
 }
 
 // What becomes of a state s, or of a gradient on its way back, over steps whose sizes are `over` in sum and `most` at
-// the largest, as a step at a time gives it.
-// The usual case: more than 0 is left of it, so that an infinite one stays infinite (a finite one moves by less
-// than 1.2e-38 of its size).
-__device__ __forceinline__ float decay_over(float A2, float over) { return __builtin_amdgcn_exp2f(__builtin_fmaxf(A2 * over, -126.0f)); }
-// The others: an infinite one, of which a step alone may leave nothing (0 x infinity), and growth past float32's range
-// (a rate above 0) of one that may not get there.
-constexpr float kUnusual = 1.0e38f;  // where a state, or what is left of one, is as large or larger
+// the largest, as a step at a time gives it, where exp2(A2 over) s does not say it: of an infinite one something is left
+// unless a step alone leaves nothing (0 x infinity), and growth past float32's range (a rate above 0) may be of one that does not
+// get there.
+constexpr float kUnusual = 1.0e38f;  // so where a state, or what is left of one, is as large or larger
 __device__ __forceinline__ float passed(float s, float A2, float over, float most) {
   if (s == 0.0f || __builtin_fabsf(s) == __builtin_inff()) return s * __builtin_amdgcn_exp2f(A2 * most);
-  const float v = __builtin_fminf(__builtin_fmaxf(A2 * over, -126.0f), 1000.0f), e = __builtin_rintf(v);
+  const float v = __builtin_fminf(__builtin_fmaxf(A2 * over, -1000.0f), 1000.0f), e = __builtin_rintf(v);
   return __builtin_ldexpf(s * __builtin_amdgcn_exp2f(v - e), (int)e);
 }
 
@@ -543,7 +540,7 @@ __global__ __launch_bounds__(64) void ssm_join_kernel(SsmParams p) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (k0 + k >= count) continue;
-      const float decay = decay_over(A2, over[k]);
+      const float decay = __builtin_amdgcn_exp2f(A2 * over[k]);
       const bool drop = over[k] < 0.0f;
       largest = __builtin_fmaxf(__builtin_fmaxf(largest, __builtin_fabsf(s)), decay);
       s = drop ? end[k] : __builtin_fmaf(decay, s, end[k]);
@@ -554,7 +551,10 @@ __global__ __launch_bounds__(64) void ssm_join_kernel(SsmParams p) {
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         if (k0 + k >= count) continue;
-        s = over[k] < 0.0f ? end[k] : passed(s, A2, over[k], span[k * span_step + most]) + end[k];
+        const float decay = __builtin_amdgcn_exp2f(A2 * over[k]);
+        if (over[k] < 0.0f) s = end[k];
+        else if (__builtin_fmaxf(__builtin_fabsf(s), decay) >= kUnusual) s = passed(s, A2, over[k], span[k * span_step + most]) + end[k];
+        else s = __builtin_fmaf(decay, s, end[k]);  // as above: a lane's result is its own
         slot[k * step] = s;
       }
     }

@@ -139,3 +139,36 @@ def test_states_that_grow_past_a_chunk(dev, T, B, H):
     # a span's exponent of 185 by 3 of its own: 400
     P.assert_within(h, want, want, 2000, "h_T")
     assert (h[..., 1] == 0).all() and h[..., 0].min() > 1e16
+
+
+# with the last step of a first chunk, and the first of one that is neither first nor second
+@pytest.mark.parametrize("T,B,H,N,last,first", [(300, 2, 24, 4, 79, 160), (1061, 40, 70, 4, 47, 960)])
+@pytest.mark.parametrize("large", [1e30, 1e38])
+def test_a_large_state_decays_to_nothing(dev, T, B, H, N, last, first, large):
+    """A finite state that a chunk's decay leaves nothing of is gone behind the chunk, however large it was, and so is a
+    gradient on its way back."""
+    t, dy, dh = _fast(T, B, H, N, dev, 45)
+    t["u"][:, 0, 3], t["h0"][0, 3], dy[:, 1, 4], dh[1, 4] = 0.0, 0.0, 0.0, 0.0
+    t["u"][last, 0, 3], dy[first, 1, 4] = large, large
+    y, _, got = _run(t, dy, dh)
+    # e^-3.2 a step: 60 steps leave 4e-84 of it
+    assert y[last, 0, 3].abs() > 1e-6 * large and (y[last + 60:, 0, 3] == 0).all()
+    assert got["u"][first - 1, 1, 4].abs() > 1e-6 * large and (got["u"][:first - 60, 1, 4] == 0).all()
+
+
+@pytest.mark.parametrize("T,B,H,N", [(300, 2, 24, 4), (1061, 40, 70, 4)])
+@pytest.mark.parametrize("large", [3e38, INF, float("nan")])
+def test_channels_do_not_see_each_other(dev, T, B, H, N, large):
+    """What is unusual in a channel changes no bit of another's results."""
+    t, dy, dh = _fast(T, B, H, N, dev, 46)
+    y, h, got = _run(t, dy, dh)
+    t["h0"][0, 3, 1], dh[0, 4, 2] = large, large
+    y1, h1, got1 = _run(t, dy, dh)
+    others = [c for c in range(H) if c not in (3, 4)]
+    assert torch.equal(y[..., others], y1[..., others]) and torch.equal(h[:, others], h1[:, others])
+    for k in ("u", "delta", "z"):
+        assert torch.equal(got[k][..., others], got1[k][..., others]), k
+    assert torch.equal(got["h0"][:, others], got1["h0"][:, others])
+    for k in ("A", "D", "delta_bias"):
+        assert torch.equal(got[k][others], got1[k][others]), k
+    assert torch.equal(y[:, 1:], y1[:, 1:]) and torch.equal(got["B"][:, 1:], got1["B"][:, 1:])
