@@ -57,7 +57,7 @@ def causal_conv_step(
     """One token for each row of ``x`` [B, C]: ``y`` [B, C], with the inputs before it in row
     ``slots[b]`` of ``state`` [S, W - 1, C] (x's type), which moves on in place. ``slots`` as in
     ``gated_linear_step``: distinct int32 rows, row b when None, a negative one for an empty row
-    of the batch (its output is zero), NaN for one past the cache. No autograd."""
+    of the batch (its output is zero), NaN for one past the cache. At most 65535 rows. No autograd."""
     act = _activation("causal_conv_step", activation)
     try:
         return (_lib._ops or _lib.ops()).causal_conv_step(x, weight, bias, state, slots, act)

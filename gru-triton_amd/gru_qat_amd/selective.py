@@ -60,7 +60,7 @@ def selective_step(
     """One token for each row of ``u``, ``delta`` and ``z`` [B, H], ``B`` and ``C`` [B, N]: advances row
     ``slots[b]`` of ``state`` [S, H, N] (float32, in place) and returns ``y`` [B, H] in u's type.
     ``slots`` as in ``gated_linear_step``: distinct int32 rows, row b when None, a negative one for an
-    empty row of the batch (its output is zero), NaN for one past the cache. No autograd."""
+    empty row of the batch (its output is zero), NaN for one past the cache. At most 65535 rows. No autograd."""
     try:
         return (_lib._ops or _lib.ops()).selective_step(u, delta, A, B, C, state, slots, D, z, delta_bias)
     except TypeError as e:

@@ -17,7 +17,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0)
     """``scale * weight[tokens]`` [..., K] for ``tokens`` [...] (int32 or int64) and ``weight`` [V, K]
     (float32 or bfloat16). A negative token marks padding: a row of zeros that sends no gradient; one
     of V or more gives NaN and sends none. Differentiable in weight (once): the gradient is dense,
-    its sums are float32, and it is the same from run to run."""
+    its sums are float32, and it is the same from run to run. At most 2^25 tokens and 2^25 rows of
+    2^20 elements."""
     try:
         return (_lib._ops or _lib.ops()).embedding(tokens, weight, scale)
     except TypeError as e:
@@ -36,7 +37,7 @@ def token_logprobs(
     -infinity, entropy 0 and no gradient. A NaN or +infinity makes a row's results NaN. A negative
     token does not count: its log probability is 0 and sends no gradient (its row's entropy does);
     one of V or more gives NaN. The logits of a row to which no gradient comes get zeros, also NaN
-    ones. Rows have at most 2^24 logits, 2^19 with ``top``. Differentiable in logits
+    ones. At most 2^23 rows of 2^24 logits, 2^19 with ``top``. Differentiable in logits
     through logprobs and entropy (once): ``-logprobs.sum() / (tokens >= 0).sum()`` is the
     cross entropy over the tokens that count."""
     try:
